@@ -275,8 +275,8 @@ SSLM_API sslm_status sslm_b200_debug_withhold_tc_load(int32_t launches);
  * `kernel` waits for more than will come in one of its exchanges. kernel 0: the weights-first linear kernel
  * where K is cut over a cluster (exchange 0); 1: attention of few rows (0 maxima, 1 sums, 2 contexts, 3 the
  * funnel's maximum); 2: attention of prefill chunks in tiles cut over a cluster (0 to 2); 3: the activation
- * site (0); 5: attention of few biased rows with the q/k/v site inside (0 the biased elements' maximum). kernel -1 takes
- * the request back. */
+ * site (0); 5: attention of few biased rows with the q/k/v site inside (0 the biased elements' maximum); 6: attention of
+ * rows that share a prefix (0 to 2); 7: the pick (0). kernel -1 takes the request back. */
 SSLM_API sslm_status sslm_b200_debug_withhold_exchange(int32_t kernel, int32_t exchange);
 /* Tests only: the first kernel of each of the next `launches` (0..16) row groups counts as refused by the CUDA
  * runtime, as for want of resources. The verb returns SSLM_ALLOCATION_FAILED and launches nothing behind it. */
@@ -350,6 +350,100 @@ SSLM_API sslm_status sslm_b200_linear_resident(const int8_t* d_x, const int8_t* 
                                                int64_t site_m, int64_t site_e, int32_t* d_out_folded,
                                                int8_t* d_out_codes, int64_t* d_out_scales,
                                                int32_t* d_row_status, void* stream);
+
+/* ---- operators on a caller's own tensors, besides the linear layer above. As there: every pointer is a
+ * device pointer on the calling thread's current device, nothing is allocated, the work is enqueued on
+ * `stream` (a cudaStream_t, NULL = the default stream) and the call returns without waiting. They have no
+ * scratch: calls may overlap, on any streams, and may be captured into graphs (the first call of a kind
+ * on a device sets its kernels up: make it before a capture begins). What a call leaves out, rows of no
+ * group or refused rows, is left as it was. `struct_size` is the size of the struct, `reserved` 0.
+ *
+ * Row statuses (row_status, int32 [rows], may be NULL): 0, or why the row was refused by the kernel: */
+#define SSLM_B200_ROW_LENGTH 7       /* a length below zero or above the room the call gave */
+#define SSLM_B200_ROW_CONSTANTS 20   /* constants outside their domain */
+#define SSLM_B200_ROW_WAIT 100       /* a bounded wait inside the kernel ran out; the row's outputs are not valid */
+#define SSLM_B200_ROW_INDEX 101      /* a page id, or a mask's number, that does not exist */
+
+/* Integer attention of rows that share prefixes, each prefix read and multiplied once for all its rows (the
+ * attention of sslm_decode_step over P + S positions of the paged pool, src/forward/forward_sites.cpp:1858-1903).
+ * Row r is one token; group g is the rows group_start[g] .. group_start[g + 1] (ascending, device memory); its
+ * rows see prefix_len[g] positions of prefix_pages[g] and then suffix_len[r] positions of suffix_pages[r]. Either
+ * length may be 0 or end inside a page; a row that sees nothing has a context of zeros. Several rows may name
+ * the same suffix pages (a draft of several tokens: lengths one apart).
+ *   s_k = q . K_k;  x = min(max s - s_k, 30 q_ln2);  z = floor(x / q_ln2);  e_k = ((q_b - x + z q_ln2)^2 + q_c) >> z
+ *   p_k = floor(2^15 e_k / sum e);  out = fold(sum p_k V_k)
+ * Query head h uses K / V head h / (heads / kv_heads). head_dim 32, 64 or 128; at most 8 query heads per K / V head;
+ * at most 32,768 positions a row, 65,535 rows and groups. Constants: 1 <= q_ln2 <= q_b < 2^24, q_c >= 0,
+ * peak = q_b^2 + q_c <= 2^47 and peak * width < 2^63, else the row is refused, as is one with a length or page
+ * id out of range (all rows of a prefix with a bad id).
+ * kv is one layer of a pool: [kv_heads][K, V][num_pages] pages of 16 positions, a K page [16][head_dim], a V page
+ * [head_dim][16]. fold (may be NULL: none): per query head (identity, multiplier, shift 0..31). out_codes / out_scales
+ * (may be NULL): the context funnel of the row with the site constant, int8 codes [rows][heads * head_dim] and
+ * (m, e) pairs, the operands sslm_b200_linear_resident takes; they need row_status.
+ * Alignment: kv and out 16 bytes, out_stride a multiple of 4 elements, q 4 bytes and q_stride a multiple of 4. */
+typedef struct sslm_b200_prefix_attention {
+	uint32_t struct_size;
+	int32_t rows, groups, heads, kv_heads, head_dim;
+	int32_t max_prefix, max_suffix;   /* no length is above these; the launch is sized by them */
+	const int8_t* q;                  /* [rows][heads][head_dim] rotated codes */
+	int64_t q_stride;                 /* elements between rows, as every stride here */
+	const int64_t* consts;            /* [rows][kv_heads][3] q_ln2, q_b, q_c */
+	const int8_t* kv;
+	int64_t num_pages;
+	const int32_t* group_start;       /* [groups + 1] */
+	const int32_t* prefix_len;        /* [groups] */
+	const int32_t* prefix_pages;      /* [groups][prefix_stride] */
+	int64_t prefix_stride;
+	const int32_t* suffix_len;        /* [rows] */
+	const int32_t* suffix_pages;      /* [rows][suffix_stride] */
+	int64_t suffix_stride;
+	const int32_t* fold;              /* [heads][3] */
+	int32_t* out;                     /* [rows][heads][head_dim] */
+	int64_t out_stride;
+	int64_t site_m, site_e;
+	int8_t* out_codes;
+	int64_t* out_scales;
+	int32_t* row_status;
+	uint64_t reserved;
+} sslm_b200_prefix_attention;
+SSLM_API sslm_status sslm_b200_attention_prefix_resident(const sslm_b200_prefix_attention* call, void* stream);
+
+/* The greedy token of logit rows that penalties, biases and masks have changed. Per token v of row r:
+ *   not allowed where the logit is INT32_MIN, or bit v of mask page mask_page[r] is clear (-1: no mask)
+ *   n = how often v is among the row's history_len[r] history ids (at most 65,535); where n > 0:
+ *       x = x > 0 ? floor(x 2^15 / repetition) : -floor(-x repetition / 2^15);  x -= presence + frequency n
+ *   x += every bias whose token is v (at most 1,024 a row; the same token twice counts twice)
+ *   x is held between -(2^31 - 1) and 2^31 - 1, INT32_MIN where v is not allowed
+ * out_tokens[r] is the lowest index of the largest x, -2 where nothing is allowed; out_best[r] that x; out_logits the
+ * changed row (may be `logits` itself, may not overlap it otherwise). Each may be NULL, not all. Ids outside
+ * the vocabulary, in either list, count for nothing. params, history, bias_tokens and mask_page may be NULL: none.
+ * A repetition below 1 (Q15: 32,768 is 1.0), a length below 0 or above its maximum or a mask number that does
+ * not exist refuses the row. */
+typedef struct sslm_b200_pick {
+	uint32_t struct_size;
+	int32_t rows, vocab, num_masks;
+	int32_t max_history, max_bias;    /* no length is above these */
+	uint32_t reserved;
+	const int32_t* logits;            /* [rows][logits_stride] */
+	int64_t logits_stride;
+	const int32_t* params;            /* [rows][3] repetition (Q15), presence, frequency (logit units) */
+	const int32_t* history;           /* [rows][history_stride] */
+	int64_t history_stride;
+	const int32_t* history_len;       /* [rows] */
+	const int32_t* bias_tokens;       /* [rows][bias_stride] */
+	const int32_t* bias_values;       /* [rows][bias_stride] */
+	int64_t bias_stride;
+	const int32_t* bias_len;          /* [rows] */
+	const uint8_t* masks;             /* [num_masks][mask_stride] bytes, bit v & 7 of byte v / 8 */
+	int64_t mask_stride;
+	const int32_t* mask_page;         /* [rows] */
+	int32_t* out_tokens;              /* [rows] */
+	int32_t* out_best;                /* [rows] */
+	int32_t* out_logits;              /* [rows][out_stride] */
+	int64_t out_stride;
+	int32_t* row_status;
+} sslm_b200_pick;
+SSLM_API sslm_status sslm_b200_pick_resident(const sslm_b200_pick* call, void* stream);
 
 #ifdef __cplusplus
 }

@@ -279,6 +279,148 @@ class Sequence:
                 self.eng.seqs.remove(self)
 
 
+# ---- operators on tensors in GPU memory (sslm_b200_*_resident). A call is prepared once from the tensors of a
+# program (anything with torch's data_ptr / shape / stride / dtype / device) and then run as often as their contents
+# change, like a batch of Engine.batch. It holds the tensors, copies none of them and keeps no result.
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("groups", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("max_prefix", C.c_int32), ("max_suffix", C.c_int32), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("consts", C.c_void_p), ("kv", C.c_void_p), ("num_pages", C.c_int64), ("group_start", C.c_void_p), ("prefix_len", C.c_void_p),
+                ("prefix_pages", C.c_void_p), ("prefix_stride", C.c_int64), ("suffix_len", C.c_void_p), ("suffix_pages", C.c_void_p),
+                ("suffix_stride", C.c_int64), ("fold", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("site_m", C.c_int64),
+                ("site_e", C.c_int64), ("out_codes", C.c_void_p), ("out_scales", C.c_void_p), ("row_status", C.c_void_p), ("reserved", C.c_uint64)]
+
+
+class PickArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("vocab", C.c_int32), ("num_masks", C.c_int32), ("max_history", C.c_int32),
+                ("max_bias", C.c_int32), ("reserved", C.c_uint32), ("logits", C.c_void_p),
+                ("logits_stride", C.c_int64), ("params", C.c_void_p), ("history", C.c_void_p), ("history_stride", C.c_int64),
+                ("history_len", C.c_void_p), ("bias_tokens", C.c_void_p), ("bias_values", C.c_void_p), ("bias_stride", C.c_int64),
+                ("bias_len", C.c_void_p), ("masks", C.c_void_p), ("mask_stride", C.c_int64), ("mask_page", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("out_best", C.c_void_p), ("out_logits", C.c_void_p), ("out_stride", C.c_int64), ("row_status", C.c_void_p)]
+
+
+class _ResidentCall:
+    def __init__(self, lib: SslmLib, verb: str, args):
+        self._fn = getattr(lib.dll, verb)
+        self._fn.restype = C.c_int
+        self._fn.argtypes = [C.c_void_p, C.c_void_p]
+        self.verb, self.args, self._held, self._device = verb, args, [], None
+        args.struct_size = C.sizeof(args)
+
+    def _hold(self, name, t, dtype, shape, rows_strided=False):
+        """The address of a tensor of this dtype and shape (None: any extent), dense but for the rows' stride."""
+        if t is None:
+            return None
+        if str(t.dtype).split(".")[-1] != dtype:
+            raise TypeError("%s: %s expected, got %s" % (name, dtype, t.dtype))
+        if len(t.shape) != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape)):
+            raise ValueError("%s: shape %s expected, got %s" % (name, list(shape), list(t.shape)))
+        if t.device.type != "cuda" or (self._device is not None and t.device != self._device):
+            raise ValueError("%s: a tensor on %s expected, got one on %s" % (name, self._device or "a GPU", t.device))
+        want = 1
+        for i in range(len(shape) - 1, -1, -1):
+            if rows_strided and i == 0:
+                if t.shape[0] > 1 and t.stride(0) < want:
+                    raise ValueError("%s: rows may not overlap" % name)
+            elif t.shape[i] > 1 and t.stride(i) != want:
+                raise ValueError("%s: dense elements expected, got strides %s" % (name, list(t.stride())))
+            want *= t.shape[i]
+        self._device = t.device
+        self._held.append(t)
+        return t.data_ptr()
+
+    @staticmethod
+    def _row_stride(t, width):
+        return t.stride(0) if t is not None and t.shape[0] > 1 else width
+
+    def run(self, stream=None):
+        """Enqueues the call on `stream` (a cudaStream_t as an int; default: torch's current stream of the tensors' device)."""
+        import torch
+        if torch.cuda.current_device() != self._device.index:
+            with torch.cuda.device(self._device):
+                return self.run(stream)
+        if stream is None:
+            stream = torch.cuda.current_stream().cuda_stream
+        st = self._fn(C.addressof(self.args), stream)
+        if st != SSLM_OK:
+            raise SslmError(self.verb, st)
+
+
+class PrefixAttention(_ResidentCall):
+    """sslm_b200_attention_prefix_resident. q int8 [rows, heads, head_dim] and out int32 of the same shape (rows may be
+    strided), consts int64 [rows, kv_heads, 3], kv int8 [kv_heads, 2, pages, 16 * head_dim], group_start int32 [groups + 1],
+    prefix_len int32 [groups], prefix_pages int32 [groups, n], suffix_len int32 [rows], suffix_pages int32 [rows, n], fold int32
+    [heads, 3] or None; out_codes int8 [rows, heads * head_dim] and out_scales int64 [rows, 2] with site = (m, e); row_status int32 [rows].
+    No length may exceed max_prefix / max_suffix (default: what the page tables hold)."""
+
+    def __init__(self, lib, q, consts, kv, group_start, prefix_len, prefix_pages, suffix_len, suffix_pages, out, fold=None, max_prefix=None,
+                 max_suffix=None, site=(0, 0), out_codes=None, out_scales=None, row_status=None):
+        a = PrefixAttentionArgs()
+        super().__init__(lib, "sslm_b200_attention_prefix_resident", a)
+        rows, heads, hd = q.shape
+        groups, kv_heads = prefix_len.shape[0], kv.shape[0]
+        a.rows, a.groups, a.heads, a.kv_heads, a.head_dim = rows, groups, heads, kv_heads, hd
+        a.q, a.q_stride = self._hold("q", q, "int8", (rows, heads, hd), True), self._row_stride(q, heads * hd)
+        a.consts = self._hold("consts", consts, "int64", (rows, kv_heads, 3))
+        a.kv, a.num_pages = self._hold("kv", kv, "int8", (kv_heads, 2, None, 16 * hd)), kv.shape[2]
+        a.group_start = self._hold("group_start", group_start, "int32", (groups + 1,))
+        a.prefix_len = self._hold("prefix_len", prefix_len, "int32", (groups,))
+        a.prefix_pages = self._hold("prefix_pages", prefix_pages, "int32", (groups, None), True)
+        a.prefix_stride = self._row_stride(prefix_pages, prefix_pages.shape[1])
+        a.suffix_len = self._hold("suffix_len", suffix_len, "int32", (rows,))
+        a.suffix_pages = self._hold("suffix_pages", suffix_pages, "int32", (rows, None), True)
+        a.suffix_stride = self._row_stride(suffix_pages, suffix_pages.shape[1])
+        a.max_prefix = min(32768, prefix_pages.shape[1] * 16) if max_prefix is None else max_prefix
+        a.max_suffix = min(32768, suffix_pages.shape[1] * 16) if max_suffix is None else max_suffix
+        if a.max_prefix > prefix_pages.shape[1] * 16 or a.max_suffix > suffix_pages.shape[1] * 16:
+            raise ValueError("max_prefix / max_suffix: more than the page tables hold")
+        a.fold = self._hold("fold", fold, "int32", (heads, 3))
+        a.out, a.out_stride = self._hold("out", out, "int32", (rows, heads, hd), True), self._row_stride(out, heads * hd)
+        a.site_m, a.site_e = site
+        a.out_codes = self._hold("out_codes", out_codes, "int8", (rows, heads * hd))
+        a.out_scales = self._hold("out_scales", out_scales, "int64", (rows, 2))
+        a.row_status = self._hold("row_status", row_status, "int32", (rows,))
+
+
+class Pick(_ResidentCall):
+    """sslm_b200_pick_resident. logits int32 [rows, vocab] (rows may be strided), params int32 [rows, 3] (repetition in Q15, presence,
+    frequency), history int32 [rows, n] with history_len int32 [rows], bias_tokens and bias_values int32 [rows, n] with bias_len int32
+    [rows], masks uint8 [pages, ceil(vocab / 8)] with mask_page int32 [rows] (-1: none), out_tokens and out_best int32 [rows],
+    out_logits int32 [rows, vocab] (may be `logits`), row_status int32 [rows]; what is None is left out."""
+
+    def __init__(self, lib, logits, params=None, history=None, history_len=None, bias_tokens=None, bias_values=None, bias_len=None, masks=None,
+                 mask_page=None, out_tokens=None, out_best=None, out_logits=None, row_status=None):
+        a = PickArgs()
+        super().__init__(lib, "sslm_b200_pick_resident", a)
+        rows, vocab = logits.shape
+        a.rows, a.vocab = rows, vocab
+        a.logits, a.logits_stride = self._hold("logits", logits, "int32", (rows, vocab), True), self._row_stride(logits, vocab)
+        a.params = self._hold("params", params, "int32", (rows, 3))
+        if (history is None) != (history_len is None) or (masks is None) != (mask_page is None) or len({bias_tokens is None, bias_values is None, bias_len is None}) > 1:
+            raise ValueError("a list comes with its lengths (and values), masks with mask_page")
+        if history is not None:
+            a.history, a.history_stride = self._hold("history", history, "int32", (rows, None), True), self._row_stride(history, history.shape[1])
+            a.max_history = history.shape[1]
+            a.history_len = self._hold("history_len", history_len, "int32", (rows,))
+        if bias_tokens is not None:
+            a.bias_tokens = self._hold("bias_tokens", bias_tokens, "int32", (rows, None))
+            a.bias_values = self._hold("bias_values", bias_values, "int32", tuple(bias_tokens.shape))
+            a.bias_stride = a.max_bias = bias_tokens.shape[1]
+            a.bias_len = self._hold("bias_len", bias_len, "int32", (rows,))
+        if masks is not None:
+            a.masks, a.num_masks = self._hold("masks", masks, "uint8", (None, None), True), masks.shape[0]
+            if masks.shape[1] < (vocab + 7) // 8:
+                raise ValueError("masks: %d bytes a page expected, got %d" % ((vocab + 7) // 8, masks.shape[1]))
+            a.mask_stride = self._row_stride(masks, masks.shape[1])
+            a.mask_page = self._hold("mask_page", mask_page, "int32", (rows,))
+        a.out_tokens = self._hold("out_tokens", out_tokens, "int32", (rows,))
+        a.out_best = self._hold("out_best", out_best, "int32", (rows,))
+        a.out_logits = self._hold("out_logits", out_logits, "int32", (rows, vocab), True)
+        a.out_stride = self._row_stride(out_logits, vocab)
+        a.row_status = self._hold("row_status", row_status, "int32", (rows,))
+
+
 def parse_save_blob(blob: bytes, hidden_size: int) -> dict:
     """Fields of an SSB3 sequence blob (src/sslm_abi.cpp:2620-2716)."""
     assert blob[0:4] == b"SSB3"

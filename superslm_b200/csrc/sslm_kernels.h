@@ -91,7 +91,8 @@ inline int sm_count() {
 // with four bytes more than will come: that block's wait runs out. One word: 0 for none, else
 // kernel << 8 | exchange + 1.
 // (4 names no kernel; 5 is the fifth exchange of attention with the q/k/v site of biased rows inside)
-enum ExchangeKernel { kExchangeLinear = 0, kExchangeAttnFew, kExchangeAttnChunk, kExchangeAct, kExchangeAttnSite = 5, kExchangeKernels };
+// (6: attention of rows that share a prefix; 7: the pick)
+enum ExchangeKernel { kExchangeLinear = 0, kExchangeAttnFew, kExchangeAttnChunk, kExchangeAct, kExchangeAttnSite = 5, kExchangeAttnPrefix, kExchangePick, kExchangeKernels };
 inline std::atomic<uint32_t> g_withheld_exchange{0};
 inline int exchange_debug_take(ExchangeKernel kernel) {
 	uint32_t w = g_withheld_exchange.load(std::memory_order_relaxed);
@@ -204,6 +205,7 @@ void launch_lora_u(const RowBatch& b, const int8_t* x, int k_in, int layer, int 
 cudaError_t attn_configure(const Dims& d);
 // slices per kv head of later attention launches (0: chosen per launch); for tuning and tests
 void attn_force_splits(int splits);
+int attn_forced_splits();
 // How the attention of m rows will run, decided ahead of the q/k/v site: site != 0 says that it takes that site over
 // (launch_qkv_post is then left out).
 struct AttnChoice {

@@ -78,6 +78,16 @@ struct RowDesc {
 	int32_t pad;
 };
 
+// What the pick of one row works on: its logits and what changes them (sslm_pick.cu).
+struct PickRow {
+	const int32_t* logits;                      // nullptr: the row has no controls
+	const int32_t* history;                     // ids that count as repeated, n_history of them, and `extra`, or -1
+	const int32_t *bias_tokens, *bias_values;
+	const uint8_t* mask;                        // allowed tokens, a bit each, or nullptr: all
+	int32_t theta, presence, frequency, n_history, extra, n_bias;
+	int32_t layer, pad;
+};
+
 struct RowSource { const int8_t* hidden; const Scale* scale; };  // nullptr hidden: embed rows[r].token
 struct RowSink { int8_t* hidden; Scale* scale; };                // nullptr hidden: drop
 
