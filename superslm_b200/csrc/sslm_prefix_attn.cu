@@ -6,13 +6,14 @@
 // A tile is ROWS query rows of one kv head: tq = ROWS / G rows of a group times the G q heads of that kv head.
 // The tile multiplies the prefix's K and V once, ROWS rows at a time; a row's own pages are multiplied
 // with the same instructions, the other rows of the tile left out. A tile is cut over the blocks of a
-// cluster, prefix in steps of 128 positions and suffixes in pages of 16, both dealt round-robin, and the
-// blocks exchange maxima, sums and shares of P.V as k_attention_chunk's do (sums and maxima of integers:
-// no order of arrival changes a result).
+// cluster, the pages of the prefix and those of the suffixes both dealt round-robin, and the blocks exchange
+// maxima, sums and shares of P.V as k_attention_chunk's do (sums and maxima of integers: no order of arrival
+// changes a result).
 //
-// The scores of a step lie in shared memory, four neighbouring positions of a row per word quad: of the
-// prefix where the thread that computed them finds them again, of suffix pages packed by (page, head), since
-// only G of the tile's rows see such a page. Both become the A fragments of P.V in place.
+// K and V go from L2 straight into the registers of the warp that multiplies them: a page of K belongs to one
+// warp, 8 or 16 channels of all V pages to one. The scores stay in shared memory, of the prefix by page and row, of suffix
+// pages by page and head, since only G of the tile's rows see such a page; (shift, base) words and then the two
+// byte planes of the probabilities take their place.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -26,13 +27,14 @@
 
 namespace sslm {
 
-constexpr int kPfxThreads = 256, kPfxStep = 128, kPfxStepPages = kPfxStep / kPageTokens;
+constexpr int kPfxThreads = 512;
 constexpr int kPfxMaxWidth = 32768;      // positions a row sees at most: the longest admitted context
 constexpr int kPfxTokens = 32;           // rows a tile holds at most (32 query rows of groups of one)
 
 struct PrefixArgs {
 	int rows, groups, G, kv_heads, tq, ginv, shift;      // ginv = ceil(65536 / G); a tile is cut over 1 << shift blocks
-	int psteps, spages;                                  // prefix steps and suffix pages a block has room for
+	int ppages, spages;                                  // prefix and suffix pages a block has room for (multiples of four)
+	int vgroups;                                         // groups of four pages whose V it has room for
 	int max_prefix, max_suffix;
 	const int8_t* q;
 	int64_t q_stride;
@@ -55,14 +57,19 @@ struct PrefixArgs {
 	int debug_withhold;            // tests only (exchange_debug_take)
 };
 
+// Scores of a page: 64 bytes per row (16 positions), and 16 more, so that the sixteen bytes of four neighbouring
+// pages that a lane quad reads together lie in different banks.
+constexpr int kPfxPad = 16;
 template <int HD, int ROWS>
 struct PrefixSmem {
-	static constexpr int kKStride = HD + 16;                                        // (padding against bank conflicts)
-	static constexpr size_t kStage = (size_t)2 * kPfxStep * kKStride;               // two K steps, two V steps, or received shares
-	static constexpr size_t kStepScores = (size_t)ROWS * kPfxStep * 4;
-	static constexpr size_t bytes(int psteps, int spages, int group) {
-		return kStage + kStepScores * psteps + (size_t)spages * group * kPageTokens * 4 + (size_t)(psteps * kPfxStepPages + spages) * 8 + (size_t)spages * 4;
+	static constexpr int kQStride = HD + 16, kSumStride = HD + 8;      // (padding against bank conflicts)
+	static constexpr size_t kShares = (size_t)ROWS * HD * 4;           // what the blocks of the cluster send of P.V
+	static constexpr size_t kSums = (size_t)ROWS * kSumStride * 4;     // the warps' shares of it, and before that the tile's q rows
+	static constexpr size_t bytes(int ppages, int spages, int group, bool cluster) {
+		return (cluster ? kShares : 0) + kSums + (size_t)ppages * (ROWS * 64 + kPfxPad) + (size_t)spages * (group * 64 + kPfxPad) + (size_t)(ppages + spages) * 12 +
+		       (size_t)spages * 4;
 	}
+	static constexpr size_t kVPage = (size_t)kPageTokens * HD + 32;    // a staged V page (padding as above)
 };
 
 // the constants of a row's softmax element lie where the kernels' short forms hold, and a row of `width` such
@@ -72,44 +79,97 @@ __device__ __forceinline__ bool softmax_gate(int64_t ln2, int64_t qb, int64_t qc
 	const int64_t peak = qb * qb + qc;      // (below 2^49)
 	return peak <= SSLM_SOFTMAX_MAX_SAFE && (unsigned long long)peak * (unsigned long long)max(width, 1) <= 0x7FFFFFFFFFFFFFFFull;
 }
+// The HD / 16 words of a head-dim row that lane column c feeds to the score MMAs: MMA j takes words 2j (k slots 4c ..) and 2j + 1
+// (16 + 4c ..), of q and of K alike.
+template <int HD>
+__device__ __forceinline__ void row_words(const int8_t* row, int c, uint32_t (&w)[HD / 16]) {
+	if constexpr (HD == 128) {
+		asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+		             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+		             : "l"(row + c * 32)
+		             : "memory");
+	} else if constexpr (HD == 64) {
+		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 16) : "memory");
+	} else {
+		asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(row + c * 8) : "memory");
+	}
+}
+__device__ __forceinline__ int4 load16(const void* p) {
+	int4 v;
+	asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+	return v;
+}
+
+// One softmax element as chunk_exp (sslm_softmax.cuh) has it, under the same gates, with the division by a product: for
+// d = q_ln2 <= 2^L, L <= 24, M = floor(2^(31 + L) / d) + 1 fits 32 bits and exceeds 2^(31 + L) / d by at most d / d, so that
+// x M / 2^(31 + L) exceeds x / d by at most x / 2^(31 + L) < 1 / d for x <= 30 d, and its floor is that of x / d.
+struct IExpMul {
+	uint32_t ln2, clip, mul, shift;      // clip = 30 ln2
+	int64_t qc;
+	uint32_t qb, pad;
+};
+__device__ __forceinline__ IExpMul iexp_mul_prepare(int64_t ln2, int64_t qb, int64_t qc) {
+	IExpMul f;
+	f.ln2 = (uint32_t)ln2;
+	f.clip = 30u * f.ln2;
+	f.shift = 31u + (f.ln2 > 1u ? 32u - (uint32_t)__clz((int)(f.ln2 - 1u)) : 0u);
+	f.mul = (uint32_t)((1ull << f.shift) / f.ln2) + 1u;
+	f.qc = qc;
+	f.qb = (uint32_t)qb;
+	f.pad = 0;
+	return f;
+}
+__device__ __forceinline__ unsigned long long iexp_mul(uint32_t dq, const IExpMul& f, uint32_t* parts) {
+	const uint32_t x = min(dq, f.clip);
+	const uint32_t z = (uint32_t)(((unsigned long long)x * f.mul) >> f.shift);
+	const uint32_t base = z * f.ln2 + (f.qb - x);      // 1 .. q_b < 2^24
+	*parts = (z << 24) + base;
+	return ((unsigned long long)base * base + (unsigned long long)f.qc) >> z;
+}
 
 template <int HD, int ROWS, bool RESIDENT>
-__global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __grid_constant__ PrefixArgs a) {
+__global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __grid_constant__ PrefixArgs a) {
 	using L = PrefixSmem<HD, ROWS>;
-	constexpr int KS = HD / 32;                       // MMA steps along the head dimension
-	constexpr int RB = ROWS / 16;                     // 16-row blocks
-	constexpr int CW = 8 / RB;                        // warps per row block: along the pages of a step, along the channels of P.V
-	constexpr int PW = kPfxStepPages / CW;            // pages of a step per warp
-	constexpr int NT = HD / 8 >= CW ? HD / 8 / CW : 1;      // 8-channel tiles a warp owns in P.V (some warps none: 32 channels, 16 rows)
-	constexpr int kSlots = RB * 32;
+	constexpr int KS = HD / 32;                 // MMA steps along the head dimension
+	constexpr int RB = ROWS / 16;               // 16-row blocks
+	constexpr int W = kPfxThreads / 32;
+	constexpr int kPageScores = ROWS * 64 + kPfxPad;
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ __align__(8) unsigned long long s_bars[3];
+	__shared__ __align__(8) unsigned long long s_bars[4];      // staged V; maxima, sums, shares of P.V
 	__shared__ unsigned long long s_sum[ROWS], s_rxsum[kPfxThreads];
-	__shared__ IExpFast s_fx[kPfxTokens];
-	__shared__ int32_t s_max[ROWS], s_rxmax[kPfxThreads], s_len[kPfxTokens], s_code[kPfxTokens], s_cum[kPfxTokens + 1], s_fold[24], s_tile[3], s_badprefix;
+	__shared__ IExpMul s_fx[kPfxTokens];
+	__shared__ float4 s_prob[ROWS];             // (c, q_c, eps) of a row's probabilities
+	__shared__ int32_t s_max[ROWS], s_rxmax[kPfxThreads], s_len[kPfxTokens], s_code[kPfxTokens], s_cum[kPfxTokens + 1], s_fold[24], s_tile[4];
 
 	const int G = a.G, kvh = (int)blockIdx.z;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
 	const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
-	int8_t* stage = (int8_t*)smem;
-	int4* sc = (int4*)(smem + L::kStage);                                                       // [step][page][row a, row b][kSlots]
-	int4* csc = (int4*)(smem + L::kStage + L::kStepScores * a.psteps);                          // [suffix page][head][4]
-	int64_t* pbase = (int64_t*)((unsigned char*)csc + (size_t)a.spages * G * kPageTokens * 4);  // page offsets inside a plane, -1: none
-	int64_t* sbase = pbase + a.psteps * kPfxStepPages;
-	int32_t* sown = (int32_t*)(sbase + a.spages);                                               // owner | positions << 8
-	int32_t* rx_ctx = (int32_t*)stage;                                                          // [sub][ROWS / sub][HD]
+	int32_t* rx_ctx = (int32_t*)smem;                                                       // [sub][ROWS / sub][HD], of a cluster
+	int32_t* ctx = (int32_t*)(smem + (sub > 1 ? L::kShares : 0));                           // [ROWS][kSumStride]
+	int8_t* qs = (int8_t*)ctx;                                                              // [ROWS][kQStride]
+	unsigned char* vst = (unsigned char*)ctx + L::kSums;                                    // [4 vgroups] staged V pages
+	unsigned char* sc = vst + (size_t)a.vgroups * 4 * L::kVPage;                            // [page][row][16] scores of prefix pages
+	unsigned char* csc = sc + (size_t)a.ppages * kPageScores;                               // [page][head][16] scores of suffix pages
+	const int csc_page = G * 64 + kPfxPad;
+	int64_t* pbase = (int64_t*)(csc + (size_t)a.spages * csc_page);                         // page offsets inside a plane, -1: none
+	int64_t* sbase = pbase + a.ppages;
+	int32_t* sown = (int32_t*)(sbase + a.spages);                                           // owner | positions << 8
+	uint32_t* redo = (uint32_t*)(sown + a.spages);                                          // [ppages, then spages] rows whose probabilities need the exact form
 
-	if (sub > 1) {
-		if (t == 0) {
+	if (t == 0) {
+		ring_init(cta_addr(&s_bars[0]), 1);
+		if (sub > 1) {
 			const int held = (blockIdx.x | blockIdx.y | blockIdx.z) == 0 ? a.debug_withhold : 0;
 			auto more = [&](int i) { return held == i + 1 ? 4u : 0u; };
-			exchange_init(cta_addr(&s_bars[0]), (uint32_t)(sub * ROWS * 4) + more(0));
-			exchange_init(cta_addr(&s_bars[1]), (uint32_t)(sub * ROWS * 8) + more(1));
-			exchange_init(cta_addr(&s_bars[2]), (uint32_t)(ROWS * HD * 4) + more(2));
-			exchange_fence_init();
+			exchange_init(cta_addr(&s_bars[1]), (uint32_t)(sub * ROWS * 4) + more(0));
+			exchange_init(cta_addr(&s_bars[2]), (uint32_t)(sub * ROWS * 8) + more(1));
+			exchange_init(cta_addr(&s_bars[3]), (uint32_t)(ROWS * HD * 4) + more(2));
 		}
-		cluster_arrive();
-		cluster_wait();
+		exchange_fence_init();
+	}
+	if (sub > 1) {
+		__syncwarp();
+		cluster_arrive();      // (waited for ahead of the first word that is sent)
 	}
 	// A caller's tensors may have been written by the kernel in front. An engine call's descriptors, lengths and page
 	// tables were uploaded, and the prefix's pages filled, before its first launch.
@@ -119,12 +179,15 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 	}
 	// ---- which tile: group after group, tq rows at a time
 	if (warp == 0) {
-		int want = (int)blockIdx.y, r0 = 0, nt = 0, group = 0;
+		int want = (int)blockIdx.y, r0 = 0, nt = 0, group = 0, prefix = 0;
 		for (int g0 = 0; g0 < a.groups; g0 += 32) {
-			int start = 0, n = 0;
+			int start = 0, n = 0, len = 0;
 			if (g0 + lane < a.groups) {
-				start = max(a.group_start[g0 + lane], 0);
-				n = max(min(a.group_start[g0 + lane + 1], a.rows) - start, 0);
+				start = a.group_start[g0 + lane];
+				n = a.group_start[g0 + lane + 1];
+				len = a.prefix_len[g0 + lane];
+				start = max(start, 0);
+				n = max(min(n, a.rows) - start, 0);
 			}
 			const int tiles = (n + a.tq - 1) / a.tq;
 			int upto = tiles;
@@ -138,6 +201,7 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 				const int src = __ffs(has) - 1, first = (want - (upto - tiles)) * a.tq;
 				r0 = __shfl_sync(0xffffffffu, start + first, src);
 				nt = __shfl_sync(0xffffffffu, min(a.tq, n - first), src);
+				prefix = __shfl_sync(0xffffffffu, len, src);
 				group = g0 + src;
 				break;
 			}
@@ -147,7 +211,7 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 			s_tile[0] = r0;
 			s_tile[1] = nt;
 			s_tile[2] = group;
-			s_badprefix = 0;
+			s_tile[3] = prefix;
 		}
 	}
 	if (t < ROWS) {
@@ -156,57 +220,55 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 	}
 	if (t < 3 * G) s_fold[t] = a.fold != nullptr ? a.fold[3 * kvh * G + t] : (t % 3 == 0 ? 1 : 0);
 	__syncthreads();
-	const int r0 = s_tile[0], nt = s_tile[1], group = s_tile[2];
-	if (nt == 0) return;      // (all blocks of the cluster alike)
-	int P = a.prefix_len[group];
-	const int32_t* prefix_pages = RESIDENT ? a.prefix_pages + (int64_t)group * a.prefix_stride : a.desc[r0].pages;
-	if (RESIDENT) {
-		// lengths, constants and page ids that are out of range refuse their row; every block of the tile comes to the
-		// same verdict by itself
-		const bool bad_len = P < 0 || P > a.max_prefix;
-		if (t < kPfxTokens) {
-			int code = kOk, len = 0;
-			if (t < nt) {
-				len = a.suffix_len[r0 + t];
-				if (bad_len || len < 0 || len > a.max_suffix || P + len > kPfxMaxWidth) {
-					code = SSLM_B200_ROW_LENGTH;
-				} else {
-					const int64_t* k = a.consts + (int64_t)(r0 + t) * a.kv_heads * 3;
-					for (int h = 0; h < a.kv_heads; ++h)
-						if (!softmax_gate(k[3 * h], k[3 * h + 1], k[3 * h + 2], P + len)) code = SSLM_B200_ROW_CONSTANTS;
-				}
-			}
-			s_len[t] = code == kOk ? len : 0;
-			s_code[t] = code;
-		}
-		if (bad_len) P = 0;
-		__syncthreads();
-		for (int i = t; i < (P + kPageTokens - 1) / kPageTokens; i += kPfxThreads)
-			if ((uint64_t)(int64_t)prefix_pages[i] >= (uint64_t)a.num_pages) s_badprefix = 1;
-		for (int tk = warp; tk < nt; tk += kPfxThreads / 32) {
-			const int32_t* pages = a.suffix_pages + (int64_t)(r0 + tk) * a.suffix_stride;
-			bool bad = false;
-			for (int i = lane; i < (s_len[tk] + kPageTokens - 1) / kPageTokens; i += 32) bad = bad || (uint64_t)(int64_t)pages[i] >= (uint64_t)a.num_pages;
-			if (__any_sync(0xffffffffu, bad) && lane == 0) {
-				s_code[tk] = SSLM_B200_ROW_INDEX;
-				s_len[tk] = 0;
-			}
-		}
-		__syncthreads();
-		if (s_badprefix != 0) {
-			P = 0;
-			if (t < nt && s_code[t] == kOk) s_code[t] = SSLM_B200_ROW_INDEX;
-			if (t < kPfxTokens) s_len[t] = 0;
-			__syncthreads();
-		}
-		// (the tiles of the first kv head start first: what a later one may have to say about a wait comes after this)
-		if (kvh == 0 && rank == 0 && t < nt && a.status != nullptr) a.status[r0 + t] = s_code[t];
-	} else if (t < kPfxTokens) {
-		s_len[t] = t < nt ? min(max(a.desc[r0 + t].pos + 1 - P, 0), a.max_suffix) : 0;
+	const int r0 = s_tile[0], nt = s_tile[1];
+	if (nt == 0) {      // (all blocks of the cluster alike)
+		if (sub > 1) cluster_wait();
+		return;
 	}
-	if (warp == 0) {      // pages of the tile's suffixes, counted up row by row
-		__syncwarp();
-		int upto = (s_len[lane] + kPageTokens - 1) / kPageTokens;
+	int P = s_tile[3];
+	const int32_t* prefix_pages = RESIDENT ? a.prefix_pages + (int64_t)s_tile[2] * a.prefix_stride : a.desc[r0].pages;
+	auto stage_q = [&](int first, int step) {      // rows of tokens that there are not: zeros
+		for (int i = first; i < ROWS * (HD / 4); i += step) {
+			const int rho = i / (HD / 4), w = i % (HD / 4), tk = rho * a.ginv >> 16;
+			*(uint32_t*)(qs + rho * L::kQStride + 4 * w) =
+			    tk < nt ? *(const uint32_t*)(a.q + (int64_t)(r0 + tk) * a.q_stride + (int64_t)(kvh * G + rho - tk * G) * HD + 4 * w) : 0u;
+		}
+	};
+	const bool bad_len = RESIDENT && (P < 0 || P > a.max_prefix);
+	if (bad_len) P = 0;
+	// ---- lengths and constants: what is out of range refuses its row; every block of the tile comes to the same verdict
+	const int64_t page_bytes = kPageTokens * HD, plane = a.num_pages * page_bytes;
+	const int8_t* kplane = a.kv + (int64_t)(2 * kvh) * plane;
+	const int8_t* vplane = kplane + plane;
+	auto mine = [&](int n) { return n > rank ? (n - rank + sub - 1) >> a.shift : 0; };      // of n things dealt out: rank, rank + sub, ...
+	auto known = [&](int id) { return !RESIDENT || (uint64_t)(int64_t)id < (uint64_t)a.num_pages; };
+	auto stage_v = [&](int at, int64_t base) {      // the page's V into place `at` (filled-up prefix pages first), while there is room
+		if (base < 0 || at >= 4 * a.vgroups) return;
+		const uint32_t bar = cta_addr(&s_bars[0]);
+		asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((uint32_t)page_bytes) : "memory");
+		asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(cta_addr(vst + (size_t)at * L::kVPage)),
+		             "l"(vplane + base), "r"((uint32_t)page_bytes), "r"(bar) : "memory");
+	};
+	const int np = min(mine((P + kPageTokens - 1) / kPageTokens), a.ppages), np4 = (np + 3) & ~3;      // (filled up to groups of four)
+	bool bad_page = false;
+	if (warp == 0) {
+		int code = lane < nt ? kOk : 1, len = 0;
+		if (lane < nt && RESIDENT) {
+			len = a.suffix_len[r0 + lane];
+			const int64_t* k = a.consts + (int64_t)(r0 + lane) * a.kv_heads * 3;
+			if (bad_len || len < 0 || len > a.max_suffix || P + len > kPfxMaxWidth) {
+				code = SSLM_B200_ROW_LENGTH;
+			} else {
+				for (int h = 0; h < a.kv_heads; ++h)
+					if (!softmax_gate(k[3 * h], k[3 * h + 1], k[3 * h + 2], P + len)) code = SSLM_B200_ROW_CONSTANTS;
+			}
+			if (code != kOk) len = 0;
+		} else if (lane < nt) {
+			len = min(max(a.desc[r0 + lane].pos + 1 - P, 0), a.max_suffix);
+		}
+		s_len[lane] = len;
+		s_code[lane] = code;
+		int upto = (len + kPageTokens - 1) / kPageTokens;      // pages of the suffixes, counted up row by row
 #pragma unroll
 		for (int o = 1; o < 32; o *= 2) {
 			const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -214,192 +276,168 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 		}
 		s_cum[lane + 1] = upto;
 		if (lane == 0) s_cum[0] = 0;
+	} else {      // (meanwhile the others: this block's prefix pages, and the tile's q rows)
+		for (int i = t - 32; i < np4; i += kPfxThreads - 32) {
+			const int id = i < np ? prefix_pages[rank + i * sub] : 0;
+			bad_page = bad_page || !known(id);
+			pbase[i] = i < np && known(id) ? (int64_t)id * page_bytes : -1;
+			redo[i] = 0u;
+			stage_v(i, pbase[i]);
+		}
+		if (RESIDENT) stage_q(t - 32, kPfxThreads - 32);
 	}
-	__syncthreads();
-	// ---- this block's part: prefix steps and suffix pages rank, rank + sub, ...
-	auto mine = [&](int n) { return n > rank ? (n - rank + sub - 1) >> a.shift : 0; };
-	const int nps = min(mine((P + kPfxStep - 1) / kPfxStep), a.psteps);
-	const int nsp = min(mine(s_cum[kPfxTokens]), a.spages);
-	const int nss = (nsp + kPfxStepPages - 1) / kPfxStepPages, steps = nps + nss;
-	const int64_t page_bytes = kPageTokens * HD, plane = a.num_pages * page_bytes;
-	const int8_t* kplane = a.kv + (int64_t)(2 * kvh) * plane;
-	const int8_t* vplane = kplane + plane;
-	for (int i = t; i < nps * kPfxStepPages; i += kPfxThreads) {
-		const int page = (rank + (i / kPfxStepPages) * sub) * kPfxStepPages + i % kPfxStepPages;
-		pbase[i] = page * kPageTokens < P ? (int64_t)prefix_pages[page] * page_bytes : -1;
-	}
-	for (int i = t; i < nss * kPfxStepPages; i += kPfxThreads) {
+	// a page id that does not exist: the rows that see the page report the largest maximum there is, which no score
+	// reaches, and every block of the tile learns of it with the maxima
+	if (__syncthreads_or((int)bad_page) && t < ROWS) s_max[t] = INT32_MAX;
+	// ---- K of this warp's first page is on its way while the suffix tables are made
+	const int krow = 4 * (g >> 1) + (g & 1);      // position of column g in the first MMA of a page, two more in the second
+	uint32_t kn[2][HD / 16];
+#pragma unroll
+	for (int w = 0; w < HD / 16; ++w) kn[0][w] = kn[1][w] = 0u;
+	auto fetch_k = [&](int64_t base) {      // (no page: nothing, the words are not used)
+		if (base >= 0) {
+			row_words<HD>(kplane + base + krow * HD, c, kn[0]);
+			row_words<HD>(kplane + base + (krow + 2) * HD, c, kn[1]);
+		}
+	};
+	if (warp < np) fetch_k(pbase[warp]);      // (of an engine call too: the prefix has been in place since its first launch)
+	const int ns = min(mine(s_cum[kPfxTokens]), a.spages), ns4 = (ns + 3) & ~3;
+	for (int i = t; i < ns4; i += kPfxThreads) {
 		int64_t base = -1;
 		int own = 255;
-		if (i < nsp) {
+		if (i < ns) {
 			const int x = rank + i * sub;
 			int tk = 0;
 			while (s_cum[tk + 1] <= x) ++tk;
 			const int page = x - s_cum[tk];
 			const int32_t* pages = RESIDENT ? a.suffix_pages + (int64_t)(r0 + tk) * a.suffix_stride : a.desc[r0 + tk].pages + P / kPageTokens;
-			base = (int64_t)pages[page] * page_bytes;
-			own = tk | min(kPageTokens, s_len[tk] - page * kPageTokens) << 8;
+			const int id = pages[page];
+			if (known(id)) {
+				base = (int64_t)id * page_bytes;
+				own = tk | min(kPageTokens, s_len[tk] - page * kPageTokens) << 8;
+			} else {
+				for (int h = 0; h < G; ++h) s_max[tk * G + h] = INT32_MAX;      // (any number of pages may write it)
+			}
 		}
 		sbase[i] = base;
 		sown[i] = own;
+		redo[a.ppages + i] = 0u;
+		if (RESIDENT) stage_v(np4 + i, base);
 	}
-	__syncthreads();
-	// step i into half i & 1 of the stage; pages that there are not are left out (their scores are masked, their
-	// probabilities zero)
-	auto base_of = [&](int i, int page) { return i < nps ? pbase[i * kPfxStepPages + page] : sbase[(i - nps) * kPfxStepPages + page]; };
-	auto load_k = [&](int i) {
-		int8_t* kd = stage + (size_t)(i & 1) * kPfxStep * L::kKStride;
-		for (int idx = t; idx < kPfxStep * (HD / 16); idx += kPfxThreads) {
-			const int row = idx / (HD / 16), piece = idx % (HD / 16);
-			const int64_t base = base_of(i, row / kPageTokens);
-			if (base >= 0) cp_async16(kd + (size_t)row * L::kKStride + piece * 16, kplane + base + (row % kPageTokens) * HD + piece * 16);
-		}
-		asm volatile("cp.async.commit_group;" ::: "memory");
-	};
-	auto load_v = [&](int i) {
-		int8_t* vd = stage + (size_t)(i & 1) * kPfxStep * HD;
-		for (int idx = t; idx < kPfxStepPages * HD; idx += kPfxThreads) {
-			const int pg = idx / HD, piece = idx % HD;
-			const int64_t base = base_of(i, pg);
-			if (base >= 0) cp_async16(vd + (size_t)pg * HD * kPageTokens + piece * 16, vplane + base + piece * 16);
-		}
-		asm volatile("cp.async.commit_group;" ::: "memory");
-	};
-	const bool early = RESIDENT || nps > 0;      // (an engine call's newest K rows come from the kernel in front)
-	if (early && steps > 0) load_k(0);
 	if (!RESIDENT) {
 		pdl_wait();
 		pdl_release();
+		stage_q(t, kPfxThreads);
+		for (int i = t; i < ns; i += kPfxThreads) stage_v(np4 + i, sbase[i]);      // (the thread's own entries)
+		if (t < nt) s_code[t] = __ldcg(&a.status[r0 + t]) != 0 ? 1 : kOk;
+		__syncthreads();
 	}
-	if (!early && steps > 0) load_k(0);
-	if (t < kPfxTokens) {
-		IExpFast f{1u, 30u, 1, 0, 0.9999995f};
-		if (t < nt) {
+	if (warp == W - 1) {      // (wanted by the softmax only)
+		IExpConsts k{1, 1, 0};      // (of a row that is left out)
+		if (s_code[lane] == kOk) {
 			if (RESIDENT) {
-				const int64_t* k = a.consts + ((int64_t)(r0 + t) * a.kv_heads + kvh) * 3;
-				if (s_code[t] == kOk) f = iexp_fast_prepare(SoftmaxConsts{{k[0], k[1], k[2]}, 0});
+				const int64_t* p = a.consts + ((int64_t)(r0 + lane) * a.kv_heads + kvh) * 3;
+				k = IExpConsts{p[0], p[1], p[2]};
 			} else {
-				s_code[t] = __ldcg(&a.status[r0 + t]) != 0 ? 1 : kOk;
-				if (s_code[t] == kOk) f = iexp_fast_prepare(a.smc[(size_t)(r0 + t) * a.kv_heads + kvh]);
+				k = a.smc[(size_t)(r0 + lane) * a.kv_heads + kvh].c;
 			}
-		} else {
-			s_code[t] = 1;
 		}
-		s_fx[t] = f;
+		s_fx[lane] = iexp_mul_prepare(k.q_ln2, k.q_b, k.q_c);
 	}
 	__syncthreads();
+	if (t == 0) ring_arrive(cta_addr(&s_bars[0]));      // (every staged page is announced)
 
-	const int rb = warp / CW, kq = warp % CW;
-	const int rho_a = rb * 16 + g, rho_b = rho_a + 8;
-	const int tok_a = rho_a * a.ginv >> 16, tok_b = rho_b * a.ginv >> 16;
-	const int head_a = rho_a - tok_a * G, head_b = rho_b - tok_b * G;
-	const bool in_a = tok_a < nt && s_code[tok_a] == kOk, in_b = tok_b < nt && s_code[tok_b] == kOk;
 	bool ok = true;
 
-	// ---- pass 1: scores and row maxima. acc[j]: MMA j = 2 * page + half; the K rows of a page are read in the order
-	// 0 1 4 5 8 9 12 13 | 2 3 6 7 10 11 14 15, which leaves a lane with four neighbouring positions
+	// ---- pass 1: scores and row maxima, a page per warp and turn, K straight into registers. The 16 positions of a page are
+	// spread over the columns of two MMAs so that a lane is left with positions 4 c .. 4 c + 3 of its rows.
 	{
-		uint32_t qa[KS][4];
-		const int8_t* qpa = a.q + (int64_t)(r0 + (in_a ? tok_a : 0)) * a.q_stride + (int64_t)(kvh * G + head_a) * HD;
-		const int8_t* qpb = a.q + (int64_t)(r0 + (in_b ? tok_b : 0)) * a.q_stride + (int64_t)(kvh * G + head_b) * HD;
+		uint32_t q[RB][2][HD / 16];
+		int tok[RB][2], head[RB][2], mx[RB][2];      // of rows 16 b + 8 e + g
 #pragma unroll
-		for (int ks = 0; ks < KS; ++ks) {
-			qa[ks][0] = in_a ? *(const uint32_t*)(qpa + 32 * ks + 4 * c) : 0u;
-			qa[ks][1] = in_b ? *(const uint32_t*)(qpb + 32 * ks + 4 * c) : 0u;
-			qa[ks][2] = in_a ? *(const uint32_t*)(qpa + 32 * ks + 16 + 4 * c) : 0u;
-			qa[ks][3] = in_b ? *(const uint32_t*)(qpb + 32 * ks + 16 + 4 * c) : 0u;
-		}
-		const int krow = 4 * ((lane & 7) >> 1) + (lane & 1);
-		int mx_a = INT32_MIN, mx_b = INT32_MIN;
-#pragma unroll 1
-		for (int i = 0; i < steps; ++i) {
-			if (i + 1 < steps) {
-				load_k(i + 1);
-				asm volatile("cp.async.wait_group 1;" ::: "memory");
-			} else {
-				asm volatile("cp.async.wait_group 0;" ::: "memory");
-			}
-			__syncthreads();
-			const uint32_t kd = cta_addr(stage + (size_t)((i & 1) * kPfxStep + kq * PW * kPageTokens) * L::kKStride);
-			int acc[2 * PW][4];
+		for (int b = 0; b < RB; ++b)
 #pragma unroll
-			for (int j = 0; j < 2 * PW; ++j)
+			for (int e = 0; e < 2; ++e) {
+				const int rho = 16 * b + 8 * e + g;
+				tok[b][e] = rho * a.ginv >> 16;
+				head[b][e] = rho - tok[b][e] * G;
+				mx[b][e] = INT32_MIN;
+				const int8_t* row = qs + rho * L::kQStride + c * (HD / 4);
+				if constexpr (HD == 32) {
+					*(uint2*)q[b][e] = *(const uint2*)row;
+				} else {
 #pragma unroll
-				for (int x = 0; x < 4; ++x) acc[j][x] = 0;
-			if constexpr (HD == 32) {
-#pragma unroll
-				for (int j = 0; j < 2 * PW; j += 2) {      // both halves of a page in one load
-					uint32_t b0, b1, b2, b3;
-					ldmatrix4(kd + (8 * j + krow + 2 * (lane >> 4)) * L::kKStride + ((lane >> 3) & 1) * 16, b0, b1, b2, b3);
-					mma_s8s8_full(acc[j], qa[0][0], qa[0][1], qa[0][2], qa[0][3], b0, b1);
-					mma_s8s8_full(acc[j + 1], qa[0][0], qa[0][1], qa[0][2], qa[0][3], b2, b3);
+					for (int w = 0; w < HD / 16; w += 4) *(uint4*)&q[b][e][w] = *(const uint4*)(row + 4 * w);
 				}
-			} else {
+			}
+		const int total = np + ns;
+		uint32_t kw[2][HD / 16];
+		if (warp >= np && warp < total) fetch_k(sbase[warp - np]);
+#pragma unroll 1
+		for (int i = warp; i < total; i += W) {
 #pragma unroll
-				for (int ks = 0; ks < KS; ks += 2) {
+			for (int w = 0; w < HD / 16; ++w) {
+				kw[0][w] = kn[0][w];
+				kw[1][w] = kn[1][w];
+			}
+			if (i + W < total) fetch_k(i + W < np ? pbase[i + W] : sbase[i + W - np]);
+			const int own = i < np ? 0 : sown[i - np];
+			const int end = i < np ? P - (rank + i * sub) * kPageTokens : own >> 8;      // positions of the page that count
 #pragma unroll
-					for (int j = 0; j < 2 * PW; ++j) {
-						uint32_t b0, b1, b2, b3;
-						ldmatrix4(kd + (16 * (j >> 1) + 2 * (j & 1) + krow) * L::kKStride + 32 * ks + (lane >> 3) * 16, b0, b1, b2, b3);
-						mma_s8s8_full(acc[j], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
-						mma_s8s8_full(acc[j], qa[ks + 1][0], qa[ks + 1][1], qa[ks + 1][2], qa[ks + 1][3], b2, b3);
+			for (int b = 0; b < RB; ++b) {
+				int acc[2][4];
+#pragma unroll
+				for (int h = 0; h < 2; ++h) {
+#pragma unroll
+					for (int x = 0; x < 4; ++x) acc[h][x] = 0;
+#pragma unroll
+					for (int j = 0; j < KS; ++j)
+						mma_s8s8_full(acc[h], q[b][0][2 * j], q[b][1][2 * j], q[b][0][2 * j + 1], q[b][1][2 * j + 1], kw[h][2 * j], kw[h][2 * j + 1]);
+				}
+#pragma unroll
+				for (int e = 0; e < 2; ++e) {
+					int4 v = make_int4(acc[0][2 * e], acc[0][2 * e + 1], acc[1][2 * e], acc[1][2 * e + 1]);
+					if (end < kPageTokens) {
+						v.x = 4 * c < end ? v.x : INT32_MIN;
+						v.y = 4 * c + 1 < end ? v.y : INT32_MIN;
+						v.z = 4 * c + 2 < end ? v.z : INT32_MIN;
+						v.w = 4 * c + 3 < end ? v.w : INT32_MIN;
+					}
+					const bool sees = i < np || tok[b][e] == (own & 255);
+					unsigned char* at = i < np ? sc + i * kPageScores + (16 * b + 8 * e + g) * 64 : csc + (i - np) * csc_page + head[b][e] * 64;
+					if (sees) {
+						*(int4*)(at + c * 16) = v;
+						mx[b][e] = max(mx[b][e], max(max(v.x, v.y), max(v.z, v.w)));
 					}
 				}
 			}
-			// row a, page p (positions 4 c ..): acc[2p][0], acc[2p][1], acc[2p + 1][0], acc[2p + 1][1]; row b: [2], [3]
+		}
 #pragma unroll
-			for (int p = 0; p < PW; ++p) {
-				int4 va = make_int4(acc[2 * p][0], acc[2 * p][1], acc[2 * p + 1][0], acc[2 * p + 1][1]);
-				int4 vb = make_int4(acc[2 * p][2], acc[2 * p][3], acc[2 * p + 1][2], acc[2 * p + 1][3]);
-				const int page = kq * PW + p;
-				bool see_a = true, see_b = true;
-				int end;      // positions of the page that count
-				if (i < nps) {
-					end = P - ((rank + i * sub) * kPfxStep + page * kPageTokens);
-				} else {
-					const int own = sown[(i - nps) * kPfxStepPages + page];
-					end = own >> 8;
-					see_a = tok_a == (own & 255);
-					see_b = tok_b == (own & 255);
-				}
-				if (end < kPageTokens) {
-					const int k0 = 4 * c;
-					va.x = k0 < end ? va.x : INT32_MIN; va.y = k0 + 1 < end ? va.y : INT32_MIN;
-					va.z = k0 + 2 < end ? va.z : INT32_MIN; va.w = k0 + 3 < end ? va.w : INT32_MIN;
-					vb.x = k0 < end ? vb.x : INT32_MIN; vb.y = k0 + 1 < end ? vb.y : INT32_MIN;
-					vb.z = k0 + 2 < end ? vb.z : INT32_MIN; vb.w = k0 + 3 < end ? vb.w : INT32_MIN;
-				}
-				if (see_a) mx_a = max(mx_a, max(max(va.x, va.y), max(va.z, va.w)));
-				if (see_b) mx_b = max(mx_b, max(max(vb.x, vb.y), max(vb.z, vb.w)));
-				if (i < nps) {
-					int4* at = sc + ((size_t)(i * kPfxStepPages + page) * 2) * kSlots + rb * 32 + lane;
-					at[0] = va;
-					at[kSlots] = vb;
-				} else {
-					int4* at = csc + (size_t)((i - nps) * kPfxStepPages + page) * G * 4 + c;
-					if (see_a) at[4 * head_a] = va;
-					if (see_b) at[4 * head_b] = vb;
-				}
+		for (int b = 0; b < RB; ++b)
+#pragma unroll
+			for (int e = 0; e < 2; ++e) {
+				int m = mx[b][e];
+				m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+				m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+				if (c == 0) atomicMax(&s_max[16 * b + 8 * e + g], m);
 			}
-			__syncthreads();      // the step may be overwritten
-		}
-		mx_a = max(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
-		mx_a = max(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
-		mx_b = max(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
-		mx_b = max(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
-		if (c == 0) {
-			atomicMax(&s_max[rho_a], mx_a);
-			atomicMax(&s_max[rho_b], mx_b);
-		}
 	}
-	// (the stage is free: V arrives during the softmax)
-	if (steps > 0) load_v(0);
-	if (steps > 1) load_v(1);
+	__syncthreads();
+	for (int i = t; i < ROWS * L::kSumStride; i += kPfxThreads) ctx[i] = 0;      // (the q rows are read)
+	// (V that is not staged: into L2 during the softmax)
+	const int pgroups = np4 >> 2, groups = pgroups + (ns4 >> 2);
+	constexpr int kLines = kPageTokens * HD / 128;
+	for (int i = t + 4 * a.vgroups * kLines; i < 4 * groups * kLines; i += kPfxThreads) {
+		const int at = i / kLines;
+		const int64_t base = at < np4 ? pbase[at] : sbase[at - np4];
+		if (base >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(vplane + base + i % kLines * 128));
+	}
 	__syncthreads();
 	if (sub > 1) {
-		if (t < sub * ROWS) exchange_send(&s_rxmax[rank * ROWS + t % ROWS], cta_addr(&s_bars[0]), (uint32_t)(t / ROWS), (uint32_t)s_max[t % ROWS]);
-		ok = exchange_wait(cta_addr(&s_bars[0]));
-		__syncthreads();
+		cluster_wait();      // (the peers run)
+		if (t < sub * ROWS) exchange_send(&s_rxmax[rank * ROWS + t % ROWS], cta_addr(&s_bars[1]), (uint32_t)(t / ROWS), (uint32_t)s_max[t % ROWS]);
+		ok = exchange_wait(cta_addr(&s_bars[1]));
+		__syncthreads();      // (all of them are sent)
 		if (t < ROWS) {
 			int m = INT32_MIN;
 			for (int i = 0; i < sub; ++i) m = max(m, s_rxmax[i * ROWS + t]);
@@ -407,219 +445,235 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 		}
 		__syncthreads();
 	}
+	if (RESIDENT) {
+		if (t < nt && s_code[t] == kOk && s_max[t * G] == INT32_MAX) s_code[t] = SSLM_B200_ROW_INDEX;
+		__syncthreads();
+		// (the tiles of the first kv head start first: what a later one may have to say about a wait comes after this)
+		if (kvh == 0 && rank == 0 && t < nt && a.status != nullptr) a.status[r0 + t] = s_code[t];
+	}
+
+	// The softmax passes deal out four positions of one row and page at a time. Of prefix pages a thread keeps to one row, two pages
+	// a turn; suffix pages have G rows each.
+	constexpr int kTurn = kPfxThreads / (ROWS * 4);      // pages side by side
+	const int my_row = (t >> 2) % ROWS, my_page = t / (ROWS * 4);
+	const int my_tok = min(my_row * a.ginv >> 16, kPfxTokens - 1);
+	const int ntask = ns * G * 4;
 
 	// ---- pass 2: exponentials and row totals; a score's place then holds the element's (shift, base)
-	const IExpFast fa = s_fx[in_a ? tok_a : 0], fb = s_fx[in_b ? tok_b : 0];
-	const int ntask = nsp * G * 4;      // four positions of one head and suffix page each
 	{
-		const uint32_t mx_a = (uint32_t)s_max[rho_a], mx_b = (uint32_t)s_max[rho_b];
-		unsigned long long sum[2] = {0ull, 0ull};
-		auto four = [](int4 v, uint32_t m, const IExpFast& f, bool whole, int4* parts) {
+		auto four = [](int4* at, uint32_t m, const IExpMul& f, bool whole) {
+			const int4 v = *at;
 			uint32_t p0, p1, p2, p3;
-			int64_t e0 = chunk_exp(m - (uint32_t)v.x, f, &p0), e1 = chunk_exp(m - (uint32_t)v.y, f, &p1);
-			int64_t e2 = chunk_exp(m - (uint32_t)v.z, f, &p2), e3 = chunk_exp(m - (uint32_t)v.w, f, &p3);
+			unsigned long long e0 = iexp_mul(m - (uint32_t)v.x, f, &p0), e1 = iexp_mul(m - (uint32_t)v.y, f, &p1);
+			unsigned long long e2 = iexp_mul(m - (uint32_t)v.z, f, &p2), e3 = iexp_mul(m - (uint32_t)v.w, f, &p3);
 			if (!whole) {      // masked positions count for nothing
 				if (v.x == INT32_MIN) { e0 = 0; p0 = kBaseOfZero; }
 				if (v.y == INT32_MIN) { e1 = 0; p1 = kBaseOfZero; }
 				if (v.z == INT32_MIN) { e2 = 0; p2 = kBaseOfZero; }
 				if (v.w == INT32_MIN) { e3 = 0; p3 = kBaseOfZero; }
 			}
-			*parts = make_int4((int)p0, (int)p1, (int)p2, (int)p3);
-			return (unsigned long long)(e0 + e1) + (unsigned long long)(e2 + e3);
+			*at = make_int4((int)p0, (int)p1, (int)p2, (int)p3);
+			return (e0 + e1) + (e2 + e3);
 		};
-#pragma unroll 1
-		for (int i = 0; i < nps; ++i) {
-			const bool whole = (rank + i * sub) * kPfxStep + kPfxStep <= P;
-#pragma unroll
-			for (int p = 0; p < PW; ++p) {
-				int4* at = sc + ((size_t)(i * kPfxStepPages + kq * PW + p) * 2) * kSlots + rb * 32 + lane;
-				sum[0] += four(at[0], mx_a, fa, whole, &at[0]);
-				sum[1] += four(at[kSlots], mx_b, fb, whole, &at[kSlots]);
-			}
-		}
-#pragma unroll
-		for (int h = 0; h < 2; ++h) {
-			sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-			sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-			if (c == 0 && nps > 0) atomicAdd(&s_sum[h ? rho_b : rho_a], sum[h]);
+		{
+			const IExpMul f = s_fx[my_tok];
+			const uint32_t m = (uint32_t)s_max[my_row];
+			unsigned long long sum = 0ull;
+			unsigned char* at = sc + my_row * 64 + c * 16;
+#pragma unroll 2
+			for (int page = my_page; page < np; page += kTurn)
+				sum += four((int4*)(at + page * kPageScores), m, f, (rank + page * sub + 1) * kPageTokens <= P);
+			sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+			sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+			if (c == 0 && sum != 0ull) atomicAdd(&s_sum[my_row], sum);
 		}
 #pragma unroll 1
 		for (int u0 = warp * 32; u0 < ntask; u0 += kPfxThreads) {
-			const int u = u0 + lane;
-			unsigned long long s = 0ull;
-			int rho = 0;
-			if (u < ntask) {
-				const int page = (u >> 2) * a.ginv >> 16, head = (u >> 2) - page * G, own = sown[page];
-				rho = (own & 255) * G + head;
-				s = four(csc[u], (uint32_t)s_max[rho], s_fx[own & 255], own >> 8 == kPageTokens, &csc[u]);
-			}
-			s += __shfl_xor_sync(0xffffffffu, s, 1);
-			s += __shfl_xor_sync(0xffffffffu, s, 2);
-			if (c == 0 && u < ntask) atomicAdd(&s_sum[rho], s);
+			const int u = (u0 + lane) >> 2, page = u * a.ginv >> 16, h = u - page * G;
+			const int own = page < ns ? sown[page] : 255;
+			unsigned long long sum = 0ull;
+			const int rho = (own & 255) * G + h;
+			if ((own & 255) < nt) sum = four((int4*)(csc + page * csc_page + h * 64 + c * 16), (uint32_t)s_max[rho], s_fx[own & 255], own >> 8 == kPageTokens);
+			sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+			sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+			if (c == 0 && sum != 0ull) atomicAdd(&s_sum[rho], sum);
 		}
 	}
 	__syncthreads();
 	if (sub > 1) {
-		if (t < sub * ROWS) exchange_send(&s_rxsum[rank * ROWS + t % ROWS], cta_addr(&s_bars[1]), (uint32_t)(t / ROWS), s_sum[t % ROWS]);
-		ok = exchange_wait(cta_addr(&s_bars[1])) && ok;
-		__syncthreads();
-		if (t < ROWS) {
-			unsigned long long s = 0ull;
-			for (int i = 0; i < sub; ++i) s += s_rxsum[i * ROWS + t];
-			s_sum[t] = s;
-		}
-		__syncthreads();
+		if (t < sub * ROWS) exchange_send(&s_rxsum[rank * ROWS + t % ROWS], cta_addr(&s_bars[2]), (uint32_t)(t / ROWS), s_sum[t % ROWS]);
+		ok = exchange_wait(cta_addr(&s_bars[2])) && ok;
+		__syncthreads();      // (all of them are sent)
 	}
+	if (t < ROWS) {
+		unsigned long long s = sub > 1 ? 0ull : s_sum[t];
+		if (sub > 1)
+			for (int i = 0; i < sub; ++i) s += s_rxsum[i * ROWS + t];
+		s_sum[t] = s;
+		const float pc = 32768.0f / (float)(s > 1ull ? s : 1ull);      // (chunk_prob)
+		const int tk = t * a.ginv >> 16;
+		const bool live = tk < nt && s_code[tk] == kOk;      // (the others' probabilities: far below 1, none of them in doubt)
+		s_prob[t] = live ? make_float4(pc, (float)s_fx[tk].qc, pc * 1.01f, 0.0f) : make_float4(8.6736174e-19f, 0.0f, -1.0f, 0.0f);
+	}
+	__syncthreads();
 
-	// ---- pass 3: probabilities, packed as the A fragments of P.V: of a prefix page (row a low, row b low, row a high, row b
-	// high plane), of a suffix page and head (low, high), four positions per word
+	// ---- pass 3: probabilities, two planes of bytes: of each page and row (low plane, 16 bytes) and (high plane, 16 bytes), in
+	// the place of the page's scores
 	{
-		auto four = [](int4 v, const ChunkProb& p, int64_t qc, unsigned long long tot, uint32_t* lo, uint32_t* hi) {
+		// true: the exact form is wanted for one of the row's sixteen positions (its four lanes are of one mind)
+		auto four = [&](int4 v, const ChunkProb& p, uint32_t* lo, uint32_t* hi) {
 			float near = 1.0f;
-			uint32_t p0 = chunk_prob_of((uint32_t)v.x, p, &near), p1 = chunk_prob_of((uint32_t)v.y, p, &near);
-			uint32_t p2 = chunk_prob_of((uint32_t)v.z, p, &near), p3 = chunk_prob_of((uint32_t)v.w, p, &near);
-			if (near < p.eps) {
-				const uint4 x = chunk_prob_exact((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w, qc, tot);
-				p0 = x.x; p1 = x.y; p2 = x.z; p3 = x.w;
-			}
+			const uint32_t p0 = chunk_prob_of((uint32_t)v.x, p, &near), p1 = chunk_prob_of((uint32_t)v.y, p, &near);
+			const uint32_t p2 = chunk_prob_of((uint32_t)v.z, p, &near), p3 = chunk_prob_of((uint32_t)v.w, p, &near);
 			*lo = pack_plane(p0, p1, p2, p3, 0);
 			*hi = pack_plane(p0, p1, p2, p3, 1);
+			return (__ballot_sync(0xffffffffu, near < p.eps) >> (lane & 28) & 15u) != 0u;      // (all lanes have read by now)
 		};
-		const unsigned long long tot_a = s_sum[rho_a], tot_b = s_sum[rho_b];
-		const ChunkProb pa = chunk_prob(tot_a, fa), pb = chunk_prob(tot_b, fb);
+		auto put = [&](unsigned char* at, uint32_t lo, uint32_t hi) {
+			*(uint32_t*)(at + c * 4) = lo;
+			*(uint32_t*)(at + 16 + c * 4) = hi;
+		};
+		auto constants = [&](int rho) {
+			const float4 x = s_prob[rho];
+			return ChunkProb{x.x, x.y, x.z};
+		};
+		{
+			const ChunkProb p = constants(my_row);
+			unsigned char* row = sc + my_row * 64;
 #pragma unroll 1
-		for (int i = 0; i < nps; ++i) {
-#pragma unroll
-			for (int p = 0; p < PW; ++p) {
-				int4* at = sc + ((size_t)(i * kPfxStepPages + kq * PW + p) * 2) * kSlots + rb * 32 + lane;
-				uint32_t lo_a, hi_a, lo_b, hi_b;
-				four(at[0], pa, fa.qc, tot_a, &lo_a, &hi_a);
-				four(at[kSlots], pb, fb.qc, tot_b, &lo_b, &hi_b);
-				at[0] = make_int4((int)lo_a, (int)lo_b, (int)hi_a, (int)hi_b);
+			for (int page = my_page; page < np; page += 2 * kTurn) {
+				const bool two = page + kTurn < np;      // (alike for the row's four lanes)
+				unsigned char *at = row + page * kPageScores, *next = two ? at + kTurn * kPageScores : at;
+				const int4 v0 = *(const int4*)(at + c * 16), v1 = *(const int4*)(next + c * 16);
+				uint32_t lo0, hi0, lo1, hi1;
+				const bool redo0 = four(v0, p, &lo0, &hi0), redo1 = four(v1, p, &lo1, &hi1);
+				if (!redo0) put(at, lo0, hi0);
+				else if (c == 0) atomicOr(&redo[page], 1u << my_row);
+				if (two && !redo1) put(next, lo1, hi1);
+				else if (two && c == 0) atomicOr(&redo[page + kTurn], 1u << my_row);
 			}
 		}
 #pragma unroll 1
-		for (int u = t; u < ntask; u += kPfxThreads) {
-			const int page = (u >> 2) * a.ginv >> 16, head = (u >> 2) - page * G, tk = sown[page] & 255;
-			const unsigned long long tot = s_sum[tk * G + head];
+		for (int u0 = warp * 32; u0 < ntask; u0 += kPfxThreads) {
+			const int u = (u0 + lane) >> 2, page = u * a.ginv >> 16, h = u - page * G;
+			const int tk = page < ns ? sown[page] & 255 : 255;
+			const bool there = tk < nt;
 			uint32_t lo, hi;
-			four(csc[u], chunk_prob(tot, s_fx[tk]), s_fx[tk].qc, tot, &lo, &hi);
-			csc[u] = make_int4((int)lo, (int)hi, 0, 0);
+			unsigned char* at = csc + page * csc_page + h * 64;
+			const bool again = four(there ? *(const int4*)(at + c * 16) : make_int4(0, 0, 0, 0), there ? constants(tk * G + h) : ChunkProb{8.6736174e-19f, 0.0f, -1.0f}, &lo, &hi);
+			if (there && !again) put(at, lo, hi);
+			else if (there && c == 0) atomicOr(&redo[a.ppages + page], 1u << h);
 		}
-	}
-
-	// ---- pass 4: P.V of this warp's rows and channels, over the pages of all warps
-	const bool owns = kq * NT * 8 < HD;
-	int accl[NT][4], acch[NT][4];
-#pragma unroll
-	for (int i = 0; i < NT; ++i)
-#pragma unroll
-		for (int x = 0; x < 4; ++x) accl[i][x] = acch[i][x] = 0;
+		// The exact form, apart from the loops above (a call in them costs a third of their time): one row and page at a time.
+		__syncthreads();
 #pragma unroll 1
-	for (int i = 0; i < steps; ++i) {
-		if (i + 1 < steps) asm volatile("cp.async.wait_group 1;" ::: "memory");
-		else asm volatile("cp.async.wait_group 0;" ::: "memory");
-		__syncthreads();      // V of the step (and, the first time, everybody's probabilities) are there
-		const uint32_t vd = cta_addr(stage + (size_t)(i & 1) * kPfxStep * HD);
-		if (owns) {
-#pragma unroll
-			for (int ks = 0; ks < kPfxStepPages / 2; ++ks) {      // two pages
-				int4 x0, x1;
-				if (i < nps) {
-					const int4* at = sc + ((size_t)(i * kPfxStepPages + 2 * ks) * 2) * kSlots + rb * 32 + lane;
-					x0 = at[0];
-					x1 = at[2 * kSlots];
-				} else {
-					const int page = (i - nps) * kPfxStepPages + 2 * ks;
-					auto fragment = [&](int pg) {
-						const int own = sown[pg] & 255;
-						int2 fa2 = make_int2(0, 0), fb2 = make_int2(0, 0);
-						if (tok_a == own) fa2 = *(const int2*)&csc[(size_t)(pg * G + head_a) * 4 + c];
-						if (tok_b == own) fb2 = *(const int2*)&csc[(size_t)(pg * G + head_b) * 4 + c];
-						return make_int4(fa2.x, fb2.x, fa2.y, fb2.y);
-					};
-					x0 = fragment(page);
-					x1 = fragment(page + 1);
+		for (int i = warp; i < np + ns; i += W) {
+			const bool shared = i < np;
+			uint32_t rows = shared ? redo[i] : redo[a.ppages + i - np];
+			while (rows != 0u) {
+				const int r = __ffs(rows) - 1, tk = shared ? r * a.ginv >> 16 : sown[i - np] & 255, rho = shared ? r : tk * G + r;
+				rows &= rows - 1u;
+				unsigned char* at = shared ? sc + i * kPageScores + r * 64 : csc + (i - np) * csc_page + r * 64;
+				uint4 x = make_uint4(0u, 0u, 0u, 0u);
+				if (lane < 4) {
+					const int4 v = *(const int4*)(at + c * 16);
+					x = chunk_prob_exact((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w, s_fx[tk].qc, s_sum[rho]);
 				}
-				if constexpr (NT == 1) {
-					const uint32_t at = vd + (uint32_t)((2 * ks + ((lane >> 3) & 1)) * HD + 8 * kq + (lane & 7)) * kPageTokens;
-					uint32_t b0, b1, b2, b3;      // (the upper half of the lanes repeats the lower half's rows)
-					ldmatrix4(at, b0, b1, b2, b3);
-					mma_u8s8_full(accl[0], x0.x, x0.y, x1.x, x1.y, b0, b1);
-					mma_u8s8_full(acch[0], x0.z, x0.w, x1.z, x1.w, b0, b1);
-				} else {
-#pragma unroll
-					for (int n = 0; n < NT; n += 2) {      // two 8-channel tiles, two pages each
-						const uint32_t at = vd + (uint32_t)((2 * ks + ((lane >> 3) & 1)) * HD + 8 * (kq * NT + n + (lane >> 4)) + (lane & 7)) * kPageTokens;
-						uint32_t b0, b1, b2, b3;
-						ldmatrix4(at, b0, b1, b2, b3);
-						mma_u8s8_full(accl[n], x0.x, x0.y, x1.x, x1.y, b0, b1);
-						mma_u8s8_full(acch[n], x0.z, x0.w, x1.z, x1.w, b0, b1);
-						mma_u8s8_full(accl[n + 1], x0.x, x0.y, x1.x, x1.y, b2, b3);
-						mma_u8s8_full(acch[n + 1], x0.z, x0.w, x1.z, x1.w, b2, b3);
-					}
-				}
+				__syncwarp();
+				if (lane < 4) put(at, pack_plane(x.x, x.y, x.z, x.w, 0), pack_plane(x.x, x.y, x.z, x.w, 1));
 			}
 		}
-		__syncthreads();      // the step may be overwritten
-		if (i + 2 < steps) load_v(i + 2);
 	}
+	__syncthreads();      // everybody's probabilities are there
+
+	// ---- pass 4: P.V. A warp has 16 channels of all rows and every KW-th group of four pages: the planes are read once per 16 channels
+	// (once per 8, a tile per warp, those reads were the bound; per 32 adding up the warps' shares costs more). Lane column c owns
+	// page 4 x + c of a group: its 16-byte row of the V page feeds two MMAs (positions 0..7 and 8..15), the row's planes
+	// the A side of both.
+	ok = ring_wait(cta_addr(&s_bars[0]), 0) && ok;
+	{
+		constexpr int CW = HD / 16, KW = W / CW;
+		const int ch0 = (warp % CW) * 16, part = warp / CW;
+		int acc[RB][2][2][4];      // [row block][8-channel tile][plane]
+#pragma unroll
+		for (int b = 0; b < RB; ++b)
+#pragma unroll
+			for (int n = 0; n < 2; ++n)
+#pragma unroll
+				for (int x = 0; x < 4; ++x) acc[b][n][0][x] = acc[b][n][1][x] = 0;
+		int4 vn[2];
+		auto fetch = [&](int x) {
+			if (x < a.vgroups) {
+#pragma unroll
+				for (int n = 0; n < 2; ++n) vn[n] = *(const int4*)(vst + (size_t)(4 * x + c) * L::kVPage + (ch0 + n * 8 + g) * kPageTokens);
+			} else {
+				const int64_t base = x < pgroups ? pbase[4 * x + c] : (x < groups ? sbase[4 * (x - pgroups) + c] : -1);
+#pragma unroll
+				for (int n = 0; n < 2; ++n) vn[n] = base >= 0 ? load16(vplane + base + (ch0 + n * 8 + g) * kPageTokens) : make_int4(0, 0, 0, 0);
+			}
+		};
+		if (part < groups) fetch(part);
+#pragma unroll 1
+		for (int x = part; x < groups; x += KW) {
+			const int4 v[2] = {vn[0], vn[1]};
+			if (x + KW < groups) fetch(x + KW);
+			const bool shared = x < pgroups;
+			const int page = shared ? 4 * x + c : 4 * (x - pgroups) + c;
+			const int own = shared ? 0 : sown[page] & 255;
+#pragma unroll
+			for (int b = 0; b < RB; ++b)
+#pragma unroll
+				for (int pl = 0; pl < 2; ++pl) {
+					int4 w[2];
+#pragma unroll
+					for (int e = 0; e < 2; ++e) {
+						const int rho = 16 * b + 8 * e + g, tk = rho * a.ginv >> 16;
+						const unsigned char* at = shared ? sc + page * kPageScores + rho * 64 : csc + page * csc_page + (rho - tk * G) * 64;
+						w[e] = (shared ? page < np : own == tk) ? *(const int4*)(at + 16 * pl) : make_int4(0, 0, 0, 0);
+					}
+#pragma unroll
+					for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w[0].x, w[1].x, w[0].y, w[1].y, v[n].x, v[n].y);
+#pragma unroll
+					for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w[0].z, w[1].z, w[0].w, w[1].w, v[n].z, v[n].w);
+				}
+		}
+		if (part < groups) {
+#pragma unroll
+			for (int b = 0; b < RB; ++b)
+#pragma unroll
+				for (int n = 0; n < 2; ++n)
+#pragma unroll
+					for (int x = 0; x < 4; ++x)
+						atomicAdd(&ctx[(16 * b + 8 * (x >> 1) + g) * L::kSumStride + ch0 + n * 8 + 2 * c + (x & 1)], acc[b][n][0][x] + 256 * acc[b][n][1][x]);
+		}
+	}
+	__syncthreads();
 
 	// ---- per-head context fold (forward_sites.cpp:1889-1896), store, row maximum for the funnel
-	if (sub == 1) {
-		uint32_t top_a = 0, top_b = 0;
-		if (owns) {
-#pragma unroll
-			for (int n = 0; n < NT; ++n) {
-				const int ch = 8 * (kq * NT + n) + 2 * c;
-				auto put = [&](int tok, int head, int v0, int v1, uint32_t& top) {
-					int2 o;
-					o.x = fold(v0, s_fold[3 * head], s_fold[3 * head + 1], s_fold[3 * head + 2]);
-					o.y = fold(v1, s_fold[3 * head], s_fold[3 * head + 1], s_fold[3 * head + 2]);
-					*(int2*)(a.out + (int64_t)(r0 + tok) * a.out_stride + (int64_t)(kvh * G + head) * HD + ch) = o;
-					top = max(top, max(abs_u32(o.x), abs_u32(o.y)));
-				};
-				if (in_a) put(tok_a, head_a, accl[n][0] + 256 * acch[n][0], accl[n][1] + 256 * acch[n][1], top_a);
-				if (in_b) put(tok_b, head_b, accl[n][2] + 256 * acch[n][2], accl[n][3] + 256 * acch[n][3], top_b);
-			}
-		}
+	auto store = [&](int rho, int ch, int32_t sum) {      // (a warp's elements lie in one row)
+		const int tk = rho * a.ginv >> 16, h = rho - tk * G;
+		const bool live = tk < nt && s_code[tk] == kOk;
+		const int32_t o = fold(sum, s_fold[3 * h], s_fold[3 * h + 1], s_fold[3 * h + 2]);
+		if (live) a.out[(int64_t)(r0 + tk) * a.out_stride + (int64_t)(kvh * G + h) * HD + ch] = o;
 		if (!RESIDENT) {
-			top_a = max(top_a, __shfl_xor_sync(0xffffffffu, top_a, 1));
-			top_a = max(top_a, __shfl_xor_sync(0xffffffffu, top_a, 2));
-			top_b = max(top_b, __shfl_xor_sync(0xffffffffu, top_b, 1));
-			top_b = max(top_b, __shfl_xor_sync(0xffffffffu, top_b, 2));
-			if (c == 0 && top_a) atomicMax(&a.rowmax[(size_t)(r0 + tok_a) * 4 + 3], (unsigned long long)top_a);
-			if (c == 0 && top_b) atomicMax(&a.rowmax[(size_t)(r0 + tok_b) * 4 + 3], (unsigned long long)top_b);
+			const uint32_t top = __reduce_max_sync(0xffffffffu, live ? abs_u32(o) : 0u);
+			if (lane == 0 && top) atomicMax(&a.rowmax[(size_t)(r0 + tk) * 4 + 3], (unsigned long long)top);
 		}
-		return;
-	}
-	// the shares go to the blocks that add them up; a peer's stage is free once the peer has got here
-	cluster_arrive();
-	cluster_wait();
-	constexpr int kRowBits = ROWS == 32 ? 5 : 4;
-	const int rows = ROWS >> a.shift, rshift = kRowBits - a.shift;
-	auto send = [&](int rho, int ch, int v0, int v1) {
-		exchange_send(&rx_ctx[(rank * rows + (rho & (rows - 1))) * HD + ch], cta_addr(&s_bars[2]), (uint32_t)(rho >> rshift), make_int2(v0, v1));
 	};
-	if (owns) {
-#pragma unroll
-		for (int n = 0; n < NT; ++n) {
-			const int ch = 8 * (kq * NT + n) + 2 * c;
-			send(rho_a, ch, accl[n][0] + 256 * acch[n][0], accl[n][1] + 256 * acch[n][1]);
-			send(rho_b, ch, accl[n][2] + 256 * acch[n][2], accl[n][3] + 256 * acch[n][3]);
+	if (sub == 1) {
+		for (int e = t; e < ROWS * HD; e += kPfxThreads) store(e / HD, e % HD, ctx[e / HD * L::kSumStride + e % HD]);
+	} else {      // the shares go to the blocks that add them up, ROWS / sub rows each
+		constexpr int kRowBits = ROWS == 32 ? 5 : 4;
+		const int rows = ROWS >> a.shift, rshift = kRowBits - a.shift;
+		for (int e = t; e < ROWS * HD / 2; e += kPfxThreads) {
+			const int rho = e / (HD / 2), ch = 2 * (e % (HD / 2));
+			exchange_send(&rx_ctx[(rank * rows + (rho & (rows - 1))) * HD + ch], cta_addr(&s_bars[3]), (uint32_t)(rho >> rshift), *(const int2*)&ctx[rho * L::kSumStride + ch]);
 		}
-	}
-	ok = exchange_wait(cta_addr(&s_bars[2])) && ok;
-	for (int e = t; e < rows * HD; e += kPfxThreads) {
-		const int rho = rank * rows + e / HD, ch = e % HD, tok = rho * a.ginv >> 16, head = rho - tok * G;      // (a warp's elements lie in one row)
-		int32_t sum = 0;
-		for (int i = 0; i < sub; ++i) sum += rx_ctx[i * rows * HD + e];
-		const int32_t o = fold(sum, s_fold[3 * head], s_fold[3 * head + 1], s_fold[3 * head + 2]);
-		const bool in = tok < nt && s_code[tok] == kOk;
-		if (in) a.out[(int64_t)(r0 + tok) * a.out_stride + (int64_t)(kvh * G + head) * HD + ch] = o;
-		if (!RESIDENT) {
-			const uint32_t top = __reduce_max_sync(0xffffffffu, in ? abs_u32(o) : 0u);
-			if (lane == 0 && top) atomicMax(&a.rowmax[(size_t)(r0 + tok) * 4 + 3], (unsigned long long)top);
+		ok = exchange_wait(cta_addr(&s_bars[3])) && ok;
+		for (int e = t; e < rows * HD; e += kPfxThreads) {
+			int32_t sum = 0;
+			for (int i = 0; i < sub; ++i) sum += rx_ctx[i * rows * HD + e];
+			store(rank * rows + e / HD, e % HD, sum);
 		}
 	}
 	if (__builtin_expect(!__all_sync(0xffffffffu, ok), 0)) {      // (the warp's lanes speak for the tile's rows)
@@ -628,7 +682,7 @@ __global__ void __launch_bounds__(kPfxThreads, 2) k_attention_prefix(const __gri
 			else atomicCAS(&a.status[r0 + lane], 0, pack_status(kInternalWaitTimeout, kSiteCtx, a.layer));
 		}
 		__syncwarp();
-		exchange_leave(cta_addr(&s_bars[0]), 3);
+		exchange_leave(cta_addr(&s_bars[0]), sub > 1 ? 4 : 1);
 	}
 }
 
@@ -672,15 +726,15 @@ namespace {
 
 struct PrefixPlan {
 	int rows;        // query rows per tile: 16 or 32
-	int tq, tiles, shift, psteps, spages;
+	int tq, tiles, shift, ppages, spages, vgroups;
 	size_t smem;
 };
-constexpr size_t kPfxSmemMax = 218 * 1024;      // (beside 9 KB of fixed arrays)
+constexpr size_t kPfxSmemMax = 216 * 1024;      // (beside 8 KB of fixed arrays)
 
-size_t prefix_smem(int hd, int rows, int psteps, int spages, int group) {
+size_t prefix_smem(int hd, int rows, int ppages, int spages, int group, bool cluster) {
 	auto of = [&](auto head) {
 		constexpr int HD = decltype(head)::value;
-		return rows == 32 ? PrefixSmem<HD, 32>::bytes(psteps, spages, group) : PrefixSmem<HD, 16>::bytes(psteps, spages, group);
+		return rows == 32 ? PrefixSmem<HD, 32>::bytes(ppages, spages, group, cluster) : PrefixSmem<HD, 16>::bytes(ppages, spages, group, cluster);
 	};
 	if (hd == 128) return of(std::integral_constant<int, 128>{});
 	return hd == 64 ? of(std::integral_constant<int, 64>{}) : of(std::integral_constant<int, 32>{});
@@ -694,11 +748,14 @@ bool prefix_shape(int hd, int rows, int group, int shift, int max_prefix, int ma
 	p->tq = rows / group;
 	p->shift = shift;
 	const int sub = 1 << shift;
-	p->psteps = ((max_prefix + kPfxStep - 1) / kPfxStep + sub - 1) / sub;
-	p->spages = (p->tq * ((max_suffix + kPageTokens - 1) / kPageTokens) + sub - 1) / sub;
-	p->spages = (p->spages + kPfxStepPages - 1) / kPfxStepPages * kPfxStepPages;
-	p->smem = prefix_smem(hd, rows, p->psteps, p->spages, group);
-	return p->smem <= kPfxSmemMax;
+	p->ppages = (((max_prefix + kPageTokens - 1) / kPageTokens + sub - 1) / sub + 3) & ~3;
+	p->spages = ((p->tq * ((max_suffix + kPageTokens - 1) / kPageTokens) + sub - 1) / sub + 3) & ~3;
+	p->smem = prefix_smem(hd, rows, p->ppages, p->spages, group, shift > 0);
+	if (p->smem > kPfxSmemMax) return false;
+	const size_t vgroup = 4 * ((size_t)kPageTokens * hd + 32);      // (kVPage)
+	p->vgroups = (int)std::min<size_t>((p->ppages + p->spages) / 4, (kPfxSmemMax - p->smem) / vgroup);
+	p->smem += p->vgroups * vgroup;
+	return true;
 }
 
 // How a call is cut. False when nothing fits (rows wider than 32,768 positions).
@@ -708,8 +765,7 @@ bool prefix_plan(int hd, int group, int kv_heads, int rows, int groups, int max_
 	for (int r : {32, 16}) {
 		PrefixPlan best{};
 		bool have = false;
-		const int top = r == 32 ? 3 : 4;
-		for (int shift = 0; shift <= top; ++shift) {
+		for (int shift = 0; shift <= 4; ++shift) {
 			PrefixPlan p;
 			if (!prefix_shape(hd, r, group, shift, max_prefix, max_suffix, &p)) continue;
 			p.tiles = prefix_tiles(rows, groups, p.tq);
@@ -720,7 +776,7 @@ bool prefix_plan(int hd, int group, int kv_heads, int rows, int groups, int max_
 				continue;
 			}
 			const int64_t blocks = (int64_t)p.tiles * kv_heads << shift;
-			if (have && (blocks > 2 * sms || p.psteps * kPfxStepPages + p.spages < kPfxStepPages)) break;
+			if (have && (blocks > 2 * sms || p.ppages + p.spages < 8)) break;
 			best = p;
 			have = true;
 		}
@@ -766,8 +822,9 @@ cudaError_t prefix_dispatch(PrefixArgs a, int hd, const PrefixPlan& p, cudaStrea
 	a.tq = p.tq;
 	a.ginv = (65536 + a.G - 1) / a.G;
 	a.shift = p.shift;
-	a.psteps = p.psteps;
+	a.ppages = p.ppages;
 	a.spages = p.spages;
+	a.vgroups = p.vgroups;
 	a.debug_withhold = p.shift > 0 ? exchange_debug_take(kExchangeAttnPrefix) : 0;
 	if (hd == 128) return p.rows == 32 ? prefix_launch<128, 32, RESIDENT>(a, p, st) : prefix_launch<128, 16, RESIDENT>(a, p, st);
 	if (hd == 64) return p.rows == 32 ? prefix_launch<64, 32, RESIDENT>(a, p, st) : prefix_launch<64, 16, RESIDENT>(a, p, st);
