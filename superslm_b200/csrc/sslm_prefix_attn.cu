@@ -32,7 +32,8 @@ constexpr int kPfxMaxWidth = 32768;      // positions a row sees at most: the lo
 constexpr int kPfxTokens = 32;           // rows a tile holds at most (32 query rows of groups of one)
 
 struct PrefixArgs {
-	int rows, groups, G, kv_heads, tq, ginv, shift;      // ginv = ceil(65536 / G); a tile is cut over 1 << shift blocks
+	int rows, groups, G, kv_heads, tq, ginv, sub;        // ginv = ceil(65536 / G); a tile is cut over `sub` blocks, one cluster
+	int per, pinv;                                       // rows of the tile that each of them adds up and stores, ceil(65536 / per)
 	int ppages, spages;                                  // prefix and suffix pages a block has room for (multiples of four)
 	int vgroups;                                         // groups of four pages whose V it has room for
 	int max_prefix, max_suffix;
@@ -63,10 +64,10 @@ constexpr int kPfxPad = 16;
 template <int HD, int ROWS>
 struct PrefixSmem {
 	static constexpr int kQStride = HD + 16, kSumStride = HD + 8;      // (padding against bank conflicts)
-	static constexpr size_t kShares = (size_t)ROWS * HD * 4;           // what the blocks of the cluster send of P.V
+	__host__ __device__ static constexpr size_t kShares(int sub) { return (size_t)sub * ((ROWS + sub - 1) / sub) * HD * 4; }      // what the blocks of the cluster send of P.V
 	static constexpr size_t kSums = (size_t)ROWS * kSumStride * 4;     // the warps' shares of it, and before that the tile's q rows
-	static constexpr size_t bytes(int ppages, int spages, int group, bool cluster) {
-		return (cluster ? kShares : 0) + kSums + (size_t)ppages * (ROWS * 64 + kPfxPad) + (size_t)spages * (group * 64 + kPfxPad) + (size_t)(ppages + spages) * 12 +
+	static constexpr size_t bytes(int ppages, int spages, int group, int sub) {
+		return (sub > 1 ? kShares(sub) : 0) + kSums + (size_t)ppages * (ROWS * 64 + kPfxPad) + (size_t)spages * (group * 64 + kPfxPad) + (size_t)(ppages + spages) * 12 +
 		       (size_t)spages * 4;
 	}
 	static constexpr size_t kVPage = (size_t)kPageTokens * HD + 32;    // a staged V page (padding as above)
@@ -113,7 +114,15 @@ __device__ __forceinline__ IExpMul iexp_mul_prepare(int64_t ln2, int64_t qb, int
 	f.ln2 = (uint32_t)ln2;
 	f.clip = 30u * f.ln2;
 	f.shift = 31u + (f.ln2 > 1u ? 32u - (uint32_t)__clz((int)(f.ln2 - 1u)) : 0u);
-	f.mul = (uint32_t)((1ull << f.shift) / f.ln2) + 1u;
+	// floor(2^shift / d) from a float quotient (off by 2^-22 of 2^32 at most) and two remainders
+	const float r = 1.0f / (float)f.ln2;
+	const unsigned long long n = 1ull << f.shift;
+	uint32_t m = (uint32_t)fminf(r * (float)n, 4294966784.0f);
+	m += (uint32_t)(int)floorf((float)(long long)(n - (unsigned long long)m * f.ln2) * r);
+	const long long rem = (long long)(n - (unsigned long long)m * f.ln2);
+	m += rem >= (long long)f.ln2 ? 1u : 0u;
+	m -= rem < 0 ? 1u : 0u;
+	f.mul = m + 1u;
 	f.qc = qc;
 	f.qb = (uint32_t)qb;
 	f.pad = 0;
@@ -142,10 +151,10 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	__shared__ int32_t s_max[ROWS], s_rxmax[kPfxThreads], s_len[kPfxTokens], s_code[kPfxTokens], s_cum[kPfxTokens + 1], s_fold[24], s_tile[4];
 
 	const int G = a.G, kvh = (int)blockIdx.z;
-	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
+	const int sub = a.sub, rank = (int)blockIdx.x;
 	const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
-	int32_t* rx_ctx = (int32_t*)smem;                                                       // [sub][ROWS / sub][HD], of a cluster
-	int32_t* ctx = (int32_t*)(smem + (sub > 1 ? L::kShares : 0));                           // [ROWS][kSumStride]
+	int32_t* rx_ctx = (int32_t*)smem;                                                       // [sub][per][HD], of a cluster
+	int32_t* ctx = (int32_t*)(smem + (sub > 1 ? L::kShares(sub) : 0));                           // [ROWS][kSumStride]
 	int8_t* qs = (int8_t*)ctx;                                                              // [ROWS][kQStride]
 	unsigned char* vst = (unsigned char*)ctx + L::kSums;                                    // [4 vgroups] staged V pages
 	unsigned char* sc = vst + (size_t)a.vgroups * 4 * L::kVPage;                            // [page][row][16] scores of prefix pages
@@ -163,7 +172,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 			auto more = [&](int i) { return held == i + 1 ? 4u : 0u; };
 			exchange_init(cta_addr(&s_bars[1]), (uint32_t)(sub * ROWS * 4) + more(0));
 			exchange_init(cta_addr(&s_bars[2]), (uint32_t)(sub * ROWS * 8) + more(1));
-			exchange_init(cta_addr(&s_bars[3]), (uint32_t)(ROWS * HD * 4) + more(2));
+			exchange_init(cta_addr(&s_bars[3]), (uint32_t)(sub * max(0, min(a.per, ROWS - rank * a.per)) * HD * 4) + more(2));
 		}
 		exchange_fence_init();
 	}
@@ -228,10 +237,17 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	int P = s_tile[3];
 	const int32_t* prefix_pages = RESIDENT ? a.prefix_pages + (int64_t)s_tile[2] * a.prefix_stride : a.desc[r0].pages;
 	auto stage_q = [&](int first, int step) {      // rows of tokens that there are not: zeros
-		for (int i = first; i < ROWS * (HD / 4); i += step) {
-			const int rho = i / (HD / 4), w = i % (HD / 4), tk = rho * a.ginv >> 16;
-			*(uint32_t*)(qs + rho * L::kQStride + 4 * w) =
-			    tk < nt ? *(const uint32_t*)(a.q + (int64_t)(r0 + tk) * a.q_stride + (int64_t)(kvh * G + rho - tk * G) * HD + 4 * w) : 0u;
+		constexpr int kWords = ROWS * (HD / 4), kTurns = (kWords + kPfxThreads - 33) / (kPfxThreads - 32);
+		uint32_t x[kTurns];
+#pragma unroll
+		for (int u = 0; u < kTurns; ++u) {      // (all of them on their way before the first is stored)
+			const int i = first + u * step, rho = i / (HD / 4), w = i % (HD / 4), tk = rho * a.ginv >> 16;
+			x[u] = i < kWords && tk < nt ? *(const uint32_t*)(a.q + (int64_t)(r0 + tk) * a.q_stride + (int64_t)(kvh * G + rho - tk * G) * HD + 4 * w) : 0u;
+		}
+#pragma unroll
+		for (int u = 0; u < kTurns; ++u) {
+			const int i = first + u * step;
+			if (i < kWords) *(uint32_t*)(qs + i / (HD / 4) * L::kQStride + 4 * (i % (HD / 4))) = x[u];
 		}
 	};
 	const bool bad_len = RESIDENT && (P < 0 || P > a.max_prefix);
@@ -240,7 +256,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	const int64_t page_bytes = kPageTokens * HD, plane = a.num_pages * page_bytes;
 	const int8_t* kplane = a.kv + (int64_t)(2 * kvh) * plane;
 	const int8_t* vplane = kplane + plane;
-	auto mine = [&](int n) { return n > rank ? (n - rank + sub - 1) >> a.shift : 0; };      // of n things dealt out: rank, rank + sub, ...
+	auto mine = [&](int n) { return n > rank ? (n - rank + sub - 1) / sub : 0; };      // of n things dealt out: rank, rank + sub, ...
 	auto known = [&](int id) { return !RESIDENT || (uint64_t)(int64_t)id < (uint64_t)a.num_pages; };
 	auto stage_v = [&](int at, int64_t base) {      // the page's V into place `at` (filled-up prefix pages first), while there is room
 		if (base < 0 || at >= 4 * a.vgroups) return;
@@ -253,16 +269,25 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	bool bad_page = false;
 	if (warp == 0) {
 		int code = lane < nt ? kOk : 1, len = 0;
-		if (lane < nt && RESIDENT) {
-			len = a.suffix_len[r0 + lane];
-			const int64_t* k = a.consts + (int64_t)(r0 + lane) * a.kv_heads * 3;
-			if (bad_len || len < 0 || len > a.max_suffix || P + len > kPfxMaxWidth) {
+		if (RESIDENT) {
+			if (lane < nt) len = a.suffix_len[r0 + lane];
+			if (lane < nt && (bad_len || len < 0 || len > a.max_suffix || P + len > kPfxMaxWidth)) {
 				code = SSLM_B200_ROW_LENGTH;
-			} else {
-				for (int h = 0; h < a.kv_heads; ++h)
-					if (!softmax_gate(k[3 * h], k[3 * h + 1], k[3 * h + 2], P + len)) code = SSLM_B200_ROW_CONSTANTS;
+				len = 0;
 			}
-			if (code != kOk) len = 0;
+			s_code[lane] = 0;
+			__syncwarp();
+			for (int x0 = 0; x0 < nt * a.kv_heads; x0 += 32) {      // a row's constants of every kv head: a lane each
+				const int x = x0 + lane, tk = min(x / a.kv_heads, nt - 1);
+				const int64_t* k = a.consts + (int64_t)r0 * a.kv_heads * 3 + 3 * min(x, nt * a.kv_heads - 1);
+				const int64_t ln2 = k[0], qb = k[1], qc = k[2];
+				if (!softmax_gate(ln2, qb, qc, P + __shfl_sync(0xffffffffu, len, tk))) s_code[tk] = SSLM_B200_ROW_CONSTANTS;
+			}
+			__syncwarp();
+			if (code == kOk && s_code[lane] != 0) {
+				code = SSLM_B200_ROW_CONSTANTS;
+				len = 0;
+			}
 		} else if (lane < nt) {
 			len = min(max(a.desc[r0 + lane].pos + 1 - P, 0), a.max_suffix);
 		}
@@ -277,7 +302,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		s_cum[lane + 1] = upto;
 		if (lane == 0) s_cum[0] = 0;
 	} else {      // (meanwhile the others: this block's prefix pages, and the tile's q rows)
-		for (int i = t - 32; i < np4; i += kPfxThreads - 32) {
+		for (int i = warp - 1 + lane * (W - 1); i < np4; i += kPfxThreads - 32) {      // (a few of the bulk copies per warp)
 			const int id = i < np ? prefix_pages[rank + i * sub] : 0;
 			bad_page = bad_page || !known(id);
 			pbase[i] = i < np && known(id) ? (int64_t)id * page_bytes : -1;
@@ -291,18 +316,22 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	if (__syncthreads_or((int)bad_page) && t < ROWS) s_max[t] = INT32_MAX;
 	// ---- K of this warp's first page is on its way while the suffix tables are made
 	const int krow = 4 * (g >> 1) + (g & 1);      // position of column g in the first MMA of a page, two more in the second
-	uint32_t kn[2][HD / 16];
+	uint32_t kn[2][2][HD / 16];      // [page on its way][MMA]
 #pragma unroll
-	for (int w = 0; w < HD / 16; ++w) kn[0][w] = kn[1][w] = 0u;
-	auto fetch_k = [&](int64_t base) {      // (no page: nothing, the words are not used)
+	for (int u = 0; u < 2; ++u)
+#pragma unroll
+		for (int w = 0; w < HD / 16; ++w) kn[u][0][w] = kn[u][1][w] = 0u;
+	auto fetch_k = [&](uint32_t (&k)[2][HD / 16], int64_t base) {      // (no page: nothing, the words are not used)
 		if (base >= 0) {
-			row_words<HD>(kplane + base + krow * HD, c, kn[0]);
-			row_words<HD>(kplane + base + (krow + 2) * HD, c, kn[1]);
+			row_words<HD>(kplane + base + krow * HD, c, k[0]);
+			row_words<HD>(kplane + base + (krow + 2) * HD, c, k[1]);
 		}
 	};
-	if (warp < np) fetch_k(pbase[warp]);      // (of an engine call too: the prefix has been in place since its first launch)
+#pragma unroll
+	for (int u = 0; u < 2; ++u)      // (of an engine call too: the prefix has been in place since its first launch)
+		if (warp + u * W < np) fetch_k(kn[u], pbase[warp + u * W]);
 	const int ns = min(mine(s_cum[kPfxTokens]), a.spages), ns4 = (ns + 3) & ~3;
-	for (int i = t; i < ns4; i += kPfxThreads) {
+	for (int i = warp + lane * W; i < ns4; i += kPfxThreads) {
 		int64_t base = -1;
 		int own = 255;
 		if (i < ns) {
@@ -328,7 +357,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		pdl_wait();
 		pdl_release();
 		stage_q(t, kPfxThreads);
-		for (int i = t; i < ns; i += kPfxThreads) stage_v(np4 + i, sbase[i]);      // (the thread's own entries)
+		for (int i = warp + lane * W; i < ns; i += kPfxThreads) stage_v(np4 + i, sbase[i]);      // (the thread's own entries)
 		if (t < nt) s_code[t] = __ldcg(&a.status[r0 + t]) != 0 ? 1 : kOk;
 		__syncthreads();
 	}
@@ -372,15 +401,19 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 			}
 		const int total = np + ns;
 		uint32_t kw[2][HD / 16];
-		if (warp >= np && warp < total) fetch_k(sbase[warp - np]);
+#pragma unroll
+		for (int u = 0; u < 2; ++u)
+			if (warp + u * W >= np && warp + u * W < total) fetch_k(kn[u], sbase[warp + u * W - np]);
 #pragma unroll 1
 		for (int i = warp; i < total; i += W) {
 #pragma unroll
 			for (int w = 0; w < HD / 16; ++w) {
-				kw[0][w] = kn[0][w];
-				kw[1][w] = kn[1][w];
+				kw[0][w] = kn[0][0][w];
+				kw[1][w] = kn[0][1][w];
+				kn[0][0][w] = kn[1][0][w];
+				kn[0][1][w] = kn[1][1][w];
 			}
-			if (i + W < total) fetch_k(i + W < np ? pbase[i + W] : sbase[i + W - np]);
+			if (i + 2 * W < total) fetch_k(kn[1], i + 2 * W < np ? pbase[i + 2 * W] : sbase[i + 2 * W - np]);
 			const int own = i < np ? 0 : sown[i - np];
 			const int end = i < np ? P - (rank + i * sub) * kPageTokens : own >> 8;      // positions of the page that count
 #pragma unroll
@@ -564,6 +597,10 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 			if (there && !again) put(at, lo, hi);
 			else if (there && c == 0) atomicOr(&redo[a.ppages + page], 1u << h);
 		}
+		for (int i = t; i < (np4 - np) * ROWS; i += kPfxThreads) {      // (pages that fill up the last group)
+			int4* at = (int4*)(sc + (np + i / ROWS) * kPageScores + i % ROWS * 64);
+			at[0] = at[1] = make_int4(0, 0, 0, 0);
+		}
 		// The exact form, apart from the loops above (a call in them costs a third of their time): one row and page at a time.
 		__syncthreads();
 #pragma unroll 1
@@ -602,40 +639,55 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 #pragma unroll
 				for (int x = 0; x < 4; ++x) acc[b][n][0][x] = acc[b][n][1][x] = 0;
 		int4 vn[2];
+		const unsigned char* vsm = vst + (size_t)c * L::kVPage + (ch0 + g) * kPageTokens;
 		auto fetch = [&](int x) {
 			if (x < a.vgroups) {
 #pragma unroll
-				for (int n = 0; n < 2; ++n) vn[n] = *(const int4*)(vst + (size_t)(4 * x + c) * L::kVPage + (ch0 + n * 8 + g) * kPageTokens);
+				for (int n = 0; n < 2; ++n) vn[n] = *(const int4*)(vsm + (size_t)x * 4 * L::kVPage + n * 8 * kPageTokens);
 			} else {
-				const int64_t base = x < pgroups ? pbase[4 * x + c] : (x < groups ? sbase[4 * (x - pgroups) + c] : -1);
+				const int64_t base = x < pgroups ? pbase[4 * x + c] : sbase[4 * (x - pgroups) + c];
 #pragma unroll
 				for (int n = 0; n < 2; ++n) vn[n] = base >= 0 ? load16(vplane + base + (ch0 + n * 8 + g) * kPageTokens) : make_int4(0, 0, 0, 0);
 			}
 		};
+		auto multiply = [&](int b, int pl, const int4& w0, const int4& w1, const int4 (&v)[2]) {
+#pragma unroll
+			for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w0.x, w1.x, w0.y, w1.y, v[n].x, v[n].y);
+#pragma unroll
+			for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w0.z, w1.z, w0.w, w1.w, v[n].z, v[n].w);
+		};
 		if (part < groups) fetch(part);
+		int x = part;
 #pragma unroll 1
-		for (int x = part; x < groups; x += KW) {
+		for (; x < pgroups; x += KW) {      // of the prefix
 			const int4 v[2] = {vn[0], vn[1]};
 			if (x + KW < groups) fetch(x + KW);
-			const bool shared = x < pgroups;
-			const int page = shared ? 4 * x + c : 4 * (x - pgroups) + c;
-			const int own = shared ? 0 : sown[page] & 255;
+			const unsigned char* at = sc + (4 * x + c) * kPageScores + g * 64;
 #pragma unroll
 			for (int b = 0; b < RB; ++b)
 #pragma unroll
-				for (int pl = 0; pl < 2; ++pl) {
-					int4 w[2];
+				for (int pl = 0; pl < 2; ++pl)
+					multiply(b, pl, *(const int4*)(at + 16 * b * 64 + 16 * pl), *(const int4*)(at + (16 * b + 8) * 64 + 16 * pl), v);
+		}
+#pragma unroll 1
+		for (; x < groups; x += KW) {      // of the suffixes: a page has planes of its owner's G rows, the others' are zero
+			const int4 v[2] = {vn[0], vn[1]};
+			if (x + KW < groups) fetch(x + KW);
+			const int page = 4 * (x - pgroups) + c, first = (sown[page] & 255) * G;
+			const unsigned char* at = csc + page * csc_page;
 #pragma unroll
-					for (int e = 0; e < 2; ++e) {
-						const int rho = 16 * b + 8 * e + g, tk = rho * a.ginv >> 16;
-						const unsigned char* at = shared ? sc + page * kPageScores + rho * 64 : csc + page * csc_page + (rho - tk * G) * 64;
-						w[e] = (shared ? page < np : own == tk) ? *(const int4*)(at + 16 * pl) : make_int4(0, 0, 0, 0);
-					}
+			for (int b = 0; b < RB; ++b) {
+				int4 w[2][2];      // [row][plane]
 #pragma unroll
-					for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w[0].x, w[1].x, w[0].y, w[1].y, v[n].x, v[n].y);
+				for (int e = 0; e < 2; ++e) {
+					const uint32_t h = (uint32_t)(16 * b + 8 * e + g - first);
+					const bool sees = h < (uint32_t)G;
 #pragma unroll
-					for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w[0].z, w[1].z, w[0].w, w[1].w, v[n].z, v[n].w);
+					for (int pl = 0; pl < 2; ++pl) w[e][pl] = sees ? *(const int4*)(at + h * 64 + 16 * pl) : make_int4(0, 0, 0, 0);
 				}
+				multiply(b, 0, w[0][0], w[1][0], v);
+				multiply(b, 1, w[0][1], w[1][1], v);
+			}
 		}
 		if (part < groups) {
 #pragma unroll
@@ -662,18 +714,17 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	};
 	if (sub == 1) {
 		for (int e = t; e < ROWS * HD; e += kPfxThreads) store(e / HD, e % HD, ctx[e / HD * L::kSumStride + e % HD]);
-	} else {      // the shares go to the blocks that add them up, ROWS / sub rows each
-		constexpr int kRowBits = ROWS == 32 ? 5 : 4;
-		const int rows = ROWS >> a.shift, rshift = kRowBits - a.shift;
+	} else {      // the shares go to the blocks that add them up, `per` rows each
 		for (int e = t; e < ROWS * HD / 2; e += kPfxThreads) {
-			const int rho = e / (HD / 2), ch = 2 * (e % (HD / 2));
-			exchange_send(&rx_ctx[(rank * rows + (rho & (rows - 1))) * HD + ch], cta_addr(&s_bars[3]), (uint32_t)(rho >> rshift), *(const int2*)&ctx[rho * L::kSumStride + ch]);
+			const int rho = e / (HD / 2), ch = 2 * (e % (HD / 2)), to = rho * a.pinv >> 16;
+			exchange_send(&rx_ctx[(rank * a.per + rho - to * a.per) * HD + ch], cta_addr(&s_bars[3]), (uint32_t)to, *(const int2*)&ctx[rho * L::kSumStride + ch]);
 		}
 		ok = exchange_wait(cta_addr(&s_bars[3])) && ok;
+		const int rows = min(a.per, ROWS - rank * a.per);
 		for (int e = t; e < rows * HD; e += kPfxThreads) {
 			int32_t sum = 0;
-			for (int i = 0; i < sub; ++i) sum += rx_ctx[i * rows * HD + e];
-			store(rank * rows + e / HD, e % HD, sum);
+			for (int i = 0; i < sub; ++i) sum += rx_ctx[i * a.per * HD + e];
+			store(rank * a.per + e / HD, e % HD, sum);
 		}
 	}
 	if (__builtin_expect(!__all_sync(0xffffffffu, ok), 0)) {      // (the warp's lanes speak for the tile's rows)
@@ -726,31 +777,31 @@ namespace {
 
 struct PrefixPlan {
 	int rows;        // query rows per tile: 16 or 32
-	int tq, tiles, shift, ppages, spages, vgroups;
+	int tq, tiles, sub, ppages, spages, vgroups;
 	size_t smem;
 };
-constexpr size_t kPfxSmemMax = 216 * 1024;      // (beside 8 KB of fixed arrays)
+constexpr size_t kPfxSmemMax = 216 * 1024;      // (beside 9 KB of fixed arrays)
+constexpr int kPfxMaxSub = 16;
 
-size_t prefix_smem(int hd, int rows, int ppages, int spages, int group, bool cluster) {
+size_t prefix_smem(int hd, int rows, int ppages, int spages, int group, int sub) {
 	auto of = [&](auto head) {
 		constexpr int HD = decltype(head)::value;
-		return rows == 32 ? PrefixSmem<HD, 32>::bytes(ppages, spages, group, cluster) : PrefixSmem<HD, 16>::bytes(ppages, spages, group, cluster);
+		return rows == 32 ? PrefixSmem<HD, 32>::bytes(ppages, spages, group, sub) : PrefixSmem<HD, 16>::bytes(ppages, spages, group, sub);
 	};
 	if (hd == 128) return of(std::integral_constant<int, 128>{});
 	return hd == 64 ? of(std::integral_constant<int, 64>{}) : of(std::integral_constant<int, 32>{});
 }
 
 // tiles of `tq` rows that `rows` rows in `groups` groups need at most
-int prefix_tiles(int rows, int groups, int tq) { return std::min<int64_t>(rows, ((int64_t)rows + (int64_t)groups * (tq - 1)) / tq); }
+int prefix_tiles(int rows, int groups, int tq) { return (int)std::min<int64_t>(rows, ((int64_t)rows + (int64_t)groups * (tq - 1)) / tq); }
 
-bool prefix_shape(int hd, int rows, int group, int shift, int max_prefix, int max_suffix, PrefixPlan* p) {
+bool prefix_shape(int hd, int rows, int group, int sub, int max_prefix, int max_suffix, PrefixPlan* p) {
 	p->rows = rows;
 	p->tq = rows / group;
-	p->shift = shift;
-	const int sub = 1 << shift;
+	p->sub = sub;
 	p->ppages = (((max_prefix + kPageTokens - 1) / kPageTokens + sub - 1) / sub + 3) & ~3;
 	p->spages = ((p->tq * ((max_suffix + kPageTokens - 1) / kPageTokens) + sub - 1) / sub + 3) & ~3;
-	p->smem = prefix_smem(hd, rows, p->ppages, p->spages, group, shift > 0);
+	p->smem = prefix_smem(hd, rows, p->ppages, p->spages, group, sub);
 	if (p->smem > kPfxSmemMax) return false;
 	const size_t vgroup = 4 * ((size_t)kPageTokens * hd + 32);      // (kVPage)
 	p->vgroups = (int)std::min<size_t>((p->ppages + p->spages) / 4, (kPfxSmemMax - p->smem) / vgroup);
@@ -758,74 +809,101 @@ bool prefix_shape(int hd, int rows, int group, int shift, int max_prefix, int ma
 	return true;
 }
 
-// How a call is cut. False when nothing fits (rows wider than 32,768 positions).
-bool prefix_plan(int hd, int group, int kv_heads, int rows, int groups, int max_prefix, int max_suffix, int forced, PrefixPlan* out) {
-	const int sms = sm_count();
-	bool found = false;
-	for (int r : {32, 16}) {
-		PrefixPlan best{};
-		bool have = false;
-		for (int shift = 0; shift <= 4; ++shift) {
-			PrefixPlan p;
-			if (!prefix_shape(hd, r, group, shift, max_prefix, max_suffix, &p)) continue;
-			p.tiles = prefix_tiles(rows, groups, p.tq);
-			if (forced > 0) {
-				best = p;
-				have = true;
-				if (1 << shift >= forced) break;
-				continue;
-			}
-			const int64_t blocks = (int64_t)p.tiles * kv_heads << shift;
-			if (have && (blocks > 2 * sms || p.ppages + p.spages < 8)) break;
-			best = p;
-			have = true;
-		}
-		if (!have) continue;
-		const int64_t blocks = (int64_t)best.tiles * kv_heads << best.shift;
-		if (!found || blocks > 0) *out = best;
-		found = true;
-		if (forced > 0 ? r == 32 : blocks >= sms / 2) break;
-	}
-	return found;
-}
-
 template <int HD, int ROWS, bool RESIDENT>
-cudaError_t prefix_launch(const PrefixArgs& a, const PrefixPlan& p, cudaStream_t st) {
-	static PerDeviceOnce once;
-	const auto kernel = k_attention_prefix<HD, ROWS, RESIDENT>;
-	cudaError_t e = once_per_device(once, [&] {
-		cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPfxSmemMax);
-		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-		return x;
-	});
-	if (e != cudaSuccess) return e;
+cudaLaunchConfig_t prefix_config(cudaLaunchAttribute (&attr)[2], int sub, int tiles, int kv_heads, size_t smem, cudaStream_t st) {
 	cudaLaunchConfig_t cfg = {};
-	cfg.gridDim = dim3(1u << p.shift, p.tiles, a.kv_heads);
+	cfg.gridDim = dim3(sub, tiles, kv_heads);
 	cfg.blockDim = dim3(kPfxThreads);
-	cfg.dynamicSmemBytes = p.smem;
+	cfg.dynamicSmemBytes = smem;
 	cfg.stream = st;
-	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
-	attr[0].val.clusterDim.x = 1u << p.shift;
+	attr[0].val.clusterDim.x = (unsigned)sub;
 	attr[0].val.clusterDim.y = 1;
 	attr[0].val.clusterDim.z = 1;
 	attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
 	attr[1].val.programmaticStreamSerializationAllowed = 1;
 	cfg.attrs = attr;
 	cfg.numAttrs = pdl_enabled() ? 2 : 1;
-	return cudaLaunchKernelEx(&cfg, kernel, a);
+	return cfg;
+}
+// Once per kernel and device: its attributes, and how many clusters of each size run at once. (Clusters lie inside a GPC, whose
+// multiprocessors a size may not divide: of 148, 140 are used by clusters of five or ten, 112 by eight, 96 by sixteen.)
+struct PrefixKernel {
+	PerDeviceOnce once;
+	int clusters[kMaxDevices][kPfxMaxSub + 1];
+};
+template <int HD, int ROWS, bool RESIDENT>
+cudaError_t prefix_setup(const int** clusters) {
+	static PrefixKernel k;
+	const auto kernel = k_attention_prefix<HD, ROWS, RESIDENT>;
+	const cudaError_t e = once_per_device(k.once, [&] {
+		cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPfxSmemMax);
+		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+		for (int sub = 1; sub <= kPfxMaxSub && x == cudaSuccess; ++sub) {
+			cudaLaunchAttribute attr[2];
+			const cudaLaunchConfig_t cfg = prefix_config<HD, ROWS, RESIDENT>(attr, sub, 1, 1, kPfxSmemMax, nullptr);
+			int n = 0;
+			if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {      // (a size the device does not have)
+				cudaGetLastError();
+				n = 0;
+			}
+			k.clusters[current_device_ordinal()][sub] = n;
+		}
+		return x;
+	});
+	*clusters = k.clusters[current_device_ordinal()];
+	return e;
+}
+template <bool RESIDENT>
+cudaError_t prefix_clusters(int hd, int rows, const int** clusters) {
+	if (hd == 128) return rows == 32 ? prefix_setup<128, 32, RESIDENT>(clusters) : prefix_setup<128, 16, RESIDENT>(clusters);
+	if (hd == 64) return rows == 32 ? prefix_setup<64, 32, RESIDENT>(clusters) : prefix_setup<64, 16, RESIDENT>(clusters);
+	return rows == 32 ? prefix_setup<32, 32, RESIDENT>(clusters) : prefix_setup<32, 16, RESIDENT>(clusters);
+}
+
+// How a call is cut: the tile height and the blocks per tile whose rounds of blocks end first.
+template <bool RESIDENT>
+cudaError_t prefix_plan(int hd, int group, int kv_heads, int rows, int groups, int max_prefix, int max_suffix, int forced, PrefixPlan* out) {
+	float least = 0.0f;
+	for (int r : {32, 16}) {
+		const int* clusters = nullptr;
+		const cudaError_t e = prefix_clusters<RESIDENT>(hd, r, &clusters);
+		if (e != cudaSuccess) return e;
+		for (int sub = 1; sub <= kPfxMaxSub; ++sub) {
+			PrefixPlan p;
+			if (clusters[sub] < 1 || !prefix_shape(hd, r, group, sub, max_prefix, max_suffix, &p)) continue;
+			p.tiles = prefix_tiles(rows, groups, p.tq);
+			const int rounds = (int)(((int64_t)p.tiles * kv_heads + clusters[sub] - 1) / clusters[sub]);
+			float cost = rounds * (8.0f + (r == 32 ? 0.28f : 0.17f) * p.ppages + 0.2f * p.spages);
+			if (forced > 0) cost = (float)(sub < forced ? 1000 + forced - sub : sub - forced);
+			if (least == 0.0f || cost + 1.0f < least) {
+				least = cost + 1.0f;
+				*out = p;
+			}
+		}
+	}
+	return least > 0.0f ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+
+template <int HD, int ROWS, bool RESIDENT>
+cudaError_t prefix_launch(const PrefixArgs& a, const PrefixPlan& p, cudaStream_t st) {
+	cudaLaunchAttribute attr[2];
+	const cudaLaunchConfig_t cfg = prefix_config<HD, ROWS, RESIDENT>(attr, p.sub, p.tiles, a.kv_heads, p.smem, st);
+	return cudaLaunchKernelEx(&cfg, k_attention_prefix<HD, ROWS, RESIDENT>, a);
 }
 
 template <bool RESIDENT>
 cudaError_t prefix_dispatch(PrefixArgs a, int hd, const PrefixPlan& p, cudaStream_t st) {
 	a.tq = p.tq;
 	a.ginv = (65536 + a.G - 1) / a.G;
-	a.shift = p.shift;
+	a.sub = p.sub;
+	a.per = (p.rows + p.sub - 1) / p.sub;
+	a.pinv = (65536 + a.per - 1) / a.per;
 	a.ppages = p.ppages;
 	a.spages = p.spages;
 	a.vgroups = p.vgroups;
-	a.debug_withhold = p.shift > 0 ? exchange_debug_take(kExchangeAttnPrefix) : 0;
+	a.debug_withhold = p.sub > 1 ? exchange_debug_take(kExchangeAttnPrefix) : 0;
 	if (hd == 128) return p.rows == 32 ? prefix_launch<128, 32, RESIDENT>(a, p, st) : prefix_launch<128, 16, RESIDENT>(a, p, st);
 	if (hd == 64) return p.rows == 32 ? prefix_launch<64, 32, RESIDENT>(a, p, st) : prefix_launch<64, 16, RESIDENT>(a, p, st);
 	return p.rows == 32 ? prefix_launch<32, 32, RESIDENT>(a, p, st) : prefix_launch<32, 16, RESIDENT>(a, p, st);
@@ -859,7 +937,10 @@ extern "C" sslm_status sslm_b200_attention_prefix_resident(const sslm_b200_prefi
 		return SSLM_MISALIGNED_BUFFER;
 	const int G = c.heads / c.kv_heads;
 	PrefixPlan p;
-	if (!prefix_plan(c.head_dim, G, c.kv_heads, c.rows, c.groups, c.max_prefix, c.max_suffix, attn_forced_splits(), &p)) return SSLM_INVALID_ARGUMENT;
+	if (prefix_plan<true>(c.head_dim, G, c.kv_heads, c.rows, c.groups, c.max_prefix, c.max_suffix, attn_forced_splits(), &p) != cudaSuccess) {
+		cudaGetLastError();
+		return SSLM_ALLOCATION_FAILED;
+	}
 	PrefixArgs a{};
 	a.rows = c.rows; a.groups = c.groups; a.G = G; a.kv_heads = c.kv_heads;
 	a.max_prefix = c.max_prefix; a.max_suffix = c.max_suffix;
