@@ -9,11 +9,13 @@
 //   x = clamp(x, -(2^31 - 1), 2^31 - 1), or INT32_MIN where v is not allowed
 // and the row's token is the lowest index of the largest x, -2 where nothing is allowed.
 //
-// One pass over the logits. A row is cut over the blocks of a cluster; a block first builds, for its slice of
-// the vocabulary, two bitmaps in shared memory -- which tokens are allowed, which ones the history or the biases
-// name -- and 16-bit counts beside them, then streams its logits. Four neighbouring tokens that nothing names,
-// nearly all of them, cost a load, two bitmap words and a maximum. Bound by the logits' bytes where rows are many, by
-// the chain (lists, bitmaps, one trip to memory, one exchange) where they are few.
+// One pass over the logits. A row is cut over the blocks of a cluster; a block first marks, for its slice of the
+// vocabulary, which tokens the history or the biases name, with counts beside them, and which ones are allowed. The
+// named tokens are few and dear (a division, a table): they are listed and dealt out one by one. All others are
+// streamed past, four at a time, and cost a load, a nibble of one bitmap and a maximum; where it lies is looked up
+// once, at the end. (With the named ones worked on in the stream nearly every other warp stopped for one: 256 rows
+// of 151,936 with histories of 1,024 took 104 us.) Bound by the logits' bytes where rows are many, by the chain
+// (lists, marks, one trip to memory, one exchange) where they are few.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -33,6 +35,7 @@ struct PickArgs {
 	int rows, vocab, shift, slice;      // a row is cut over 1 << shift blocks of `slice` tokens (a multiple of 32)
 	int pass;                           // tokens per pass over a slice (a multiple of 32)
 	int hash;                           // places of the bias table, a power of two, or 0
+	int list;                           // room for named tokens of a pass: all of it, or all that the lists can name
 	// a caller's tensors
 	const int32_t* logits;
 	int64_t logits_stride;
@@ -56,8 +59,8 @@ struct PickArgs {
 };
 
 struct PickSmem {
-	// counts u16 [pass + 8], allowed bits [pass / 32 + 2], named bits [pass / 32 + 2], bias keys [hash], bias sums [hash]
-	static size_t bytes(int pass, int hash) { return (size_t)hash * 12 + (size_t)(pass + 8) * 2 + (size_t)(pass / 32 + 2) * 8; }
+	// bias sums [hash], bias keys [hash], counts u16 [pass + 8], allowed and named bits [pass / 32 + 2], list of named tokens u16 [list]
+	static size_t bytes(int pass, int hash, int list) { return (size_t)hash * 12 + (size_t)(pass + 8) * 2 + (size_t)(pass / 32 + 2) * 8 + (size_t)list * 2; }
 };
 
 __device__ __forceinline__ unsigned long long pick_key(int32_t x, int v) {
@@ -65,9 +68,10 @@ __device__ __forceinline__ unsigned long long pick_key(int32_t x, int v) {
 }
 
 template <bool RESIDENT>
-__global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ PickArgs a) {
+__global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant__ PickArgs a) {
 	extern __shared__ __align__(16) unsigned char smem[];
 	__shared__ __align__(8) unsigned long long s_bar, s_rx[16], s_warp[kPickThreads / 32];
+	__shared__ int s_listed;
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
 	const int64_t r = blockIdx.y;
@@ -76,14 +80,15 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ P
 	uint32_t* counts = (uint32_t*)(bkey + a.hash);                          // u16 pairs
 	uint32_t* allow = counts + (a.pass + 8) / 2;                            // bit i: token v0 + i
 	uint32_t* named = allow + a.pass / 32 + 2;
+	uint16_t* list = (uint16_t*)(named + a.pass / 32 + 2);
 	if (sub > 1) {
 		if (t == 0 && rank == 0) {
 			const int held = blockIdx.x == 0 && blockIdx.y == 0 ? a.debug_withhold : 0;
 			exchange_init(cta_addr(&s_bar), (uint32_t)(sub * 8) + (held == 1 ? 4u : 0u));
 			exchange_fence_init();
 		}
-		cluster_arrive();
-		cluster_wait();
+		__syncwarp();
+		cluster_arrive();      // (waited for ahead of the word that is sent)
 	}
 	pdl_wait();
 	pdl_release();
@@ -129,18 +134,31 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ P
 		if (w.logits == nullptr) code = 1;      // (a row without controls)
 		else if (w.extra >= 0 && rank == 0 && t == 0) const_cast<int32_t*>(w.history)[w.n_history] = w.extra;      // (its blocks count it from the descriptor)
 	}
-	if (code != 0) return;      // (all blocks of the cluster alike)
+	if (code != 0) {      // (all blocks of the cluster alike)
+		if (sub > 1) cluster_wait();
+		return;
+	}
 
+	auto place = [&](int v) { return ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1); };
 	const bool listed = w.n_history > 0 || w.extra >= 0 || w.n_bias > 0;
-	int32_t top = INT32_MIN;
-	int top_at = 0;
+	unsigned long long key = 0ull;      // of the named tokens and the ends
+	const double inv_theta = 1.0 / (double)w.theta;
 	const int s0 = min(V, rank * a.slice), s1 = min(V, s0 + a.slice);
 	// four neighbouring tokens of the row lie in one aligned 16-byte word; mis: tokens by which the row's first is off
 	const int mis = (int)(((uintptr_t)w.logits >> 2) & 3);
 	const int mis_out = (int)(((uintptr_t)out >> 2) & 3);
+	constexpr int U = 5, kStride = 4 * kPickThreads;
 	for (int v0 = s0; v0 < s1; v0 += a.pass) {
 		const int v1 = min(s1, v0 + a.pass), n = v1 - v0, words = (n + 31) / 32;
-		// ---- bitmaps and counts of tokens v0 .. v1
+		// whole aligned words of four tokens, `first` to `last`; the ends of the pass one by one
+		const int first = min(v1, v0 + ((4 - ((v0 + mis) & 3)) & 3)), last = first + ((v1 - first) & ~3);
+		const int32_t* mine = w.logits + first + 4 * t;
+		const int turns = first + 4 * t < last ? (last - first - 4 * t + kStride - 1) / kStride : 0;      // this thread's words
+		int4 x[U];      // (on their way while the marks are made)
+#pragma unroll
+		for (int u = 0; u < U; ++u)
+			if (u < turns) x[u] = __ldcs((const int4*)(mine + u * kStride));
+		// ---- marks and counts of tokens v0 .. v1
 		for (int i = t; i < words + 2; i += kPickThreads) {
 			uint32_t bits = 0;
 			const int left = n - i * 32;
@@ -148,9 +166,10 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ P
 				bits = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
 				if (w.mask != nullptr) {      // (v0 is a multiple of 32; a page has ceil(V / 8) bytes and any address)
 					const uint8_t* m = w.mask + (v0 >> 3) + 4 * i;
-					const int nbytes = min(4, (left + 7) >> 3);
 					uint32_t page = 0;
-					for (int j = 0; j < nbytes; ++j) page |= (uint32_t)m[j] << (8 * j);
+					if (left >= 32 && ((uintptr_t)m & 3) == 0) page = *(const uint32_t*)m;
+					else
+						for (int j = 0; j < min(4, (left + 7) >> 3); ++j) page |= (uint32_t)m[j] << (8 * j);
 					bits &= page;
 				}
 			}
@@ -158,123 +177,161 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ P
 			named[i] = 0u;
 		}
 		if (listed) {
-			for (int i = t; i < (n + 8) / 2; i += kPickThreads) counts[i] = 0u;
+			for (int i = t; i < (n + 8) / 8; i += kPickThreads) ((int4*)counts)[i] = make_int4(0, 0, 0, 0);
 			for (int i = t; i < a.hash; i += kPickThreads) {
 				bkey[i] = -1;
 				bsum[i] = 0ull;
 			}
-		}
-		__syncthreads();
-		if (listed) {
+			if (t == 0) s_listed = 0;
+			__syncthreads();
+			auto name = [&](uint32_t i) {      // the first to name a token enters it into the list
+				if ((atomicOr(&named[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u) == 0u) list[atomicAdd(&s_listed, 1)] = (uint16_t)i;
+			};
 			auto seen = [&](int v) {
 				const uint32_t i = (uint32_t)(v - v0);
 				if (i >= (uint32_t)n) return;
 				atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
-				atomicOr(&named[i >> 5], 1u << (i & 31));
+				name(i);
 			};
-			for (int i = t; i < w.n_history; i += kPickThreads) seen(w.history[i]);
+			{      // (ids of any alignment: single ones up to the first 16-byte word, then words)
+				const int head = min(w.n_history, (int)((4 - (((uintptr_t)w.history >> 2) & 3)) & 3)), whole = (w.n_history - head) >> 2;
+				if (t < head) seen(w.history[t]);
+				const int4* ids = (const int4*)(w.history + head);
+#pragma unroll 2
+				for (int i = t; i < whole; i += kPickThreads) {
+					const int4 id = ids[i];
+					seen(id.x);
+					seen(id.y);
+					seen(id.z);
+					seen(id.w);
+				}
+				const int tail = head + 4 * whole + t;
+				if (tail < w.n_history) seen(w.history[tail]);
+			}
 			if (t == 0 && w.extra >= 0) seen(w.extra);
 			for (int i = t; i < w.n_bias; i += kPickThreads) {
 				const int v = bt[i];
 				const uint32_t at = (uint32_t)(v - v0);
 				if (at >= (uint32_t)n) continue;
-				uint32_t h = ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1);
+				uint32_t h = place(v);
 				for (;;) {      // (at least half of the places stay free)
 					const int was = atomicCAS(&bkey[h], -1, v);
 					if (was == -1 || was == v) break;
 					h = (h + 1) & (uint32_t)(a.hash - 1);
 				}
 				atomicAdd(&bsum[h], (unsigned long long)(long long)bv[i]);
-				atomicOr(&named[at >> 5], 1u << (at & 31));
+				name(at);
 			}
 			__syncthreads();
+			// ---- the named tokens
+#pragma unroll 2
+			for (int k = t; k < s_listed; k += kPickThreads) {
+				const int i = list[k], v = v0 + i;
+				int32_t y = w.logits[v];
+				if (y != INT32_MIN) {
+					long long z = y;
+					const uint32_t cnt = counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
+					if (cnt != 0u) {
+						if (z > 0) {      // floor(2^15 z / theta): a quotient in doubles, off by one at most, settled by its remainder
+							const long long num = z << 15;
+							long long q = (long long)((double)num * inv_theta);
+							const long long rem = num - q * (long long)w.theta;
+							z = q + (rem >= (long long)w.theta ? 1 : 0) - (rem < 0 ? 1 : 0);
+						} else {
+							z = -((-z * (long long)w.theta) >> 15);
+						}
+						z -= (long long)w.presence + (long long)w.frequency * (long long)cnt;
+					}
+					if (w.n_bias > 0) {
+						uint32_t h = place(v);
+						while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
+						if (bkey[h] == v) z += (long long)bsum[h];
+					}
+					y = (int32_t)max(-2147483647ll, min(2147483647ll, z));
+				}
+				if ((allow[i >> 5] >> (i & 31) & 1u) == 0u) y = INT32_MIN;
+				key = max(key, pick_key(y, v));
+				if (out != nullptr) out[v] = y;
+			}
+		} else {
+			__syncthreads();
 		}
-		// ---- the logits
-		auto changed = [&](int32_t x32, int v) {      // a token that a list names
+		// ---- all others
+		auto one = [&](int v) {
 			const int i = v - v0;
-			long long x = x32;
-			const uint32_t cnt = counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
-			if (cnt != 0u) {
-				x = x > 0 ? (x << 15) / w.theta : -((-x * (long long)w.theta) >> 15);
-				x -= (long long)w.presence + (long long)w.frequency * (long long)cnt;
-			}
-			if (w.n_bias > 0) {
-				uint32_t h = ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1);
-				while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
-				if (bkey[h] == v) x += (long long)bsum[h];
-			}
-			return (int32_t)max(-2147483647ll, min(2147483647ll, x));
+			if ((named[i >> 5] >> (i & 31) & 1u) != 0u) return;
+			const int32_t y = (allow[i >> 5] >> (i & 31) & 1u) != 0u ? w.logits[v] : INT32_MIN;
+			key = max(key, pick_key(y, v));
+			if (out != nullptr) out[v] = y;
 		};
-		auto take = [&](int32_t x, int v) {
-			if (x > top) {
-				top = x;
-				top_at = v;
+		if (t < first - v0) one(v0 + t);
+		if (t < v1 - last) one(last + t);
+		// the words of a thread lie a multiple of 32 tokens apart: their bits at one place of their bitmap words
+		const int bit = (first - v0 + 4 * t) & 31, word = (first - v0 + 4 * t) >> 5;
+		const bool straddles = bit > 28;
+		auto nibble = [&](const uint32_t* map, int k) {
+			const uint32_t* p = map + word + k * (kStride / 32);
+			return __funnelshift_r(p[0], straddles ? p[1] : 0u, bit) & 15u;
+		};
+		auto words_of = [&](int4 q, uint32_t use, int32_t (&y)[4]) {
+			y[0] = q.x; y[1] = q.y; y[2] = q.z; y[3] = q.w;
+			if (use != 15u) {
+#pragma unroll
+				for (int j = 0; j < 4; ++j) y[j] = (use >> j & 1u) != 0u ? y[j] : INT32_MIN;
 			}
 		};
-		auto one = [&](int32_t x, int v) {
-			const int i = v - v0;
-			if (x != INT32_MIN && (named[i >> 5] >> (i & 31) & 1u) != 0u) x = changed(x, v);
-			if ((allow[i >> 5] >> (i & 31) & 1u) == 0u) x = INT32_MIN;
-			take(x, v);
-			if (out != nullptr) out[v] = x;
-		};
-		// whole aligned words of the pass, and its ends one by one
-		const int first = v0 + ((4 - ((v0 + mis) & 3)) & 3), last = first + (v1 > first ? (v1 - first) & ~3 : 0);
-		if (t < min(first, v1) - v0) one(w.logits[v0 + t], v0 + t);
-		constexpr int U = 4;
-		for (int b = first + 4 * t; b < last; b += 4 * U * kPickThreads) {
-			int4 x[U];
+		int32_t top = INT32_MIN;
+		int top_at = 0;      // the word that has it first
+		for (int k0 = 0; k0 < turns; k0 += U) {
 #pragma unroll
 			for (int u = 0; u < U; ++u) {
-				const int v = b + 4 * u * kPickThreads;
-				if (v < last) x[u] = __ldcs((const int4*)(w.logits + v));
-			}
-#pragma unroll
-			for (int u = 0; u < U; ++u) {
-				const int v = b + 4 * u * kPickThreads, i = v - v0;
-				if (v >= last) break;
-				const uint32_t al = __funnelshift_r(allow[i >> 5], allow[(i >> 5) + 1], i & 31) & 15u;
-				const uint32_t nm = __funnelshift_r(named[i >> 5], named[(i >> 5) + 1], i & 31) & 15u;
-				int32_t y[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-				if (nm != 0u) {
-#pragma unroll
-					for (int j = 0; j < 4; ++j)
-						if ((nm >> j & 1u) != 0u && y[j] != INT32_MIN) y[j] = changed(y[j], v + j);
-				}
-				if (al != 15u) {
-#pragma unroll
-					for (int j = 0; j < 4; ++j) y[j] = (al >> j & 1u) != 0u ? y[j] : INT32_MIN;
-				}
-				if (max(max(y[0], y[1]), max(y[2], y[3])) > top) {
-#pragma unroll
-					for (int j = 0; j < 4; ++j) take(y[j], v + j);
+				const int k = k0 + u;
+				if (k >= turns) break;
+				const int4 q = x[u];
+				if (k + U < turns) x[u] = __ldcs((const int4*)(mine + (k + U) * kStride));
+				const uint32_t nm = listed ? nibble(named, k) : 0u;
+				int32_t y[4];
+				words_of(q, nibble(allow, k) & ~nm, y);
+				const int32_t m = max(max(y[0], y[1]), max(y[2], y[3]));
+				if (m > top) {
+					top = m;
+					top_at = k;
 				}
 				if (out != nullptr) {
-					if (mis_out == mis) {
-						__stcs((int4*)(out + v), make_int4(y[0], y[1], y[2], y[3]));
+					int32_t* to = out + first + 4 * t + k * kStride;
+					if (mis_out == mis && nm == 0u) {
+						__stcs((int4*)to, make_int4(y[0], y[1], y[2], y[3]));
 					} else {
 #pragma unroll
-						for (int j = 0; j < 4; ++j) out[v + j] = y[j];
+						for (int j = 0; j < 4; ++j)
+							if ((nm >> j & 1u) == 0u) to[j] = y[j];
 					}
 				}
 			}
 		}
-		const int tail = max(first, last);
-		if (tail < v1 && t < v1 - tail) one(w.logits[tail + t], tail + t);
+		if (top != INT32_MIN) {      // (in place, the word reads as it was but for what the bitmaps leave out)
+			int32_t y[4];
+			words_of(*(const int4*)(mine + top_at * kStride), nibble(allow, top_at) & ~(listed ? nibble(named, top_at) : 0u), y);
+			const int j = y[0] == top ? 0 : (y[1] == top ? 1 : (y[2] == top ? 2 : 3));
+			key = max(key, pick_key(top, first + 4 * t + top_at * kStride + j));
+		}
 		__syncthreads();      // the tables may be overwritten
 	}
 	// ---- the row's largest key: larger values first, then lower indices
-	unsigned long long key = pick_key(top, top_at);
 #pragma unroll
 	for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
 	if (lane == 0) s_warp[warp] = key;
 	__syncthreads();
-	if (warp != 0) return;
+	if (warp != 0) {
+		if (sub > 1) cluster_wait();
+		return;
+	}
 	key = lane < kPickThreads / 32 ? s_warp[lane] : 0ull;
 #pragma unroll
 	for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
 	bool ok = true;
 	if (sub > 1) {
+		cluster_wait();      // (the first block runs)
 		if (lane == 0) exchange_send(&s_rx[rank], cta_addr(&s_bar), 0u, key);
 		if (rank != 0) return;      // (nothing is sent to it)
 		ok = exchange_wait(cta_addr(&s_bar));
@@ -303,11 +360,14 @@ __global__ void __launch_bounds__(kPickThreads) k_pick(const __grid_constant__ P
 namespace {
 
 // Blocks per row: slices of at least 4,096 tokens, eight blocks at most.
-void pick_plan(int vocab, int bias, PickArgs* a) {
+// names: how many tokens the lists of a row can name.
+void pick_plan(int vocab, int names, int bias, PickArgs* a) {
 	a->shift = 0;
 	while (a->shift < 3 && vocab >> (a->shift + 1) >= 4096) ++a->shift;
+	if (a->shift == 3 && a->rows * 16 <= sm_count() && vocab >= 16 * 4096) a->shift = 4;      // (few rows: the chain is shorter)
 	a->slice = (((vocab + (1 << a->shift) - 1) >> a->shift) + 31) & ~31;
 	a->pass = std::min(a->slice, kPickPass);
+	a->list = std::min(a->pass, names);
 	a->hash = 0;
 	if (bias > 0) {
 		a->hash = 16;
@@ -319,14 +379,16 @@ template <bool RESIDENT>
 cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 	static PerDeviceOnce once;
 	cudaError_t e = once_per_device(once, [&] {
-		return cudaFuncSetAttribute(k_pick<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PickSmem::bytes(kPickPass, 2 * kPickMaxBias));
+		cudaError_t x = cudaFuncSetAttribute(k_pick<RESIDENT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+		if (x != cudaSuccess) return x;
+		return cudaFuncSetAttribute(k_pick<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PickSmem::bytes(kPickPass, 2 * kPickMaxBias, kPickPass));
 	});
 	if (e != cudaSuccess) return e;
 	a.debug_withhold = a.shift > 0 ? exchange_debug_take(kExchangePick) : 0;
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3(1u << a.shift, a.rows);
 	cfg.blockDim = dim3(kPickThreads);
-	cfg.dynamicSmemBytes = PickSmem::bytes(a.pass, a.hash);
+	cfg.dynamicSmemBytes = PickSmem::bytes(a.pass, a.hash, a.list);
 	cfg.stream = st;
 	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -370,7 +432,7 @@ extern "C" sslm_status sslm_b200_pick_resident(const sslm_b200_pick* call, void*
 	a.out_tokens = c.out_tokens; a.out_best = c.out_best; a.out_logits = c.out_logits; a.out_stride = c.out_stride;
 	a.status = c.row_status;
 	a.max_history = c.max_history; a.max_bias = c.max_bias;
-	pick_plan(c.vocab, c.bias_tokens ? c.max_bias : 0, &a);
+	pick_plan(c.vocab, (c.history ? c.max_history : 0) + (c.bias_tokens ? c.max_bias : 0), c.bias_tokens ? c.max_bias : 0, &a);
 	if (pick_launch<true>(a, (cudaStream_t)stream) != cudaSuccess) {
 		cudaGetLastError();
 		return SSLM_ALLOCATION_FAILED;
