@@ -276,7 +276,7 @@ SSLM_API sslm_status sslm_b200_debug_withhold_tc_load(int32_t launches);
  * where K is cut over a cluster (exchange 0); 1: attention of few rows (0 maxima, 1 sums, 2 contexts, 3 the
  * funnel's maximum); 2: attention of prefill chunks in tiles cut over a cluster (0 to 2); 3: the activation
  * site (0); 5: attention of few biased rows with the q/k/v site inside (0 the biased elements' maximum); 6: attention of
- * rows that share a prefix (0 to 2); 7: the pick (0). kernel -1 takes the request back. */
+ * rows that share a prefix (0 to 2, 3 its copies of V); 7: the pick (0, 1 its first copy of logits). kernel -1 takes the request back. */
 SSLM_API sslm_status sslm_b200_debug_withhold_exchange(int32_t kernel, int32_t exchange);
 /* Tests only: the first kernel of each of the next `launches` (0..16) row groups counts as refused by the CUDA
  * runtime, as for want of resources. The verb returns SSLM_ALLOCATION_FAILED and launches nothing behind it. */

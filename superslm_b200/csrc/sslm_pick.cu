@@ -28,14 +28,19 @@ namespace sslm {
 
 constexpr int kPickThreads = 512;
 constexpr int kPickPass = 24576;            // tokens whose counts a block holds at a time (a multiple of 32)
+constexpr int kPickBits = 262144;           // and tokens whose two bits it holds at a time, where the counts lie in a table
+constexpr int kPickTable = 3072;            // names of a row that the table takes
+constexpr int kPickChunk = 1024, kPickStages = 4;      // words of four logits that arrive at once, and places for them
 constexpr int kPickMaxHistory = 65535;      // (a count is 16 bits)
 constexpr int kPickMaxBias = 1024;
 
 struct PickArgs {
 	int rows, vocab, shift, slice;      // a row is cut over 1 << shift blocks of `slice` tokens (a multiple of 32)
 	int pass;                           // tokens per pass over a slice (a multiple of 32)
-	int hash;                           // places of the bias table, a power of two, or 0
-	int list;                           // room for named tokens of a pass: all of it, or all that the lists can name
+	int hash;                           // places of the table, a power of two, or 0
+	int list;                           // counts by token: room for named tokens of a pass, all of it or all that the lists can name
+	int sums;                           // 1: there are biases
+	int stages;
 	// a caller's tensors
 	const int32_t* logits;
 	int64_t logits_stride;
@@ -58,35 +63,46 @@ struct PickArgs {
 	int debug_withhold;                 // tests only (exchange_debug_take)
 };
 
+// What the lists of a row name is kept in one of two ways. In a table (TABLE) of places found by the token's hash, with the
+// count and the sum of the biases beside each: its size goes by the lists, so a block may have a slice of any length. Or, for
+// long lists, as counts of 16 bits by token, a list of those that are named, and a table for the biases alone.
 struct PickSmem {
-	// bias sums [hash], bias keys [hash], counts u16 [pass + 8], allowed and named bits [pass / 32 + 2], list of named tokens u16 [list]
-	static size_t bytes(int pass, int hash, int list) { return (size_t)hash * 12 + (size_t)(pass + 8) * 2 + (size_t)(pass / 32 + 2) * 8 + (size_t)list * 2; }
+	// logits on their way [stages][kPickChunk], sums [hash] if there are biases, tokens [hash], TABLE: counts [hash], else counts u16
+	// [pass + 8], allowed and named bits [pass / 32 + 2], else list u16 [list]
+	static size_t bytes(bool table, int stages, int sums, int pass, int hash, int list) {
+		return (size_t)stages * kPickChunk * 16 + (size_t)hash * ((table ? 8 : 4) + 8 * sums) + (table ? 0 : (size_t)(pass + 8) * 2) + (size_t)(pass / 32 + 2) * 8 +
+		       (table ? 0 : (size_t)list * 2);
+	}
 };
 
 __device__ __forceinline__ unsigned long long pick_key(int32_t x, int v) {
 	return x == INT32_MIN ? 0ull : (unsigned long long)((uint32_t)x ^ 0x80000000u) << 32 | (0xFFFFFFFFu - (uint32_t)v);
 }
 
-template <bool RESIDENT>
+template <bool RESIDENT, bool TABLE, bool OUT>
 __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant__ PickArgs a) {
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ __align__(8) unsigned long long s_bar, s_rx[16], s_warp[kPickThreads / 32];
-	__shared__ int s_listed;
+	__shared__ __align__(8) unsigned long long s_bar, s_full[kPickStages], s_rx[16], s_warp[kPickThreads / 32];
+	__shared__ PickRow s_row;
+	__shared__ int s_listed, s_code, s_late;
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
 	const int64_t r = blockIdx.y;
-	unsigned long long* bsum = (unsigned long long*)smem;                   // [hash]
-	int32_t* bkey = (int32_t*)(bsum + a.hash);                              // [hash] token, -1: free
-	uint32_t* counts = (uint32_t*)(bkey + a.hash);                          // u16 pairs
-	uint32_t* allow = counts + (a.pass + 8) / 2;                            // bit i: token v0 + i
+	const int4* ring = (const int4*)smem;                                   // [stages][kPickChunk]
+	unsigned long long* bsum = (unsigned long long*)(smem + (size_t)a.stages * kPickChunk * 16);      // [hash], if there are biases
+	int32_t* bkey = (int32_t*)(bsum + (a.sums ? a.hash : 0));               // [hash] token, -1: free
+	uint32_t* counts = (uint32_t*)(bkey + a.hash);                          // TABLE: [hash], else u16 pairs by token
+	uint32_t* allow = counts + (TABLE ? a.hash : (a.pass + 8) / 2);         // bit i: token v0 + i
 	uint32_t* named = allow + a.pass / 32 + 2;
 	uint16_t* list = (uint16_t*)(named + a.pass / 32 + 2);
+	const int held = (blockIdx.x | blockIdx.y) == 0 ? a.debug_withhold : 0;
+	if (t == 0) {
+		if (sub > 1 && rank == 0) exchange_init(cta_addr(&s_bar), (uint32_t)(sub * 8) + (held == 1 ? 4u : 0u));
+		for (int i = 0; i < kPickStages; ++i) ring_init(cta_addr(&s_full[i]), 1);
+		exchange_fence_init();
+		s_late = 0;
+	}
 	if (sub > 1) {
-		if (t == 0 && rank == 0) {
-			const int held = blockIdx.x == 0 && blockIdx.y == 0 ? a.debug_withhold : 0;
-			exchange_init(cta_addr(&s_bar), (uint32_t)(sub * 8) + (held == 1 ? 4u : 0u));
-			exchange_fence_init();
-		}
 		__syncwarp();
 		cluster_arrive();      // (waited for ahead of the word that is sent)
 	}
@@ -94,70 +110,78 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 	pdl_release();
 
 	// ---- the row
-	PickRow w{};
-	int32_t code = 0;
-	const int32_t* bt = nullptr;
-	const int32_t* bv = nullptr;
+	const int32_t* logits = RESIDENT ? a.logits + r * a.logits_stride : a.desc[r].logits;
 	int32_t* out = nullptr;
-	if (RESIDENT) {
-		w.logits = a.logits + r * a.logits_stride;
-		w.theta = 32768;
-		w.extra = -1;
-		if (a.params != nullptr) {
-			w.theta = a.params[3 * r];
-			w.presence = a.params[3 * r + 1];
-			w.frequency = a.params[3 * r + 2];
-			if (w.theta < 1) code = SSLM_B200_ROW_CONSTANTS;
-		}
-		if (a.history != nullptr) {
-			w.history = a.history + r * a.history_stride;
-			w.n_history = a.history_len[r];
-			if (w.n_history < 0 || w.n_history > a.max_history) code = SSLM_B200_ROW_LENGTH;
-		}
-		if (a.bias_tokens != nullptr) {
-			bt = a.bias_tokens + r * a.bias_stride;
-			bv = a.bias_values + r * a.bias_stride;
-			w.n_bias = a.bias_len[r];
-			if (w.n_bias < 0 || w.n_bias > a.max_bias) code = SSLM_B200_ROW_LENGTH;
-		}
-		if (a.mask_page != nullptr) {
-			const int page = a.mask_page[r];
+	if (OUT) out = a.out_logits + r * a.out_stride;
+	if (t == 0) {
+		PickRow x{};
+		int32_t code = 0;
+		if (RESIDENT) {
+			x.theta = 32768;
+			x.extra = -1;
+			const int page = a.mask_page != nullptr ? a.mask_page[r] : -1;
+			if (a.params != nullptr) {
+				x.theta = a.params[3 * r];
+				x.presence = a.params[3 * r + 1];
+				x.frequency = a.params[3 * r + 2];
+			}
+			if (a.history != nullptr) {
+				x.history = a.history + r * a.history_stride;
+				x.n_history = a.history_len[r];
+			}
+			if (a.bias_tokens != nullptr) {
+				x.bias_tokens = a.bias_tokens + r * a.bias_stride;
+				x.bias_values = a.bias_values + r * a.bias_stride;
+				x.n_bias = a.bias_len[r];
+			}
+			if (page >= 0 && page < a.num_masks) x.mask = a.masks + (int64_t)page * a.mask_stride;
+			if (x.theta < 1) code = SSLM_B200_ROW_CONSTANTS;
+			if (x.n_history < 0 || x.n_history > a.max_history || x.n_bias < 0 || x.n_bias > a.max_bias) code = SSLM_B200_ROW_LENGTH;
 			if (page >= a.num_masks) code = SSLM_B200_ROW_INDEX;
-			else if (page >= 0) w.mask = a.masks + (int64_t)page * a.mask_stride;
+			if (rank == 0 && a.status != nullptr) a.status[r] = code;
+		} else {
+			x = a.desc[r];
+			if (x.logits == nullptr) code = 1;      // (a row without controls)
+			else if (x.extra >= 0 && rank == 0) const_cast<int32_t*>(x.history)[x.n_history] = x.extra;      // (its blocks count it from the record)
 		}
-		if (a.out_logits != nullptr) out = a.out_logits + r * a.out_stride;
-		if (rank == 0 && t == 0 && a.status != nullptr) a.status[r] = code;
-	} else {
-		w = a.desc[r];
-		bt = w.bias_tokens;
-		bv = w.bias_values;
-		if (w.logits == nullptr) code = 1;      // (a row without controls)
-		else if (w.extra >= 0 && rank == 0 && t == 0) const_cast<int32_t*>(w.history)[w.n_history] = w.extra;      // (its blocks count it from the descriptor)
+		s_row = x;
+		s_code = code;
 	}
-	if (code != 0) {      // (all blocks of the cluster alike)
+	const PickRow& w = s_row;
+	unsigned long long key = 0ull;      // of the named tokens and the ends
+	const int s0 = min(V, rank * a.slice), s1 = min(V, s0 + a.slice);
+	// four neighbouring tokens of the row lie in one aligned 16-byte word; mis: tokens by which the row's first is off
+	const int mis = (int)(((uintptr_t)logits >> 2) & 3);
+	int v0 = s0, v1, first, last, chunks;
+	uint32_t seq = 0;      // chunks of earlier passes
+	// a pass: tokens v0 .. v1; whole aligned words of four tokens lie from `first` to `last`, the ends are taken one by one
+	auto issue = [&](int chunk) {      // (one thread; the place is free)
+		const uint32_t at = (seq + (uint32_t)chunk) % (uint32_t)a.stages, bar = cta_addr(&s_full[at]);
+		const uint32_t bytes = (uint32_t)min(4 * kPickChunk, last - first - 4 * kPickChunk * chunk) * 4u;
+		asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes + (held == 2 && seq + chunk == 0 ? 16u : 0u)) : "memory");
+		asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(cta_addr(ring + at * kPickChunk)),
+		             "l"(logits + first + 4 * kPickChunk * chunk), "r"(bytes), "r"(bar) : "memory");
+	};
+	auto begin = [&]() {
+		v1 = min(s1, v0 + a.pass);
+		first = min(v1, v0 + ((4 - ((v0 + mis) & 3)) & 3));
+		last = first + ((v1 - first) & ~3);
+		chunks = ((last - first) / 4 + kPickChunk - 1) / kPickChunk;
+		if (t == 0)      // (the first of them on their way while the marks are made)
+			for (int i = 0; i < min(chunks, a.stages); ++i) issue(i);
+	};
+	__syncthreads();
+	if (s_code != 0) {      // (all blocks of the cluster alike)
 		if (sub > 1) cluster_wait();
 		return;
 	}
 
 	auto place = [&](int v) { return ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1); };
 	const bool listed = w.n_history > 0 || w.extra >= 0 || w.n_bias > 0;
-	unsigned long long key = 0ull;      // of the named tokens and the ends
-	const double inv_theta = 1.0 / (double)w.theta;
-	const int s0 = min(V, rank * a.slice), s1 = min(V, s0 + a.slice);
-	// four neighbouring tokens of the row lie in one aligned 16-byte word; mis: tokens by which the row's first is off
-	const int mis = (int)(((uintptr_t)w.logits >> 2) & 3);
 	const int mis_out = (int)(((uintptr_t)out >> 2) & 3);
-	constexpr int U = 5, kStride = 4 * kPickThreads;
-	for (int v0 = s0; v0 < s1; v0 += a.pass) {
-		const int v1 = min(s1, v0 + a.pass), n = v1 - v0, words = (n + 31) / 32;
-		// whole aligned words of four tokens, `first` to `last`; the ends of the pass one by one
-		const int first = min(v1, v0 + ((4 - ((v0 + mis) & 3)) & 3)), last = first + ((v1 - first) & ~3);
-		const int32_t* mine = w.logits + first + 4 * t;
-		const int turns = first + 4 * t < last ? (last - first - 4 * t + kStride - 1) / kStride : 0;      // this thread's words
-		int4 x[U];      // (on their way while the marks are made)
-#pragma unroll
-		for (int u = 0; u < U; ++u)
-			if (u < turns) x[u] = __ldcs((const int4*)(mine + u * kStride));
+	if (v0 < s1) begin();
+	while (v0 < s1) {
+		const int n = v1 - v0, words = (n + 31) / 32;
 		// ---- marks and counts of tokens v0 .. v1
 		for (int i = t; i < words + 2; i += kPickThreads) {
 			uint32_t bits = 0;
@@ -177,60 +201,86 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			named[i] = 0u;
 		}
 		if (listed) {
-			for (int i = t; i < (n + 8) / 8; i += kPickThreads) ((int4*)counts)[i] = make_int4(0, 0, 0, 0);
+			if constexpr (!TABLE) {
+				for (int i = t; i < (n + 8) / 8; i += kPickThreads) ((int4*)counts)[i] = make_int4(0, 0, 0, 0);
+			}
 			for (int i = t; i < a.hash; i += kPickThreads) {
 				bkey[i] = -1;
-				bsum[i] = 0ull;
+				if (a.sums) bsum[i] = 0ull;
+				if constexpr (TABLE) counts[i] = 0u;
 			}
 			if (t == 0) s_listed = 0;
 			__syncthreads();
+			auto bits_of = [&](uint32_t i) { return named[i >> 5] >> (i & 31) & 1u; };
 			auto name = [&](uint32_t i) {      // the first to name a token enters it into the list
-				if ((atomicOr(&named[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u) == 0u) list[atomicAdd(&s_listed, 1)] = (uint16_t)i;
+				if (bits_of(i) == 0u && (atomicOr(&named[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u) == 0u) list[atomicAdd(&s_listed, 1)] = (uint16_t)i;
+			};
+			auto enter = [&](int v) {      // its place in the table (a quarter of the places at least stay free)
+				uint32_t h = place(v);
+				for (;;) {
+					int was = *(volatile int32_t*)&bkey[h];
+					if (was == -1) was = atomicCAS(&bkey[h], -1, v);
+					if (was == -1 || was == v) break;
+					h = (h + 1) & (uint32_t)(a.hash - 1);
+				}
+				return h;
 			};
 			auto seen = [&](int v) {
 				const uint32_t i = (uint32_t)(v - v0);
 				if (i >= (uint32_t)n) return;
-				atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
-				name(i);
+				if constexpr (TABLE) {
+					atomicAdd(&counts[enter(v)], 1u);
+					if (bits_of(i) == 0u) atomicOr(&named[i >> 5], 1u << (i & 31));
+				} else {
+					atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
+					name(i);
+				}
 			};
 			{      // (ids of any alignment: single ones up to the first 16-byte word, then words)
 				const int head = min(w.n_history, (int)((4 - (((uintptr_t)w.history >> 2) & 3)) & 3)), whole = (w.n_history - head) >> 2;
 				if (t < head) seen(w.history[t]);
 				const int4* ids = (const int4*)(w.history + head);
-#pragma unroll 2
-				for (int i = t; i < whole; i += kPickThreads) {
-					const int4 id = ids[i];
-					seen(id.x);
-					seen(id.y);
-					seen(id.z);
-					seen(id.w);
+				for (int i0 = t; i0 < whole; i0 += 4 * kPickThreads) {
+					int4 id[4];
+#pragma unroll
+					for (int u = 0; u < 4; ++u) id[u] = i0 + u * kPickThreads < whole ? ids[i0 + u * kPickThreads] : make_int4(-1, -1, -1, -1);
+#pragma unroll 1
+					for (int u = 0; u < 4; ++u) {
+						seen(id[0].x);
+						seen(id[0].y);
+						seen(id[0].z);
+						seen(id[0].w);
+						id[0] = id[1];
+						id[1] = id[2];
+						id[2] = id[3];
+					}
 				}
 				const int tail = head + 4 * whole + t;
 				if (tail < w.n_history) seen(w.history[tail]);
 			}
 			if (t == 0 && w.extra >= 0) seen(w.extra);
 			for (int i = t; i < w.n_bias; i += kPickThreads) {
-				const int v = bt[i];
+				const int v = w.bias_tokens[i];
 				const uint32_t at = (uint32_t)(v - v0);
 				if (at >= (uint32_t)n) continue;
-				uint32_t h = place(v);
-				for (;;) {      // (at least half of the places stay free)
-					const int was = atomicCAS(&bkey[h], -1, v);
-					if (was == -1 || was == v) break;
-					h = (h + 1) & (uint32_t)(a.hash - 1);
+				atomicAdd(&bsum[enter(v)], (unsigned long long)(long long)w.bias_values[i]);
+				if constexpr (TABLE) {
+					if (bits_of(at) == 0u) atomicOr(&named[at >> 5], 1u << (at & 31));
+				} else {
+					name(at);
 				}
-				atomicAdd(&bsum[h], (unsigned long long)(long long)bv[i]);
-				name(at);
 			}
 			__syncthreads();
 			// ---- the named tokens
+			const double inv_theta = 1.0 / (double)w.theta;
 #pragma unroll 2
-			for (int k = t; k < s_listed; k += kPickThreads) {
-				const int i = list[k], v = v0 + i;
-				int32_t y = w.logits[v];
+			for (int k = t; k < (TABLE ? a.hash : s_listed); k += kPickThreads) {
+				const int v = TABLE ? bkey[k] : v0 + list[k], i = v - v0;
+				if (TABLE && v < 0) continue;
+				int32_t y = logits[v];
 				if (y != INT32_MIN) {
 					long long z = y;
-					const uint32_t cnt = counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
+					const uint32_t cnt = TABLE ? counts[k] : counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
 					if (cnt != 0u) {
 						if (z > 0) {      // floor(2^15 z / theta): a quotient in doubles, off by one at most, settled by its remainder
 							const long long num = z << 15;
@@ -242,7 +292,9 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 						}
 						z -= (long long)w.presence + (long long)w.frequency * (long long)cnt;
 					}
-					if (w.n_bias > 0) {
+					if (TABLE) {
+						if (a.sums) z += (long long)bsum[k];
+					} else if (w.n_bias > 0) {
 						uint32_t h = place(v);
 						while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
 						if (bkey[h] == v) z += (long long)bsum[h];
@@ -251,22 +303,27 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 				}
 				if ((allow[i >> 5] >> (i & 31) & 1u) == 0u) y = INT32_MIN;
 				key = max(key, pick_key(y, v));
-				if (out != nullptr) out[v] = y;
+				if (OUT) out[v] = y;
 			}
-		} else {
-			__syncthreads();
 		}
+		__syncthreads();
 		// ---- all others
 		auto one = [&](int v) {
 			const int i = v - v0;
 			if ((named[i >> 5] >> (i & 31) & 1u) != 0u) return;
-			const int32_t y = (allow[i >> 5] >> (i & 31) & 1u) != 0u ? w.logits[v] : INT32_MIN;
+			const int32_t y = (allow[i >> 5] >> (i & 31) & 1u) != 0u ? logits[v] : INT32_MIN;
 			key = max(key, pick_key(y, v));
-			if (out != nullptr) out[v] = y;
+			if (OUT) out[v] = y;
 		};
 		if (t < first - v0) one(v0 + t);
 		if (t < v1 - last) one(last + t);
-		// the words of a thread lie a multiple of 32 tokens apart: their bits at one place of their bitmap words
+		if (listed) {      // (from here on the words' own tokens only)
+			__syncthreads();
+			for (int i = t; i < words; i += kPickThreads) allow[i] &= ~named[i];
+			__syncthreads();
+		}
+		// a thread has every 512th word: their bits lie at one place of their bitmap words
+		constexpr int kStride = 4 * kPickThreads;
 		const int bit = (first - v0 + 4 * t) & 31, word = (first - v0 + 4 * t) >> 5;
 		const bool straddles = bit > 28;
 		auto nibble = [&](const uint32_t* map, int k) {
@@ -282,22 +339,24 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		};
 		int32_t top = INT32_MIN;
 		int top_at = 0;      // the word that has it first
-		for (int k0 = 0; k0 < turns; k0 += U) {
+		const int total = (last - first) / 4;
+#pragma unroll 1
+		for (int i = 0; i < chunks; ++i) {
+			const uint32_t at = (seq + (uint32_t)i) % (uint32_t)a.stages, turn = (seq + (uint32_t)i) / (uint32_t)a.stages;
+			if (s_late == 0 && !ring_wait(cta_addr(&s_full[at]), turn & 1u)) s_late = 1;      // (what is read then does not count)
 #pragma unroll
-			for (int u = 0; u < U; ++u) {
-				const int k = k0 + u;
-				if (k >= turns) break;
-				const int4 q = x[u];
-				if (k + U < turns) x[u] = __ldcs((const int4*)(mine + (k + U) * kStride));
-				const uint32_t nm = listed ? nibble(named, k) : 0u;
+			for (int u = 0; u < kPickChunk / kPickThreads; ++u) {
+				const int k = i * (kPickChunk / kPickThreads) + u;
+				if (k * kPickThreads + t >= total) break;
 				int32_t y[4];
-				words_of(q, nibble(allow, k) & ~nm, y);
+				words_of(ring[at * kPickChunk + u * kPickThreads + t], nibble(allow, k), y);
 				const int32_t m = max(max(y[0], y[1]), max(y[2], y[3]));
 				if (m > top) {
 					top = m;
 					top_at = k;
 				}
-				if (out != nullptr) {
+				if (OUT) {
+					const uint32_t nm = listed ? nibble(named, k) : 0u;
 					int32_t* to = out + first + 4 * t + k * kStride;
 					if (mis_out == mis && nm == 0u) {
 						__stcs((int4*)to, make_int4(y[0], y[1], y[2], y[3]));
@@ -308,19 +367,26 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 					}
 				}
 			}
+			__syncthreads();      // the place is free
+			if (t == 0 && s_late == 0 && i + a.stages < chunks) issue(i + a.stages);
 		}
 		if (top != INT32_MIN) {      // (in place, the word reads as it was but for what the bitmaps leave out)
 			int32_t y[4];
-			words_of(*(const int4*)(mine + top_at * kStride), nibble(allow, top_at) & ~(listed ? nibble(named, top_at) : 0u), y);
+			words_of(*(const int4*)(logits + first + 4 * t + top_at * kStride), nibble(allow, top_at), y);
 			const int j = y[0] == top ? 0 : (y[1] == top ? 1 : (y[2] == top ? 2 : 3));
 			key = max(key, pick_key(top, first + 4 * t + top_at * kStride + j));
 		}
 		__syncthreads();      // the tables may be overwritten
+		seq += (uint32_t)chunks;
+		v0 += a.pass;
+		if (v0 < s1) begin();
 	}
 	// ---- the row's largest key: larger values first, then lower indices
 #pragma unroll
 	for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
 	if (lane == 0) s_warp[warp] = key;
+	if (t == 0 && s_late != 0)      // (a copy that is late may still come)
+		for (uint32_t i = seq > (uint32_t)a.stages ? seq - (uint32_t)a.stages : 0u; i < seq; ++i) ring_wait(cta_addr(&s_full[i % (uint32_t)a.stages]), i / (uint32_t)a.stages & 1u);
 	__syncthreads();
 	if (warp != 0) {
 		if (sub > 1) cluster_wait();
@@ -329,13 +395,15 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 	key = lane < kPickThreads / 32 ? s_warp[lane] : 0ull;
 #pragma unroll
 	for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-	bool ok = true;
+	bool ok = s_late == 0;
 	if (sub > 1) {
 		cluster_wait();      // (the first block runs)
+		if (!ok) key = 1ull;      // (no token's key: theirs have an index below 2^30)
 		if (lane == 0) exchange_send(&s_rx[rank], cta_addr(&s_bar), 0u, key);
 		if (rank != 0) return;      // (nothing is sent to it)
-		ok = exchange_wait(cta_addr(&s_bar));
+		ok = exchange_wait(cta_addr(&s_bar)) && ok;
 		key = lane < sub ? s_rx[lane] : 0ull;
+		ok = !__any_sync(0xffffffffu, key == 1ull) && ok;
 #pragma unroll
 		for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
 	}
@@ -359,36 +427,46 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 
 namespace {
 
-// Blocks per row: slices of at least 4,096 tokens, eight blocks at most.
-// names: how many tokens the lists of a row can name.
-void pick_plan(int vocab, int names, int bias, PickArgs* a) {
+// names: how many tokens the lists of a row can name; biases of them. True: the table.
+bool pick_plan(int names, int biases, PickArgs* a) {
+	const bool table = names <= kPickTable;
+	// blocks per row: as many as run at once, two a multiprocessor, with slices of at least 4,096 tokens; without the table
+	// the passes of a slice repeat the lists, so one pass if possible
+	const int most = std::max(1, 2 * sm_count() / a->rows);
 	a->shift = 0;
-	while (a->shift < 3 && vocab >> (a->shift + 1) >= 4096) ++a->shift;
-	if (a->shift == 3 && a->rows * 16 <= sm_count() && vocab >= 16 * 4096) a->shift = 4;      // (few rows: the chain is shorter)
-	a->slice = (((vocab + (1 << a->shift) - 1) >> a->shift) + 31) & ~31;
-	a->pass = std::min(a->slice, kPickPass);
+	while (a->shift < 4 && a->vocab >> (a->shift + 1) >= 4096 && (2 << a->shift <= most || (!table && a->vocab >> a->shift > kPickPass))) ++a->shift;
+	a->slice = (((a->vocab + (1 << a->shift) - 1) >> a->shift) + 31) & ~31;
+	a->pass = std::min(a->slice, table ? kPickBits : kPickPass);
 	a->list = std::min(a->pass, names);
+	a->sums = biases > 0 ? 1 : 0;
 	a->hash = 0;
-	if (bias > 0) {
-		a->hash = 16;
-		while (a->hash < 2 * bias) a->hash *= 2;
+	const int kept = table ? names : biases;
+	if (kept > 0) {
+		a->hash = 64;
+		while (3 * a->hash < 4 * kept) a->hash *= 2;
 	}
+	// logits on their way: what a pass has, four chunks at most, two where that lets two blocks share a multiprocessor
+	const size_t half = 112 * 1024, kept_bytes = PickSmem::bytes(table, 0, a->sums, a->pass, a->hash, a->list), chunk = kPickChunk * 16;
+	a->stages = std::max(1, std::min(kPickStages, (a->pass / 4 + kPickChunk - 1) / kPickChunk));
+	while (a->stages > 2 && kept_bytes + a->stages * chunk > half && kept_bytes + 2 * chunk <= half) --a->stages;
+	return table;
 }
 
-template <bool RESIDENT>
+template <bool RESIDENT, bool TABLE, bool OUT>
 cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 	static PerDeviceOnce once;
+	const auto kernel = k_pick<RESIDENT, TABLE, OUT>;
 	cudaError_t e = once_per_device(once, [&] {
-		cudaError_t x = cudaFuncSetAttribute(k_pick<RESIDENT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-		if (x != cudaSuccess) return x;
-		return cudaFuncSetAttribute(k_pick<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PickSmem::bytes(kPickPass, 2 * kPickMaxBias, kPickPass));
+		const size_t most = TABLE ? PickSmem::bytes(true, kPickStages, 1, kPickBits, 4096, 0) : PickSmem::bytes(false, kPickStages, 1, kPickPass, 2 * kPickMaxBias, kPickPass);
+		const cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+		return x != cudaSuccess ? x : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
 	});
 	if (e != cudaSuccess) return e;
-	a.debug_withhold = a.shift > 0 ? exchange_debug_take(kExchangePick) : 0;
+	a.debug_withhold = exchange_debug_take(kExchangePick);
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3(1u << a.shift, a.rows);
 	cfg.blockDim = dim3(kPickThreads);
-	cfg.dynamicSmemBytes = PickSmem::bytes(a.pass, a.hash, a.list);
+	cfg.dynamicSmemBytes = PickSmem::bytes(TABLE, a.stages, a.sums, a.pass, a.hash, a.list);
 	cfg.stream = st;
 	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -399,7 +477,7 @@ cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 	attr[1].val.programmaticStreamSerializationAllowed = 1;
 	cfg.attrs = attr;
 	cfg.numAttrs = pdl_enabled() ? 2 : 1;
-	return cudaLaunchKernelEx(&cfg, k_pick<RESIDENT>, a);
+	return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 }  // namespace
@@ -432,8 +510,11 @@ extern "C" sslm_status sslm_b200_pick_resident(const sslm_b200_pick* call, void*
 	a.out_tokens = c.out_tokens; a.out_best = c.out_best; a.out_logits = c.out_logits; a.out_stride = c.out_stride;
 	a.status = c.row_status;
 	a.max_history = c.max_history; a.max_bias = c.max_bias;
-	pick_plan(c.vocab, (c.history ? c.max_history : 0) + (c.bias_tokens ? c.max_bias : 0), c.bias_tokens ? c.max_bias : 0, &a);
-	if (pick_launch<true>(a, (cudaStream_t)stream) != cudaSuccess) {
+	const int biases = c.bias_tokens ? c.max_bias : 0;
+	const bool table = pick_plan((c.history ? c.max_history : 0) + biases, biases, &a);
+	const auto launch = table ? (c.out_logits ? pick_launch<true, true, true> : pick_launch<true, true, false>)
+	                          : (c.out_logits ? pick_launch<true, false, true> : pick_launch<true, false, false>);
+	if (launch(a, (cudaStream_t)stream) != cudaSuccess) {
 		cudaGetLastError();
 		return SSLM_ALLOCATION_FAILED;
 	}

@@ -166,9 +166,9 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	uint32_t* redo = (uint32_t*)(sown + a.spages);                                          // [ppages, then spages] rows whose probabilities need the exact form
 
 	if (t == 0) {
-		ring_init(cta_addr(&s_bars[0]), 1);
+		const int held = (blockIdx.x | blockIdx.y | blockIdx.z) == 0 ? a.debug_withhold : 0;
+		ring_init(cta_addr(&s_bars[0]), held == 4 ? 2 : 1);
 		if (sub > 1) {
-			const int held = (blockIdx.x | blockIdx.y | blockIdx.z) == 0 ? a.debug_withhold : 0;
 			auto more = [&](int i) { return held == i + 1 ? 4u : 0u; };
 			exchange_init(cta_addr(&s_bars[1]), (uint32_t)(sub * ROWS * 4) + more(0));
 			exchange_init(cta_addr(&s_bars[2]), (uint32_t)(sub * ROWS * 8) + more(1));
@@ -903,7 +903,7 @@ cudaError_t prefix_dispatch(PrefixArgs a, int hd, const PrefixPlan& p, cudaStrea
 	a.ppages = p.ppages;
 	a.spages = p.spages;
 	a.vgroups = p.vgroups;
-	a.debug_withhold = p.sub > 1 ? exchange_debug_take(kExchangeAttnPrefix) : 0;
+	a.debug_withhold = exchange_debug_take(kExchangeAttnPrefix);
 	if (hd == 128) return p.rows == 32 ? prefix_launch<128, 32, RESIDENT>(a, p, st) : prefix_launch<128, 16, RESIDENT>(a, p, st);
 	if (hd == 64) return p.rows == 32 ? prefix_launch<64, 32, RESIDENT>(a, p, st) : prefix_launch<64, 16, RESIDENT>(a, p, st);
 	return p.rows == 32 ? prefix_launch<32, 32, RESIDENT>(a, p, st) : prefix_launch<32, 16, RESIDENT>(a, p, st);

@@ -215,18 +215,20 @@ def test_calls_on_two_streams(gpu_lib, torch):
         c.compare()
 
 
-def test_an_exchange_that_runs_out(gpu_lib, torch):
+@pytest.mark.parametrize("rows,vocab,exchange", [(3, 100000, 0), (3, 100000, 1), (200, 30000, 1)])
+def test_a_wait_that_runs_out(gpu_lib, torch, rows, vocab, exchange):
+    """block 0 waits for more than its peers send, or than its copy of logits brings: its row is reported, the next call is right"""
     arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
     arm.argtypes = [C.c_int32, C.c_int32]
-    assert arm(7, 1) == abi.ST["SSLM_INVALID_ARGUMENT"]
-    c = Call(gpu_lib, torch, make(30, 3, 100000, 10, 0, None))
+    assert arm(7, 2) == abi.ST["SSLM_INVALID_ARGUMENT"]
+    c = Call(gpu_lib, torch, make(30, rows, vocab, 10, 0, None))
     try:
-        assert arm(7, 0) == 0
+        assert arm(7, exchange) == 0
         c.call.run()
         torch.cuda.synchronize()
     finally:
         arm(-1, 0)
-    assert c.status.tolist() == [100, 0, 0]
+    assert c.status.tolist() == [100] + [0] * (rows - 1)
     c.check()
 
 

@@ -278,13 +278,13 @@ def test_calls_on_two_streams(gpu_lib, torch):
         c.compare()
 
 
-@pytest.mark.parametrize("exchange", [0, 1, 2])
-def test_an_exchange_that_runs_out(gpu_lib, torch, splits, exchange):
-    """block 0 waits for more than its peers send: its rows are reported, the next call is right"""
+@pytest.mark.parametrize("splits_n,exchange", [(4, 0), (4, 1), (4, 2), (4, 3), (1, 3)])
+def test_a_wait_that_runs_out(gpu_lib, torch, splits, splits_n, exchange):
+    """block 0 waits for more than its peers send, or its copies of V bring: its rows are reported, the next call is right"""
     arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
     arm.argtypes = [C.c_int32, C.c_int32]
-    assert arm(6, 3) == abi.ST["SSLM_INVALID_ARGUMENT"]
-    splits(4)
+    assert arm(6, 4) == abi.ST["SSLM_INVALID_ARGUMENT"]
+    splits(splits_n)
     c = Call(gpu_lib, torch, attention_case(40, SHAPES["1.5b"], [600], lengths(40, 5, 1, 50)))
     try:
         assert arm(6, exchange) == 0
@@ -292,7 +292,8 @@ def test_an_exchange_that_runs_out(gpu_lib, torch, splits, exchange):
         torch.cuda.synchronize()
     finally:
         arm(-1, 0)
-    assert (c.status == 100).all()
+    # (exchanges of a cluster of four: two rows a tile, or five)
+    assert c.status[0] == 100 and all(s in (0, 100) for s in c.status.tolist())
     c.out.fill_(JUNK)
     c.check()
 
