@@ -10,12 +10,13 @@
 // and the row's token is the lowest index of the largest x, -2 where nothing is allowed.
 //
 // One pass over the logits. A row is cut over the blocks of a cluster; a block first marks, for its slice of the
-// vocabulary, which tokens the history or the biases name, with counts beside them, and which ones are allowed. The
-// named tokens are few and dear (a division, a table): they are listed and dealt out one by one. All others are
-// streamed past, four at a time, and cost a load, a nibble of one bitmap and a maximum; where it lies is looked up
-// once, at the end. (With the named ones worked on in the stream nearly every other warp stopped for one: 256 rows
-// of 151,936 with histories of 1,024 took 104 us.) Bound by the logits' bytes where rows are many, by the chain
-// (lists, marks, one trip to memory, one exchange) where they are few.
+// vocabulary, which tokens the history or the biases name, with counts beside them, and which of the others are
+// allowed. The others, nearly all, are streamed past, four at a time, and cost a word of shared memory, a nibble of
+// one bitmap and a maximum; where it lies is looked up once, at the end. The named tokens are dear (a division, a
+// table) and come last, each to one thread: then their logits are in L2 (asked for ahead of the stream, a thousand
+// single words a row cost as much as 20 MB of it; worked on in the stream, nearly every other warp stops for one).
+// Bound by the logits' bytes where rows are many, by the chain (lists, marks, one trip to memory, one exchange)
+// where they are few.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -28,11 +29,11 @@ namespace sslm {
 
 constexpr int kPickThreads = 512;
 constexpr int kPickPass = 24576;            // tokens whose counts a block holds at a time (a multiple of 32)
-constexpr int kPickBits = 262144;           // and tokens whose two bits it holds at a time, where the counts lie in a table
-constexpr int kPickTable = 3072;            // names of a row that the table takes
-constexpr int kPickChunk = 1024, kPickStages = 4;      // words of four logits that arrive at once, and places for them
+constexpr int kPickBits = 262144;           // and tokens whose bits it holds at a time, where the counts lie in a table
 constexpr int kPickMaxHistory = 65535;      // (a count is 16 bits)
 constexpr int kPickMaxBias = 1024;
+constexpr int kPickTable = 3072;            // names of a row that the table takes
+constexpr int kPickChunk = 1024, kPickStages = 4;      // words of four logits that arrive at once, and places for them
 
 struct PickArgs {
 	int rows, vocab, shift, slice;      // a row is cut over 1 << shift blocks of `slice` tokens (a multiple of 32)
@@ -64,14 +65,16 @@ struct PickArgs {
 };
 
 // What the lists of a row name is kept in one of two ways. In a table (TABLE) of places found by the token's hash, with the
-// count and the sum of the biases beside each: its size goes by the lists, so a block may have a slice of any length. Or, for
-// long lists, as counts of 16 bits by token, a list of those that are named, and a table for the biases alone.
+// count and the sum of the biases beside each: its size goes by the lists, so a block may have a slice of any length, and a
+// thread keeps its ids of the lists in registers from the start of the call. Or, for long lists, as counts of 16 bits by
+// token, a list of those that are named, and a table for the biases alone.
 struct PickSmem {
 	// logits on their way [stages][kPickChunk], sums [hash] if there are biases, tokens [hash], TABLE: counts [hash], else counts u16
-	// [pass + 8], allowed and named bits [pass / 32 + 2], else list u16 [list]
-	static size_t bytes(bool table, int stages, int sums, int pass, int hash, int list) {
-		return (size_t)stages * kPickChunk * 16 + (size_t)hash * ((table ? 8 : 4) + 8 * sums) + (table ? 0 : (size_t)(pass + 8) * 2) + (size_t)(pass / 32 + 2) * 8 +
-		       (table ? 0 : (size_t)list * 2);
+	// [pass + 8], bits of the tokens that are allowed and not named, bits of the named ones if kept, else list u16 [list]
+	__host__ __device__ static int words(int pass) { return (pass / 32 + 11) & ~3; }      // of a bitmap: filled four at a time (16-byte stores), read one further
+	static size_t bytes(bool table, bool out, int stages, int sums, int pass, int hash, int list) {
+		return (size_t)stages * kPickChunk * 16 + (size_t)hash * ((table ? 8 : 4) + 8 * sums) + (table ? 0 : (size_t)(pass + 8) * 2) +
+		       (size_t)words(pass) * (table && !out ? 4 : 8) + (table ? 0 : (size_t)list * 2);
 	}
 };
 
@@ -81,10 +84,12 @@ __device__ __forceinline__ unsigned long long pick_key(int32_t x, int v) {
 
 template <bool RESIDENT, bool TABLE, bool OUT>
 __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant__ PickArgs a) {
+	constexpr bool NAMED = OUT || !TABLE;      // the named bits are kept
+	constexpr int kStride = 4 * kPickThreads;
 	extern __shared__ __align__(16) unsigned char smem[];
 	__shared__ __align__(8) unsigned long long s_bar, s_full[kPickStages], s_rx[16], s_warp[kPickThreads / 32];
 	__shared__ PickRow s_row;
-	__shared__ int s_listed, s_code, s_late;
+	__shared__ int s_listed, s_code, s_late, s_part[kPickThreads / 32];
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
 	const int64_t r = blockIdx.y;
@@ -92,9 +97,9 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 	unsigned long long* bsum = (unsigned long long*)(smem + (size_t)a.stages * kPickChunk * 16);      // [hash], if there are biases
 	int32_t* bkey = (int32_t*)(bsum + (a.sums ? a.hash : 0));               // [hash] token, -1: free
 	uint32_t* counts = (uint32_t*)(bkey + a.hash);                          // TABLE: [hash], else u16 pairs by token
-	uint32_t* allow = counts + (TABLE ? a.hash : (a.pass + 8) / 2);         // bit i: token v0 + i
-	uint32_t* named = allow + a.pass / 32 + 2;
-	uint16_t* list = (uint16_t*)(named + a.pass / 32 + 2);
+	uint32_t* dense = counts + (TABLE ? a.hash : (a.pass + 8) / 2);         // bit i: token v0 + i is allowed and not named
+	uint32_t* named = dense + (NAMED ? PickSmem::words(a.pass) : 0);
+	uint16_t* list = (uint16_t*)(named + PickSmem::words(a.pass));
 	const int held = (blockIdx.x | blockIdx.y) == 0 ? a.debug_withhold : 0;
 	if (t == 0) {
 		if (sub > 1 && rank == 0) exchange_init(cta_addr(&s_bar), (uint32_t)(sub * 8) + (held == 1 ? 4u : 0u));
@@ -147,11 +152,23 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		s_row = x;
 		s_code = code;
 	}
-	const PickRow& w = s_row;
-	unsigned long long key = 0ull;      // of the named tokens and the ends
+	// TABLE: this thread's ids, asked for with the row's record (of the lists' whole room: how much of it counts is known later)
+	constexpr int IH = TABLE ? kPickTable / kPickThreads : 0, IB = TABLE ? kPickMaxBias / kPickThreads : 0, IN = IH + IB + 1;
+	int32_t id[IN], add[IB + 1];
+	if constexpr (TABLE && RESIDENT) {
+#pragma unroll
+		for (int u = 0; u < IH; ++u) id[u] = a.history != nullptr && t + u * kPickThreads < a.max_history ? a.history[r * a.history_stride + t + u * kPickThreads] : -1;
+#pragma unroll
+		for (int u = 0; u < IB; ++u) {
+			const bool there = a.bias_tokens != nullptr && t + u * kPickThreads < a.max_bias;
+			id[IH + u] = there ? a.bias_tokens[r * a.bias_stride + t + u * kPickThreads] : -1;
+			add[u] = there ? a.bias_values[r * a.bias_stride + t + u * kPickThreads] : 0;
+		}
+	}
+	const PickRow& w = s_row;      // (in shared memory: the registers are wanted elsewhere)
 	const int s0 = min(V, rank * a.slice), s1 = min(V, s0 + a.slice);
 	// four neighbouring tokens of the row lie in one aligned 16-byte word; mis: tokens by which the row's first is off
-	const int mis = (int)(((uintptr_t)logits >> 2) & 3);
+	const int mis = (int)(((uintptr_t)logits >> 2) & 3), mis_out = (int)(((uintptr_t)out >> 2) & 3);
 	int v0 = s0, v1, first, last, chunks;
 	uint32_t seq = 0;      // chunks of earlier passes
 	// a pass: tokens v0 .. v1; whole aligned words of four tokens lie from `first` to `last`, the ends are taken one by one
@@ -175,155 +192,159 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		if (sub > 1) cluster_wait();
 		return;
 	}
-
-	auto place = [&](int v) { return ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1); };
-	const bool listed = w.n_history > 0 || w.extra >= 0 || w.n_bias > 0;
-	const int mis_out = (int)(((uintptr_t)out >> 2) & 3);
 	if (v0 < s1) begin();
+	const bool listed = w.n_history > 0 || w.extra >= 0 || w.n_bias > 0;
+	if constexpr (TABLE) {
+#pragma unroll
+		for (int u = 0; u < IH; ++u) {
+			if (!RESIDENT) id[u] = t + u * kPickThreads < w.n_history ? w.history[t + u * kPickThreads] : -1;
+			else if (t + u * kPickThreads >= w.n_history) id[u] = -1;
+		}
+#pragma unroll
+		for (int u = 0; u < IB; ++u) {
+			const bool there = t + u * kPickThreads < w.n_bias;
+			if (!RESIDENT) add[u] = there ? w.bias_values[t + u * kPickThreads] : 0;
+			id[IH + u] = there ? (RESIDENT ? id[IH + u] : w.bias_tokens[t + u * kPickThreads]) : -1;
+		}
+		id[IN - 1] = !RESIDENT && t == 0 ? w.extra : -1;
+	}
+	auto place = [&](int v) { return ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1); };
+	unsigned long long key = 0ull;
 	while (v0 < s1) {
 		const int n = v1 - v0, words = (n + 31) / 32;
 		// ---- marks and counts of tokens v0 .. v1
-		for (int i = t; i < words + 2; i += kPickThreads) {
-			uint32_t bits = 0;
-			const int left = n - i * 32;
-			if (left > 0) {
-				bits = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
-				if (w.mask != nullptr) {      // (v0 is a multiple of 32; a page has ceil(V / 8) bytes and any address)
-					const uint8_t* m = w.mask + (v0 >> 3) + 4 * i;
+		for (int i = 4 * t; i < words + 2; i += 4 * kPickThreads) {
+			uint32_t bits[4];
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				const int left = n - (i + j) * 32;
+				bits[j] = left >= 32 ? 0xFFFFFFFFu : (left > 0 ? (1u << left) - 1u : 0u);
+				if (w.mask != nullptr && left > 0) {      // (v0 is a multiple of 32; a page has ceil(V / 8) bytes and any address)
+					const uint8_t* m = w.mask + (v0 >> 3) + 4 * (i + j);
 					uint32_t page = 0;
 					if (left >= 32 && ((uintptr_t)m & 3) == 0) page = *(const uint32_t*)m;
 					else
-						for (int j = 0; j < min(4, (left + 7) >> 3); ++j) page |= (uint32_t)m[j] << (8 * j);
-					bits &= page;
+						for (int b = 0; b < min(4, (left + 7) >> 3); ++b) page |= (uint32_t)m[b] << (8 * b);
+					bits[j] &= page;
 				}
 			}
-			allow[i] = bits;
-			named[i] = 0u;
+			*(uint4*)(dense + i) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+			if constexpr (NAMED) *(uint4*)(named + i) = make_uint4(0u, 0u, 0u, 0u);
 		}
+		int at[IN];      // TABLE: the place of an id that this thread was the first to enter, or -1
+#pragma unroll
+		for (int u = 0; u < IN; ++u) at[u] = -1;
 		if (listed) {
-			if constexpr (!TABLE) {
+			if constexpr (!TABLE)
 				for (int i = t; i < (n + 8) / 8; i += kPickThreads) ((int4*)counts)[i] = make_int4(0, 0, 0, 0);
-			}
 			for (int i = t; i < a.hash; i += kPickThreads) {
 				bkey[i] = -1;
 				if (a.sums) bsum[i] = 0ull;
 				if constexpr (TABLE) counts[i] = 0u;
 			}
-			if (t == 0) s_listed = 0;
 			__syncthreads();
-			auto bits_of = [&](uint32_t i) { return named[i >> 5] >> (i & 31) & 1u; };
-			auto name = [&](uint32_t i) {      // the first to name a token enters it into the list
-				if (bits_of(i) == 0u && (atomicOr(&named[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u) == 0u) list[atomicAdd(&s_listed, 1)] = (uint16_t)i;
+			auto name = [&](uint32_t i) {
+				if constexpr (NAMED) {
+					if ((named[i >> 5] >> (i & 31) & 1u) != 0u) return;
+					atomicOr(&named[i >> 5], 1u << (i & 31));
+				}
+				if ((dense[i >> 5] >> (i & 31) & 1u) != 0u) atomicAnd(&dense[i >> 5], ~(1u << (i & 31)));
 			};
-			auto enter = [&](int v) {      // its place in the table (a quarter of the places at least stay free)
+			auto enter = [&](int v, bool* new_to_it) {      // its place in the table (a quarter of the places at least stay free)
 				uint32_t h = place(v);
 				for (;;) {
 					int was = *(volatile int32_t*)&bkey[h];
-					if (was == -1) was = atomicCAS(&bkey[h], -1, v);
-					if (was == -1 || was == v) break;
+					if (was == -1) {
+						was = atomicCAS(&bkey[h], -1, v);
+						*new_to_it = was == -1;
+						if (was == -1) break;
+					}
+					if (was == v) break;
 					h = (h + 1) & (uint32_t)(a.hash - 1);
 				}
 				return h;
 			};
-			auto seen = [&](int v) {
-				const uint32_t i = (uint32_t)(v - v0);
-				if (i >= (uint32_t)n) return;
-				if constexpr (TABLE) {
-					atomicAdd(&counts[enter(v)], 1u);
-					if (bits_of(i) == 0u) atomicOr(&named[i >> 5], 1u << (i & 31));
-				} else {
-					atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
+			if constexpr (TABLE) {
+#pragma unroll
+				for (int u = 0; u < IN; ++u) {
+					const uint32_t i = (uint32_t)(id[u] - v0);
+					if (i >= (uint32_t)n) continue;
+					bool new_to_it = false;
+					const uint32_t h = enter(id[u], &new_to_it);
+					if (new_to_it) at[u] = (int)h;
+					if (u < IH || u == IN - 1) atomicAdd(&counts[h], 1u);
+					else atomicAdd(&bsum[h], (unsigned long long)(long long)add[u - IH]);
 					name(i);
 				}
-			};
-			{      // (ids of any alignment: single ones up to the first 16-byte word, then words)
+			} else {
+				auto seen = [&](int v) {
+					const uint32_t i = (uint32_t)(v - v0);
+					if (i >= (uint32_t)n) return;
+					atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
+					name(i);
+				};
+				// (ids of any alignment: single ones up to the first 16-byte word, then words)
 				const int head = min(w.n_history, (int)((4 - (((uintptr_t)w.history >> 2) & 3)) & 3)), whole = (w.n_history - head) >> 2;
 				if (t < head) seen(w.history[t]);
 				const int4* ids = (const int4*)(w.history + head);
 				for (int i0 = t; i0 < whole; i0 += 4 * kPickThreads) {
-					int4 id[4];
+					int4 x[4];
 #pragma unroll
-					for (int u = 0; u < 4; ++u) id[u] = i0 + u * kPickThreads < whole ? ids[i0 + u * kPickThreads] : make_int4(-1, -1, -1, -1);
+					for (int u = 0; u < 4; ++u) x[u] = i0 + u * kPickThreads < whole ? ids[i0 + u * kPickThreads] : make_int4(-1, -1, -1, -1);
 #pragma unroll 1
 					for (int u = 0; u < 4; ++u) {
-						seen(id[0].x);
-						seen(id[0].y);
-						seen(id[0].z);
-						seen(id[0].w);
-						id[0] = id[1];
-						id[1] = id[2];
-						id[2] = id[3];
+						seen(x[0].x);
+						seen(x[0].y);
+						seen(x[0].z);
+						seen(x[0].w);
+						x[0] = x[1];
+						x[1] = x[2];
+						x[2] = x[3];
 					}
 				}
 				const int tail = head + 4 * whole + t;
 				if (tail < w.n_history) seen(w.history[tail]);
-			}
-			if (t == 0 && w.extra >= 0) seen(w.extra);
-			for (int i = t; i < w.n_bias; i += kPickThreads) {
-				const int v = w.bias_tokens[i];
-				const uint32_t at = (uint32_t)(v - v0);
-				if (at >= (uint32_t)n) continue;
-				atomicAdd(&bsum[enter(v)], (unsigned long long)(long long)w.bias_values[i]);
-				if constexpr (TABLE) {
-					if (bits_of(at) == 0u) atomicOr(&named[at >> 5], 1u << (at & 31));
-				} else {
-					name(at);
+				if (t == 0 && w.extra >= 0) seen(w.extra);
+				for (int i = t; i < w.n_bias; i += kPickThreads) {
+					const int v = w.bias_tokens[i];
+					if ((uint32_t)(v - v0) >= (uint32_t)n) continue;
+					bool new_to_it;
+					atomicAdd(&bsum[enter(v, &new_to_it)], (unsigned long long)(long long)w.bias_values[i]);
+					name((uint32_t)(v - v0));
 				}
-			}
-			__syncthreads();
-			// ---- the named tokens
-			const double inv_theta = 1.0 / (double)w.theta;
-#pragma unroll 2
-			for (int k = t; k < (TABLE ? a.hash : s_listed); k += kPickThreads) {
-				const int v = TABLE ? bkey[k] : v0 + list[k], i = v - v0;
-				if (TABLE && v < 0) continue;
-				int32_t y = logits[v];
-				if (y != INT32_MIN) {
-					long long z = y;
-					const uint32_t cnt = TABLE ? counts[k] : counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
-					if (cnt != 0u) {
-						if (z > 0) {      // floor(2^15 z / theta): a quotient in doubles, off by one at most, settled by its remainder
-							const long long num = z << 15;
-							long long q = (long long)((double)num * inv_theta);
-							const long long rem = num - q * (long long)w.theta;
-							z = q + (rem >= (long long)w.theta ? 1 : 0) - (rem < 0 ? 1 : 0);
-						} else {
-							z = -((-z * (long long)w.theta) >> 15);
-						}
-						z -= (long long)w.presence + (long long)w.frequency * (long long)cnt;
-					}
-					if (TABLE) {
-						if (a.sums) z += (long long)bsum[k];
-					} else if (w.n_bias > 0) {
-						uint32_t h = place(v);
-						while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
-						if (bkey[h] == v) z += (long long)bsum[h];
-					}
-					y = (int32_t)max(-2147483647ll, min(2147483647ll, z));
+				__syncthreads();
+				// the list of named tokens, from the bits: a thread's words, the warps' shares, a place each
+				int have = 0;
+				for (int i = t; i < words; i += kPickThreads) have += __popc(named[i]);
+				int upto = have;
+#pragma unroll
+				for (int o = 1; o < 32; o *= 2) {
+					const int y = __shfl_up_sync(0xffffffffu, upto, o);
+					if (lane >= o) upto += y;
 				}
-				if ((allow[i >> 5] >> (i & 31) & 1u) == 0u) y = INT32_MIN;
-				key = max(key, pick_key(y, v));
-				if (OUT) out[v] = y;
+				if (lane == 31) s_part[warp] = upto;
+				__syncthreads();
+				int to = upto - have;
+				for (int i = 0; i < warp; ++i) to += s_part[i];
+				if (t == kPickThreads - 1) s_listed = to + have;
+				for (int i = t; i < words; i += kPickThreads)
+					for (uint32_t bits = named[i]; bits != 0u; bits &= bits - 1u) list[to++] = (uint16_t)(32 * i + __ffs(bits) - 1);
 			}
 		}
 		__syncthreads();
-		// ---- all others
-		auto one = [&](int v) {
+		// ---- the tokens that nothing names
+		auto single = [&](int v) {
 			const int i = v - v0;
-			if ((named[i >> 5] >> (i & 31) & 1u) != 0u) return;
-			const int32_t y = (allow[i >> 5] >> (i & 31) & 1u) != 0u ? logits[v] : INT32_MIN;
+			const bool use = (dense[i >> 5] >> (i & 31) & 1u) != 0u;
+			const int32_t y = use ? logits[v] : INT32_MIN;
 			key = max(key, pick_key(y, v));
-			if (OUT) out[v] = y;
+			if constexpr (OUT) {
+				if ((named[i >> 5] >> (i & 31) & 1u) == 0u) out[v] = y;
+			}
 		};
-		if (t < first - v0) one(v0 + t);
-		if (t < v1 - last) one(last + t);
-		if (listed) {      // (from here on the words' own tokens only)
-			__syncthreads();
-			for (int i = t; i < words; i += kPickThreads) allow[i] &= ~named[i];
-			__syncthreads();
-		}
+		if (t < first - v0) single(v0 + t);
+		if (t < v1 - last) single(last + t);
 		// a thread has every 512th word: their bits lie at one place of their bitmap words
-		constexpr int kStride = 4 * kPickThreads;
 		const int bit = (first - v0 + 4 * t) & 31, word = (first - v0 + 4 * t) >> 5;
 		const bool straddles = bit > 28;
 		auto nibble = [&](const uint32_t* map, int k) {
@@ -342,20 +363,20 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		const int total = (last - first) / 4;
 #pragma unroll 1
 		for (int i = 0; i < chunks; ++i) {
-			const uint32_t at = (seq + (uint32_t)i) % (uint32_t)a.stages, turn = (seq + (uint32_t)i) / (uint32_t)a.stages;
-			if (s_late == 0 && !ring_wait(cta_addr(&s_full[at]), turn & 1u)) s_late = 1;      // (what is read then does not count)
+			const uint32_t slot = (seq + (uint32_t)i) % (uint32_t)a.stages, turn = (seq + (uint32_t)i) / (uint32_t)a.stages;
+			if (s_late == 0 && !ring_wait(cta_addr(&s_full[slot]), turn & 1u)) s_late = 1;      // (what is read then does not count)
 #pragma unroll
 			for (int u = 0; u < kPickChunk / kPickThreads; ++u) {
 				const int k = i * (kPickChunk / kPickThreads) + u;
 				if (k * kPickThreads + t >= total) break;
 				int32_t y[4];
-				words_of(ring[at * kPickChunk + u * kPickThreads + t], nibble(allow, k), y);
+				words_of(ring[slot * kPickChunk + u * kPickThreads + t], nibble(dense, k), y);
 				const int32_t m = max(max(y[0], y[1]), max(y[2], y[3]));
 				if (m > top) {
 					top = m;
 					top_at = k;
 				}
-				if (OUT) {
+				if constexpr (OUT) {
 					const uint32_t nm = listed ? nibble(named, k) : 0u;
 					int32_t* to = out + first + 4 * t + k * kStride;
 					if (mis_out == mis && nm == 0u) {
@@ -372,9 +393,60 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		}
 		if (top != INT32_MIN) {      // (in place, the word reads as it was but for what the bitmaps leave out)
 			int32_t y[4];
-			words_of(*(const int4*)(logits + first + 4 * t + top_at * kStride), nibble(allow, top_at), y);
+			words_of(*(const int4*)(logits + first + 4 * t + top_at * kStride), nibble(dense, top_at), y);
 			const int j = y[0] == top ? 0 : (y[1] == top ? 1 : (y[2] == top ? 2 : 3));
 			key = max(key, pick_key(top, first + 4 * t + top_at * kStride + j));
+		}
+		// ---- the named tokens: (in place, they read as they were)
+		if (listed) {
+			const double inv_theta = 1.0 / (double)w.theta;
+			auto change = [&](int v, int32_t y, uint32_t cnt, long long sum) {      // its logit, its occurrences, what the biases add
+				if (y != INT32_MIN) {
+					long long z = y;
+					if (cnt != 0u) {
+						if (z > 0) {      // floor(2^15 z / theta): a quotient in doubles, off by one at most, settled by its remainder
+							const long long num = z << 15;
+							const long long q = (long long)((double)num * inv_theta), rem = num - q * (long long)w.theta;
+							z = q + (rem >= (long long)w.theta ? 1 : 0) - (rem < 0 ? 1 : 0);
+						} else {
+							z = -((-z * (long long)w.theta) >> 15);
+						}
+						z -= (long long)w.presence + (long long)w.frequency * (long long)cnt;
+					}
+					y = (int32_t)max(-2147483647ll, min(2147483647ll, z + sum));
+				}
+				if (w.mask != nullptr && (w.mask[v >> 3] >> (v & 7) & 1) == 0) y = INT32_MIN;
+				key = max(key, pick_key(y, v));
+				if constexpr (OUT) out[v] = y;
+			};
+			if constexpr (TABLE) {
+				int32_t raw[IN];
+#pragma unroll
+				for (int u = 0; u < IN; ++u) raw[u] = at[u] >= 0 ? logits[id[u]] : INT32_MIN;
+#pragma unroll
+				for (int u = 0; u < IN; ++u)
+					if (at[u] >= 0) change(id[u], raw[u], counts[at[u]], a.sums ? (long long)bsum[at[u]] : 0ll);
+			} else {
+				for (int k0 = t; k0 < s_listed; k0 += 4 * kPickThreads) {
+					int32_t y[4];
+#pragma unroll
+					for (int u = 0; u < 4; ++u) y[u] = k0 + u * kPickThreads < s_listed ? logits[v0 + list[k0 + u * kPickThreads]] : INT32_MIN;
+#pragma unroll 1
+					for (int k = k0; k < min(s_listed, k0 + 4 * kPickThreads); k += kPickThreads) {
+						const int i = list[k], v = v0 + i;
+						long long sum = 0;
+						if (w.n_bias > 0) {
+							uint32_t h = place(v);
+							while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
+							if (bkey[h] == v) sum = (long long)bsum[h];
+						}
+						change(v, y[0], counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, sum);
+						y[0] = y[1];
+						y[1] = y[2];
+						y[2] = y[3];
+					}
+				}
+			}
 		}
 		__syncthreads();      // the tables may be overwritten
 		seq += (uint32_t)chunks;
@@ -446,7 +518,7 @@ bool pick_plan(int names, int biases, PickArgs* a) {
 		while (3 * a->hash < 4 * kept) a->hash *= 2;
 	}
 	// logits on their way: what a pass has, four chunks at most, two where that lets two blocks share a multiprocessor
-	const size_t half = 112 * 1024, kept_bytes = PickSmem::bytes(table, 0, a->sums, a->pass, a->hash, a->list), chunk = kPickChunk * 16;
+	const size_t half = 112 * 1024, kept_bytes = PickSmem::bytes(table, a->out_logits != nullptr, 0, a->sums, a->pass, a->hash, a->list), chunk = kPickChunk * 16;
 	a->stages = std::max(1, std::min(kPickStages, (a->pass / 4 + kPickChunk - 1) / kPickChunk));
 	while (a->stages > 2 && kept_bytes + a->stages * chunk > half && kept_bytes + 2 * chunk <= half) --a->stages;
 	return table;
@@ -457,7 +529,7 @@ cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 	static PerDeviceOnce once;
 	const auto kernel = k_pick<RESIDENT, TABLE, OUT>;
 	cudaError_t e = once_per_device(once, [&] {
-		const size_t most = TABLE ? PickSmem::bytes(true, kPickStages, 1, kPickBits, 4096, 0) : PickSmem::bytes(false, kPickStages, 1, kPickPass, 2 * kPickMaxBias, kPickPass);
+		const size_t most = TABLE ? PickSmem::bytes(true, true, kPickStages, 1, kPickBits, 4096, 0) : PickSmem::bytes(false, true, kPickStages, 1, kPickPass, 2 * kPickMaxBias, kPickPass);
 		const cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 		return x != cudaSuccess ? x : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
 	});
@@ -466,7 +538,7 @@ cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3(1u << a.shift, a.rows);
 	cfg.blockDim = dim3(kPickThreads);
-	cfg.dynamicSmemBytes = PickSmem::bytes(TABLE, a.stages, a.sums, a.pass, a.hash, a.list);
+	cfg.dynamicSmemBytes = PickSmem::bytes(TABLE, OUT, a.stages, a.sums, a.pass, a.hash, a.list);
 	cfg.stream = st;
 	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
