@@ -254,6 +254,12 @@ SSLM_API sslm_status sslm_b200_tc_variant_counts(uint64_t* counts, int32_t n);
  * Results do not depend on it. For tuning and for tests that walk every cut. */
 SSLM_API sslm_status sslm_b200_set_attention_splits(int32_t splits);
 
+/* Decode rows whose sequences adopted the same frozen prefix are attended together, the prefix's K and V read and
+ * multiplied once for all of them. mode 1 (the default): where that is faster; 0: never; 2: wherever two rows of a call share
+ * a whole page. Results do not depend on it. For tuning and for tests; the second verb counts the launches so far. */
+SSLM_API sslm_status sslm_b200_set_prefix_attention(int32_t mode);
+SSLM_API uint64_t sslm_b200_prefix_attention_launches(void);
+
 /* Bisection aid (the counterpart of the reference's per-site trace hook,
  * src/forward/checked_chain_funnel.cpp:338-361). With a buffer set, every later sslm_prefill /
  * sslm_decode_step on this workspace appends one record per traced site, layer and row:
@@ -324,6 +330,26 @@ SSLM_API sslm_status sslm_b200_profile_read(sslm_workspace ws, double* ms, uint6
  * sslm_decode_step calls on `ws` into host memory ([tokens in call order][vocab]);
  * pass NULL to stop. */
 SSLM_API sslm_status sslm_b200_capture_logits(sslm_workspace ws, int32_t* host_rows);
+
+/* Penalties for repeated tokens and biases of a sequence's picks. From this call on sslm_decode_step chooses the sequence's
+ * tokens from its logit row as sslm_b200_pick_resident (below) changes it: the history is the tokens the sequence has
+ * produced, and with count_given those it was given as well (prompts and an adopted prefix), since it was created, reset or
+ * restored. A bound schema's mask applies as before, and where it allows nothing the step answers as before. Other sequences of a
+ * call are chosen for as ever, and a save blob has nothing of this: a restored sequence has no controls and an empty history.
+ * NULL takes the controls away; a second call replaces them; sslm_seq_reset leaves them attached and empties the history.
+ * repetition below 1, more than 1,024 biases, or a missing list: SSLM_INVALID_ARGUMENT; a bias token outside the vocabulary:
+ * SSLM_TOKEN_ID_OUT_OF_RANGE; nothing changes then. The first decode call of a workspace that has such a sequence allocates room
+ * for its logit rows. */
+typedef struct sslm_b200_controls {
+	uint32_t struct_size;
+	int32_t repetition;              /* Q15: 32,768 is 1.0 */
+	int32_t presence, frequency;     /* logit units */
+	int32_t count_given;
+	int32_t n_bias;
+	const int32_t* bias_tokens;
+	const int32_t* bias_values;
+} sslm_b200_controls;
+SSLM_API sslm_status sslm_b200_seq_set_controls(sslm_seq seq, const sslm_b200_controls* controls);
 
 /* Bytes of HBM held by the model's weights, tables and constants. */
 SSLM_API size_t sslm_b200_model_device_bytes(sslm_model model);

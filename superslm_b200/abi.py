@@ -47,6 +47,11 @@ class SslmDecodeParams(C.Structure):
                 ("q_ln2", C.c_int64), ("q_b", C.c_int64), ("q_c", C.c_int64)]
 
 
+class SslmControls(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("repetition", C.c_int32), ("presence", C.c_int32), ("frequency", C.c_int32),
+                ("count_given", C.c_int32), ("n_bias", C.c_int32), ("bias_tokens", C.POINTER(C.c_int32)), ("bias_values", C.POINTER(C.c_int32))]
+
+
 _H = C.c_void_p  # opaque handle
 
 
@@ -248,6 +253,20 @@ class Sequence:
 
     def set_adapter(self, adapter_handle):
         _chk("sslm_seq_set_adapter", self.eng.lib.sslm_seq_set_adapter(self.handle, adapter_handle))
+
+    def set_controls(self, repetition=32768, presence=0, frequency=0, count_given=False, biases=()):
+        """sslm_b200_seq_set_controls: penalties for repeated tokens (repetition in Q15, the others in logit units) and biases, pairs of
+        (token, value); repetition=None takes them away."""
+        fn = self.eng.lib.dll.sslm_b200_seq_set_controls
+        fn.restype, fn.argtypes = C.c_int, [_H, C.c_void_p]
+        if repetition is None:
+            _chk("sslm_b200_seq_set_controls", fn(self.handle, None))
+            return
+        biases = list(biases)
+        tokens, values = ((C.c_int32 * len(biases))(*[b[i] for b in biases]) for i in range(2))
+        c = SslmControls(C.sizeof(SslmControls), repetition, presence, frequency, int(count_given), len(biases),
+                         C.cast(tokens, C.POINTER(C.c_int32)), C.cast(values, C.POINTER(C.c_int32)))
+        _chk("sslm_b200_seq_set_controls", fn(self.handle, C.addressof(c)))
 
     def save(self) -> bytes:
         n = C.c_size_t(0)

@@ -37,6 +37,9 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // one hidden-state slot of a sequence: codes, then the carried scale
 size_t seq_scale_offset(const Dims& d) { return align_up(d.hidden, 16); }
 size_t seq_state_stride(const Dims& d) { return align_up(seq_scale_offset(d) + sizeof(Scale), 256); }
+// ids that count as repeated (every position holds one token, and one more has been produced), and biases with their tokens
+size_t seq_history_bytes(const Dims& d) { return align_up(((size_t)d.context_cap + 16) * 4, 256); }
+size_t seq_control_bytes(const Dims& d) { return seq_history_bytes(d) + (size_t)kPickMaxBias * 8; }
 
 sslm_status map_forward_status(int32_t st) {
 	// MapForwardStatus, src/sslm_abi.cpp:1352-1370
@@ -352,7 +355,7 @@ extern "C" sslm_status sslm_kv_pool_create(sslm_model model, void* buf, size_t b
 	p->pages_per_block = (d.context_cap + kPageTokens - 1) / kPageTokens;
 	p->dev.num_pages = (int64_t)p->pages_per_block * block_count;
 	const size_t bytes = (size_t)d.layers * d.kv_heads * 2 * p->dev.num_pages * kPageTokens * d.head_dim;
-	p->seq_stride = 2 * seq_state_stride(d) + align_up((size_t)p->pages_per_block * 4, 256);
+	p->seq_stride = 2 * seq_state_stride(d) + align_up((size_t)p->pages_per_block * 4, 256) + seq_control_bytes(d);
 	const size_t kv_bytes = align_up(bytes, 256);
 	if (!cuda_ok(cudaMalloc((void**)&p->dev.base, kv_bytes + p->seq_stride * block_count))) {
 		delete p;
@@ -393,7 +396,7 @@ bool config_ok(const sslm_model_s* model, const sslm_config* c) {
 	return c->reserved == 0;
 }
 
-constexpr size_t kUpBytesPerRow = sizeof(RowDesc) + sizeof(RowSource) + sizeof(RowSink) + sizeof(void*);
+constexpr size_t kUpBytesPerRow = sizeof(RowDesc) + sizeof(RowSource) + sizeof(RowSink) + 4 * sizeof(int32_t) + sizeof(void*) + sizeof(PickRow);
 constexpr size_t kDownBytesPerRow = 8 + 8 + 4 + 4;      // arg-max key, saturations, status, finished layers
 
 // Lay the upload and read-back blocks out for a call of n rows.
@@ -407,7 +410,9 @@ void bind_rows(sslm_workspace_s* w, int n) {
 	up(w->h_rows, w->d_rows, n * sizeof(RowDesc));
 	up(w->h_src, w->d_src, n * sizeof(RowSource));
 	up(w->h_sink, w->d_sink, n * sizeof(RowSink));
+	up(w->h_group, w->d_group, n * 4 * sizeof(int32_t));
 	up(w->h_row_mask, w->d_row_mask, n * sizeof(void*));
+	up(w->h_pick, w->d_pick, n * sizeof(PickRow));
 	w->h_best = (unsigned long long*)w->h_down;
 	w->h_sat = w->h_best + n;
 	w->h_status = (int32_t*)(w->h_sat + n);
@@ -494,6 +499,7 @@ static void destroy_workspace(sslm_workspace_s* w) {
 	cudaFree(w->d_scratch);
 	cudaFree(w->d_tc_partial);
 	cudaFree(w->d_tc_counters);
+	cudaFree(w->d_pick_logits);
 	cudaFree(w->d_up);
 	cudaFree(w->d_down);
 	cudaFreeHost(w->h_up);
@@ -610,6 +616,14 @@ extern "C" sslm_status sslm_b200_set_attention_splits(int32_t splits) {
 	attn_force_splits(splits);
 	return SSLM_OK;
 }
+
+extern "C" sslm_status sslm_b200_set_prefix_attention(int32_t mode) {
+	if (mode < 0 || mode > 2) return SSLM_INVALID_ARGUMENT;
+	g_prefix_mode.store(mode);
+	return SSLM_OK;
+}
+
+extern "C" uint64_t sslm_b200_prefix_attention_launches(void) { return g_prefix_launches.load(); }
 
 extern "C" sslm_status sslm_b200_profile(sslm_workspace ws, int32_t enable) {
 	if (!ws) return SSLM_INVALID_ARGUMENT;

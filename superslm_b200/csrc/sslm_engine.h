@@ -47,6 +47,8 @@ struct sslm_workspace_s {
 	sslm::RowSink *h_sink = nullptr, *d_sink = nullptr;
 	// head rows of constrained sequences: the mask page of the row's DFA state (else nullptr)
 	const uint8_t **h_row_mask = nullptr, **d_row_mask = nullptr;
+	// of a decode call, per row: first rows of the groups that share a prefix (two places a row), shared positions (two places a row)
+	int32_t *h_group = nullptr, *d_group = nullptr;
 	unsigned long long *h_best = nullptr, *h_sat = nullptr;
 	int32_t *h_status = nullptr, *h_done = nullptr;
 	// carved row buffers (base pointers for row 0)
@@ -59,6 +61,10 @@ struct sslm_workspace_s {
 	unsigned int* d_tc_counters = nullptr;
 	int32_t* logit_capture = nullptr;   // host buffer for full logit rows (tests), or nullptr
 	int32_t* d_logits = nullptr;
+	// full logit rows of a decode call in which some sequence has controls, allocated by the first such call; records of their picks
+	int32_t* d_pick_logits = nullptr;
+	size_t pick_rows = 0;
+	sslm::PickRow *h_pick = nullptr, *d_pick = nullptr;
 	cudaEvent_t ev[2][2] = {};    // start and end: of the call at hand [ev_now] and of the last completed one [ev_now ^ 1]
 	int ev_now = 0;
 	float last_ms = 0.f;
@@ -170,6 +176,17 @@ struct sslm_seq_s {
 	int32_t* d_pages = nullptr;     // device page table, pages_per_block entries
 	size_t pages_on_device = 0;     // entries of it that are in place
 	uint64_t batch_mark = 0;        // the decode batch the sequence was last put into
+	uint64_t uid = 0;               // of the sequences created so far
+	// the first pages are those of the frozen prefix with this uid (0: none): sequences of one prefix have the same ones
+	// tokens the sequence was given and tokens it produced, in order (since it was created, reset or restored)
+	std::vector<int32_t> given, produced;
+	// penalties and biases of its picks (sslm_b200_seq_set_controls); their ids and the biases lie in the sequence's slot of the pool
+	bool controlled = false, count_given = false;
+	int32_t theta = 0, presence = 0, frequency = 0, n_bias = 0;
+	int32_t *d_history = nullptr, *d_bias = nullptr;
+	size_t given_on_device = 0, produced_on_device = 0;      // ids that count and are in d_history (given ones before later produced ones or behind)
+	uint64_t shared_uid = 0;
+	int32_t shared_pages = 0;
 	int64_t context_length = 0;
 	uint32_t layer_index = 0;
 	int32_t current_token = -1;

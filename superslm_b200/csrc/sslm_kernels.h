@@ -201,6 +201,11 @@ void tc_variant_counts(unsigned long long* counts, int n);
 void launch_lora_u(const RowBatch& b, const int8_t* x, int k_in, int layer, int nproj,
                    const int* lora_slots, cudaStream_t st);
 
+// ---- the pick of rows whose sequences carry controls (sslm_pick.cu)
+constexpr int kPickMaxBias = 1024;      // biases of a row
+// best[r] of the rows whose record has logits; names: ids that a row's history, its extra one and its biases have at most, biases of them
+cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* status, cudaStream_t st);
+
 // ---- attention over the paged KV pool (sslm_attn.cu)
 cudaError_t attn_configure(const Dims& d);
 // slices per kv head of later attention launches (0: chosen per launch); for tuning and tests
@@ -218,6 +223,22 @@ AttnChoice attn_choose(const Dims& d, const LayerDev& h, int m, int max_width, i
 bool launch_attention(const RowBatch& b, const Dims& d, const LayerDev& layer, int layer_index,
                       KvPoolDev pool, int max_width, int reverse_rows, const AttnChoice& choice, const int32_t* cos, const int32_t* sin,
                       cudaStream_t st, cudaError_t* err);
+// ---- attention of decode rows that share a prefix's pages (sslm_prefix_attn.cu): the first of a batch's rows, group by group.
+// How the launches of a call are cut, decided once per call.
+struct PrefixPlan {
+	int rows;                // query rows per tile: 16 or 32
+	int tq, tiles, sub, ppages, spages, vgroups;
+	size_t smem;
+	int groups, max_suffix;  // of the call
+};
+bool prefix_attention_plan(const Dims& d, int rows, int groups, int max_prefix, int max_suffix, PrefixPlan* out);
+// rows [0, group_start[groups]) of the batch; device arrays: first row of each group, and positions each group shares (whole
+// pages, the same in all its rows' tables). launch_ctx_funnel must follow.
+cudaError_t launch_attention_prefix(const RowBatch& b, const Dims& d, const LayerDev& layer, int layer_index, KvPoolDev pool, const PrefixPlan& plan,
+                                    const int32_t* group_start, const int32_t* prefix_len, cudaStream_t st);
+// 0: never, 1: where it is the better of the two, 2: wherever two rows share a page; and the launches so far
+inline std::atomic<int> g_prefix_mode{1};
+inline std::atomic<uint64_t> g_prefix_launches{0};
 // gather `planes` planes of a sequence's pages, from plane0 on, into the reference's canonical block layout
 // [layer][K|V][kv_head][position][head_dim] with `span` positions per plane; positions beyond
 // `valid(layer)` are zero

@@ -31,7 +31,6 @@ constexpr int kPickThreads = 512;
 constexpr int kPickPass = 24576;            // tokens whose counts a block holds at a time (a multiple of 32)
 constexpr int kPickBits = 262144;           // and tokens whose bits it holds at a time, where the counts lie in a table
 constexpr int kPickMaxHistory = 65535;      // (a count is 16 bits)
-constexpr int kPickMaxBias = 1024;
 constexpr int kPickTable = 3072;            // names of a row that the table takes
 constexpr int kPickChunk = 1024, kPickStages = 4;      // words of four logits that arrive at once, and places for them
 
@@ -553,6 +552,15 @@ cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 }
 
 }  // namespace
+
+cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* status, cudaStream_t st) {
+	PickArgs a{};
+	a.rows = m; a.vocab = vocab;
+	a.desc = rows; a.best = best; a.status = status;
+	const bool table = pick_plan(names, biases, &a);
+	return table ? pick_launch<false, true, false>(a, st) : pick_launch<false, false, false>(a, st);
+}
+
 }  // namespace sslm
 
 using namespace sslm;

@@ -775,11 +775,6 @@ __global__ void __launch_bounds__(256) k_prefix_codes(const int32_t* out, int64_
 
 namespace {
 
-struct PrefixPlan {
-	int rows;        // query rows per tile: 16 or 32
-	int tq, tiles, sub, ppages, spages, vgroups;
-	size_t smem;
-};
 constexpr size_t kPfxSmemMax = 216 * 1024;      // (beside 9 KB of fixed arrays)
 constexpr int kPfxMaxSub = 16;
 
@@ -910,6 +905,33 @@ cudaError_t prefix_dispatch(PrefixArgs a, int hd, const PrefixPlan& p, cudaStrea
 }
 
 }  // namespace
+
+bool prefix_attention_plan(const Dims& d, int rows, int groups, int max_prefix, int max_suffix, PrefixPlan* out) {
+	if (prefix_plan<false>(d.head_dim, d.heads / d.kv_heads, d.kv_heads, rows, groups, max_prefix, max_suffix, attn_forced_splits(), out) != cudaSuccess) {
+		cudaGetLastError();
+		return false;
+	}
+	out->groups = groups;
+	out->max_suffix = max_suffix;
+	return true;
+}
+
+cudaError_t launch_attention_prefix(const RowBatch& b, const Dims& d, const LayerDev& layer, int layer_index, KvPoolDev pool, const PrefixPlan& plan,
+                                    const int32_t* group_start, const int32_t* prefix_len, cudaStream_t st) {
+	PrefixArgs a{};
+	a.rows = b.m; a.groups = plan.groups; a.G = d.heads / d.kv_heads; a.kv_heads = d.kv_heads;
+	a.max_suffix = plan.max_suffix;
+	a.q = b.qrot; a.q_stride = d.hidden;
+	a.kv = pool.base + kv_plane_offset(d, pool, layer_index, 0, 0); a.num_pages = pool.num_pages;
+	a.group_start = group_start; a.prefix_len = prefix_len;
+	a.desc = b.rows; a.smc = b.smc; a.rowmax = b.rowmax; a.layer = b.layer;
+	a.fold = layer.f_ctx;
+	a.out = b.ctxw; a.out_stride = d.hidden;
+	a.status = b.status;
+	g_prefix_launches.fetch_add(1, std::memory_order_relaxed);
+	return prefix_dispatch<false>(a, d.head_dim, plan, st);
+}
+
 }  // namespace sslm
 
 using namespace sslm;
