@@ -459,11 +459,9 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	for (int i = t; i < ROWS * L::kSumStride; i += kPfxThreads) ctx[i] = 0;      // (the q rows are read)
 	// (V that is not staged: into L2 during the softmax)
 	const int pgroups = np4 >> 2, groups = pgroups + (ns4 >> 2);
-	constexpr int kLines = kPageTokens * HD / 128;
-	for (int i = t + 4 * a.vgroups * kLines; i < 4 * groups * kLines; i += kPfxThreads) {
-		const int at = i / kLines;
-		const int64_t base = at < np4 ? pbase[at] : sbase[at - np4];
-		if (base >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(vplane + base + i % kLines * 128));
+	for (int i = 4 * a.vgroups + t; i < 4 * groups; i += kPfxThreads) {
+		const int64_t base = i < np4 ? pbase[i] : sbase[i - np4];
+		if (base >= 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(vplane + base), "r"((uint32_t)page_bytes) : "memory");
 	}
 	__syncthreads();
 	if (sub > 1) {
@@ -623,44 +621,46 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	}
 	__syncthreads();      // everybody's probabilities are there
 
-	// ---- pass 4: P.V. A warp has 16 channels of all rows and every KW-th group of four pages: the planes are read once per 16 channels
-	// (once per 8, a tile per warp, those reads were the bound; per 32 adding up the warps' shares costs more). Lane column c owns
+	// ---- pass 4: P.V. A warp has 16 channels of 32 rows, or 32 of 16, and every KW-th group of four pages: the planes are read once per
+	// so many channels (once per 8, a tile per warp, those reads were the bound; per 32 of 32 rows adding up the warps' shares costs more). Lane column c owns
 	// page 4 x + c of a group: its 16-byte row of the V page feeds two MMAs (positions 0..7 and 8..15), the row's planes
 	// the A side of both.
 	ok = ring_wait(cta_addr(&s_bars[0]), 0) && ok;
 	{
-		constexpr int CW = HD / 16, KW = W / CW;
-		const int ch0 = (warp % CW) * 16, part = warp / CW;
-		int acc[RB][2][2][4];      // [row block][8-channel tile][plane]
+		constexpr int NT = 4 / RB, CW = HD / (8 * NT), KW = W / CW;      // 8-channel tiles of a warp; warps along channels and pages
+		const int ch0 = (warp % CW) * 8 * NT, part = warp / CW;
+		int acc[RB][NT][2][4];      // [row block][8-channel tile][plane]
 #pragma unroll
 		for (int b = 0; b < RB; ++b)
 #pragma unroll
-			for (int n = 0; n < 2; ++n)
+			for (int n = 0; n < NT; ++n)
 #pragma unroll
 				for (int x = 0; x < 4; ++x) acc[b][n][0][x] = acc[b][n][1][x] = 0;
-		int4 vn[2];
+		int4 vn[NT];
 		const unsigned char* vsm = vst + (size_t)c * L::kVPage + (ch0 + g) * kPageTokens;
 		auto fetch = [&](int x) {
 			if (x < a.vgroups) {
 #pragma unroll
-				for (int n = 0; n < 2; ++n) vn[n] = *(const int4*)(vsm + (size_t)x * 4 * L::kVPage + n * 8 * kPageTokens);
+				for (int n = 0; n < NT; ++n) vn[n] = *(const int4*)(vsm + (size_t)x * 4 * L::kVPage + n * 8 * kPageTokens);
 			} else {
 				const int64_t base = x < pgroups ? pbase[4 * x + c] : sbase[4 * (x - pgroups) + c];
 #pragma unroll
-				for (int n = 0; n < 2; ++n) vn[n] = base >= 0 ? load16(vplane + base + (ch0 + n * 8 + g) * kPageTokens) : make_int4(0, 0, 0, 0);
+				for (int n = 0; n < NT; ++n) vn[n] = base >= 0 ? load16(vplane + base + (ch0 + n * 8 + g) * kPageTokens) : make_int4(0, 0, 0, 0);
 			}
 		};
-		auto multiply = [&](int b, int pl, const int4& w0, const int4& w1, const int4 (&v)[2]) {
+		auto multiply = [&](int b, int pl, const int4& w0, const int4& w1, const int4 (&v)[NT]) {
 #pragma unroll
-			for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w0.x, w1.x, w0.y, w1.y, v[n].x, v[n].y);
+			for (int n = 0; n < NT; ++n) mma_u8s8_full(acc[b][n][pl], w0.x, w1.x, w0.y, w1.y, v[n].x, v[n].y);
 #pragma unroll
-			for (int n = 0; n < 2; ++n) mma_u8s8_full(acc[b][n][pl], w0.z, w1.z, w0.w, w1.w, v[n].z, v[n].w);
+			for (int n = 0; n < NT; ++n) mma_u8s8_full(acc[b][n][pl], w0.z, w1.z, w0.w, w1.w, v[n].z, v[n].w);
 		};
 		if (part < groups) fetch(part);
 		int x = part;
 #pragma unroll 1
 		for (; x < pgroups; x += KW) {      // of the prefix
-			const int4 v[2] = {vn[0], vn[1]};
+			int4 v[NT];
+#pragma unroll
+			for (int n = 0; n < NT; ++n) v[n] = vn[n];
 			if (x + KW < groups) fetch(x + KW);
 			const unsigned char* at = sc + (4 * x + c) * kPageScores + g * 64;
 #pragma unroll
@@ -671,7 +671,9 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		}
 #pragma unroll 1
 		for (; x < groups; x += KW) {      // of the suffixes: a page has planes of its owner's G rows, the others' are zero
-			const int4 v[2] = {vn[0], vn[1]};
+			int4 v[NT];
+#pragma unroll
+			for (int n = 0; n < NT; ++n) v[n] = vn[n];
 			if (x + KW < groups) fetch(x + KW);
 			const int page = 4 * (x - pgroups) + c, first = (sown[page] & 255) * G;
 			const unsigned char* at = csc + page * csc_page;
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 #pragma unroll
 			for (int b = 0; b < RB; ++b)
 #pragma unroll
-				for (int n = 0; n < 2; ++n)
+				for (int n = 0; n < NT; ++n)
 #pragma unroll
 					for (int x = 0; x < 4; ++x)
 						atomicAdd(&ctx[(16 * b + 8 * (x >> 1) + g) * L::kSumStride + ch0 + n * 8 + 2 * c + (x & 1)], acc[b][n][0][x] + 256 * acc[b][n][1][x]);
