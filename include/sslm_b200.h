@@ -410,7 +410,7 @@ SSLM_API sslm_status sslm_b200_linear_resident(const int8_t* d_x, const int8_t* 
 typedef struct sslm_b200_prefix_attention {
 	uint32_t struct_size;
 	int32_t rows, groups, heads, kv_heads, head_dim;
-	int32_t max_prefix, max_suffix;   /* no length is above these; the launch is sized by them */
+	int32_t max_prefix, max_suffix;   /* no length is above these (each at most 32,768); the launch is sized by them */
 	const int8_t* q;                  /* [rows][heads][head_dim] rotated codes */
 	int64_t q_stride;                 /* elements between rows, as every stride here */
 	const int64_t* consts;            /* [rows][kv_heads][3] q_ln2, q_b, q_c */
@@ -448,7 +448,7 @@ SSLM_API sslm_status sslm_b200_attention_prefix_resident(const sslm_b200_prefix_
 typedef struct sslm_b200_pick {
 	uint32_t struct_size;
 	int32_t rows, vocab, num_masks;
-	int32_t max_history, max_bias;    /* no length is above these */
+	int32_t max_history, max_bias;    /* no length is above these; every row's lists have room for as many (all of it may be read) */
 	uint32_t reserved;
 	const int32_t* logits;            /* [rows][logits_stride] */
 	int64_t logits_stride;

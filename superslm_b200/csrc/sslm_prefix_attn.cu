@@ -792,9 +792,9 @@ size_t prefix_smem(int hd, int rows, int ppages, int spages, int group, int sub)
 // tiles of `tq` rows that `rows` rows in `groups` groups need at most
 int prefix_tiles(int rows, int groups, int tq) { return (int)std::min<int64_t>(rows, ((int64_t)rows + (int64_t)groups * (tq - 1)) / tq); }
 
-bool prefix_shape(int hd, int rows, int group, int sub, int max_prefix, int max_suffix, PrefixPlan* p) {
+bool prefix_shape(int hd, int rows, int group, int cut, int sub, int max_prefix, int max_suffix, PrefixPlan* p) {
 	p->rows = rows;
-	p->tq = rows / group;
+	p->tq = std::max(rows / group / cut, 1);
 	p->sub = sub;
 	p->ppages = (((max_prefix + kPageTokens - 1) / kPageTokens + sub - 1) / sub + 3) & ~3;
 	p->spages = ((p->tq * ((max_suffix + kPageTokens - 1) / kPageTokens) + sub - 1) / sub + 3) & ~3;
@@ -824,7 +824,7 @@ cudaLaunchConfig_t prefix_config(cudaLaunchAttribute (&attr)[2], int sub, int ti
 	return cfg;
 }
 // Once per kernel and device: its attributes, and how many clusters of each size run at once. (Clusters lie inside a GPC, whose
-// multiprocessors a size may not divide: of 148, 140 are used by clusters of five or ten, 112 by eight, 96 by sixteen.)
+// multiprocessors a size may not divide: of 148, 132 are used by clusters of four or six, 130 by five, 120 by eight, 112 by sixteen.)
 struct PrefixKernel {
 	PerDeviceOnce once;
 	int clusters[kMaxDevices][kPfxMaxSub + 1];
@@ -859,17 +859,19 @@ cudaError_t prefix_clusters(int hd, int rows, const int** clusters) {
 	return rows == 32 ? prefix_setup<32, 32, RESIDENT>(clusters) : prefix_setup<32, 16, RESIDENT>(clusters);
 }
 
-// How a call is cut: the tile height and the blocks per tile whose rounds of blocks end first.
+// How a call is cut: the tile height and the blocks per tile whose rounds of blocks end first. A block holds its share of the
+// prefix's scores and of every suffix of the tile; where both may be so long that no number of blocks has room for a full tile
+// (32,768 each: 16 rows of one head need 330 KB a block), tiles of a half or a quarter of the rows are taken, which always fit.
 template <bool RESIDENT>
 cudaError_t prefix_plan(int hd, int group, int kv_heads, int rows, int groups, int max_prefix, int max_suffix, int forced, PrefixPlan* out) {
 	float least = 0.0f;
-	for (int r : {32, 16}) {
+	for (int cut = 1; cut <= kPfxMaxSub && least == 0.0f; cut *= 2) for (int r : {32, 16}) {
 		const int* clusters = nullptr;
 		const cudaError_t e = prefix_clusters<RESIDENT>(hd, r, &clusters);
 		if (e != cudaSuccess) return e;
 		for (int sub = 1; sub <= kPfxMaxSub; ++sub) {
 			PrefixPlan p;
-			if (clusters[sub] < 1 || !prefix_shape(hd, r, group, sub, max_prefix, max_suffix, &p)) continue;
+			if (clusters[sub] < 1 || !prefix_shape(hd, r, group, cut, sub, max_prefix, max_suffix, &p)) continue;
 			p.tiles = prefix_tiles(rows, groups, p.tq);
 			const int rounds = (int)(((int64_t)p.tiles * kv_heads + clusters[sub] - 1) / clusters[sub]);
 			float cost = rounds * (8.0f + (r == 32 ? 0.28f : 0.17f) * p.ppages + 0.2f * p.spages);

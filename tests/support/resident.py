@@ -5,8 +5,9 @@ PAGE = 16
 LOWEST = -(1 << 31)
 
 
-def attention_case(seed, shape, prefix, suffix, per_group=None, deviation=40.0, consts=None, spare_pages=3):
-    """prefix: positions of each group; suffix: positions of each row; per_group: rows of each group (default: even)."""
+def attention_case(seed, shape, prefix, suffix, per_group=None, deviation=40.0, consts=None, spare_pages=3, widths=(0, 0)):
+    """prefix: positions of each group; suffix: positions of each row; per_group: rows of each group (default: even);
+    widths: pages that the tables have room for at least, those behind a length without a page (-1)."""
     heads, kv_heads, hd = shape
     g = np.random.default_rng(seed)
     rows, groups = len(suffix), len(prefix)
@@ -29,9 +30,11 @@ def attention_case(seed, shape, prefix, suffix, per_group=None, deviation=40.0, 
     fold[:, 1] = g.integers(-(1 << 31) + 1, (1 << 31) - 1, heads)
     fold[:, 2] = g.integers(0, 12, heads)
     fold[::3, 0] = 1
+    def table(ids, width):
+        return np.concatenate([ids, np.full((len(ids), max(0, width - ids.shape[1])), -1, dtype=np.int32)], axis=1)
     return dict(q=codes((rows, heads, hd)), consts=consts, kv=codes((kv_heads, 2, pages, PAGE * hd)), group_start=start,
-                prefix_len=np.asarray(prefix, dtype=np.int32), prefix_pages=order[:groups * pp].reshape(groups, pp).copy(),
-                suffix_len=np.asarray(suffix, dtype=np.int32), suffix_pages=order[groups * pp:groups * pp + rows * sp].reshape(rows, sp).copy(), fold=fold)
+                prefix_len=np.asarray(prefix, dtype=np.int32), prefix_pages=table(order[:groups * pp].reshape(groups, pp), widths[0]),
+                suffix_len=np.asarray(suffix, dtype=np.int32), suffix_pages=table(order[groups * pp:groups * pp + rows * sp].reshape(rows, sp), widths[1]), fold=fold)
 
 
 def fold64(x, identity, mult, shift):

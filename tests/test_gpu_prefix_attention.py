@@ -11,7 +11,7 @@ from tests.support.resident import attention_case, attention_rows
 pytestmark = pytest.mark.gpu
 
 SHAPES = {"0.5b": (14, 2, 64), "1.5b": (12, 2, 128), "3b": (16, 2, 128), "tiny": (4, 2, 32), "mha": (3, 3, 64), "mqa": (5, 1, 32), "wide": (8, 8, 128),
-          "g7": (7, 1, 128), "g1": (2, 2, 32), "g3": (6, 2, 64)}
+          "g7": (7, 1, 128), "g1": (2, 2, 32), "g3": (6, 2, 64), "g1w": (2, 2, 128)}
 
 
 @pytest.fixture()
@@ -85,9 +85,17 @@ def test_larger_batches(gpu_lib, torch, shape, rows, prefix, lo, hi):
 
 
 @pytest.mark.parametrize("shape,prefix,suffix", [("3b", [32768], [0, 0, 0]), ("tiny", [32700], [68, 1]), ("1.5b", [0], [32768, 5]), ("mqa", [16385], [16383, 0, 7]),
-                                                 ("g1", [0, 0], [32768] * 3)])
+                                                 ("g1", [0, 0], [32768] * 3), ("g1w", [0], [32768, 32000] + [31000] * 14), ("g1w", [16384], [16384] * 16),
+                                                 ("g3", [30000], [2768] * 11), ("0.5b", [0], [32768] * 2)])
 def test_widest_rows(gpu_lib, torch, shape, prefix, suffix):
     Call(gpu_lib, torch, attention_case(5, SHAPES[shape], prefix, suffix)).check()
+
+
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+@pytest.mark.parametrize("prefix,suffix", [([300, 0], [40, 0, 7] + [100] * 30), ([20000], [12768, 12767] + [60] * 9)])
+def test_both_maxima_at_their_limit(gpu_lib, torch, shape, prefix, suffix):
+    """page tables that hold 32,768 positions each: tiles of fewer rows, whatever the shape"""
+    Call(gpu_lib, torch, attention_case(6, SHAPES[shape], prefix, suffix, widths=(2048, 2048))).check()
 
 
 @pytest.mark.parametrize("consts", [(1, 1, 0), (1, 11_863_283, 0), ((1 << 23), (1 << 23), 0), (5, 11, (1 << 40)), (3000, 6000, 0), (1 << 20, 1 << 21, 1 << 46),
@@ -115,6 +123,34 @@ def test_rows_outside_the_groups_are_left_alone(gpu_lib, torch):
     Call(gpu_lib, torch, case).check()
     case["group_start"] = np.array([4, 4, 4], dtype=np.int32)
     Call(gpu_lib, torch, case).check(want={})
+
+
+def test_more_groups_than_a_warp_looks_at_at_once(gpu_lib, torch):
+    """groups of none, one and several rows, in tiles that lie behind 32, 64, ... groups"""
+    g = np.random.default_rng(9)
+    per = g.choice([0, 1, 2, 5, 11], 150)
+    per[[0, 31, 32, 63, 64, 149]] = [0, 7, 0, 9, 1, 3]
+    n = int(per.sum())
+    case = attention_case(9, SHAPES["tiny"], g.integers(0, 40, 150).tolist(), lengths(9, n, 0, 20), per_group=per.tolist())
+    Call(gpu_lib, torch, case).check()
+
+
+@pytest.mark.parametrize("per_group", [65535, 1])
+def test_as_many_rows_as_a_call_takes(gpu_lib, torch, per_group):
+    """65,535 rows of one group, and as many groups of a row: copies of 13 rows"""
+    n, one = 65535, attention_case(10, SHAPES["mqa"], [33], lengths(10, 13, 0, 40))
+    want = attention_rows(one)
+    at = np.arange(n) % 13
+    case = dict(one, **{k: one[k][at] for k in ("q", "consts", "suffix_len", "suffix_pages")})
+    if per_group == 1:
+        case.update(group_start=np.arange(n + 1, dtype=np.int32), prefix_len=np.full(n, 33, dtype=np.int32), prefix_pages=np.repeat(one["prefix_pages"], n, 0))
+    else:
+        case["group_start"] = np.array([0, n], dtype=np.int32)
+    c = Call(gpu_lib, torch, case)
+    c.call.run()
+    torch.cuda.synchronize()
+    assert (c.status.cpu().numpy() == 0).all()
+    assert (c.out.cpu().numpy() == np.stack([want[r] for r in range(13)])[at]).all()
 
 
 def test_draft_tokens_share_their_suffix_pages(gpu_lib, torch):
