@@ -31,7 +31,7 @@ constexpr int kPickThreads = 512;
 constexpr int kPickPass = 24576;            // tokens whose counts a block holds at a time (a multiple of 32)
 constexpr int kPickBits = 262144;           // and tokens whose bits it holds at a time, where the counts lie in a table
 constexpr int kPickMaxHistory = 65535;      // (a count is 16 bits)
-constexpr int kPickTable = 3072;            // names of a row that the table takes
+constexpr int kPickTable = 2560;            // names of a row that the table takes
 constexpr int kPickChunk = 1024, kPickStages = 4;      // words of four logits that arrive at once, and places for them
 
 struct PickArgs {

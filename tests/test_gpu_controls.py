@@ -232,6 +232,46 @@ def test_save_blobs_and_restored_sequences(gpu_lib):
         eng.close()
 
 
+def test_a_sequence_listed_twice(gpu_lib):
+    eng = engine(gpu_lib, "tiny", 64, 3)
+    sh = A.SHAPES["tiny"]
+    try:
+        a, b = eng.new_seq(), eng.new_seq()
+        for s in (a, b):
+            s.prefill(A.stream_uniform(1, "prompt", 9, 0, 40), 64)
+            s.set_controls(repetition=60000, presence=9000, frequency=4000, count_given=True)
+        got = []
+        for _ in range(4):
+            st, toks = eng.decode_step([a, a], sh.layers)
+            assert st == 0
+            got += toks
+        assert got == b.decode(8, sh.layers)
+    finally:
+        eng.close()
+
+
+def test_a_slot_taken_again(gpu_lib):
+    """controls, ids and biases end with their sequence, though the next one lies where it lay"""
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model("tiny", 0xC0, 64), blocks=1, max_batch=1, max_chunk=64)
+    sh = A.SHAPES["tiny"]
+    prompt = A.stream_uniform(1, "prompt", 9, 0, 40)
+
+    def fresh(**controls):
+        s = eng.new_seq()
+        s.prefill(prompt, 64)
+        if controls:
+            s.set_controls(**controls)
+        got = s.decode(6, sh.layers)
+        s.release()
+        return got
+    try:
+        plain, mild = fresh(), fresh(repetition=45000, count_given=True)
+        assert fresh(repetition=60000, presence=1 << 28, biases=[(5, 1 << 30)]) != plain
+        assert fresh() == plain and fresh(repetition=45000, count_given=True) == mild
+    finally:
+        eng.close()
+
+
 def test_refusals(gpu_lib):
     eng = engine(gpu_lib, "tiny", 32, 1)
     sh = A.SHAPES["tiny"]

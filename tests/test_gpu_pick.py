@@ -98,6 +98,20 @@ def test_a_vocabulary_of_several_passes(gpu_lib, torch):
     Call(gpu_lib, torch, make(2, 3, 500_003, 5000, 1024, 0.4)).check()
 
 
+@pytest.mark.parametrize("history,bias", [(2560, 0), (2561, 0), (1536, 1024), (1537, 1024), (2048, 512), (512, 1), (511, 1024)])
+def test_lists_where_the_table_ends(gpu_lib, torch, history, bias):
+    Call(gpu_lib, torch, make(history, 3, 40000, history, bias, 0.5)).check()
+
+
+def test_as_many_rows_as_a_call_takes(gpu_lib, torch):
+    case = make(5, 65535, 70, params=False)
+    c = Call(gpu_lib, torch, case)
+    c.call.run()
+    torch.cuda.synchronize()
+    assert (c.tokens.cpu().numpy() == case["logits"].argmax(1)).all() and (c.best.cpu().numpy() == case["logits"].max(1)).all()
+    assert (c.out.cpu().numpy() == case["logits"]).all() and (c.status.cpu().numpy() == 0).all()
+
+
 def test_longest_lists(gpu_lib, torch):
     case = make(3, 2, 5000, 65535, 1024, None)
     case["history"][1, :] = 4321                     # one token counts 65,535 times

@@ -39,13 +39,16 @@ class Prefix:
         assert self.eng.lib.sslm_prefix_release(self.h) == 0
 
 
-def run(dll, lib, shape, mode, prefixes, members, steps=3, budget=None, splits=0, **model):
-    """members: (prefix number or None, tokens of its own) per sequence. Tokens of every step and the save blobs."""
+def run(dll, lib, shape, mode, prefixes, members, steps=3, budget=None, splits=0, adapted=(), twice=(), **model):
+    """members: (prefix number or None, tokens of its own) per sequence. adapted: which of them have an adapter, in turn one of
+    two; twice: which are listed a second time at the end of the batch. Tokens of every step and the save blobs."""
     dll.sslm_b200_set_prefix_attention(mode)
     dll.sslm_b200_set_attention_splits(splits)
     sh = A.SHAPES[shape]
     cap = max((prefixes[p] if p is not None else 0) + n for p, n in members) + steps + 2
-    eng = abi.Engine(lib, A.build_synthetic_model(shape, 0x5A17, cap, **model), blocks=len(members) + len(prefixes), max_batch=len(members), max_chunk=128)
+    cap += steps if twice else 0
+    art = A.build_synthetic_model(shape, 0x5A17, cap, **model)
+    eng = abi.Engine(lib, art, blocks=len(members) + len(prefixes), max_batch=len(members), max_chunk=128)
     try:
         pf = [Prefix(eng, A.stream_uniform(0x900 + i, "prefix", n, 0, sh.vocab - 1)) for i, n in enumerate(prefixes)]
         seqs = []
@@ -54,12 +57,15 @@ def run(dll, lib, shape, mode, prefixes, members, steps=3, budget=None, splits=0
             if n:
                 s.prefill(A.stream_uniform(0x500 + i, "own", n, 0, sh.vocab - 1), 128)
             seqs.append(s)
+        adapters = [eng.map_adapter(A.build_synthetic_adapter(art, 0x77 + i, 16 * (i + 1))) for i in range(2 if adapted else 0)]
+        for i in adapted:
+            seqs[i].set_adapter(adapters[i % 2])
         for p in pf:
             p.release()
         before = dll.sslm_b200_prefix_attention_launches()
         tokens = []
         for _ in range(steps * (1 if budget is None else -(-sh.layers // budget)) + 1):
-            st, got = eng.decode_step(seqs, budget or sh.layers)
+            st, got = eng.decode_step(seqs + [seqs[i] for i in twice], budget or sh.layers)
             assert st == 0
             tokens.append(got)
         return tokens, [s.save() for s in seqs], dll.sslm_b200_prefix_attention_launches() - before
@@ -107,6 +113,21 @@ def test_biased_projections(dll, gpu_lib):
     prefixes, members = [120], [(0, 1 + 5 * i) for i in range(7)]
     apart = run(dll, gpu_lib, "tiny", 0, prefixes, members, bias_bits=28)
     together = run(dll, gpu_lib, "tiny", 2, prefixes, members, bias_bits=28)
+    assert together[2] > 0 and together[:2] == apart[:2]
+
+
+@pytest.mark.parametrize("shape", ["small", "mini0.5b"])
+def test_adapters_beside_it(dll, gpu_lib, shape):
+    prefixes, members = [120, 33], [(i % 2, 1 + 5 * i) for i in range(8)] + [(None, 9), (None, 30)]
+    apart = run(dll, gpu_lib, shape, 0, prefixes, members, adapted=(0, 3, 4, 7, 8))
+    together = run(dll, gpu_lib, shape, 2, prefixes, members, adapted=(0, 3, 4, 7, 8))
+    assert together[2] > 0 and together[:2] == apart[:2]
+
+
+def test_sequences_listed_twice(dll, gpu_lib):
+    prefixes, members = [70], [(0, 1 + 5 * i) for i in range(5)] + [(None, 9)]
+    apart = run(dll, gpu_lib, "small", 0, prefixes, members, twice=(0, 2, 5))
+    together = run(dll, gpu_lib, "small", 2, prefixes, members, twice=(0, 2, 5))
     assert together[2] > 0 and together[:2] == apart[:2]
 
 
