@@ -278,56 +278,79 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			} else {
 				auto seen = [&](int v) {
 					const uint32_t i = (uint32_t)(v - v0);
-					if (i >= (uint32_t)n) return;
-					atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));
-					name(i);
+					if (i < (uint32_t)n) atomicAdd(&counts[i >> 1], 1u << (16 * (i & 1)));      // (nothing waits for it)
 				};
-				// (ids of any alignment: single ones up to the first 16-byte word, then words)
+				// (ids of any alignment: single ones up to the first 16-byte word, then words, the next ones asked for ahead)
 				const int head = min(w.n_history, (int)((4 - (((uintptr_t)w.history >> 2) & 3)) & 3)), whole = (w.n_history - head) >> 2;
-				if (t < head) seen(w.history[t]);
 				const int4* ids = (const int4*)(w.history + head);
-				for (int i0 = t; i0 < whole; i0 += 4 * kPickThreads) {
-					int4 x[4];
+				auto fetch = [&](int4 (&x)[4], int i0) {
 #pragma unroll
 					for (int u = 0; u < 4; ++u) x[u] = i0 + u * kPickThreads < whole ? ids[i0 + u * kPickThreads] : make_int4(-1, -1, -1, -1);
-#pragma unroll 1
+				};
+				int4 x[4], y[4];
+				fetch(x, t);
+				for (int i = t; i < w.n_bias; i += kPickThreads) {
+					const int v = w.bias_tokens[i];
+					const uint32_t at_bit = (uint32_t)(v - v0);
+					if (at_bit >= (uint32_t)n) continue;
+					bool new_to_it = false;
+					atomicAdd(&bsum[enter(v, &new_to_it)], (unsigned long long)(long long)w.bias_values[i]);
+					if (new_to_it) atomicOr(&named[at_bit >> 5], 1u << (at_bit & 31));
+				}
+				if (t < head) seen(w.history[t]);
+				for (int i0 = t; i0 < whole; i0 += 4 * kPickThreads) {
+					fetch(y, i0 + 4 * kPickThreads);
+#pragma unroll
 					for (int u = 0; u < 4; ++u) {
-						seen(x[0].x);
-						seen(x[0].y);
-						seen(x[0].z);
-						seen(x[0].w);
-						x[0] = x[1];
-						x[1] = x[2];
-						x[2] = x[3];
+						seen(x[u].x);
+						seen(x[u].y);
+						seen(x[u].z);
+						seen(x[u].w);
+						x[u] = y[u];
 					}
 				}
 				const int tail = head + 4 * whole + t;
 				if (tail < w.n_history) seen(w.history[tail]);
 				if (t == 0 && w.extra >= 0) seen(w.extra);
-				for (int i = t; i < w.n_bias; i += kPickThreads) {
-					const int v = w.bias_tokens[i];
-					if ((uint32_t)(v - v0) >= (uint32_t)n) continue;
-					bool new_to_it;
-					atomicAdd(&bsum[enter(v, &new_to_it)], (unsigned long long)(long long)w.bias_values[i]);
-					name((uint32_t)(v - v0));
-				}
 				__syncthreads();
-				// the list of named tokens, from the bits: a thread's words, the warps' shares, a place each
+				// a thread's words of the bitmaps, from the counts; the list is of tokens that are counted and have no bias
+				constexpr int kWords = (kPickPass / 32 + kPickThreads - 1) / kPickThreads;
+				uint32_t counted[kWords];
 				int have = 0;
-				for (int i = t; i < words; i += kPickThreads) have += __popc(named[i]);
+#pragma unroll
+				for (int u = 0; u < kWords; ++u) {
+					const int i = t + u * kPickThreads;
+					counted[u] = 0u;
+					if (i >= words) continue;
+#pragma unroll
+					for (int j = 0; j < 4; ++j) {      // (behind the last token lies something else, which does not count)
+						const uint4 q = ((const uint4*)counts)[4 * i + j];
+						const uint32_t pair[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+						for (int k = 0; k < 4; ++k)
+							counted[u] |= ((pair[k] & 0xFFFFu) != 0u ? 1u << (8 * j + 2 * k) : 0u) | (pair[k] >> 16 != 0u ? 2u << (8 * j + 2 * k) : 0u);
+					}
+					if (n - 32 * i < 32) counted[u] &= (1u << (n - 32 * i)) - 1u;
+					const uint32_t biased = named[i];
+					counted[u] &= ~biased;
+					named[i] = biased | counted[u];
+					dense[i] &= ~(biased | counted[u]);
+					have += __popc(counted[u]);
+				}
 				int upto = have;
 #pragma unroll
 				for (int o = 1; o < 32; o *= 2) {
-					const int y = __shfl_up_sync(0xffffffffu, upto, o);
-					if (lane >= o) upto += y;
+					const int z = __shfl_up_sync(0xffffffffu, upto, o);
+					if (lane >= o) upto += z;
 				}
 				if (lane == 31) s_part[warp] = upto;
 				__syncthreads();
 				int to = upto - have;
 				for (int i = 0; i < warp; ++i) to += s_part[i];
 				if (t == kPickThreads - 1) s_listed = to + have;
-				for (int i = t; i < words; i += kPickThreads)
-					for (uint32_t bits = named[i]; bits != 0u; bits &= bits - 1u) list[to++] = (uint16_t)(32 * i + __ffs(bits) - 1);
+#pragma unroll
+				for (int u = 0; u < kWords; ++u)
+					for (uint32_t bits = counted[u]; bits != 0u; bits &= bits - 1u) list[to++] = (uint16_t)(32 * (t + u * kPickThreads) + __ffs(bits) - 1);
 			}
 		}
 		__syncthreads();
@@ -426,20 +449,18 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 				for (int u = 0; u < IN; ++u)
 					if (at[u] >= 0) change(id[u], raw[u], counts[at[u]], a.sums ? (long long)bsum[at[u]] : 0ll);
 			} else {
+				for (int h = t; h < a.hash; h += kPickThreads) {
+					const int v = bkey[h];
+					if (v >= 0) change(v, logits[v], counts[(v - v0) >> 1] >> (16 * ((v - v0) & 1)) & 0xFFFFu, (long long)bsum[h]);
+				}
 				for (int k0 = t; k0 < s_listed; k0 += 4 * kPickThreads) {
 					int32_t y[4];
 #pragma unroll
 					for (int u = 0; u < 4; ++u) y[u] = k0 + u * kPickThreads < s_listed ? logits[v0 + list[k0 + u * kPickThreads]] : INT32_MIN;
 #pragma unroll 1
 					for (int k = k0; k < min(s_listed, k0 + 4 * kPickThreads); k += kPickThreads) {
-						const int i = list[k], v = v0 + i;
-						long long sum = 0;
-						if (w.n_bias > 0) {
-							uint32_t h = place(v);
-							while (bkey[h] != v && bkey[h] != -1) h = (h + 1) & (uint32_t)(a.hash - 1);
-							if (bkey[h] == v) sum = (long long)bsum[h];
-						}
-						change(v, y[0], counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, sum);
+						const int i = list[k];
+						change(v0 + i, y[0], counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, 0);
 						y[0] = y[1];
 						y[1] = y[2];
 						y[2] = y[3];
