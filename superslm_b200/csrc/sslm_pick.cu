@@ -242,13 +242,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 				if constexpr (TABLE) counts[i] = 0u;
 			}
 			__syncthreads();
-			auto name = [&](uint32_t i) {
-				if constexpr (NAMED) {
-					if ((named[i >> 5] >> (i & 31) & 1u) != 0u) return;
-					atomicOr(&named[i >> 5], 1u << (i & 31));
-				}
-				if ((dense[i >> 5] >> (i & 31) & 1u) != 0u) atomicAnd(&dense[i >> 5], ~(1u << (i & 31)));
-			};
+			// (a token that is not allowed is the stream's, whoever names it)
 			auto enter = [&](int v, bool* new_to_it) {      // its place in the table (a quarter of the places at least stay free)
 				uint32_t h = place(v);
 				for (;;) {
@@ -270,10 +264,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 					if (i >= (uint32_t)n) continue;
 					bool new_to_it = false;
 					const uint32_t h = enter(id[u], &new_to_it);
-					if (new_to_it) at[u] = (int)h;
+					if (new_to_it && (atomicAnd(&dense[i >> 5], ~(1u << (i & 31))) >> (i & 31) & 1u) != 0u) {
+						at[u] = (int)h;
+						if constexpr (NAMED) atomicOr(&named[i >> 5], 1u << (i & 31));
+					}
 					if (u < IH || u == IN - 1) atomicAdd(&counts[h], 1u);
 					else atomicAdd(&bsum[h], (unsigned long long)(long long)add[u - IH]);
-					name(i);
 				}
 			} else {
 				auto seen = [&](int v) {
@@ -331,10 +327,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 							counted[u] |= ((pair[k] & 0xFFFFu) != 0u ? 1u << (8 * j + 2 * k) : 0u) | (pair[k] >> 16 != 0u ? 2u << (8 * j + 2 * k) : 0u);
 					}
 					if (n - 32 * i < 32) counted[u] &= (1u << (n - 32 * i)) - 1u;
-					const uint32_t biased = named[i];
-					counted[u] &= ~biased;
+					const uint32_t allowed = dense[i], biased = named[i] & allowed;
+					counted[u] &= allowed & ~biased;
 					named[i] = biased | counted[u];
-					dense[i] &= ~(biased | counted[u]);
+					dense[i] = allowed & ~(biased | counted[u]);
 					have += __popc(counted[u]);
 				}
 				int upto = have;
@@ -437,7 +433,6 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 					}
 					y = (int32_t)max(-2147483647ll, min(2147483647ll, z + sum));
 				}
-				if (w.mask != nullptr && (w.mask[v >> 3] >> (v & 7) & 1) == 0) y = INT32_MIN;
 				key = max(key, pick_key(y, v));
 				if constexpr (OUT) out[v] = y;
 			};
@@ -451,20 +446,20 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			} else {
 				for (int h = t; h < a.hash; h += kPickThreads) {
 					const int v = bkey[h];
-					if (v >= 0) change(v, logits[v], counts[(v - v0) >> 1] >> (16 * ((v - v0) & 1)) & 0xFFFFu, (long long)bsum[h]);
+					if (v >= 0 && (named[(v - v0) >> 5] >> ((v - v0) & 31) & 1u) != 0u) change(v, logits[v], counts[(v - v0) >> 1] >> (16 * ((v - v0) & 1)) & 0xFFFFu, (long long)bsum[h]);
 				}
-				for (int k0 = t; k0 < s_listed; k0 += 4 * kPickThreads) {
-					int32_t y[4];
+				int32_t y[4];      // (logits of the next four turns)
 #pragma unroll
-					for (int u = 0; u < 4; ++u) y[u] = k0 + u * kPickThreads < s_listed ? logits[v0 + list[k0 + u * kPickThreads]] : INT32_MIN;
+				for (int u = 0; u < 4; ++u) y[u] = t + u * kPickThreads < s_listed ? logits[v0 + list[t + u * kPickThreads]] : INT32_MIN;
 #pragma unroll 1
-					for (int k = k0; k < min(s_listed, k0 + 4 * kPickThreads); k += kPickThreads) {
-						const int i = list[k];
-						change(v0 + i, y[0], counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, 0);
-						y[0] = y[1];
-						y[1] = y[2];
-						y[2] = y[3];
-					}
+				for (int k = t; k < s_listed; k += kPickThreads) {
+					const int i = list[k], ahead = k + 4 * kPickThreads;
+					const int32_t x = y[0];
+					y[0] = y[1];
+					y[1] = y[2];
+					y[2] = y[3];
+					y[3] = ahead < s_listed ? logits[v0 + list[ahead]] : INT32_MIN;
+					change(v0 + i, x, counts[i >> 1] >> (16 * (i & 1)) & 0xFFFFu, 0);
 				}
 			}
 		}
