@@ -15,8 +15,15 @@
 // one bitmap and a maximum; where it lies is looked up once, at the end. The named tokens are dear (a division, a
 // table) and come last, each to one thread: then their logits are in L2 (asked for ahead of the stream, a thousand
 // single words a row cost as much as 20 MB of it; worked on in the stream, nearly every other warp stops for one).
-// Bound by the logits' bytes where rows are many, by the chain (lists, marks, one trip to memory, one exchange)
-// where they are few.
+//
+// Counts lie in a table of the names (TABLE: 1,536 of few rows and 2,560 of many at most, a thread's ids in registers, whoever enters a token works on it),
+// or, for longer lists, by token: an id then costs one atomic that nothing waits for, and the bitmaps and the list of named
+// tokens are made from the counts (40 rows of 32,768 ids: 33 us with the bitmaps marked id by id, 18.6 so).
+//
+// What bounds it (us, one B200, logits not in L2): one row of 151,936 7.1 and 21 rows under a schema 11: the chain (record,
+// lists, marks, one trip to memory, one exchange). 256 rows 45, of which the stream takes 28 at 5.6 TB/s (a kernel that only reads:
+// 5.9); the marks in front and the named tokens behind it are not hidden, since one row fills a block and two blocks a
+// multiprocessor. 64 rows written out 24: 79 MB both ways.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -516,7 +523,10 @@ namespace {
 
 // names: how many tokens the lists of a row can name; biases of them. True: the table.
 bool pick_plan(int names, int biases, PickArgs* a) {
-	const bool table = names <= kPickTable;
+	// The table or counts by token, us: 151,936 tokens and one row 12.3 / 12.3 with 1,600 names and 14.3 / 12.3 with 2,400, 21 rows
+	// 16.4 / 18.4 and 20.4 / 18.4 (2,560), but 64 rows 24.6 / 32.8 and 256 rows 74 / 102 (2,560): there the passes that the counts
+	// need cost more than a table's turns. 32,003 tokens: one and 21 rows 14.3 / 12.3 (2,400), 64 16.4 / 16.4, 256 31 / 33.
+	const bool table = names <= (a->rows <= 32 ? 1536 : kPickTable);
 	// blocks per row: as many as run at once, two a multiprocessor, with slices of at least 4,096 tokens; without the table
 	// the passes of a slice repeat the lists, so one pass if possible
 	const int most = std::max(1, 2 * sm_count() / a->rows);

@@ -98,9 +98,10 @@ def test_a_vocabulary_of_several_passes(gpu_lib, torch):
     Call(gpu_lib, torch, make(2, 3, 500_003, 5000, 1024, 0.4)).check()
 
 
-@pytest.mark.parametrize("history,bias", [(2560, 0), (2561, 0), (1536, 1024), (1537, 1024), (2048, 512), (512, 1), (511, 1024)])
-def test_lists_where_the_table_ends(gpu_lib, torch, history, bias):
-    Call(gpu_lib, torch, make(history, 3, 40000, history, bias, 0.5)).check()
+@pytest.mark.parametrize("rows", [3, 33])
+@pytest.mark.parametrize("history,bias", [(2560, 0), (2561, 0), (1536, 1024), (1537, 1024), (1536, 0), (1537, 0), (512, 1024), (513, 1024), (512, 1)])
+def test_lists_where_the_table_ends(gpu_lib, torch, rows, history, bias):
+    Call(gpu_lib, torch, make(history, rows, 40000, history, bias, 0.5)).check()
 
 
 def test_as_many_rows_as_a_call_takes(gpu_lib, torch):
