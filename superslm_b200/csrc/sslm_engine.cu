@@ -37,8 +37,10 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // one hidden-state slot of a sequence: codes, then the carried scale
 size_t seq_scale_offset(const Dims& d) { return align_up(d.hidden, 16); }
 size_t seq_state_stride(const Dims& d) { return align_up(seq_scale_offset(d) + sizeof(Scale), 256); }
-// ids that count as repeated (every position holds one token, and one more has been produced), and biases with their tokens
-size_t seq_history_bytes(const Dims& d) { return align_up(((size_t)d.context_cap + 16) * 4, 256); }
+// Ids that count as repeated, and biases with their tokens. A produced token is dropped where a prefill follows it, so a sequence
+// may be given a token and produce one for every position: a pick needs a position, or a token given since the last one, of its
+// own. With the longest context, 32,768, a pick finds 65,535 ids at most, what it counts in 16 bits.
+size_t seq_history_bytes(const Dims& d) { return align_up(((size_t)2 * d.context_cap + 16) * 4, 256); }
 size_t seq_control_bytes(const Dims& d) { return seq_history_bytes(d) + (size_t)kPickMaxBias * 8; }
 
 sslm_status map_forward_status(int32_t st) {

@@ -301,6 +301,34 @@ def test_refusals(gpu_lib):
         eng.close()
 
 
+def test_a_token_given_and_one_produced_for_every_position(gpu_lib, capture):
+    """produced tokens that a prefill drops count all the same: twice as many ids as positions, biases and neighbours untouched"""
+    cap = 40
+    eng = engine(gpu_lib, "tiny", cap, 2)
+    eng.vocab = A.SHAPES["tiny"].vocab
+    try:
+        a, b = eng.new_seq(), eng.new_seq()
+        biases, own = [(7, 30000), (9, -20000), (11, 25000)], A.stream_uniform(3, "own", cap, 0, 60)
+        for s in (a, b):
+            s.set_controls(repetition=50000, presence=500, frequency=900, count_given=True, biases=biases)
+        history = [[], []]
+        for n in range(cap):
+            for s, h in ((a, history[0]), (b, history[1])):
+                s.prefill(own[n:n + 1], 64)
+                h.append(int(own[n]))
+            if n == cap - 1:      # (taken away and put back: all ids go to the device at once)
+                a.set_controls(repetition=None)
+                a.set_controls(repetition=50000, presence=500, frequency=900, count_given=True, biases=biases)
+            toks, rows = step(eng, capture, [a, b])
+            for i in range(2):
+                assert toks[i] == picked(changed_logits(rows[i], (50000, 500, 900), history[i], biases))[0], n
+                history[i].append(toks[i])
+        assert len(history[0]) == 2 * cap and history[0] == history[1]
+        assert eng.decode_step([a], eng.num_layers)[0] == abi.ST["SSLM_CONTEXT_CAP_EXCEEDED"]
+    finally:
+        eng.close()
+
+
 def test_long_histories(gpu_lib, capture):
     """more ids than the table takes, and a context that is full"""
     cap = 3400
