@@ -98,6 +98,11 @@ def test_both_maxima_at_their_limit(gpu_lib, torch, shape, prefix, suffix):
     Call(gpu_lib, torch, attention_case(6, SHAPES[shape], prefix, suffix, widths=(2048, 2048))).check()
 
 
+def test_a_row_longer_than_the_longest(gpu_lib, torch):
+    case = attention_case(7, SHAPES["tiny"], [32760], [8, 9, 0, 300, 1])
+    Call(gpu_lib, torch, case).check(refused={1: 7, 3: 7})
+
+
 @pytest.mark.parametrize("consts", [(1, 1, 0), (1, 11_863_283, 0), ((1 << 23), (1 << 23), 0), (5, 11, (1 << 40)), (3000, 6000, 0), (1 << 20, 1 << 21, 1 << 46),
                                     (11_863_283, 11_863_283, 0)])
 @pytest.mark.parametrize("deviation", [0.0, 3.0, 400.0])
