@@ -44,6 +44,7 @@ constexpr int kPfxTokens = 32;           // rows a tile holds at most (32 query 
 
 struct PrefixArgs {
 	int rows, groups, G, kv_heads, tq, ginv, sub;        // ginv = ceil(65536 / G); a tile is cut over `sub` blocks, one cluster
+	uint32_t sinv;                                       // ceil(2^32 / sub), of more than one block
 	int per, pinv;                                       // rows of the tile that each of them adds up and stores, ceil(65536 / per)
 	int ppages, spages;                                  // prefix and suffix pages a block has room for (multiples of four)
 	int vgroups;                                         // groups of four pages whose V it has room for
@@ -197,10 +198,19 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		pdl_wait();
 		pdl_release();
 	}
+	const int fold_word = t < 3 * G ? (a.fold != nullptr ? a.fold[3 * kvh * G + t] : (t % 3 == 0 ? 1 : 0)) : 0;      // (wanted at the end)
 	// ---- which tile: group after group, tq rows at a time
 	if (warp == 0) {
 		int want = (int)blockIdx.y, r0 = 0, nt = 0, group = 0, prefix = 0;
-		for (int g0 = 0; g0 < a.groups; g0 += 32) {
+		if (a.groups == 1) {      // (alike for all lanes)
+			const int start = max(a.group_start[0], 0), n = max(min(a.group_start[1], a.rows) - start, 0), len = a.prefix_len[0];
+			if (want < (n + a.tq - 1) / a.tq) {
+				r0 = start + want * a.tq;
+				nt = min(a.tq, n - want * a.tq);
+				prefix = len;
+			}
+		}
+		for (int g0 = 0; g0 < a.groups && a.groups > 1; g0 += 32) {
 			int start = 0, n = 0, len = 0;
 			if (g0 + lane < a.groups) {
 				start = a.group_start[g0 + lane];
@@ -238,7 +248,6 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		s_max[t] = INT32_MIN;
 		s_sum[t] = 0ull;
 	}
-	if (t < 3 * G) s_fold[t] = a.fold != nullptr ? a.fold[3 * kvh * G + t] : (t % 3 == 0 ? 1 : 0);
 	__syncthreads();
 	const int r0 = s_tile[0], nt = s_tile[1];
 	if (nt == 0) {      // (all blocks of the cluster alike)
@@ -267,7 +276,9 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 	const int64_t page_bytes = kPageTokens * HD, plane = a.num_pages * page_bytes;
 	const int8_t* kplane = a.kv + (int64_t)(2 * kvh) * plane;
 	const int8_t* vplane = kplane + plane;
-	auto mine = [&](int n) { return n > rank ? (n - rank + sub - 1) / sub : 0; };      // of n things dealt out: rank, rank + sub, ...
+	auto mine = [&](int n) {      // of n things dealt out: rank, rank + sub, ... (n <= 65,536: the product's error is below 1 / sub)
+		return n > rank ? (sub > 1 ? (int)__umulhi((uint32_t)(n - rank + sub - 1), a.sinv) : n) : 0;
+	};
 	auto known = [&](int id) { return !RESIDENT || (uint64_t)(int64_t)id < (uint64_t)a.num_pages; };
 	auto stage_v = [&](int at, int64_t base) {      // the page's V into place `at` (filled-up prefix pages first), while there is room
 		if (base < 0 || at >= 4 * a.vgroups) return;
@@ -277,22 +288,33 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		             "l"(vplane + base), "r"((uint32_t)page_bytes), "r"(bar) : "memory");
 	};
 	const int np = min(mine((P + kPageTokens - 1) / kPageTokens), a.ppages), np4 = (np + 3) & ~3;      // (filled up to groups of four)
+	// Page ids of the rows' own pages, all that the tables have room for, are asked for beside the lengths if a thread each is enough.
+	// They lie where the sums of other blocks come in, which are sent when this block's maxima are known.
+	int32_t* ids = (int32_t*)s_rxsum;
+	const int room = (a.max_suffix + kPageTokens - 1) / kPageTokens, own_room = RESIDENT && nt * room <= kPfxThreads - 32 ? room : 0;
 	bool bad_page = false;
 	if (warp == 0) {
 		int code = lane < nt ? kOk : 1, len = 0;
 		if (RESIDENT) {
 			if (lane < nt) len = a.suffix_len[r0 + lane];
+			const int all = nt * a.kv_heads;
+			int64_t k[3];
+			auto consts_of = [&](int x) {
+				const int64_t* from = a.consts + ((int64_t)r0 * a.kv_heads + min(x, all - 1)) * 3;
+#pragma unroll
+				for (int i = 0; i < 3; ++i) k[i] = from[i];
+			};
+			consts_of(lane);      // (with the lengths)
 			if (lane < nt && (bad_len || len < 0 || len > a.max_suffix || P + len > kPfxMaxWidth)) {
 				code = SSLM_B200_ROW_LENGTH;
 				len = 0;
 			}
 			s_code[lane] = 0;
 			__syncwarp();
-			for (int x0 = 0; x0 < nt * a.kv_heads; x0 += 32) {      // a row's constants of every kv head: a lane each
-				const int x = x0 + lane, tk = min(x / a.kv_heads, nt - 1);
-				const int64_t* k = a.consts + (int64_t)r0 * a.kv_heads * 3 + 3 * min(x, nt * a.kv_heads - 1);
-				const int64_t ln2 = k[0], qb = k[1], qc = k[2];
-				if (!softmax_gate(ln2, qb, qc, P + __shfl_sync(0xffffffffu, len, tk))) s_code[tk] = SSLM_B200_ROW_CONSTANTS;
+			for (int x0 = 0; x0 < all; x0 += 32) {      // a row's constants of every kv head: a lane each
+				const int tk = min((x0 + lane) / a.kv_heads, nt - 1);
+				if (x0 > 0) consts_of(x0 + lane);
+				if (!softmax_gate(k[0], k[1], k[2], P + __shfl_sync(0xffffffffu, len, tk))) s_code[tk] = SSLM_B200_ROW_CONSTANTS;
 			}
 			__syncwarp();
 			if (code == kOk && s_code[lane] != 0) {
@@ -320,7 +342,10 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 			redo[i] = 0u;
 			stage_v(i, pbase[i]);
 		}
-		if (RESIDENT) stage_q(t - 32, kPfxThreads - 32);
+		if (RESIDENT) {
+			if (t - 32 < nt * own_room) ids[t - 32] = a.suffix_pages[(int64_t)(r0 + (t - 32) / own_room) * a.suffix_stride + (t - 32) % own_room];
+			stage_q(t - 32, kPfxThreads - 32);
+		}
 	}
 	// a page id that does not exist: the rows that see the page report the largest maximum there is, which no score
 	// reaches, and every block of the tile learns of it with the maxima
@@ -351,7 +376,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 			while (s_cum[tk + 1] <= x) ++tk;
 			const int page = x - s_cum[tk];
 			const int32_t* pages = RESIDENT ? a.suffix_pages + (int64_t)(r0 + tk) * a.suffix_stride : a.desc[r0 + tk].pages + P / kPageTokens;
-			const int id = pages[page];
+			const int id = own_room > 0 ? ids[tk * own_room + page] : pages[page];
 			if (known(id)) {
 				base = (int64_t)id * page_bytes;
 				own = tk | min(kPageTokens, s_len[tk] - page * kPageTokens) << 8;
@@ -384,6 +409,7 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		}
 		s_fx[lane] = iexp_mul_prepare(k.q_ln2, k.q_b, k.q_c);
 	}
+	if (t < 3 * G) s_fold[t] = fold_word;
 	__syncthreads();
 	if (t == 0) ring_arrive(cta_addr(&s_bars[0]));      // (every staged page is announced)
 
@@ -914,6 +940,7 @@ cudaError_t prefix_dispatch(PrefixArgs a, int hd, const PrefixPlan& p, cudaStrea
 	a.tq = p.tq;
 	a.ginv = (65536 + a.G - 1) / a.G;
 	a.sub = p.sub;
+	a.sinv = (uint32_t)(((1ull << 32) + p.sub - 1) / p.sub);
 	a.per = (p.rows + p.sub - 1) / p.sub;
 	a.pinv = (65536 + a.per - 1) / a.per;
 	a.ppages = p.ppages;
