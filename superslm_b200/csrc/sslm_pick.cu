@@ -190,8 +190,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		first = min(v1, v0 + ((4 - ((v0 + mis) & 3)) & 3));
 		last = first + ((v1 - first) & ~3);
 		chunks = ((last - first) / 4 + kPickChunk - 1) / kPickChunk;
-		if (t == 0)      // (the first of them on their way while the marks are made)
-			for (int i = 0; i < min(chunks, a.stages); ++i) issue(i);
+		if (t < min(chunks, a.stages)) issue(t);      // (the first of them on their way while the marks are made; one thread for all took 0.5 us longer)
 	};
 	__syncthreads();
 	if (s_code != 0) {      // (all blocks of the cluster alike)
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			}
 		};
 		int32_t top = INT32_MIN;
-		int top_at = 0;      // the word that has it first
+		int top_at = 0;      // the word that has it first, and where in it
 		const int total = (last - first) / 4;
 #pragma unroll 1
 		for (int i = 0; i < chunks; ++i) {
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 				const int32_t m = max(max(y[0], y[1]), max(y[2], y[3]));
 				if (m > top) {
 					top = m;
-					top_at = k;
+					top_at = 4 * k + (y[0] == m ? 0 : (y[1] == m ? 1 : (y[2] == m ? 2 : 3)));
 				}
 				if constexpr (OUT) {
 					const uint32_t nm = listed ? nibble(named, k) : 0u;
@@ -416,12 +415,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			__syncthreads();      // the place is free
 			if (t == 0 && s_late == 0 && i + a.stages < chunks) issue(i + a.stages);
 		}
-		if (top != INT32_MIN) {      // (in place, the word reads as it was but for what the bitmaps leave out)
-			int32_t y[4];
-			words_of(*(const int4*)(logits + first + 4 * t + top_at * kStride), nibble(dense, top_at), y);
-			const int j = y[0] == top ? 0 : (y[1] == top ? 1 : (y[2] == top ? 2 : 3));
-			key = max(key, pick_key(top, first + 4 * t + top_at * kStride + j));
-		}
+		if (top != INT32_MIN) key = max(key, pick_key(top, first + 4 * t + (top_at >> 2) * kStride + (top_at & 3)));
 		// ---- the named tokens: (in place, they read as they were)
 		if (listed) {
 			const double inv_theta = 1.0 / (double)w.theta;
