@@ -18,9 +18,9 @@
 //
 // Counts lie in a table of the names (TABLE: 1,536 of few rows and 2,560 of many at most, a thread's ids in registers, whoever enters a token works on it),
 // or, for longer lists, by token: an id then costs one atomic that nothing waits for, and the bitmaps and the list of named
-// tokens are made from the counts (40 rows of 32,768 ids: 33 us with the bitmaps marked id by id, 18.6 so).
+// tokens are made from the counts (40 rows of 32,768 ids: 33 us with the bitmaps marked id by id, 18.5 so).
 //
-// What bounds it (us, one B200, logits not in L2): one row of 151,936 7.1 and 21 rows under a schema 11: the chain (record,
+// What bounds it (us, one B200, logits not in L2): one row of 151,936 6.8 and 21 rows under a schema 11: the chain (record,
 // lists, marks, one trip to memory, one exchange). 256 rows 45, of which the stream takes 28 at 5.6 TB/s (a kernel that only reads:
 // 5.9); the marks in front and the named tokens behind it are not hidden, since one row fills a block and two blocks a
 // multiprocessor. 64 rows written out 24: 79 MB both ways.
