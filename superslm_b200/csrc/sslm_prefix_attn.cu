@@ -93,14 +93,13 @@ __device__ __forceinline__ bool softmax_gate(int64_t ln2, int64_t qb, int64_t qc
 	return peak <= SSLM_SOFTMAX_MAX_SAFE && (unsigned long long)peak * (unsigned long long)max(width, 1) <= 0x7FFFFFFFFFFFFFFFull;
 }
 // The HD / 16 words of a head-dim row that lane column c feeds to the score MMAs: MMA j takes words 2j (k slots 4c ..) and 2j + 1
-// (16 + 4c ..), of q and of K alike.
+// (16 + 4c ..), of q and of K alike. Rows of 128 channels are taken as two halves of 64, 16 bytes a lane of each: the pool may begin at any
+// 16-byte boundary, and one load of 32 bytes wants a 32-byte one.
 template <int HD>
 __device__ __forceinline__ void row_words(const int8_t* row, int c, uint32_t (&w)[HD / 16]) {
 	if constexpr (HD == 128) {
-		asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-		             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-		             : "l"(row + c * 32)
-		             : "memory");
+		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 16) : "memory");
+		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(row + 64 + c * 16) : "memory");
 	} else if constexpr (HD == 64) {
 		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 16) : "memory");
 	} else {
@@ -428,12 +427,12 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 				tok[b][e] = rho * a.ginv >> 16;
 				head[b][e] = rho - tok[b][e] * G;
 				mx[b][e] = INT32_MIN;
-				const int8_t* row = qs + rho * L::kQStride + c * (HD / 4);
+				const int8_t* row = qs + rho * L::kQStride;      // (in row_words' order)
 				if constexpr (HD == 32) {
-					*(uint2*)q[b][e] = *(const uint2*)row;
+					*(uint2*)q[b][e] = *(const uint2*)(row + c * 8);
 				} else {
 #pragma unroll
-					for (int w = 0; w < HD / 16; w += 4) *(uint4*)&q[b][e][w] = *(const uint4*)(row + 4 * w);
+					for (int w = 0; w < HD / 16; w += 4) *(uint4*)&q[b][e][w] = *(const uint4*)(row + 16 * w + c * 16);
 				}
 			}
 		const int total = np + ns;

@@ -346,3 +346,22 @@ def test_empty_calls(gpu_lib, torch):
     c.check(want={})
     c.call.args.rows, c.call.args.groups = 2, 0
     c.check(want={})
+
+
+@pytest.mark.parametrize("shape", ["1.5b", "g7", "0.5b", "tiny"])
+@pytest.mark.parametrize("splits_n", [1, 4])
+def test_a_pool_at_any_16_byte_boundary(gpu_lib, torch, splits, splits_n, shape):
+    splits(splits_n)
+    case = attention_case(60, SHAPES[shape], [130, 33], lengths(60, 9, 0, 50))
+    want = attention_rows(case)
+    c = Call(gpu_lib, torch, case)
+    raw = torch.zeros(c.d["kv"].numel() + 64, dtype=torch.int8, device="cuda")
+    for first in (16, 48, 32):
+        kv = raw[first:first + c.d["kv"].numel()].view(c.d["kv"].shape)
+        kv.copy_(c.d["kv"])
+        assert kv.data_ptr() % 32 == first % 32
+        c.out.fill_(JUNK)
+        c.status.fill_(77)
+        abi.PrefixAttention(gpu_lib, out=c.out, row_status=c.status, **dict(c.d, kv=kv)).run()
+        torch.cuda.synchronize()
+        c.compare(want)
