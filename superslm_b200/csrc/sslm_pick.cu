@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			else atomicCAS(&a.status[r], 0, pack_status(kInternalWaitTimeout, kSiteLogits, a.desc[r].layer));
 		}
 		__syncwarp();
-		exchange_leave(cta_addr(&s_bar), 1);
+		if (sub > 1) exchange_leave(cta_addr(&s_bar), 1);      // (a block by itself has no exchange: its barrier was never set up)
 	}
 }
 

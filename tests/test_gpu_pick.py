@@ -247,6 +247,26 @@ def test_a_wait_that_runs_out(gpu_lib, torch, rows, vocab, exchange):
     c.check()
 
 
+def test_a_block_by_itself_has_no_peers_to_outlast(gpu_lib, torch):
+    """a row of one block, its copy late: a wait for the copy (0.25 s) and one more for what is under way, and no third for words of a peer"""
+    import time
+    arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
+    arm.argtypes = [C.c_int32, C.c_int32]
+    c = Call(gpu_lib, torch, make(33, 200, 9000))
+    c.check()
+    try:
+        assert arm(7, 1) == 0
+        begun = time.perf_counter()
+        c.call.run()
+        torch.cuda.synchronize()
+        took = time.perf_counter() - begun
+    finally:
+        arm(-1, 0)
+    assert c.status.tolist() == [100] + [0] * 199
+    assert 0.25 <= took < 0.75
+    c.check()
+
+
 def test_no_rows(gpu_lib, torch):
     c = Call(gpu_lib, torch, make(31, 2, 50))
     c.call.args.rows = 0
