@@ -30,6 +30,7 @@
 
 #include "../../include/sslm_b200.h"
 #include "sslm_cluster.cuh"
+#include "sslm_copies.h"
 #include "sslm_kernels.h"
 
 namespace sslm {
@@ -177,9 +178,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 	const int mis = (int)(((uintptr_t)logits >> 2) & 3), mis_out = (int)(((uintptr_t)out >> 2) & 3);
 	int v0 = s0, v1, first, last, chunks;
 	uint32_t seq = 0;      // chunks of earlier passes
+	CopyAccount copies{(uint32_t)a.stages, 0u};      // (kept by the first thread, which asks for all but a pass's first copies)
 	// a pass: tokens v0 .. v1; whole aligned words of four tokens lie from `first` to `last`, the ends are taken one by one
 	auto issue = [&](int chunk) {      // (one thread; the place is free)
-		const uint32_t at = (seq + (uint32_t)chunk) % (uint32_t)a.stages, bar = cta_addr(&s_full[at]);
+		const uint32_t at = copies.place(seq + (uint32_t)chunk), bar = cta_addr(&s_full[at]);
 		const uint32_t bytes = (uint32_t)min(4 * kPickChunk, last - first - 4 * kPickChunk * chunk) * 4u;
 		asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes + (held == 2 && seq + chunk == 0 ? 16u : 0u)) : "memory");
 		asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(cta_addr(ring + at * kPickChunk)),
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		first = min(v1, v0 + ((4 - ((v0 + mis) & 3)) & 3));
 		last = first + ((v1 - first) & ~3);
 		chunks = ((last - first) / 4 + kPickChunk - 1) / kPickChunk;
-		if (t < min(chunks, a.stages)) issue(t);      // (the first of them on their way while the marks are made; one thread for all took 0.5 us longer)
+		if ((uint32_t)t < copies.begin(seq, (uint32_t)chunks)) issue(t);      // (the first of them on their way while the marks are made; one thread for all took 0.5 us longer)
 	};
 	__syncthreads();
 	if (s_code != 0) {      // (all blocks of the cluster alike)
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 	}
 	auto place = [&](int v) { return ((uint32_t)v * 2654435761u) >> 7 & (uint32_t)(a.hash - 1); };
 	unsigned long long key = 0ull;
-	while (v0 < s1) {
+	while (v0 < s1 && s_late == 0) {      // (alike for all: it changes behind a pass's barriers only)
 		const int n = v1 - v0, words = (n + 31) / 32;
 		// ---- marks and counts of tokens v0 .. v1
 		for (int i = 4 * t; i < words + 2; i += 4 * kPickThreads) {
@@ -387,8 +389,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		const int total = (last - first) / 4;
 #pragma unroll 1
 		for (int i = 0; i < chunks; ++i) {
-			const uint32_t slot = (seq + (uint32_t)i) % (uint32_t)a.stages, turn = (seq + (uint32_t)i) / (uint32_t)a.stages;
-			if (s_late == 0 && !ring_wait(cta_addr(&s_full[slot]), turn & 1u)) s_late = 1;      // (what is read then does not count)
+			const uint32_t slot = copies.place(seq + (uint32_t)i);
+			if (s_late == 0 && !ring_wait(cta_addr(&s_full[slot]), copies.parity(seq + (uint32_t)i))) s_late = 1;      // (what is read then does not count)
 #pragma unroll
 			for (int u = 0; u < kPickChunk / kPickThreads; ++u) {
 				const int k = i * (kPickChunk / kPickThreads) + u;
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 				}
 			}
 			__syncthreads();      // the place is free
-			if (t == 0 && s_late == 0 && i + a.stages < chunks) issue(i + a.stages);
+			if (t == 0 && copies.follows((uint32_t)i, (uint32_t)chunks, s_late != 0)) issue(i + a.stages);
 		}
 		if (top != INT32_MIN) key = max(key, pick_key(top, first + 4 * t + (top_at >> 2) * kStride + (top_at & 3)));
 		// ---- the named tokens: (in place, they read as they were)
@@ -467,14 +469,14 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 		__syncthreads();      // the tables may be overwritten
 		seq += (uint32_t)chunks;
 		v0 += a.pass;
-		if (v0 < s1) begin();
+		if (v0 < s1 && s_late == 0) begin();
 	}
 	// ---- the row's largest key: larger values first, then lower indices
 #pragma unroll
 	for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
 	if (lane == 0) s_warp[warp] = key;
-	if (t == 0 && s_late != 0)      // (a copy that is late may still come)
-		for (uint32_t i = seq > (uint32_t)a.stages ? seq - (uint32_t)a.stages : 0u; i < seq; ++i) ring_wait(cta_addr(&s_full[i % (uint32_t)a.stages]), i / (uint32_t)a.stages & 1u);
+	if (t == 0 && s_late != 0)      // (a copy that is late may still come, into memory that the next block owns: every place's last one is waited for)
+		for (uint32_t i = copies.open(); i < copies.issued; ++i) ring_wait(cta_addr(&s_full[copies.place(i)]), copies.parity(i));
 	__syncthreads();
 	if (warp != 0) {
 		if (sub > 1) cluster_wait();

@@ -273,3 +273,30 @@ def test_no_rows(gpu_lib, torch):
     c.call.run()
     torch.cuda.synchronize()
     assert c.tokens.tolist() == [55, 55]
+
+
+@pytest.mark.parametrize("logits", [False, True])
+@pytest.mark.parametrize("rows,vocab,history", [(160, 600_001, 0), (160, 60_000, 3000), (1, 600_001, 0)])
+def test_a_copy_that_is_late_ahead_of_other_chunks_and_passes(gpu_lib, torch, rows, vocab, history, logits):
+    """more chunks than places, and passes behind the one whose copy is late: its row is reported, the others and the next call are right"""
+    arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
+    arm.argtypes = [C.c_int32, C.c_int32]
+    case = make(32, rows, vocab, history, 0, None)
+    c = Call(gpu_lib, torch, case, logits=logits)
+    try:
+        assert arm(7, 1) == 0
+        c.call.run()
+        torch.cuda.synchronize()
+    finally:
+        arm(-1, 0)
+    assert c.status.tolist() == [100] + [0] * (rows - 1)
+    some = sorted({1, rows // 2, rows - 1} - {0, rows})
+    for r in some:
+        assert (int(c.tokens[r]), int(c.best[r])) == picked(row_of(case, r))
+    c.call.run()
+    torch.cuda.synchronize()
+    assert c.status.tolist() == [0] * rows
+    for r in [0] + some:
+        assert (int(c.tokens[r]), int(c.best[r])) == picked(row_of(case, r))
+        if logits:
+            assert (c.out[r].cpu().numpy() == row_of(case, r)).all()
