@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) k_pick(const __grid_constant_
 			if (page >= 0 && page < a.num_masks) x.mask = a.masks + (int64_t)page * a.mask_stride;
 			if (x.theta < 1) code = SSLM_B200_ROW_CONSTANTS;
 			if (x.n_history < 0 || x.n_history > a.max_history || x.n_bias < 0 || x.n_bias > a.max_bias) code = SSLM_B200_ROW_LENGTH;
-			if (page >= a.num_masks) code = SSLM_B200_ROW_INDEX;
+			if (page >= a.num_masks || (page < -1 && code == 0)) code = SSLM_B200_ROW_INDEX;      // (-1, and nothing else below zero, says: no mask)
 			if (rank == 0 && a.status != nullptr) a.status[r] = code;
 		} else {
 			x = a.desc[r];

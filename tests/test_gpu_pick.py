@@ -300,3 +300,10 @@ def test_a_copy_that_is_late_ahead_of_other_chunks_and_passes(gpu_lib, torch, ro
         assert (int(c.tokens[r]), int(c.best[r])) == picked(row_of(case, r))
         if logits:
             assert (c.out[r].cpu().numpy() == row_of(case, r)).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 20001), (6, 900)])
+def test_only_minus_one_says_no_mask(gpu_lib, torch, rows, vocab):
+    case = make(34, rows, vocab, 50, 20, 0.5)
+    case["mask_page"][:] = [-2, -1, 3, LOWEST, 0, 5]
+    Call(gpu_lib, torch, case).check({0: 101, 3: 101, 5: 101})
