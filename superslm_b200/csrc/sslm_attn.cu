@@ -1713,6 +1713,8 @@ static AttnPlan attn_plan(const Dims& d, int m, int max_width, int forced) {
 	}
 	return p;
 }
+// blocks of such a launch (0: whole rows by one block each, in any number)
+int attn_blocks(const Dims& d, int m, int max_width) { return m * d.kv_heads * attn_plan(d, m, max_width, attn_forced_splits()).splits; }
 constexpr size_t kFewSmemMax = 223 * 1024;
 static size_t few_smem(const Dims& d, int cp) {
 	const int G = d.heads / d.kv_heads;

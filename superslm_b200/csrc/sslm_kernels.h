@@ -211,6 +211,8 @@ cudaError_t attn_configure(const Dims& d);
 // slices per kv head of later attention launches (0: chosen per launch); for tuning and tests
 void attn_force_splits(int splits);
 int attn_forced_splits();
+// blocks of a launch over m decode rows of up to max_width positions that cuts their widths, 0 where it cuts none
+int attn_blocks(const Dims& d, int m, int max_width);
 // How the attention of m rows will run, decided ahead of the q/k/v site: site != 0 says that it takes that site over
 // (launch_qkv_post is then left out).
 struct AttnChoice {

@@ -202,3 +202,20 @@ def test_a_wait_that_runs_out_inside_a_step(dll, gpu_lib):
         assert twin.decode(2, sh.layers)[1] == got[0]
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("prefixes,members,chosen", [
+    ([1024], [(0, 1 + i % 7) for i in range(64)], True),                                                    # many rows behind one prefix
+    ([1024], [(0, 1 + i % 7) for i in range(64)] + [(None, 20 + i) for i in range(4)], False),              # the same beside four others
+    ([2048], [(0, 1 + i % 7) for i in range(12)], False),                                                   # few rows
+    ([4096], [(0, 1 + i) for i in range(4)], False),
+    ([4096], [(0, 1 + i) for i in range(8)], True),
+    ([1024] * 32, [(i % 32, 1 + i % 5) for i in range(128)], False),                                        # many small groups
+    ([1024], [(0, 300 + 20 * (i % 5)) for i in range(64)], False),                                          # suffixes that are not short
+    ([2048, 128], [(0, 1 + i % 7) for i in range(40)] + [(1, 1 + i % 7) for i in range(4)], True),          # alike enough to be cut together
+    ([8192, 64], [(0, 1), (0, 2)] + [(1, 1 + i % 7) for i in range(30)], False),                            # a long prefix of few, a short one of many
+    ([8192, 64], [(0, 1 + i) for i in range(30)] + [(1, 1 + i % 7) for i in range(30)], True)])
+def test_where_it_is_the_faster_one(dll, gpu_lib, prefixes, members, chosen):
+    """mode 1 takes what was measured to gain, and leaves what was measured to lose"""
+    got = run(dll, gpu_lib, "tiny", 1, prefixes, members, steps=1)
+    assert (got[2] > 0) == chosen
