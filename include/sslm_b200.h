@@ -339,7 +339,8 @@ SSLM_API sslm_status sslm_b200_capture_logits(sslm_workspace ws, int32_t* host_r
  * NULL takes the controls away; a second call replaces them; sslm_seq_reset leaves them attached and empties the history.
  * repetition below 1, more than 1,024 biases, or a missing list: SSLM_INVALID_ARGUMENT; a bias token outside the vocabulary:
  * SSLM_TOKEN_ID_OUT_OF_RANGE; nothing changes then. The first decode call of a workspace that has such a sequence allocates room
- * for its logit rows. */
+ * for the logit rows of max_batch sequences, and the first one of more sequences for the rows of as many as the workspace takes at once;
+ * no other call allocates. */
 typedef struct sslm_b200_controls {
 	uint32_t struct_size;
 	int32_t repetition;              /* Q15: 32,768 is 1.0 */

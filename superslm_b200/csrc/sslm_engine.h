@@ -61,7 +61,7 @@ struct sslm_workspace_s {
 	unsigned int* d_tc_counters = nullptr;
 	int32_t* logit_capture = nullptr;   // host buffer for full logit rows (tests), or nullptr
 	int32_t* d_logits = nullptr;
-	// full logit rows of a decode call in which some sequence has controls, allocated by the first such call; records of their picks
+	// full logit rows of a decode call in which some sequence has controls (pick_room: allocated by the first such call); records of their picks
 	int32_t* d_pick_logits = nullptr;
 	size_t pick_rows = 0;
 	sslm::PickRow *h_pick = nullptr, *d_pick = nullptr;

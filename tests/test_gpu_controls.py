@@ -347,3 +347,30 @@ def test_long_histories(gpu_lib, capture):
         assert eng.decode_step([s], eng.num_layers)[0] == abi.ST["SSLM_CONTEXT_CAP_EXCEEDED"]
     finally:
         eng.close()
+
+
+def test_a_batch_that_grows_allocates_once(gpu_lib):
+    """room for the logit rows of max_batch sequences with the first step that needs any; of all the workspace takes with the first larger one"""
+    torch = pytest.importorskip("torch")
+    shape = A.Shape("wide vocabulary", 128, 2, 4, 2, 32, 256, 151936)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC2, 64), blocks=48, max_batch=24, max_chunk=96)
+    try:
+        seqs = []
+        for i in range(48):
+            s = eng.new_seq()
+            s.prefill(A.stream_uniform(i, "prompt", 3, 0, shape.vocab - 1), 64)
+            seqs.append(s)
+        for s in seqs[:2]:
+            assert eng.decode_step([s], shape.layers)[0] == 0      # (what kernels need to be loaded is)
+        free = []
+        for n in (1, 2, 3, 5, 8, 13, 24, 25, 33, 48):
+            for s in seqs[:n]:
+                s.set_controls(repetition=40000)
+            assert eng.decode_step(seqs[:n], shape.layers)[0] == 0
+            torch.cuda.synchronize()
+            free.append(torch.cuda.mem_get_info()[0])
+        row = shape.vocab * 4
+        assert max(free[:7]) - min(free[:7]) < row
+        assert max(free[7:]) - min(free[7:]) < row and 22 * row < free[6] - free[7] < 27 * row
+    finally:
+        eng.close()
