@@ -595,9 +595,8 @@ extern "C" sslm_status sslm_b200_pick_resident(const sslm_b200_pick* call, void*
 	if (c.history && (!c.history_len || c.max_history < 0 || c.max_history > kPickMaxHistory || c.history_stride < c.max_history)) return SSLM_INVALID_ARGUMENT;
 	if (c.bias_tokens && (!c.bias_values || !c.bias_len || c.max_bias < 0 || c.max_bias > kPickMaxBias || c.bias_stride < c.max_bias)) return SSLM_INVALID_ARGUMENT;
 	if (c.mask_page && ((!c.masks && c.num_masks > 0) || c.mask_stride < (c.vocab + 7) / 8)) return SSLM_INVALID_ARGUMENT;
-	if (!c.out_tokens && !c.out_best && !c.out_logits) return SSLM_INVALID_ARGUMENT;
-	if (c.rows == 0) return SSLM_OK;
-	if (!c.logits) return SSLM_INVALID_ARGUMENT;
+	if (c.rows == 0) return SSLM_OK;      // (tensors without elements have no address)
+	if (!c.logits || (!c.out_tokens && !c.out_best && !c.out_logits)) return SSLM_INVALID_ARGUMENT;
 	for (const void* p : {(const void*)c.logits, (const void*)c.params, (const void*)c.history, (const void*)c.history_len, (const void*)c.bias_tokens,
 	                      (const void*)c.bias_values, (const void*)c.bias_len, (const void*)c.mask_page, (const void*)c.out_tokens, (const void*)c.out_best,
 	                      (const void*)c.out_logits, (const void*)c.row_status})

@@ -77,3 +77,12 @@ def test_prepared_calls_check_their_tensors():
         abi.Pick(lib, logits=torch.zeros((2, 8), dtype=torch.int32), out_tokens=torch.zeros(2, dtype=torch.int32))
     with pytest.raises(TypeError, match="logits"):
         abi.Pick(lib, logits=torch.zeros((2, 8)), out_tokens=torch.zeros(2, dtype=torch.int32))
+
+
+def test_nothing_to_do_on_tensors_without_elements(dll):
+    """whose addresses are null"""
+    none = {k: None for k in ("logits", "params", "history", "history_len", "bias_tokens", "bias_values", "bias_len", "mask_page", "out_tokens", "out_best", "out_logits")}
+    assert dll.sslm_b200_pick_resident(C.byref(pick(rows=0, **none)), None) == 0
+    none = {k: None for k in ("q", "consts", "suffix_len", "suffix_pages", "out", "row_status")}
+    assert dll.sslm_b200_attention_prefix_resident(C.byref(attention(rows=0, **none)), None) == 0
+    assert dll.sslm_b200_pick_resident(C.byref(pick(rows=1, out_tokens=None, out_best=None, out_logits=None)), None) == BAD
