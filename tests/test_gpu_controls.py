@@ -374,3 +374,123 @@ def test_a_batch_that_grows_allocates_once(gpu_lib):
         assert max(free[7:]) - min(free[7:]) < row and 22 * row < free[6] - free[7] < 27 * row
     finally:
         eng.close()
+
+
+def large_vocabulary(vocab):
+    return A.Shape("v%d" % vocab, 128, 2, 4, 2, 32, 256, vocab)
+
+
+@pytest.mark.parametrize("vocab", [32003, 151936])
+@pytest.mark.parametrize("rows", [1, 3, 21, 64])
+def test_vocabularies_that_are_cut_over_blocks(gpu_lib, capture, vocab, rows):
+    """rows of several blocks: lists on both sides of where the table of names ends, a schema, and rows without controls among them"""
+    shape = large_vocabulary(vocab)
+    table = A.synthetic_schemas(0xC3, vocab, 2)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC3, 1700, schemas=2), blocks=rows, max_batch=rows, max_chunk=1024)
+    eng.vocab = vocab
+    kinds = [dict(repetition=45000, presence=3000, frequency=700), dict(repetition=40000, frequency=90, count_given=True),
+             dict(repetition=36000, presence=500, biases=[(7 * i % vocab, 400 * (i % 9) - 1500) for i in range(900)], count_given=True), None, "schema"]
+    try:
+        seqs, history, state, handles = [], [], [], []
+        for name in (table[0]["name"], table[1]["name"]):
+            h = C.c_void_p()
+            assert gpu_lib.sslm_schema_lookup(eng.model, name.encode(), C.byref(h)) == 0
+            handles.append(h)
+        for i in range(rows):
+            kind = kinds[i % len(kinds)] if rows > 1 else kinds[2]
+            s = eng.new_seq()
+            state.append(0 if kind == "schema" else None)
+            if kind == "schema":
+                assert gpu_lib.sslm_seq_set_schema(s.handle, handles[i % 2]) == 0
+            # (1,600 ids and 900 biases are more than any table of names takes, 600 and 900 what some do)
+            p = A.stream_uniform(20 + i, "prompt", 1600 if i % 15 == 2 else (600 if i % 15 == 7 else 12 + i % 30), 0, 4000)
+            s.prefill(p, 1024)
+            history.append([int(t) for t in p] if isinstance(kind, dict) and kind.get("count_given") else [])
+            if kind == "schema":
+                s.set_controls(repetition=60000, presence=20000)
+            elif kind is not None:
+                s.set_controls(**kind)
+            seqs.append(s)
+        dead = set()
+        for _ in range(3):
+            toks, raw = step(eng, capture, seqs)
+            for i in range(rows):
+                kind = kinds[i % len(kinds)] if rows > 1 else kinds[2]
+                if kind is None:
+                    assert toks[i] == int(raw[i].argmax())
+                    continue
+                mask = None
+                if kind == "schema":
+                    mask = np.zeros((vocab + 7) // 8, dtype=np.uint8)
+                    allowed = dict(table[i % 2]["rows"][state[i]])
+                    for t in allowed:
+                        mask[t >> 3] |= 1 << (t & 7)
+                    kind = dict(repetition=60000, presence=20000)
+                want = picked(changed_logits(raw[i], (kind["repetition"], kind.get("presence", 0), kind.get("frequency", 0)), history[i], kind.get("biases", ()), mask))[0]
+                assert toks[i] == want, (i, toks[i], want)
+                if want == -2:
+                    dead.add(i)
+                    continue
+                history[i].append(want)
+                if state[i] is not None:
+                    state[i] = allowed[want]
+            if dead:      # (a dead end ends the sequence)
+                break
+    finally:
+        eng.close()
+
+
+@pytest.mark.parametrize("vocab", [32003, 151936])
+def test_more_rows_than_are_cut(gpu_lib, vocab):
+    """200 rows, three of them with biases that decide: the others choose as in a batch without controls"""
+    shape = large_vocabulary(vocab)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC4, 40), blocks=200, max_batch=200, max_chunk=64)
+    try:
+        seqs = []
+        for i in range(200):
+            s = eng.new_seq()
+            s.prefill(A.stream_uniform(i, "prompt", 3 + i % 9, 0, vocab - 1), 64)
+            seqs.append(s)
+        def tokens(steps):
+            return [eng.decode_step(seqs, shape.layers)[1] for _ in range(steps)]
+        plain = tokens(3)
+        for i, s in enumerate(seqs):
+            s.reset()
+            s.prefill(A.stream_uniform(i, "prompt", 3 + i % 9, 0, vocab - 1), 64)
+        decided = {0: 5, 77: vocab - 1, 199: 16001}
+        for i, t in decided.items():
+            seqs[i].set_controls(biases=[(t, (1 << 31) - 1)])
+        for got, want in zip(tokens(3), plain):
+            assert got == [decided.get(i, t) for i, t in enumerate(want)]
+    finally:
+        eng.close()
+
+
+@pytest.mark.parametrize("rows,exchange", [(1, 0), (1, 1), (5, 0), (5, 1), (160, 1)])
+def test_a_wait_that_runs_out_inside_a_step(gpu_lib, rows, exchange):
+    """the step fails, and the same step made again is right"""
+    arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
+    arm.argtypes = [C.c_int32, C.c_int32]
+    shape = large_vocabulary(32003)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC5, 40), blocks=2 * rows, max_batch=rows, max_chunk=64)
+    try:
+        twins = []
+        for _ in range(2):
+            seqs = []
+            for i in range(rows):
+                s = eng.new_seq()
+                s.prefill(A.stream_uniform(i, "prompt", 3 + i % 9, 0, 40), 64)
+                s.set_controls(repetition=60000, presence=9000, frequency=4000, count_given=True)
+                seqs.append(s)
+            twins.append(seqs)
+        try:
+            assert arm(7, exchange) == 0
+            assert eng.decode_step(twins[0], shape.layers)[0] == abi.ST["SSLM_ALLOCATION_FAILED"]
+        finally:
+            arm(-1, 0)
+        # the call ended at its first row, whose wait it was; the others were not advanced
+        for _ in range(2):
+            st, got = eng.decode_step(twins[0], shape.layers)
+            assert st == 0 and (st, got) == eng.decode_step(twins[1], shape.layers)
+    finally:
+        eng.close()

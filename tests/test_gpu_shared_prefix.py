@@ -219,3 +219,55 @@ def test_where_it_is_the_faster_one(dll, gpu_lib, prefixes, members, chosen):
     """mode 1 takes what was measured to gain, and leaves what was measured to lose"""
     got = run(dll, gpu_lib, "tiny", 1, prefixes, members, steps=1)
     assert (got[2] > 0) == chosen
+
+
+@pytest.mark.parametrize("shape", ["tiny", "mini0.5b"])
+def test_where_it_is_chosen_the_outputs_are_the_same(dll, gpu_lib, shape):
+    """the default mode, with as many rows as it wants and groups that it leaves out"""
+    prefixes, members = [1040, 80], [(0, 1 + i % 7) for i in range(70)]
+    apart, chosen = (run(dll, gpu_lib, shape, mode, prefixes, members, steps=2) for mode in (0, 1))
+    assert apart[2] == 0 and chosen[2] > 0 and chosen[:2] == apart[:2]
+
+
+def test_groups_that_are_left_out(dll, gpu_lib):
+    """short groups stay with the others where long ones are attended together without them"""
+    prefixes, members = [4096, 64], [(0, 1 + i % 7) for i in range(36)] + [(1, 1 + i % 5) for i in range(60)] + [(None, 1 + i % 9) for i in range(10)]
+    apart, chosen = (run(dll, gpu_lib, "tiny", mode, prefixes, members, steps=2) for mode in (0, 1))
+    assert apart[2] == 0 and chosen[2] > 0 and chosen[:2] == apart[:2]
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+def test_sequences_at_different_layers(dll, gpu_lib, mode):
+    """rows that start on several layers share in parts of their own, each with its groups"""
+    sh = A.SHAPES["small"]
+    length = 1040 if mode == 1 else 90
+    each = 66 if mode == 1 else 4
+    got = []
+    for m in (0, mode):
+        dll.sslm_b200_set_prefix_attention(m)
+        eng = abi.Engine(gpu_lib, A.build_synthetic_model("small", 5, length + 60), blocks=3 * each + 6, max_batch=3 * each, max_chunk=256)
+        try:
+            pf = [Prefix(eng, A.stream_uniform(80 + i, "prefix", n, 0, sh.vocab - 1)) for i, n in enumerate((length, 40))]
+            seqs = []
+            for i in range(3 * each):
+                s = pf[0 if mode == 1 or i % 4 < 3 else 1].adopt() if i % 9 != 8 or mode == 1 else eng.new_seq()
+                s.prefill(A.stream_uniform(90 + i, "own", 1 + i % 5, 0, sh.vocab - 1), 128)
+                seqs.append(s)
+            assert eng.decode_step(seqs, sh.layers)[0] == 0                    # (the token that the prompt leaves)
+            assert eng.decode_step(seqs[:2 * each], 1)[0] == 0                 # two thirds are a layer on
+            assert eng.decode_step(seqs[:each], 1)[0] == 0                     # one third two
+            before = dll.sslm_b200_prefix_attention_launches()
+            tokens = []
+            order = np.random.default_rng(3).permutation(len(seqs))
+            for _ in range(2 * sh.layers):
+                st, t = eng.decode_step([seqs[i] for i in order], 1)
+                assert st == 0
+                tokens.append(t)
+            launches = dll.sslm_b200_prefix_attention_launches() - before
+            assert launches == (0 if m == 0 else 2 * sh.layers * sh.layers)    # (a part for each layer that rows start on)
+            got.append((tokens, [s.save() for s in seqs]))
+            for p in pf:
+                p.release()
+        finally:
+            eng.close()
+    assert got[0] == got[1]
