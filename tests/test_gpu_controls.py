@@ -494,3 +494,41 @@ def test_a_wait_that_runs_out_inside_a_step(gpu_lib, rows, exchange):
             assert st == 0 and (st, got) == eng.decode_step(twins[1], shape.layers)
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("rows,exchange,budget", [(1, 1, 2), (3, 0, 2), (3, 1, 1)])
+def test_a_wait_that_runs_out_between_tokens(gpu_lib, rows, exchange, budget):
+    """the layers of the failed step stay done, its token is chosen by the next one: tokens, K/V and counts as if nothing had been"""
+    arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
+    arm.argtypes = [C.c_int32, C.c_int32]
+    shape = large_vocabulary(32003)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC6, 40), blocks=2 * rows, max_batch=rows, max_chunk=64)
+    try:
+        twins = []
+        for _ in range(2):
+            seqs = []
+            for i in range(rows):
+                s = eng.new_seq()
+                s.prefill(A.stream_uniform(i, "prompt", 3 + i, 0, 40), 64)
+                s.set_controls(repetition=60000, presence=9000, frequency=4000, count_given=True)
+                seqs.append(s)
+            twins.append(seqs)
+        for seqs in twins:
+            assert eng.decode_step(seqs, budget)[0] == 0
+        for _ in range(shape.layers // budget - 1):
+            assert [eng.decode_step(seqs, budget)[0] for seqs in twins] == [0, 0]
+        try:
+            assert arm(7, exchange) == 0
+            assert eng.decode_step(twins[0], budget)[0] == abi.ST["SSLM_ALLOCATION_FAILED"]
+        finally:
+            arm(-1, 0)
+        # (the first row is where it ended: the rows behind it take the failed step again)
+        st, first = eng.decode_step(twins[0][:1], budget)
+        assert st == 0
+        rest = eng.decode_step(twins[0][1:], budget) if rows > 1 else (0, [])
+        assert rest[0] == 0 and (0, first + rest[1]) == eng.decode_step(twins[1], budget)
+        for _ in range(4):
+            assert eng.decode_step(twins[0], budget) == eng.decode_step(twins[1], budget)
+        assert [s.save() for s in twins[0]] == [s.save() for s in twins[1]]
+    finally:
+        eng.close()
