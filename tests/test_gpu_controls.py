@@ -532,3 +532,38 @@ def test_a_wait_that_runs_out_between_tokens(gpu_lib, rows, exchange, budget):
         assert [s.save() for s in twins[0]] == [s.save() for s in twins[1]]
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("rows", [257, 300, 520])
+def test_more_rows_than_one_launch_of_the_head_stores(gpu_lib, rows):
+    """batches whose head rows run in several launches: schemas and controls on both sides of where they are cut, the others choose as ever"""
+    vocab = 8191
+    shape = large_vocabulary(vocab)
+    table = A.synthetic_schemas(0xC7, vocab, 1)
+    eng = abi.Engine(gpu_lib, A.build_synthetic_model(shape, 0xC7, 40, schemas=1), blocks=rows, max_batch=rows, max_chunk=64)
+    try:
+        h = C.c_void_p()
+        assert gpu_lib.sslm_schema_lookup(eng.model, table[0]["name"].encode(), C.byref(h)) == 0
+        bound = [3, 255, 256, rows - 1]
+        decided = {0: 5, 100: vocab - 1, 254: 77, 256: sorted(t for t, _ in table[0]["rows"][0])[-1], rows - 2: 4000}
+        got = []
+        for controlled in (False, True):
+            seqs = []
+            for i in range(rows):
+                s = eng.new_seq()
+                if i in bound:
+                    assert gpu_lib.sslm_seq_set_schema(s.handle, h) == 0
+                s.prefill(A.stream_uniform(i, "prompt", 3 + i % 9, 0, vocab - 1), 64)
+                if controlled and i in decided:
+                    s.set_controls(biases=[(decided[i], (1 << 31) - 1)])
+                seqs.append(s)
+            st, toks = eng.decode_step(seqs, shape.layers)
+            assert st == 0
+            got.append(toks)
+            for s in seqs:
+                s.release()
+        plain, chosen = got
+        allowed = {t for t, _ in table[0]["rows"][0]}      # (a bias brings no token in that the schema leaves out)
+        assert chosen == [decided[i] if i in decided and (i not in bound or decided[i] in allowed) else t for i, t in enumerate(plain)]
+    finally:
+        eng.close()
