@@ -20,7 +20,7 @@
 // probability on the row's sum. So a tile walks its scores three times (maximum; exponentials and sum; probabilities), and holds
 // them: 16 or 32 rows x 4 bytes a position, which is what sets the least number of blocks a long prefix takes.
 //
-// What bounds it (us, one B200, tensors not in L2): one row behind 512 positions of 14 x 64 heads 8.4, eight rows behind 300
+// What bounds it (us, one B200, tensors not in L2): one row behind 512 positions of 12 x 128 heads 8.5, eight rows behind 300
 // 8.9: the chain (lists and pages 2.5, scores 0.7, three exchanges or barriers 2, softmax 1.5, P.V and store 1.5), bytes under 0.1.
 // 64 rows behind 2,048 of 12 x 128 19; 256 rows in six ragged groups 35, of which the longest tile takes 34 and half of the
 // blocks 22; 32 rows behind 16,384 of 16 x 128 66: softmax elements, some 80 instructions each with the contractions, issued in
@@ -93,13 +93,21 @@ __device__ __forceinline__ bool softmax_gate(int64_t ln2, int64_t qb, int64_t qc
 	return peak <= SSLM_SOFTMAX_MAX_SAFE && (unsigned long long)peak * (unsigned long long)max(width, 1) <= 0x7FFFFFFFFFFFFFFFull;
 }
 // The HD / 16 words of a head-dim row that lane column c feeds to the score MMAs: MMA j takes words 2j (k slots 4c ..) and 2j + 1
-// (16 + 4c ..), of q and of K alike. Rows of 128 channels are taken as two halves of 64, 16 bytes a lane of each: the pool may begin at any
-// 16-byte boundary, and one load of 32 bytes wants a 32-byte one.
-template <int HD>
+// (16 + 4c ..), of q and of K alike. A lane's 32 bytes of a row of 128 channels come by one load, which wants them on a 32-byte
+// boundary, or (WHOLE false: the pool does not begin on one) by two of 16. A kernel each: with the choice in one, 64 rows behind 2,048 positions took
+// 20.0 us in place of 19.8, 256 in six groups 37.5 in place of 37.0, and as much with two loads for all.
+template <int HD, bool WHOLE>
 __device__ __forceinline__ void row_words(const int8_t* row, int c, uint32_t (&w)[HD / 16]) {
 	if constexpr (HD == 128) {
-		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 16) : "memory");
-		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(row + 64 + c * 16) : "memory");
+		if constexpr (WHOLE) {
+			asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+			             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+			             : "l"(row + c * 32)
+			             : "memory");
+		} else {
+			asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 32) : "memory");
+			asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(row + c * 32 + 16) : "memory");
+		}
 	} else if constexpr (HD == 64) {
 		asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + c * 16) : "memory");
 	} else {
@@ -147,7 +155,7 @@ __device__ __forceinline__ unsigned long long iexp_mul(uint32_t dq, const IExpMu
 	return ((unsigned long long)base * base + (unsigned long long)f.qc) >> z;
 }
 
-template <int HD, int ROWS, bool RESIDENT>
+template <int HD, int ROWS, bool RESIDENT, bool WHOLE>
 __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __grid_constant__ PrefixArgs a) {
 	using L = PrefixSmem<HD, ROWS>;
 	constexpr int KS = HD / 32;                 // MMA steps along the head dimension
@@ -191,8 +199,9 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		__syncwarp();
 		cluster_arrive();      // (waited for ahead of the first word that is sent)
 	}
-	// A caller's tensors may have been written by the kernel in front. An engine call's descriptors, lengths and page
-	// tables were uploaded, and the prefix's pages filled, before its first launch.
+	// A caller's tensors may have been written by the kernel in front. Of an engine call the descriptors, lengths and page tables were uploaded, and
+	// the prefix's pages filled, before its first launch, but for the ids of pages that the call opens: k_begin enters those. Two kernels lie between
+	// (the projections and the q/k/v site), and each waits for the one in front before it lets the next one start, so k_begin is over here.
 	if (RESIDENT) {
 		pdl_wait();
 		pdl_release();
@@ -358,8 +367,8 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 		for (int w = 0; w < HD / 16; ++w) kn[u][0][w] = kn[u][1][w] = 0u;
 	auto fetch_k = [&](uint32_t (&k)[2][HD / 16], int64_t base) {      // (no page: nothing, the words are not used)
 		if (base >= 0) {
-			row_words<HD>(kplane + base + krow * HD, c, k[0]);
-			row_words<HD>(kplane + base + (krow + 2) * HD, c, k[1]);
+			row_words<HD, WHOLE>(kplane + base + krow * HD, c, k[0]);
+			row_words<HD, WHOLE>(kplane + base + (krow + 2) * HD, c, k[1]);
 		}
 	};
 #pragma unroll
@@ -427,12 +436,12 @@ __global__ void __launch_bounds__(kPfxThreads, 1) k_attention_prefix(const __gri
 				tok[b][e] = rho * a.ginv >> 16;
 				head[b][e] = rho - tok[b][e] * G;
 				mx[b][e] = INT32_MIN;
-				const int8_t* row = qs + rho * L::kQStride;      // (in row_words' order)
+				const int8_t* row = qs + rho * L::kQStride + c * (HD / 4);
 				if constexpr (HD == 32) {
-					*(uint2*)q[b][e] = *(const uint2*)(row + c * 8);
+					*(uint2*)q[b][e] = *(const uint2*)row;
 				} else {
 #pragma unroll
-					for (int w = 0; w < HD / 16; w += 4) *(uint4*)&q[b][e][w] = *(const uint4*)(row + 16 * w + c * 16);
+					for (int w = 0; w < HD / 16; w += 4) *(uint4*)&q[b][e][w] = *(const uint4*)(row + 4 * w);
 				}
 			}
 		const int total = np + ns;
@@ -868,11 +877,16 @@ struct PrefixKernel {
 template <int HD, int ROWS, bool RESIDENT>
 cudaError_t prefix_setup(const int** clusters) {
 	static PrefixKernel k;
-	const auto kernel = k_attention_prefix<HD, ROWS, RESIDENT>;
+	const auto kernel = k_attention_prefix<HD, ROWS, RESIDENT, true>;
+	const auto set = [](auto f) {
+		cudaError_t x = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPfxSmemMax);
+		if (x == cudaSuccess) x = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+		if (x == cudaSuccess) x = cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+		return x;
+	};
 	const cudaError_t e = once_per_device(k.once, [&] {
-		cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPfxSmemMax);
-		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-		if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+		cudaError_t x = set(kernel);
+		if constexpr (RESIDENT && HD == 128) x = x == cudaSuccess ? set(k_attention_prefix<HD, ROWS, true, false>) : x;
 		for (int sub = 1; sub <= kPfxMaxSub && x == cudaSuccess; ++sub) {
 			cudaLaunchAttribute attr[2];
 			const cudaLaunchConfig_t cfg = prefix_config<HD, ROWS, RESIDENT>(attr, sub, 1, 1, kPfxSmemMax, nullptr);
@@ -931,7 +945,9 @@ template <int HD, int ROWS, bool RESIDENT>
 cudaError_t prefix_launch(const PrefixArgs& a, const PrefixPlan& p, cudaStream_t st) {
 	cudaLaunchAttribute attr[2];
 	const cudaLaunchConfig_t cfg = prefix_config<HD, ROWS, RESIDENT>(attr, p.sub, p.tiles, a.kv_heads, p.smem, st);
-	return cudaLaunchKernelEx(&cfg, k_attention_prefix<HD, ROWS, RESIDENT>, a);
+	if constexpr (RESIDENT && HD == 128)      // (a caller's pool may begin at any 16-byte boundary)
+		if (((uintptr_t)a.kv & 31) != 0) return cudaLaunchKernelEx(&cfg, k_attention_prefix<HD, ROWS, true, false>, a);
+	return cudaLaunchKernelEx(&cfg, k_attention_prefix<HD, ROWS, RESIDENT, true>, a);
 }
 
 template <bool RESIDENT>
