@@ -20,10 +20,10 @@
 // or, for longer lists, by token: an id then costs one atomic that nothing waits for, and the bitmaps and the list of named
 // tokens are made from the counts (40 rows of 32,768 ids: 33 us with the bitmaps marked id by id, 18.5 so).
 //
-// What bounds it (us, one B200, logits not in L2): one row of 151,936 6.8 and 21 rows under a schema 11: the chain (record,
-// lists, marks, one trip to memory, one exchange). 256 rows 45, of which the stream takes 28 at 5.6 TB/s (a kernel that only reads:
+// What bounds it (us, one B200, logits not in L2): one row of 151,936 6.9 and 21 rows under a schema 10.6: the chain (record,
+// lists, marks, one trip to memory, one exchange). 256 rows 43.5, of which the stream takes 28 at 5.6 TB/s (a kernel that only reads:
 // 5.9); the marks in front and the named tokens behind it are not hidden, since one row fills a block and two blocks a
-// multiprocessor. 64 rows written out 24: 79 MB both ways.
+// multiprocessor. 64 rows written out 22.6: 79 MB both ways.
 #include <cuda_runtime.h>
 
 #include <algorithm>

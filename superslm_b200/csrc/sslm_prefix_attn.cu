@@ -20,9 +20,9 @@
 // probability on the row's sum. So a tile walks its scores three times (maximum; exponentials and sum; probabilities), and holds
 // them: 16 or 32 rows x 4 bytes a position, which is what sets the least number of blocks a long prefix takes.
 //
-// What bounds it (us, one B200, tensors not in L2): one row behind 512 positions of 12 x 128 heads 8.5, eight rows behind 300
-// 8.9: the chain (lists and pages 2.5, scores 0.7, three exchanges or barriers 2, softmax 1.5, P.V and store 1.5), bytes under 0.1.
-// 64 rows behind 2,048 of 12 x 128 19; 256 rows in six ragged groups 35, of which the longest tile takes 34 and half of the
+// What bounds it (us, one B200, tensors not in L2): one row behind 512 positions of 12 x 128 heads 8.6, eight rows behind 300
+// 8.8: the chain (lists and pages 2.5, scores 0.7, three exchanges or barriers 2, softmax 1.5, P.V and store 1.5), bytes under 0.1.
+// 64 rows behind 2,048 of 12 x 128 19.6; 256 rows in six ragged groups 35.8, of which the longest tile takes 34 and half of the
 // blocks 22; 32 rows behind 16,384 of 16 x 128 66: softmax elements, some 80 instructions each with the contractions, issued in
 // 42 % of the slots by sixteen warps, in two rounds, since 192 blocks are needed to hold the scores.
 #include <cuda_runtime.h>
