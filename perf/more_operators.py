@@ -219,6 +219,7 @@ def _prepare_pages(case, seed):
     s["counts"] = torch.zeros(2, dtype=torch.int32, device="cuda")
     if case["op"] == "fork":
         s["out_lengths"] = torch.zeros(n, dtype=torch.int32, device="cuda")
+        s["drawn"] = torch.zeros(N, dtype=torch.int32, device="cuda")
         s["status"] = torch.zeros(n, dtype=torch.int32, device="cuda")
     else:
         s["new_of"] = torch.zeros(N, dtype=torch.int32, device="cuda")
@@ -395,10 +396,11 @@ def _plain_fork(s):
     s["out_tables"].copy_(out)
     s["out_holders"].copy_(held)
     s["out_lengths"].copy_(after)
+    s["drawn"].copy_(torch.where(torch.arange(N, device=tables.device) < want.sum(), fresh, s["drawn"].to(torch.int64)))
     s["moves"].copy_(torch.where((me < count)[:, None], moves, s["moves"].to(torch.int64)))
     s["counts"].copy_(torch.stack([count, want.sum()]))
     s["status"].zero_()
-    return [s[x] for x in ("out_tables", "out_lengths", "out_holders", "moves", "counts", "status", "kv")]
+    return [s[x] for x in ("out_tables", "out_lengths", "out_holders", "drawn", "moves", "counts", "status", "kv")]
 
 
 def _plain_compact(s):
@@ -432,7 +434,7 @@ def run(state):
     if own:
         state["call"].run()
         names = {"site": ("q_codes", "q_scales", "consts", "saturations", "kv"), "sample": ("tokens", "mass", "kept"),
-                 "fork": ("out_tables", "out_lengths", "out_holders", "moves", "counts", "status", "kv"),
+                 "fork": ("out_tables", "out_lengths", "out_holders", "drawn", "moves", "counts", "status", "kv"),
                  "compact": ("out_tables", "out_holders", "new_of", "moves", "counts", "kv")}[state["op"]]
         return [state[x] for x in names]
     return {"site": _plain_site, "sample": _plain_sample, "fork": _plain_fork, "compact": _plain_compact}[state["op"]](state)
@@ -588,7 +590,8 @@ def _exact_fork(case, seed):
         s["kv"][:, b] = s["kv"][:, a]
         s["moves"][j] = a, b
     s["out_holders"], s["counts"] = held, np.array([len(copies), taken], np.int32)
-    return [s[x] for x in ("out_tables", "out_lengths", "out_holders", "moves", "counts", "status", "kv")]
+    s["drawn"][:taken] = free[:taken]
+    return [s[x] for x in ("out_tables", "out_lengths", "out_holders", "drawn", "moves", "counts", "status", "kv")]
 
 
 def _exact_compact(case, seed):
