@@ -472,6 +472,152 @@ typedef struct sslm_b200_pick {
 } sslm_b200_pick;
 SSLM_API sslm_status sslm_b200_pick_resident(const sslm_b200_pick* call, void* stream);
 
+/* The q/k/v site of a layer: what lies between its projections and its attention (src/forward/forward_sites.cpp:1114-1146, :1281-1415,
+ * :663-761, :1806-1856), for heads of any number, with norms of the heads and other rotations. Row r is one token at position
+ * positions[r]; q, k and v are rows of int32 projections (out_folded of sslm_b200_linear_resident), in_scales the (m, e) of the rows
+ * that were projected, 2^30 <= m < 2^31 and |e| <= 4,096.
+ *   q    without q_gain: the funnel of the whole row with the site constant q_site, codes and (m, e) as out_codes and out_scales there
+ *        with q_gain: each head by itself normed to a mean square of one, times the gains, as codes of the scale q_site
+ *   K    without k_gain: landed on its head's scale, round(x m R / 2^(62 - e + e_t)), k_landing = (m_t, e_t, R = round(2^62 / m_t))
+ *        with k_gain: normed as q
+ *   V    landed as K, with v_landing
+ *   norm of a head x:  y = x 2^s, 2^23 <= max |y| <= 2^24;  root = floor(sqrt(64 sum y^2 / head_dim));
+ *        u = round(y floor(2^54 / root) / 2^36) (15 bits behind the point);  code = round(u gain / 2^shift);  a head of zeros: zeros
+ * Every code is held between -127 and 127; roundings are to the nearest, halves away from zero. The first `rotary` channels of q and K
+ * then turn by row positions[r] of the tables (30 bits behind the point), channels (2 i, 2 i + 1) or, with `halves`, (i, i + rotary / 2):
+ *   a' = round(a cos - b sin),  b' = round(a sin + b cos), between -127 and 127
+ * K and V go to place places[r] (NULL: positions[r]) of page table table_of[r] (NULL: r): page pages[table][place / 16] of kv, which is
+ * laid out as for sslm_b200_attention_prefix_resident. consts: the softmax constants of each K / V head from q's scale and khead's (m, e).
+ * saturations: the K and V codes of the row that were held. q, or k and v, may be NULL: that part is left out.
+ * A position of -1 leaves its row out (a padded batch). Refused, and nothing of it written, is a row with a position outside the tables of
+ * angles or a place outside its page table (SSLM_B200_ROW_LENGTH), scales outside their domain (_CONSTANTS), a page or table that does not
+ * exist (_INDEX). SSLM_B200_ROW_SOFTMAX: the row is written, but some head has no constants: zeros, which attention refuses.
+ * No two rows of a call may name the same place: which of them it holds then is not said.
+ * head_dim 32, 64 or 128; (heads + 2 kv_heads) head_dim at most 32,768; rotary a multiple of 8, 0 .. head_dim; shifts 1 .. 62. Alignment: q,
+ * k, v, cos and sin 16 bytes and their strides a multiple of 4 elements, q_codes 4 bytes and its stride a multiple of 4, kv 16 bytes. */
+#define SSLM_B200_ROW_SOFTMAX 23
+typedef struct sslm_b200_qkv_site {
+	uint32_t struct_size;
+	int32_t rows, heads, kv_heads, head_dim;
+	int32_t rotary, halves;
+	int32_t num_positions;            /* rows of cos and sin */
+	int32_t num_tables, table_pages;  /* page tables, and entries of each */
+	int32_t q_shift, k_shift;
+	const int32_t *q, *k, *v;         /* [rows][heads, kv_heads, kv_heads][head_dim] */
+	int64_t q_stride, k_stride, v_stride;
+	const int64_t* in_scales;         /* [rows][2] */
+	const int32_t* positions;         /* [rows] */
+	const int32_t* places;            /* [rows] */
+	const int32_t* table_of;          /* [rows] */
+	const int32_t* pages;             /* [num_tables][pages_stride] */
+	int64_t pages_stride;
+	const int32_t *cos, *sin;         /* [num_positions][rotary / 2] */
+	const int16_t *q_gain, *k_gain;   /* [head_dim] */
+	int64_t q_site_m, q_site_e;
+	const int64_t *k_landing, *v_landing;      /* [kv_heads][3] */
+	const int64_t* khead;             /* [kv_heads][2] */
+	int8_t* kv;
+	int64_t num_pages;
+	int8_t* q_codes;                  /* [rows][heads][head_dim] */
+	int64_t q_codes_stride;
+	int64_t* q_scales;                /* [rows][2], may be NULL */
+	int64_t* consts;                  /* [rows][kv_heads][3], may be NULL */
+	int32_t* saturations;             /* [rows], may be NULL */
+	int32_t* row_status;
+	uint64_t reserved;
+} sslm_b200_qkv_site;
+SSLM_API sslm_status sslm_b200_qkv_site_resident(const sslm_b200_qkv_site* call, void* stream);
+
+/* A token drawn from the logits of each row, in integers. Per row, over the tokens v with a logit x_v other than INT32_MIN (as
+ * sslm_b200_pick_resident writes one that is not allowed), with params[r] = slope, cut, top_k, top_p, min_p and d_v = max x - x_v:
+ *   t = floor(d slope / 2^cut);  w_v = floor(P(t mod 2^24) / 2^floor(t / 2^24)), 0 from t = 2^29 on: 2^31 2^(-t / 2^24), P 2^31 at 0 and falling,
+ *       3.4e-6 off at most: P = c0 - hi(f, c1 - hi(f, c2 - hi(f, c3 - hi(f, c4)))), f = 2^8 (t mod 2^24), hi(f, c) = floor(f c / 2^32),
+ *       c = 2147483648, 1488326151, 514119776, 114090822, 14555373
+ *   slope / 2^cut is thus 2^24 times the octaves a logit unit is worth: 2^24 scale / (temperature ln 2)
+ *   kept are, in the order of falling logits, equal ones by rising index: the first top_k (0: all); of these, with S the sum of their w, those in
+ *       front of which less than floor(S top_p / 2^30) lies (2^30: all); of these those with w >= 2 min_p; and never one with w = 0
+ *   the token is the lowest v for which the kept w up to and including it, by index, are more than floor(T draws[r] / 2^31), T their sum
+ * out_tokens[r] is the token, -2 where every logit is INT32_MIN; out_mass[r] its w and T (the token's probability is their quotient), zeros
+ * there; out_kept[r] how many are kept. Each may be NULL, not all. A slope or draw below 0, a cut outside 0 .. 63, a top_k below 0, a top_p outside
+ * 1 .. 2^30 or a min_p outside 0 .. 2^30 refuses the row (SSLM_B200_ROW_CONSTANTS). At most 65,535 rows and 2^20 tokens. */
+typedef struct sslm_b200_sample {
+	uint32_t struct_size;
+	int32_t rows, vocab;
+	uint32_t reserved;
+	const int32_t* logits;            /* [rows][logits_stride] */
+	int64_t logits_stride;
+	const int32_t* params;            /* [rows][5] */
+	const int32_t* draws;             /* [rows] 0 .. 2^31 - 1 */
+	int32_t* out_tokens;              /* [rows] */
+	int64_t* out_mass;                /* [rows][2] */
+	int32_t* out_kept;                /* [rows] */
+	int32_t* row_status;
+} sslm_b200_sample;
+SSLM_API sslm_status sslm_b200_sample_resident(const sslm_b200_sample* call, void* stream);
+
+/* The sequences of a paged cache continue from others, grow or end, all at once: a beam search's step, several answers to one question,
+ * room for the next positions. Sequence i has lengths[i] positions in the pages tables[i]; holders[p] says how many tables (or whoever else) hold
+ * page p, 0: it is free. All inputs are read as they were before the call:
+ *   parents[i] = i    it stays, and takes grow[i] more positions
+ *   parents[i] = p    it becomes a copy of p with grow[i] more positions: p's full pages are held in common, a partly filled one is copied
+ *   parents[i] = -1   it ends
+ * What a sequence held and no longer holds it lets go. Pages that are drawn were free before the call, lowest first, in the order of the
+ * sequences: drawn[0 .. counts[1]) (behind these, free pages that were too few for a sequence may follow). moves[0 .. counts[0]) are the pages
+ * copied, (from, to), whole, in every plane of kv (NULL: none are copied, for a caller whose planes lie apart). Entries of out_tables behind a
+ * sequence's pages, and of moves behind the count, stay as they were. status[i]: 0, or why the sequence stays what it was: a parent that does not exist or a page id of it that does not
+ * (SSLM_B200_ROW_INDEX), a length or growth below 0 or together above the table's room (_LENGTH), not enough free pages for it (_PAGES: those
+ * in front of it are served). Outputs may not overlap inputs. At most 65,535 sequences and 65,536 pages a table; page_bytes a multiple of
+ * 16, kv on a 16-byte boundary, moves on an 8-byte one. Two launches. */
+#define SSLM_B200_ROW_PAGES 102
+typedef struct sslm_b200_fork {
+	uint32_t struct_size;
+	int32_t sequences, table_pages, planes, page_bytes;
+	uint32_t reserved;
+	int64_t num_pages;
+	int8_t* kv;                       /* [planes][num_pages][page_bytes]: of the pool of sslm_b200_attention_prefix_resident, 2 kv_heads planes a layer */
+	const int32_t* holders;           /* [num_pages] */
+	const int32_t* tables;            /* [sequences][tables_stride] */
+	int64_t tables_stride;
+	const int32_t* lengths;           /* [sequences] */
+	const int32_t* parents;           /* [sequences] */
+	const int32_t* grow;              /* [sequences], NULL: zeros */
+	int32_t* out_holders;             /* [num_pages] */
+	int32_t* out_tables;              /* [sequences][out_stride] */
+	int64_t out_stride;
+	int32_t* out_lengths;             /* [sequences] */
+	int32_t* drawn;                   /* [num_pages] */
+	int32_t* moves;                   /* [sequences][2] */
+	int32_t* counts;                  /* [2] moves, pages drawn */
+	int32_t* status;                  /* [sequences] */
+} sslm_b200_fork;
+SSLM_API sslm_status sslm_b200_fork_resident(const sslm_b200_fork* call, void* stream);
+
+/* The pages in use (holders above or below 0) move to the front of the pool: with `live` of them, those at live and behind go to the free ones
+ * in front of it, the lowest to the lowest. new_of[p] is page p's new id, -1 where it is free; moves[0 .. counts[0]) are (from, to), copied in every
+ * plane of kv (NULL: not); counts[1] = live. out_holders and out_tables are holders and tables under the new ids; entries behind a sequence's
+ * pages, and of moves behind the count, stay as they were. status[i] (may be NULL): 0, or a length below 0 or above the table's room
+ * (SSLM_B200_ROW_LENGTH), a page id that does not exist or is free (_INDEX): such a table is not written. out_tables may be tables; other
+ * outputs may not overlap inputs. Limits and alignment as above. Two launches. */
+typedef struct sslm_b200_compact {
+	uint32_t struct_size;
+	int32_t sequences, table_pages, planes, page_bytes;
+	uint32_t reserved;
+	int64_t num_pages;
+	int8_t* kv;
+	const int32_t* holders;           /* [num_pages] */
+	const int32_t* tables;            /* [sequences][tables_stride] */
+	int64_t tables_stride;
+	const int32_t* lengths;           /* [sequences] */
+	int32_t* out_holders;             /* [num_pages] */
+	int32_t* out_tables;              /* [sequences][out_stride] */
+	int64_t out_stride;
+	int32_t* new_of;                  /* [num_pages] */
+	int32_t* moves;                   /* [num_pages / 2][2] */
+	int32_t* counts;                  /* [2] moves, pages in use */
+	int32_t* status;                  /* [sequences], may be NULL */
+} sslm_b200_compact;
+SSLM_API sslm_status sslm_b200_compact_resident(const sslm_b200_compact* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

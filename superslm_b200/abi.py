@@ -16,6 +16,7 @@ chunked prefill, per-call decode.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 import struct
 
@@ -319,6 +320,35 @@ class PickArgs(C.Structure):
                 ("out_best", C.c_void_p), ("out_logits", C.c_void_p), ("out_stride", C.c_int64), ("row_status", C.c_void_p)]
 
 
+class QkvSiteArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32 if n == "struct_size" else C.c_int32) for n in ("struct_size", "rows", "heads", "kv_heads", "head_dim", "rotary", "halves", "num_positions",
+                                                                               "num_tables", "table_pages", "q_shift", "k_shift")] +
+                [(n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride")] +
+                [(n, C.c_void_p) for n in ("in_scales", "positions", "places", "table_of", "pages")] + [("pages_stride", C.c_int64)] +
+                [(n, C.c_void_p) for n in ("cos", "sin", "q_gain", "k_gain")] + [("q_site_m", C.c_int64), ("q_site_e", C.c_int64)] +
+                [(n, C.c_void_p) for n in ("k_landing", "v_landing", "khead", "kv")] + [("num_pages", C.c_int64), ("q_codes", C.c_void_p), ("q_codes_stride", C.c_int64)] +
+                [(n, C.c_void_p) for n in ("q_scales", "consts", "saturations", "row_status")] + [("reserved", C.c_uint64)])
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("vocab", C.c_int32), ("reserved", C.c_uint32), ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+                ("params", C.c_void_p), ("draws", C.c_void_p), ("out_tokens", C.c_void_p), ("out_mass", C.c_void_p), ("out_kept", C.c_void_p), ("row_status", C.c_void_p)]
+
+
+_PAGES_HEAD = [("struct_size", C.c_uint32), ("sequences", C.c_int32), ("table_pages", C.c_int32), ("planes", C.c_int32), ("page_bytes", C.c_int32), ("reserved", C.c_uint32),
+               ("num_pages", C.c_int64), ("kv", C.c_void_p), ("holders", C.c_void_p), ("tables", C.c_void_p), ("tables_stride", C.c_int64), ("lengths", C.c_void_p)]
+
+
+class ForkArgs(C.Structure):
+    _fields_ = _PAGES_HEAD + [("parents", C.c_void_p), ("grow", C.c_void_p), ("out_holders", C.c_void_p), ("out_tables", C.c_void_p), ("out_stride", C.c_int64),
+                              ("out_lengths", C.c_void_p), ("drawn", C.c_void_p), ("moves", C.c_void_p), ("counts", C.c_void_p), ("status", C.c_void_p)]
+
+
+class CompactArgs(C.Structure):
+    _fields_ = _PAGES_HEAD + [("out_holders", C.c_void_p), ("out_tables", C.c_void_p), ("out_stride", C.c_int64), ("new_of", C.c_void_p), ("moves", C.c_void_p),
+                              ("counts", C.c_void_p), ("status", C.c_void_p)]
+
+
 class _ResidentCall:
     def __init__(self, lib: SslmLib, verb: str, args):
         self._fn = getattr(lib.dll, verb)
@@ -438,6 +468,124 @@ class Pick(_ResidentCall):
         a.out_logits = self._hold("out_logits", out_logits, "int32", (rows, vocab), True)
         a.out_stride = self._row_stride(out_logits, vocab)
         a.row_status = self._hold("row_status", row_status, "int32", (rows,))
+
+
+class QkvSite(_ResidentCall):
+    """sslm_b200_qkv_site_resident. q int32 [rows, heads, head_dim], k and v int32 [rows, kv_heads, head_dim] (rows may be strided: parts of one
+    projection's rows; q, or k and v, may be None), in_scales int64 [rows, 2], positions int32 [rows], cos and sin int32 [positions, rotary / 2];
+    kv int8 [kv_heads, 2, pages, 16 * head_dim] with pages int32 [tables, n], places and table_of int32 [rows] or None; q_codes int8 [rows, heads,
+    head_dim] (rows may be strided), q_scales int64 [rows, 2], consts int64 [rows, kv_heads, 3] with khead int64 [kv_heads, 2], saturations and row_status
+    int32 [rows]. q_site = (m, e). k_landing and v_landing int64 [kv_heads, 3]; q_gain and k_gain int16 [head_dim] with gain_shift (k_gain_shift: K's, where it
+    is another one). halves: channels i and i + rotary / 2 turn together, else neighbours."""
+
+    def __init__(self, lib, q, k, v, in_scales, positions, cos, sin, q_codes=None, kv=None, pages=None, places=None, table_of=None, q_site=(1 << 30, -30), khead=None,
+                 k_landing=None, v_landing=None, q_gain=None, k_gain=None, gain_shift=1, k_gain_shift=None, halves=False, q_scales=None, consts=None, saturations=None,
+                 row_status=None):
+        a = QkvSiteArgs()
+        super().__init__(lib, "sslm_b200_qkv_site_resident", a)
+        if (k is None) != (v is None) or (q is None and k is None):
+            raise ValueError("q, or k and v, or all three")
+        rows, hd = (q if q is not None else k).shape[0], (q if q is not None else k).shape[2]
+        heads, kv_heads = 0 if q is None else q.shape[1], k.shape[1] if k is not None else (khead.shape[0] if khead is not None else 1)
+        a.rows, a.heads, a.kv_heads, a.head_dim, a.halves = rows, heads, kv_heads, hd, int(halves)
+        a.q, a.q_stride = self._hold("q", q, "int32", (rows, heads, hd), True), self._row_stride(q, heads * hd)
+        a.k, a.k_stride = self._hold("k", k, "int32", (rows, kv_heads, hd), True), self._row_stride(k, kv_heads * hd)
+        a.v, a.v_stride = self._hold("v", v, "int32", (rows, kv_heads, hd), True), self._row_stride(v, kv_heads * hd)
+        a.in_scales = self._hold("in_scales", in_scales, "int64", (rows, 2))
+        a.positions = self._hold("positions", positions, "int32", (rows,))
+        a.num_positions, a.rotary = cos.shape[0], 2 * cos.shape[1]
+        a.cos, a.sin = self._hold("cos", cos, "int32", (None, None)), self._hold("sin", sin, "int32", tuple(cos.shape))
+        a.q_site_m, a.q_site_e = q_site
+        a.q_gain, a.k_gain = self._hold("q_gain", q_gain, "int16", (hd,)), self._hold("k_gain", k_gain, "int16", (hd,))
+        a.q_shift, a.k_shift = gain_shift, gain_shift if k_gain_shift is None else k_gain_shift
+        a.khead = self._hold("khead", khead, "int64", (kv_heads, 2))
+        if k is not None:
+            a.places, a.table_of = self._hold("places", places, "int32", (rows,)), self._hold("table_of", table_of, "int32", (rows,))
+            a.pages, a.pages_stride = self._hold("pages", pages, "int32", (None, None), True), self._row_stride(pages, pages.shape[1])
+            a.num_tables, a.table_pages = pages.shape
+            a.k_landing, a.v_landing = self._hold("k_landing", k_landing, "int64", (kv_heads, 3)), self._hold("v_landing", v_landing, "int64", (kv_heads, 3))
+            a.kv, a.num_pages = self._hold("kv", kv, "int8", (kv_heads, 2, None, 16 * hd)), kv.shape[2]
+        a.q_codes, a.q_codes_stride = self._hold("q_codes", q_codes, "int8", (rows, heads, hd), True), self._row_stride(q_codes, heads * hd)
+        a.q_scales = self._hold("q_scales", q_scales, "int64", (rows, 2))
+        a.consts = self._hold("consts", consts, "int64", (rows, kv_heads, 3))
+        a.saturations = self._hold("saturations", saturations, "int32", (rows,))
+        a.row_status = self._hold("row_status", row_status, "int32", (rows,))
+
+
+def sample_params(scale, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A row of `params` for Sample: scale is what a logit unit is worth in natural units (logit = int32 value * scale)."""
+    octaves = scale / (temperature * math.log(2)) * (1 << 24)
+    f, e = math.frexp(octaves)                       # octaves = f 2^e, 1/2 <= f < 1
+    slope, cut = int(round(f * (1 << 31))), 31 - e
+    if slope == 1 << 31:
+        slope, cut = 1 << 30, cut - 1
+    if cut > 63:
+        slope, cut = slope >> min(31, cut - 63), 63
+    elif cut < 0:                                    # (64 octaves a unit are as good as more)
+        slope, cut = 1 << 30, 0
+    return [slope, cut, top_k, max(1, min(1 << 30, int(top_p * (1 << 30)))), int(min_p * (1 << 30))]
+
+
+class Sample(_ResidentCall):
+    """sslm_b200_sample_resident. logits int32 [rows, vocab] (rows may be strided), params int32 [rows, 5] (slope, cut, top_k, top_p, min_p; sample_params
+    makes a row), draws int32 [rows]; out_tokens and out_kept int32 [rows], out_mass int64 [rows, 2], row_status int32 [rows]; what is None is left out."""
+
+    def __init__(self, lib, logits, params, draws, out_tokens=None, out_mass=None, out_kept=None, row_status=None):
+        a = SampleArgs()
+        super().__init__(lib, "sslm_b200_sample_resident", a)
+        rows, vocab = logits.shape
+        a.rows, a.vocab = rows, vocab
+        a.logits, a.logits_stride = self._hold("logits", logits, "int32", (rows, vocab), True), self._row_stride(logits, vocab)
+        a.params = self._hold("params", params, "int32", (rows, 5))
+        a.draws = self._hold("draws", draws, "int32", (rows,))
+        a.out_tokens = self._hold("out_tokens", out_tokens, "int32", (rows,))
+        a.out_mass = self._hold("out_mass", out_mass, "int64", (rows, 2))
+        a.out_kept = self._hold("out_kept", out_kept, "int32", (rows,))
+        a.row_status = self._hold("row_status", row_status, "int32", (rows,))
+
+
+class _PagesCall(_ResidentCall):
+    def _cache(self, a, kv, holders, tables, lengths, out_holders, out_tables, moves, most_moves, counts, status):
+        n, pages = tables.shape[0], holders.shape[0]
+        a.sequences, a.table_pages, a.num_pages = n, tables.shape[1], pages
+        if kv is not None:
+            if len(kv.shape) < 3 or kv.shape[-2] != pages:
+                raise ValueError("kv: [..., %d pages, bytes] expected, got %s" % (pages, list(kv.shape)))
+            a.kv, a.page_bytes, a.planes = self._hold("kv", kv, "int8", tuple(kv.shape)), kv.shape[-1], math.prod(kv.shape[:-2])
+        a.holders = self._hold("holders", holders, "int32", (pages,))
+        a.tables, a.tables_stride = self._hold("tables", tables, "int32", (n, None), True), self._row_stride(tables, tables.shape[1])
+        a.lengths = self._hold("lengths", lengths, "int32", (n,))
+        a.out_holders = self._hold("out_holders", out_holders, "int32", (pages,))
+        a.out_tables, a.out_stride = self._hold("out_tables", out_tables, "int32", tuple(tables.shape), True), self._row_stride(out_tables, tables.shape[1])
+        a.moves, a.counts = self._hold("moves", moves, "int32", (most_moves, 2)), self._hold("counts", counts, "int32", (2,))
+        a.status = self._hold("status", status, "int32", (n,))
+
+
+class Fork(_PagesCall):
+    """sslm_b200_fork_resident. kv int8 [..., pages, page bytes] (all planes of the pool, or None: nothing is copied), holders int32 [pages], tables int32 [sequences, n]
+    (rows may be strided), lengths, parents and grow (or None) int32 [sequences]; out_holders, out_tables and out_lengths as their inputs, drawn int32
+    [pages], moves int32 [sequences, 2], counts int32 [2], status int32 [sequences]."""
+
+    def __init__(self, lib, kv, holders, tables, lengths, parents, out_holders, out_tables, out_lengths, drawn, moves, counts, status, grow=None):
+        a = ForkArgs()
+        super().__init__(lib, "sslm_b200_fork_resident", a)
+        n, pages = tables.shape[0], holders.shape[0]
+        self._cache(a, kv, holders, tables, lengths, out_holders, out_tables, moves, n, counts, status)
+        a.parents, a.grow = self._hold("parents", parents, "int32", (n,)), self._hold("grow", grow, "int32", (n,))
+        a.out_lengths = self._hold("out_lengths", out_lengths, "int32", (n,))
+        a.drawn = self._hold("drawn", drawn, "int32", (pages,))
+
+
+class Compact(_PagesCall):
+    """sslm_b200_compact_resident. kv, holders, tables, lengths as for Fork; out_holders and out_tables as their inputs (out_tables may be tables), new_of int32
+    [pages], moves int32 [pages // 2, 2], counts int32 [2], status int32 [sequences] or None."""
+
+    def __init__(self, lib, kv, holders, tables, lengths, out_holders, out_tables, new_of, moves, counts, status=None):
+        a = CompactArgs()
+        super().__init__(lib, "sslm_b200_compact_resident", a)
+        pages = holders.shape[0]
+        self._cache(a, kv, holders, tables, lengths, out_holders, out_tables, moves, pages // 2, counts, status)
+        a.new_of = self._hold("new_of", new_of, "int32", (pages,))
 
 
 def parse_save_blob(blob: bytes, hidden_size: int) -> dict:

@@ -91,8 +91,8 @@ inline int sm_count() {
 // with four bytes more than will come: that block's wait runs out. One word: 0 for none, else
 // kernel << 8 | exchange + 1.
 // (4 names no kernel; 5 is the fifth exchange of attention with the q/k/v site of biased rows inside)
-// (6: attention of rows that share a prefix; 7: the pick)
-enum ExchangeKernel { kExchangeLinear = 0, kExchangeAttnFew, kExchangeAttnChunk, kExchangeAct, kExchangeAttnSite = 5, kExchangeAttnPrefix, kExchangePick, kExchangeKernels };
+// (6: attention of rows that share a prefix; 7: the pick; 8: the draw)
+enum ExchangeKernel { kExchangeLinear = 0, kExchangeAttnFew, kExchangeAttnChunk, kExchangeAct, kExchangeAttnSite = 5, kExchangeAttnPrefix, kExchangePick, kExchangeSample, kExchangeKernels };
 inline std::atomic<uint32_t> g_withheld_exchange{0};
 inline int exchange_debug_take(ExchangeKernel kernel) {
 	uint32_t w = g_withheld_exchange.load(std::memory_order_relaxed);
@@ -205,6 +205,10 @@ void launch_lora_u(const RowBatch& b, const int8_t* x, int k_in, int layer, int 
 constexpr int kPickMaxBias = 1024;      // biases of a row
 // best[r] of the rows whose record has logits; names: ids that a row's history, its extra one and its biases have at most, biases of them
 cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* status, cudaStream_t st);
+
+// ---- the draw of rows whose sequences are sampled (sslm_sample.cu): best[r] of the rows whose record has logits; scales: of the rows
+// that the head multiplied
+cudaError_t launch_sample(const SampleRow* rows, int m, int vocab, const Scale* scales, unsigned long long* best, int32_t* status, cudaStream_t st);
 
 // ---- attention over the paged KV pool (sslm_attn.cu)
 cudaError_t attn_configure(const Dims& d);

@@ -88,6 +88,14 @@ struct PickRow {
 	int32_t layer, pad;
 };
 
+// What the token of one row is drawn from (sslm_sample.cu).
+struct SampleRow {
+	const int32_t* logits;                      // nullptr: the row is not sampled
+	int64_t slope_m, slope_e;                   // octaves a logit unit of a row of scale one
+	uint32_t draw, top_p, min_p;                // 31 bits, and shares of 2^30
+	int32_t top_k, layer, pad;
+};
+
 struct RowSource { const int8_t* hidden; const Scale* scale; };  // nullptr hidden: embed rows[r].token
 struct RowSink { int8_t* hidden; Scale* scale; };                // nullptr hidden: drop
 
