@@ -11,12 +11,15 @@
 // The polynomial is the fit of the smallest largest relative error (3.3e-6) with the values 1 and 1/2 at the ends, its last coefficients rounded
 // up by less than one part in 10^7, which leaves it falling from octave to octave too (checked for all 2^24 arguments): w falls with d.
 //
-// Two passes over the logits. The first finds the row's maximum and a bound that is likely to lie below what is kept and above nearly all else: the
-// least of the maxima of some hundred groups of threads. g groups leave about g ln g tokens above it (and g at least). The second pass
-// lists these tokens, a few hundred to a few thousand, and adds up all weights where top-p needs that. What is kept is then cut and drawn
-// from the list by counting into 2,048 places. Where the list does not reach far enough (its weights, or its length, tell) or overflows, the
-// same counting goes over the whole row. Rows without top-k and top-p need no list: sums of 128 neighbouring tokens are enough to find
-// the token.
+// Two passes over the logits. The first finds the row's maximum and a bound that is likely to lie below what is kept and above nearly all else:
+// the least of the maxima of g groups of threads, which leaves about g (ln g + 0.6) tokens above it, and g at least. The second pass lists these tokens,
+// a few hundred to two thousand, and adds up the weights where top-p needs that. The list is sorted, cut by its running sums, and what is kept
+// sorted by index for the draw. Rows without top-k and top-p need no list: sums of 128 neighbouring tokens are enough to find the token.
+//
+// Where top-p keeps more than the list has (the sums tell), a sample of the row says where the end of what is kept must lie; a pass adds up
+// what is surely kept and lists a window around that end, which is cut as the list is; then the sums of 128 tokens as above. Whatever
+// does not work out that way (a list that overflows, a top-k beyond some thousands) is counted into 2,048 places, and those of the place that holds
+// the end again, by one block over the whole row.
 //
 // A row is cut over the blocks of a cluster while rows are few; they exchange maxima and sums, and send their lists to the first one.
 #include <cuda_runtime.h>
@@ -37,6 +40,9 @@ constexpr int kIndexBits = 20;                // of a token
 constexpr int kMostVocab = 1 << kIndexBits;
 constexpr int kMostSlice = (kPlaces - 2) * 128 & ~127;      // a sum for every 128 tokens, and for the ends
 constexpr uint32_t kLate = 0xFFFFFFFFu;
+// exchanges, in order: maxima and bounds; sums and lists' lengths; the lists; and where the list is too short the window's ends, its sums, its
+// lists, the last key that is kept, sums and numbers of what is kept
+enum { kTop = 0, kSums, kLists, kEnds, kWindow, kWindowLists, kBound, kKept, kBars };
 
 struct SampleArgs {
 	int rows, vocab, shift, slice;      // a row is cut over 1 << shift blocks of `slice` tokens (a multiple of 128)
@@ -99,6 +105,71 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, un
 #pragma unroll
 	for (int i = 0; i < kWarps; ++i) all += s[i];
 	return all;
+}
+
+// ---- the keys of a block in rising order, E of them a thread (thread t those at E t ..), by a bitonic network: partners in the thread, in the warp,
+// or by way of `room` (E * kThreads words)
+template <int E>
+__device__ __forceinline__ void sort_keys(unsigned long long (&x)[E], unsigned long long* room) {
+	const int t = threadIdx.x;
+#pragma unroll 1
+	for (int k = 2; k <= E * kThreads; k *= 2) {
+#pragma unroll 1
+		for (int j = k / 2; j >= E; j /= 2) {
+			const int far = j / E;      // threads apart
+			const bool up = ((E * t) & k) == 0, low = (t & far) == 0;
+			unsigned long long y[E];
+			if (far >= 32) {
+				__syncthreads();
+#pragma unroll
+				for (int e = 0; e < E; ++e) room[e * kThreads + t] = x[e];
+				__syncthreads();
+#pragma unroll
+				for (int e = 0; e < E; ++e) y[e] = room[e * kThreads + (t ^ far)];
+			} else {
+#pragma unroll
+				for (int e = 0; e < E; ++e) y[e] = __shfl_xor_sync(0xffffffffu, x[e], far);
+			}
+#pragma unroll
+			for (int e = 0; e < E; ++e) x[e] = (low == up) == (x[e] < y[e]) ? x[e] : y[e];
+		}
+#pragma unroll
+		for (int j = E / 2; j > 0; j /= 2) {
+			if (j >= k) continue;
+#pragma unroll
+			for (int e = 0; e < E; ++e) {
+				if ((e & j) != 0) continue;
+				const bool up = ((E * t + e) & k) == 0;
+				const unsigned long long a = x[e], b = x[e | j];
+				x[e] = (a < b) == up ? a : b;
+				x[e | j] = (a < b) == up ? b : a;
+			}
+		}
+	}
+}
+// sums of v over the elements in front of each of a thread's own, in that order
+template <int E>
+__device__ __forceinline__ void sums_before(const uint32_t (&v)[E], unsigned long long (&before)[E], unsigned long long* s) {
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	unsigned long long mine = 0;
+#pragma unroll
+	for (int e = 0; e < E; ++e) mine += v[e];
+	unsigned long long upto = mine;
+#pragma unroll
+	for (int o = 1; o < 32; o *= 2) {
+		const unsigned long long z = __shfl_up_sync(0xffffffffu, upto, o);
+		if (lane >= o) upto += z;
+	}
+	__syncthreads();
+	if (lane == 31) s[warp] = upto;
+	__syncthreads();
+	unsigned long long at = upto - mine;
+	for (int i = 0; i < warp; ++i) at += s[i];
+#pragma unroll
+	for (int e = 0; e < E; ++e) {
+		before[e] = at;
+		at += v[e];
+	}
 }
 
 // ---- selection: of elements with keys that differ and weights, the first one, by rising keys, up to which (itself included) more than
@@ -193,13 +264,90 @@ struct SampleSmem {
 	static size_t bytes(int keep, int slice) { return (size_t)kList * 8 + (size_t)kPlaces * 12 + (keep ? (size_t)slice * 4 + 16 : 0); }
 };
 
+// What a list of a row is cut by, and what came of it.
+struct Cut {
+	uint32_t most, slope, cut, floor_w, top_p, draw;
+	int top_k;
+	unsigned long long sum;      // of all weights, where top-k does not say what counts
+};
+struct Drawn {
+	int token;
+	uint32_t weight, number;
+	unsigned long long sum;
+};
+__device__ __forceinline__ uint32_t key_weight(unsigned long long key, const Cut& c) { return weight_of((uint32_t)(key >> kIndexBits), c.most, c.slope, c.cut); }
+
+// The list in the order of falling logits, cut, and drawn from. n <= E * kThreads keys, which are overwritten. For the threads of a whole block.
+template <int E>
+__device__ __noinline__ Drawn draw_sorted(unsigned long long* list, int n, const Cut& c, unsigned long long* s_scan, Drawn* s_drawn) {
+	const int t = threadIdx.x, lane = t & 31;
+	unsigned long long x[E], before[E];
+	uint32_t w[E];
+#pragma unroll
+	for (int e = 0; e < E; ++e) x[e] = E * t + e < n ? list[E * t + e] : ~0ull;
+	__syncthreads();
+	sort_keys<E>(x, list);
+	unsigned long long sum = 0;
+	const int limit = c.top_k > 0 ? min(n, c.top_k) : n;
+#pragma unroll
+	for (int e = 0; e < E; ++e) {
+		w[e] = E * t + e < limit ? key_weight(x[e], c) : 0u;
+		sum += w[e];
+	}
+	sum = c.top_k > 0 ? block_sum(sum, s_scan) : c.sum;
+	const unsigned long long enough = c.top_p < (1u << 30) ? share_of(sum, c.top_p, 30) : ~0ull;
+	sums_before<E>(w, before, s_scan);
+	unsigned long long mass = 0;
+	uint32_t many = 0;
+#pragma unroll
+	for (int e = 0; e < E; ++e) {
+		const bool yes = before[e] < enough && w[e] >= c.floor_w;
+		if (!yes) w[e] = 0u;
+		mass += w[e];
+		many += yes ? 1u : 0u;
+	}
+	mass = block_sum(mass, s_scan);
+	const int kept = (int)block_sum(many, s_scan);      // (the first so many)
+	const unsigned long long mark = share_of(mass, c.draw, 31);
+	// by index
+	if (kept <= 32) {
+#pragma unroll
+		for (int e = 0; e < E; ++e)
+			if (E * t + e < kept) list[E * t + e] = (x[e] & (kMostVocab - 1)) << 32 | w[e];
+		__syncthreads();
+		if (t < 32) {
+			const unsigned long long mine = lane < kept ? list[lane] : ~0ull;
+			unsigned long long less = 0;
+			for (int i = 0; i < kept; ++i) {
+				const unsigned long long y = list[i];
+				if (y < mine) less += (uint32_t)y;
+			}
+			if (lane < kept && less <= mark && mark < less + (uint32_t)mine) *s_drawn = Drawn{(int)(mine >> 32), (uint32_t)mine, (uint32_t)kept, mass};
+		}
+	} else {
+#pragma unroll
+		for (int e = 0; e < E; ++e) x[e] = E * t + e < kept ? (x[e] & (kMostVocab - 1)) << 32 | w[e] : ~0ull;
+		sort_keys<E>(x, list);
+#pragma unroll
+		for (int e = 0; e < E; ++e) w[e] = E * t + e < kept ? (uint32_t)x[e] : 0u;
+		sums_before<E>(w, before, s_scan);
+#pragma unroll
+		for (int e = 0; e < E; ++e)
+			if (before[e] <= mark && mark < before[e] + w[e]) *s_drawn = Drawn{(int)(x[e] >> 32), w[e], (uint32_t)kept, mass};
+	}
+	__syncthreads();
+	return *s_drawn;
+}
+
 template <bool RESIDENT, bool KEEP>
 __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_constant__ SampleArgs a) {
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ __align__(8) unsigned long long s_bar[3], s_sum[16], s_scan[kWarps];
-	__shared__ int2 s_top[16], s_warp[kWarps];
-	__shared__ uint32_t s_count[16], s_n;
+	__shared__ __align__(8) unsigned long long s_bar[kBars], s_sum[2][16], s_scan[kWarps], s_bound;
+	__shared__ int2 s_top[16], s_warp[kWarps], s_ends;
+	__shared__ uint32_t s_count[2][16], s_n;
 	__shared__ Row s_row;
+	__shared__ Drawn s_drawn;
+	__shared__ unsigned long long s_listed[2][16];
 	__shared__ SelectSmem s_select;
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
@@ -207,12 +355,19 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	unsigned long long* list = (unsigned long long*)smem;
 	const Place places{list + kList, (uint32_t*)(list + kList + kPlaces)};
 	int4* kept = (int4*)(places.count + kPlaces);
-	const int held = (blockIdx.x | blockIdx.y) == 0 ? a.debug_withhold : 0;
+	// 1 + the exchange that is made to run out, in the first block, or where the first one only sends, in the second
+	const bool sends = a.debug_withhold == 1 + kEnds || a.debug_withhold == 1 + kBound;
+	const int held = blockIdx.y == 0 && rank == (sends ? 1 : 0) ? a.debug_withhold : 0;
 	if (t == 0) {
 		if (sub > 1) {
-			exchange_init(cta_addr(&s_bar[0]), (uint32_t)(sub * 8) + (held == 1 ? 4u : 0u));
-			exchange_init(cta_addr(&s_bar[1]), (uint32_t)(sub * 12) + (held == 2 ? 4u : 0u));
-			ring_init(cta_addr(&s_bar[2]), 1);      // (armed when the lists' lengths are known)
+			exchange_init(cta_addr(&s_bar[kTop]), (uint32_t)(sub * 8) + (held == 1 + kTop ? 4u : 0u));
+			exchange_init(cta_addr(&s_bar[kSums]), (uint32_t)(sub * 20) + (held == 1 + kSums ? 4u : 0u));
+			ring_init(cta_addr(&s_bar[kLists]), 1);      // (armed when the lists' lengths are known)
+			exchange_init(cta_addr(&s_bar[kEnds]), 8u + (held == 1 + kEnds ? 4u : 0u));
+			exchange_init(cta_addr(&s_bar[kWindow]), (uint32_t)(sub * 20) + (held == 1 + kWindow ? 4u : 0u));
+			ring_init(cta_addr(&s_bar[kWindowLists]), 1);
+			exchange_init(cta_addr(&s_bar[kBound]), 8u + (held == 1 + kBound ? 4u : 0u));
+			exchange_init(cta_addr(&s_bar[kKept]), (uint32_t)(sub * 12) + (held == 1 + kKept ? 4u : 0u));
 			exchange_fence_init();
 		}
 		s_n = 0u;
@@ -267,18 +422,45 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	const int heads = first - s0, tails = s1 - last;
 	const int end = t < heads ? s0 + t : (t >= 4 && t - 4 < tails ? last + t - 4 : -1);      // the token of the ends that is this thread's
 	const int32_t end_x = end >= 0 ? w.logits[end] : INT32_MIN;
+	constexpr int U = 4;
+	const int rounds = (words + U * kThreads - 1) / (U * kThreads);      // of U words a thread
+	auto word = [&](int k) { return KEEP ? kept[k] : __ldcg(from + k); };
+	// f(the word, its first token), over the block's words, from the last ones on (what was read last is likelier still in L2)
+	auto each_word = [&](auto f) {
+#pragma unroll 1
+		for (int i = rounds - 1; i >= 0; --i) {
+			const int k = i * U * kThreads + t;
+			int4 q[U];
+#pragma unroll
+			for (int u = 0; u < U; ++u)
+				if (k + u * kThreads < words) q[u] = word(k + u * kThreads);
+#pragma unroll
+			for (int u = 0; u < U; ++u)
+				if (k + u * kThreads < words) f(q[u], first + 4 * (k + u * kThreads));
+		}
+	};
+	// a wait ran out: the row is reported, and the block stays until nothing can be sent to it any more
+	auto give_up = [&](bool stay) {
+		if (t == 0) {
+			if (RESIDENT) {
+				if (a.status != nullptr) a.status[r] = kInternalWaitTimeout;
+			} else {
+				atomicCAS(&a.status[r], 0, pack_status(kInternalWaitTimeout, kSiteLogits, w.layer));
+			}
+		}
+		if (stay) exchange_leave(cta_addr(&s_bar[0]), kBars);
+	};
 
 	// ---- the maximum, and the least of the groups' maxima
 	int32_t top = end_x;
-	constexpr int U = 8;
 #pragma unroll 1
-	for (int k = t; k < words; k += U * kThreads) {
-		int4 q[U];
+	for (int k = t; k < words; k += 2 * U * kThreads) {
+		int4 q[2 * U];
 #pragma unroll
-		for (int u = 0; u < U; ++u)
+		for (int u = 0; u < 2 * U; ++u)
 			if (k + u * kThreads < words) q[u] = __ldcg(from + k + u * kThreads);
 #pragma unroll
-		for (int u = 0; u < U; ++u)
+		for (int u = 0; u < 2 * U; ++u)
 			if (k + u * kThreads < words) {
 				if (KEEP) kept[k + u * kThreads] = q[u];
 				top = max(top, max(max(q[u].x, q[u].y), max(q[u].z, q[u].w)));
@@ -286,14 +468,21 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	}
 	const bool cuts = w.top_k > 0 || w.top_p < (1u << 30);
 	int32_t least = INT32_MAX;
+	int group = 1;      // threads of a group, over all blocks 256 groups, or as many as there are tokens to keep
 	if (cuts) {
-		const int wanted = w.top_k > 0 && w.top_k <= 64 ? 128 : 512, lanes = max(1, min(32, sub * kThreads / wanted));
-		least = t < words || end >= 0 ? top : INT32_MIN;
-		for (int o = 1; o < lanes; o *= 2) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
+		int wanted = 256;
+		if (w.top_k > 0) {
+			wanted = 32;
+			while (wanted < min(w.top_k, 512)) wanted *= 2;
+		}
+		group = max(1, min(kThreads, sub * kThreads / wanted));
+		const bool has = t < words || end >= 0;
+		least = has ? top : INT32_MIN;
+		for (int o = 1; o < min(group, 32); o *= 2) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
 		// (threads without a token count only where their whole group has none)
-		const uint32_t has = __ballot_sync(0xffffffffu, t < words || end >= 0);
-		const uint32_t group = lanes == 32 ? 0xFFFFFFFFu : ((1u << lanes) - 1u) << (lane & ~(lanes - 1));
-		if ((has & group) == 0u) least = INT32_MAX;
+		const uint32_t any = __ballot_sync(0xffffffffu, has);
+		const uint32_t mates = group >= 32 ? 0xFFFFFFFFu : ((1u << group) - 1u) << (lane & ~(group - 1));
+		if ((any & mates) == 0u) least = INT32_MAX;
 	}
 	{
 		const int32_t m = __reduce_max_sync(0xffffffffu, top), l = __reduce_min_sync(0xffffffffu, least);
@@ -303,165 +492,389 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	{
 		const int2 x = s_warp[lane & (kWarps - 1)];
 		top = __reduce_max_sync(0xffffffffu, x.x);
-		least = __reduce_min_sync(0xffffffffu, x.y);
+		least = x.y;
+		for (int o = 1; o < group / 32; o *= 2) {
+			const int32_t y = __shfl_xor_sync(0xffffffffu, least, o);
+			least = least == INT32_MAX ? y : (y == INT32_MAX ? least : max(least, y));
+		}
+		least = __reduce_min_sync(0xffffffffu, least);
 		if (top == INT32_MIN) least = INT32_MAX;      // (nothing is allowed here)
 	}
 	bool late = false;
 	if (sub > 1) {
 		cluster_wait();      // (all blocks run)
-		if (t < sub) exchange_send(&s_top[rank], cta_addr(&s_bar[0]), (uint32_t)t, make_int2(top, least));
-		late = !exchange_wait(cta_addr(&s_bar[0]));
+		if (t < sub) exchange_send(&s_top[rank], cta_addr(&s_bar[kTop]), (uint32_t)t, make_int2(top, least));
+		late = !exchange_wait(cta_addr(&s_bar[kTop]));
 		const int2 x = s_top[lane & (sub - 1)];
 		top = __reduce_max_sync(0xffffffffu, x.x);
 		least = __reduce_min_sync(0xffffffffu, x.y);
+		late = __syncthreads_or(late) != 0;
 	}
-	late = __syncthreads_or(late) != 0;
 	const bool none = top == INT32_MIN;
+	const uint32_t most = farthest(w.slope, w.cut), floor_w = max(1u, 2u * w.min_p);
+	auto weight = [&](int32_t x) { return x != INT32_MIN ? weight_of((uint32_t)top - (uint32_t)x, most, w.slope, w.cut) : 0u; };
+	auto put = [&](int32_t x, int v) {
+		const uint32_t at = atomicAdd(&s_n, 1u);
+		if (at < (uint32_t)kList) list[at] = (unsigned long long)((uint32_t)top - (uint32_t)x) << kIndexBits | (uint32_t)v;
+	};
+	// sums over all tokens that counts() names, of 128 neighbours each: places 1 .. , the ends at 0 and behind
+	unsigned long long sum = 0, listed = 0;
+	uint32_t count = 0;
+	const int steps = (words + 31) / 32 + 2;
+	auto add_steps = [&](auto counts) {
+		if (t < 2) places.sum[t == 0 ? 0 : steps - 1] = 0ull;
+		__syncthreads();
+		if (end >= 0) {
+			const uint32_t g = counts(end_x, end);
+			sum += g;
+			count += g != 0u ? 1u : 0u;
+			atomicAdd(&places.sum[t < 4 ? 0 : steps - 1], (unsigned long long)g);
+		}
+#pragma unroll 1
+		for (int i = rounds - 1; i >= 0; --i) {
+			const int k = i * U * kThreads + t;
+			int4 q[U];
+#pragma unroll
+			for (int u = 0; u < U; ++u) q[u] = k + u * kThreads < words ? word(k + u * kThreads) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+#pragma unroll
+			for (int u = 0; u < U; ++u) {
+				const int at = k + u * kThreads, v = first + 4 * at;
+				const uint32_t g0 = counts(q[u].x, v), g1 = counts(q[u].y, v + 1), g2 = counts(q[u].z, v + 2), g3 = counts(q[u].w, v + 3);
+				const unsigned long long g = (unsigned long long)g0 + g1 + g2 + g3;
+				sum += g;
+				count += (g0 != 0u ? 1u : 0u) + (g1 != 0u ? 1u : 0u) + (g2 != 0u ? 1u : 0u) + (g3 != 0u ? 1u : 0u);
+				const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(g >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)g & 0xFFFFu);
+				if (lane == 0 && at < words) places.sum[1 + (at >> 5)] = ((unsigned long long)high << 16) + low;
+			}
+		}
+	};
 
 	// ---- the second pass
-	const uint32_t most = farthest(w.slope, w.cut), floor_w = max(1u, 2u * w.min_p);
 	const uint32_t reach = least == INT32_MIN ? 0xFFFFFFFFu : (uint32_t)top - (uint32_t)max(least, INT32_MIN + 1), far = min(reach, most);      // the list's farthest
-	unsigned long long sum = 0;
-	uint32_t count = 0;
-	auto word = [&](int k) { return KEEP ? kept[k] : __ldcg(from + k); };
+	const bool complete = reach >= most;      // the list has every token that has a weight
 	if (!late && !none) {
 		if (!cuts) {
-			// sums of what is kept of 128 neighbouring tokens: places 1 .. , the ends at 0 and behind
-			const int steps = (words + 31) / 32;
-			auto keep_of = [&](int32_t x) {
-				const uint32_t g = weight_of((uint32_t)top - (uint32_t)x, most, w.slope, w.cut);
-				const bool yes = x != INT32_MIN && g >= floor_w;
-				count += yes ? 1u : 0u;
-				return yes ? g : 0u;
-			};
-			if (t < 2) places.sum[t == 0 ? 0 : steps + 1] = 0ull;
-			__syncthreads();
-			if (end >= 0) {
-				const uint32_t g = keep_of(end_x);
-				sum += g;
-				atomicAdd(&places.sum[t < 4 ? 0 : steps + 1], (unsigned long long)g);
-			}
-#pragma unroll 4
-			for (int k = t; k - lane < words; k += kThreads) {
-				unsigned long long g = 0;
-				if (k < words) {
-					const int4 q = word(k);
-					g = (unsigned long long)keep_of(q.x) + keep_of(q.y) + keep_of(q.z) + keep_of(q.w);
-				}
-				sum += g;
-				const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(g >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)g & 0xFFFFu);
-				if (lane == 0) places.sum[1 + (k >> 5)] = ((unsigned long long)high << 16) + low;
-			}
+			add_steps([&](int32_t x, int) {
+				const uint32_t g = weight(x);
+				return g >= floor_w ? g : 0u;
+			});
 		} else {
-			const bool all = w.top_k == 0;      // all weights are added up
-			auto look = [&](int32_t x, int v) {
-				const uint32_t d = (uint32_t)top - (uint32_t)x;
-				if (all && x != INT32_MIN) sum += weight_of(d, most, w.slope, w.cut);
-				const bool yes = x != INT32_MIN && d <= far;
-				const uint32_t who = __ballot_sync(0xffffffffu, yes);
-				if (who == 0u) return;
-				uint32_t at = 0;
-				if (lane == 0) at = atomicAdd(&s_n, __popc(who));
-				at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-				if (yes && at < (uint32_t)kList) list[at] = (unsigned long long)d << kIndexBits | (uint32_t)v;
-			};
-			if (warp == 0) look(end_x, end);
-#pragma unroll 4
-			for (int k = t; k - lane < words; k += kThreads) {
-				const int4 q = k < words ? word(k) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-				const int v = first + 4 * k;
-				look(q.x, v);
-				look(q.y, v + 1);
-				look(q.z, v + 2);
-				look(q.w, v + 3);
+			const int32_t from_x = (int32_t)max((long long)top - (long long)far, -2147483647ll);
+			if (w.top_k == 0) {      // all weights are added up, and those of the list
+				auto one = [&](int32_t x, int v) {
+					const uint32_t g = weight(x);
+					sum += g;
+					if (x >= from_x) {
+						listed += g;
+						put(x, v);
+					}
+				};
+				one(end_x, end);
+				each_word([&](int4 q, int v) {
+					one(q.x, v);
+					one(q.y, v + 1);
+					one(q.z, v + 2);
+					one(q.w, v + 3);
+				});
+			} else {
+				if (end_x >= from_x) put(end_x, end);
+				each_word([&](int4 q, int v) {
+					if (max(max(q.x, q.y), max(q.z, q.w)) < from_x) return;
+					if (q.x >= from_x) put(q.x, v);
+					if (q.y >= from_x) put(q.y, v + 1);
+					if (q.z >= from_x) put(q.z, v + 2);
+					if (q.w >= from_x) put(q.w, v + 3);
+				});
 			}
 		}
 	}
-	sum = block_sum(sum, s_scan);
-	if (!cuts) count = (uint32_t)block_sum(count, s_scan);
-	else count = s_n;
-	int owner = 0;                          // the block that finds the token
-	unsigned long long mark = 0;            // and how much of what is kept lies before what it looks for
-	uint32_t others = 0;                    // tokens of the lists of lower blocks
-	if (sub > 1) {
+	sum = block_sum(sum, s_scan);      // (a barrier, behind which the list is whole)
+	if (!cuts) {
+		count = (uint32_t)block_sum(count, s_scan);
+	} else {
+		if (w.top_k == 0) listed = block_sum(listed, s_scan);
+		count = s_n;
+	}
+	int owner = 0;                          // the block that finds the token among its sums
+	unsigned long long mark = 0;            // what it looks for
+	// sums of all blocks: of `what` words; false where a wait ran out here or elsewhere
+	auto tell = [&](int bar, int slot, bool both) {
 		if (t < sub) {
-			exchange_send(&s_sum[rank], cta_addr(&s_bar[1]), (uint32_t)t, sum);
-			exchange_send(&s_count[rank], cta_addr(&s_bar[1]), (uint32_t)t, late ? kLate : count);
+			exchange_send(&s_sum[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, sum);
+			if (both) exchange_send(&s_listed[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, listed);
+			exchange_send(&s_count[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, late ? kLate : count);
 		}
-		const bool waited = exchange_wait(cta_addr(&s_bar[1]));
+		const bool waited = exchange_wait(cta_addr(&s_bar[bar]));
 		const bool gave_up = __syncthreads_or(late || !waited) != 0;
-		const uint32_t c = s_count[lane & (sub - 1)];
-		late = __any_sync(0xffffffffu, c == kLate) || gave_up;
-		if (late) {
-			if (rank == 0 && t == 0) {
-				if (RESIDENT) {
-					if (a.status != nullptr) a.status[r] = kInternalWaitTimeout;
-				} else {
-					atomicCAS(&a.status[r], 0, pack_status(kInternalWaitTimeout, kSiteLogits, w.layer));
-				}
-			}
-			if (gave_up || rank == 0) exchange_leave(cta_addr(&s_bar[0]), 3);
-			return;
-		}
-		sum = 0;
-		uint32_t total = 0;
-		if (!cuts)
-			for (int i = 0; i < sub; ++i) sum += s_sum[i];
+		const uint32_t c = s_count[slot][lane & (sub - 1)];
+		if (!__any_sync(0xffffffffu, c == kLate) && !gave_up) return true;
+		give_up(gave_up || rank == 0);
+		return false;
+	};
+	// of a total that all blocks have, what lies before the mark in other blocks
+	auto find_owner = [&](int slot) {
+		unsigned long long before = 0;
+		owner = 0;
 		for (int i = 0; i < sub; ++i) {
-			if (i < rank) others += s_count[i];
-			total += s_count[i];
-		}
-		if (cuts) {
-			for (int i = 0; i < sub; ++i) sum += s_sum[i];
-			if (rank == 0) {
-				if (t == 0 && total <= (uint32_t)kList) {
-					const uint32_t bytes = (total - count) * 8u + (held == 3 ? 8u : 0u);
-					asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[2])), "r"(bytes) : "memory");
-				}
-			} else {
-				if (total <= (uint32_t)kList)
-					for (uint32_t i = t; i < count; i += kThreads) exchange_send(list + others + i, cta_addr(&s_bar[2]), 0u, list[i]);
-				return;      // (nothing is sent to it any more)
+			if (before <= mark && mark < before + s_sum[slot][i]) {
+				owner = i;
+				break;
 			}
-		} else {
-			mark = share_of(sum, w.draw, 31);
-			unsigned long long before = 0;
-			for (int i = 0; i < sub; ++i) {
-				if (before <= mark && mark < before + s_sum[i]) {
-					owner = i;
-					break;
-				}
-				before += s_sum[i];
-			}
-			if (rank != owner) return;
-			mark -= before;
+			before += s_sum[slot][i];
 		}
-		count = total;
-		if (cuts && total <= (uint32_t)kList) {
-			late = !exchange_wait(cta_addr(&s_bar[2]));
-			if (__syncthreads_or(late)) {
-				if (t == 0) {
-					if (RESIDENT) {
-						if (a.status != nullptr) a.status[r] = kInternalWaitTimeout;
-					} else {
-						atomicCAS(&a.status[r], 0, pack_status(kInternalWaitTimeout, kSiteLogits, w.layer));
+		mark -= rank == owner ? before : 0ull;
+	};
+	uint32_t others = 0;                    // tokens of the lists of lower blocks
+	uint32_t total = count;
+	if (sub > 1) {
+		if (!tell(kSums, 0, true)) return;
+		sum = listed = 0;
+		total = 0;
+		for (int i = 0; i < sub; ++i) {
+			sum += s_sum[0][i];
+			listed += s_listed[0][i];
+			if (i < rank) others += s_count[0][i];
+			total += s_count[0][i];
+		}
+	}
+	Drawn out{-2, 0u, 0u, 0ull};
+	bool by_steps = !cuts;
+	if (cuts && !none) {
+		const Cut cut{most, w.slope, w.cut, floor_w, w.top_p, w.draw, w.top_k, sum};
+		const unsigned long long enough = w.top_k == 0 ? share_of(sum, w.top_p, 30) : 0ull;
+		bool wide = false;
+		unsigned long long bound = ~0ull, sure = 0;      // the last key that is kept; weights in front of the window
+		const bool fits = total <= (uint32_t)kList && (complete || (w.top_k > 0 ? total >= (uint32_t)w.top_k : listed >= enough));
+		if (!fits) {
+			wide = w.top_k == 0 && total <= (uint32_t)kList;
+			if (wide) {
+				// ---- a sample (32,768 to 65,536 of the first block's tokens, or all) of what lies behind the list says where the share that is still wanted
+				// ends, to one or two in a hundred; the window is three to either side
+				if (rank == 0) {
+					const int down = max(0, 32 - __clz((int)(most - far)) - 11);
+					for (int i = t; i < kPlaces; i += kThreads) places.count[i] = 0u;
+					__syncthreads();
+					const int every = max(1, words / 8192);
+					for (int k = t * every; k < words; k += kThreads * every) {
+						const int4 q = word(k);
+						const int32_t y[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+						for (int j = 0; j < 4; ++j) {
+							const uint32_t d = (uint32_t)top - (uint32_t)y[j];
+							if (y[j] != INT32_MIN && d > far && d <= most) atomicAdd(&places.count[min((d - far - 1u) >> down, (uint32_t)kPlaces - 1u)], 1u);
+						}
+					}
+					__syncthreads();
+					// weights of the places, in units such that none is above 2^15 (and no place's sum above 2^31)
+					const int shift = max(0, 17 - __clz((int)weight_of(far, most, w.slope, w.cut)));
+					uint32_t v[4];
+					unsigned long long before[4], all = 0;
+#pragma unroll
+					for (int j = 0; j < 4; ++j) {
+						const uint32_t i = 4 * t + j, mid = far + 1u + (i << down) + ((1u << down) >> 1);
+						v[j] = mid > far ? places.count[i] * (weight_of(mid, most, w.slope, w.cut) >> shift) : 0u;
+						all += v[j];
+					}
+					all = block_sum(all, s_scan);
+					sums_before<4>(v, before, s_scan);
+					const double want = (double)(enough - listed) / (double)(sum - listed), slack = 0.03;
+					const double low = (want - slack) * (double)all, high = (want + slack) * (double)all;
+					if (t == 0) s_ends = make_int2((int)far, (int)most);
+					__syncthreads();
+#pragma unroll
+					for (int j = 0; j < 4; ++j) {
+						const uint32_t i = 4 * t + j;
+						if ((double)before[j] <= low && low < (double)(before[j] + v[j])) s_ends.x = (int)(far + (i << down));
+						if ((double)before[j] <= high && high < (double)(before[j] + v[j])) s_ends.y = (int)min((unsigned long long)most, (unsigned long long)far + ((unsigned long long)(i + 1) << down));
+					}
+					__syncthreads();
+					if (sub > 1 && t < sub && t != 0) exchange_send(&s_ends, cta_addr(&s_bar[kEnds]), (uint32_t)t, s_ends);
+				} else {
+					late = !exchange_wait(cta_addr(&s_bar[kEnds]));
+					if (__syncthreads_or(late)) {
+						give_up(true);
+						return;
 					}
 				}
-				exchange_leave(cta_addr(&s_bar[0]), 3);
-				return;
+				const uint32_t begin = (uint32_t)s_ends.x, stop = (uint32_t)s_ends.y;      // the window: begin < d <= stop
+				__syncthreads();
+				if (t == 0) s_n = 0u;
+				__syncthreads();
+				sum = listed = 0;
+				auto one = [&](int32_t x, int v) {
+					const uint32_t d = (uint32_t)top - (uint32_t)x;
+					if (x == INT32_MIN || d > stop) return;
+					const uint32_t g = weight_of(d, most, w.slope, w.cut);
+					if (d <= begin) sum += g;
+					else {
+						listed += g;
+						put(x, v);
+					}
+				};
+				one(end_x, end);
+				each_word([&](int4 q, int v) {
+					one(q.x, v);
+					one(q.y, v + 1);
+					one(q.z, v + 2);
+					one(q.w, v + 3);
+				});
+				sum = block_sum(sum, s_scan);
+				listed = block_sum(listed, s_scan);
+				count = total = s_n;
+				if (sub > 1) {
+					if (!tell(kWindow, 1, true)) return;
+					sum = listed = 0;
+					others = total = 0;
+					for (int i = 0; i < sub; ++i) {
+						sum += s_sum[1][i];
+						listed += s_listed[1][i];
+						if (i < rank) others += s_count[1][i];
+						total += s_count[1][i];
+					}
+				}
+				sure = sum;
+				wide = total <= (uint32_t)kList && sure < enough && enough <= sure + listed;      // (the last kept one is the first up to which `enough` lies)
+			}
+			if (!wide && rank != 0) return;
+		}
+		const bool do_list = wide || fits;
+		if (sub > 1 && do_list) {      // the lists, to the first block
+			const uint32_t bar = cta_addr(&s_bar[wide ? kWindowLists : kLists]);
+			if (rank != 0) {
+				for (uint32_t i = t; i < count; i += kThreads) exchange_send(list + others + i, bar, 0u, list[i]);
+				if (!wide) return;      // (nothing is sent to it any more)
+			} else {
+				if (t == 0) {
+					const uint32_t bytes = (total - count) * 8u + (held == 1 + (wide ? kWindowLists : kLists) ? 8u : 0u);
+					asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+				}
+				late = !exchange_wait(bar);
+				if (__syncthreads_or(late)) {
+					give_up(true);
+					return;
+				}
 			}
 		}
-	} else if (!cuts) {
-		mark = share_of(sum, w.draw, 31);
+		if (wide) {
+			if (rank == 0) {
+				bound = select_key(
+				    [&](auto f) {
+					    for (int i = t; i < (int)total; i += kThreads) f(list[i], key_weight(list[i], cut));
+				    },
+				    kIndexBits + 32 - __clz((int)most), enough - 1ull - sure, places, s_select);
+				if (t == 0) s_bound = bound;
+				__syncthreads();
+				if (sub > 1 && t < sub && t != 0) exchange_send(&s_bound, cta_addr(&s_bar[kBound]), (uint32_t)t, bound);
+			} else {
+				late = !exchange_wait(cta_addr(&s_bar[kBound]));
+				if (__syncthreads_or(late)) {
+					give_up(true);
+					return;
+				}
+				bound = s_bound;
+			}
+			sum = 0;
+			count = 0;
+			add_steps([&](int32_t x, int v) {
+				const uint32_t d = (uint32_t)top - (uint32_t)x;
+				const unsigned long long key = (unsigned long long)d << kIndexBits | (uint32_t)v;
+				if (x == INT32_MIN || key > bound) return 0u;
+				const uint32_t g = weight_of(d, most, w.slope, w.cut);
+				return g >= floor_w ? g : 0u;
+			});
+			sum = block_sum(sum, s_scan);
+			count = total = (uint32_t)block_sum(count, s_scan);
+			if (sub > 1) {
+				if (!tell(kKept, 0, false)) return;
+				sum = 0;
+				total = 0;
+				for (int i = 0; i < sub; ++i) {
+					sum += s_sum[0][i];
+					total += s_count[0][i];
+				}
+			}
+			by_steps = true;
+		} else if (do_list && total <= 8u * kThreads) {
+			out = total <= (uint32_t)kThreads ? draw_sorted<1>(list, (int)total, cut, s_scan, &s_drawn)
+			                                  : (total <= 4u * kThreads ? draw_sorted<4>(list, (int)total, cut, s_scan, &s_drawn) : draw_sorted<8>(list, (int)total, cut, s_scan, &s_drawn));
+		} else {
+			// every element: of the list, or of the whole row
+			auto each_key = [&](auto f) {
+				if (do_list) {
+					for (int i = t; i < (int)total; i += kThreads) f(list[i]);
+				} else {
+					const int head = min(V, (4 - mis) & 3), whole = (V - head) >> 2;
+					auto one = [&](int32_t x, int v) {
+						const uint32_t d = (uint32_t)top - (uint32_t)x;
+						if (x != INT32_MIN && d <= most) f((unsigned long long)d << kIndexBits | (uint32_t)v);
+					};
+					const int4* q = (const int4*)(w.logits + head);
+#pragma unroll 1
+					for (int k = t; k < whole; k += 4 * kThreads) {
+						int4 y[4];
+#pragma unroll
+						for (int u = 0; u < 4; ++u)
+							if (k + u * kThreads < whole) y[u] = __ldcg(q + k + u * kThreads);
+#pragma unroll
+						for (int u = 0; u < 4; ++u) {
+							if (k + u * kThreads >= whole) break;
+							const int v = head + 4 * (k + u * kThreads);
+							one(y[u].x, v);
+							one(y[u].y, v + 1);
+							one(y[u].z, v + 2);
+							one(y[u].w, v + 3);
+						}
+					}
+					if (t < head) one(w.logits[t], t);
+					const int behind = head + 4 * whole + t;
+					if (behind < V) one(w.logits[behind], behind);
+				}
+			};
+			auto added = [&](auto counts) {        // weights (or ones) of the elements that counts() names
+				unsigned long long x = 0;
+				each_key([&](unsigned long long key) { x += counts(key); });
+				return block_sum(x, s_scan);
+			};
+			const int bits = kIndexBits + 32 - __clz((int)most);
+			if (w.top_k > 0) {
+				if (added([&](unsigned long long) { return 1ull; }) > (unsigned long long)w.top_k)
+					bound = select_key([&](auto f) { each_key([&](unsigned long long key) { f(key, 1u); }); }, bits, (unsigned long long)w.top_k - 1ull, places, s_select);
+				if (w.top_p < (1u << 30)) sum = added([&](unsigned long long key) { return key <= bound ? (unsigned long long)key_weight(key, cut) : 0ull; });
+			} else {
+				sum = cut.sum;
+			}
+			if (w.top_p < (1u << 30))
+				bound = select_key([&](auto f) { each_key([&](unsigned long long key) { if (key <= bound) f(key, key_weight(key, cut)); }); }, bits, share_of(sum, w.top_p, 30) - 1ull,
+				                   places, s_select);
+			auto is_kept = [&](unsigned long long key, uint32_t g) { return key <= bound && g >= floor_w; };
+			unsigned long long mass = 0, many = 0;
+			each_key([&](unsigned long long key) {
+				const uint32_t g = key_weight(key, cut);
+				if (is_kept(key, g)) {
+					mass += g;
+					++many;
+				}
+			});
+			out.sum = block_sum(mass, s_scan);
+			out.number = (uint32_t)block_sum(many, s_scan);
+			out.token = (int)select_key(
+			    [&](auto f) {
+				    each_key([&](unsigned long long key) {
+					    const uint32_t g = key_weight(key, cut);
+					    if (is_kept(key, g)) f(key & (kMostVocab - 1), g);
+				    });
+			    },
+			    kIndexBits, share_of(out.sum, w.draw, 31), places, s_select);
+			if (t == 0) out.weight = weight(w.logits[out.token]);
+		}
 	}
-	int token = -2;
-	uint32_t weight = 0, number = 0;
-	if (none) {
-		sum = 0;
-	} else if (!cuts) {
+	if (by_steps && !none) {
 		// the 128 tokens that the mark lies in, then the token
-		number = count;
-		const int steps = (words + 31) / 32 + 2;
+		mark = share_of(sum, w.draw, 31);
+		if (sub > 1) find_owner(0);
+		if (rank != owner) return;
+		out.sum = sum;
+		out.number = total;
 		unsigned long long v[4], mine = 0;
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
@@ -490,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		if (warp != 0) return;
 		const int step = (int)s_select.place;
 		mark = s_select.target;
+		const unsigned long long bound = cuts ? s_bound : ~0ull;
 		const int v0 = step == 0 ? s0 : (step == steps - 1 ? last : first + 128 * (step - 1)), v1 = step == 0 ? first : (step == steps - 1 ? s1 : min(last, v0 + 128));
 		uint32_t g[4];
 		unsigned long long own_sum = 0;
@@ -497,8 +911,8 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		for (int j = 0; j < 4; ++j) {
 			const int at = v0 + 4 * lane + j;
 			const int32_t x = at < v1 ? w.logits[at] : INT32_MIN;
-			g[j] = x != INT32_MIN ? weight_of((uint32_t)top - (uint32_t)x, most, w.slope, w.cut) : 0u;
-			if (g[j] < floor_w) g[j] = 0u;
+			g[j] = weight(x);
+			if (g[j] < floor_w || ((unsigned long long)((uint32_t)top - (uint32_t)x) << kIndexBits | (uint32_t)at) > bound) g[j] = 0u;
 			own_sum += g[j];
 		}
 		upto = own_sum;
@@ -511,109 +925,27 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		const uint32_t who = __ballot_sync(0xffffffffu, before <= mark && mark < upto);
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			if (token < 0 && before <= mark && mark < before + g[j]) {
-				token = v0 + 4 * lane + j;
-				weight = g[j];
+			if (out.token < 0 && before <= mark && mark < before + g[j]) {
+				out.token = v0 + 4 * lane + j;
+				out.weight = g[j];
 			}
 			before += g[j];
 		}
-		token = __shfl_sync(0xffffffffu, token, __ffs(who) - 1);
-		weight = __shfl_sync(0xffffffffu, weight, __ffs(who) - 1);
-	} else {
-		const int n = (int)min(count, (uint32_t)kList);
-		const bool complete = reach >= most;      // the list has every token that has a weight
-		bool listed = count <= (uint32_t)kList && (complete || w.top_k == 0 || n >= w.top_k);
-		// every element: of the list, or of the whole row
-		auto each_key = [&](auto f) {
-			if (listed) {
-				for (int i = t; i < n; i += kThreads) f(list[i]);
-			} else {
-				const int head = min(V, (4 - mis) & 3), whole = (V - head) >> 2;
-				auto one = [&](int32_t x, int v) {
-					const uint32_t d = (uint32_t)top - (uint32_t)x;
-					if (x != INT32_MIN && d <= most) f((unsigned long long)d << kIndexBits | (uint32_t)v);
-				};
-				const int4* q = (const int4*)(w.logits + head);
-#pragma unroll 1
-				for (int k = t; k < whole; k += 4 * kThreads) {
-					int4 y[4];
-#pragma unroll
-					for (int u = 0; u < 4; ++u)
-						if (k + u * kThreads < whole) y[u] = __ldcg(q + k + u * kThreads);
-#pragma unroll
-					for (int u = 0; u < 4; ++u) {
-						if (k + u * kThreads >= whole) break;
-						const int v = head + 4 * (k + u * kThreads);
-						one(y[u].x, v);
-						one(y[u].y, v + 1);
-						one(y[u].z, v + 2);
-						one(y[u].w, v + 3);
-					}
-				}
-				if (t < head) one(w.logits[t], t);
-				const int behind = head + 4 * whole + t;
-				if (behind < V) one(w.logits[behind], behind);
-			}
-		};
-		auto weight_of_key = [&](unsigned long long key) { return weight_of((uint32_t)(key >> kIndexBits), most, w.slope, w.cut); };
-		unsigned long long bound = ~0ull;      // the last key that is kept
-		auto added = [&](auto counts) {        // weights (or ones) of the elements that counts() names
-			unsigned long long x = 0;
-			each_key([&](unsigned long long key) { x += counts(key); });
-			return block_sum(x, s_scan);
-		};
-		const int bits = kIndexBits + 32 - __clz((int)(listed ? far : most));
-		if (w.top_k > 0) {
-			if (!listed || n > w.top_k) {
-				const unsigned long long have = listed ? (unsigned long long)n : added([&](unsigned long long) { return 1ull; });
-				if (have > (unsigned long long)w.top_k)
-					bound = select_key([&](auto f) { each_key([&](unsigned long long key) { f(key, 1u); }); }, bits, (unsigned long long)w.top_k - 1ull, places, s_select);
-			}
-			if (w.top_p < (1u << 30)) sum = added([&](unsigned long long key) { return key <= bound ? (unsigned long long)weight_of_key(key) : 0ull; });
-		}
-		if (w.top_p < (1u << 30)) {
-			const unsigned long long enough = share_of(sum, w.top_p, 30);      // (sum is 2^31 at least, so this is 2 at least)
-			// the last kept one is the first up to which `enough` lies
-			if (w.top_k == 0 && listed && !complete) {
-				const unsigned long long have = added([&](unsigned long long key) { return (unsigned long long)weight_of_key(key); });
-				listed = have >= enough;
-			}
-			const int b = kIndexBits + 32 - __clz((int)(listed ? far : most));
-			bound = select_key([&](auto f) { each_key([&](unsigned long long key) { if (key <= bound) f(key, weight_of_key(key)); }); }, b, enough - 1ull, places, s_select);
-		}
-		auto is_kept = [&](unsigned long long key, uint32_t g) { return key <= bound && g >= floor_w; };
-		// (sums are below 2^51, counts below 2^20: one word has no room for both, so two sums)
-		unsigned long long mass = 0, many = 0;
-		each_key([&](unsigned long long key) {
-			const uint32_t g = weight_of_key(key);
-			if (is_kept(key, g)) {
-				mass += g;
-				++many;
-			}
-		});
-		sum = block_sum(mass, s_scan);
-		number = (uint32_t)block_sum(many, s_scan);
-		mark = share_of(sum, w.draw, 31);
-		token = (int)select_key(
-		    [&](auto f) {
-			    each_key([&](unsigned long long key) {
-				    const uint32_t g = weight_of_key(key);
-				    if (is_kept(key, g)) f(key & (kMostVocab - 1), g);
-			    });
-		    },
-		    kIndexBits, mark, places, s_select);
-		if (t == 0) weight = weight_of((uint32_t)top - (uint32_t)w.logits[token], most, w.slope, w.cut);
+		out.token = __shfl_sync(0xffffffffu, out.token, __ffs(who) - 1);
+		out.weight = __shfl_sync(0xffffffffu, out.weight, __ffs(who) - 1);
+	} else if (rank != 0) {
+		return;
 	}
 	if (t != 0) return;
 	if (RESIDENT) {
-		if (a.out_tokens != nullptr) a.out_tokens[r] = token;
+		if (a.out_tokens != nullptr) a.out_tokens[r] = out.token;
 		if (a.out_mass != nullptr) {
-			a.out_mass[2 * r] = weight;
-			a.out_mass[2 * r + 1] = (int64_t)sum;
+			a.out_mass[2 * r] = out.weight;
+			a.out_mass[2 * r + 1] = (int64_t)out.sum;
 		}
-		if (a.out_kept != nullptr) a.out_kept[r] = (int32_t)number;
+		if (a.out_kept != nullptr) a.out_kept[r] = (int32_t)out.number;
 	} else {
-		a.best[r] = token < 0 ? 0ull : 1ull << 32 | (0xFFFFFFFFu - (uint32_t)token);
+		a.best[r] = out.token < 0 ? 0ull : 1ull << 32 | (0xFFFFFFFFu - (uint32_t)out.token);
 	}
 }
 

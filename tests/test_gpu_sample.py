@@ -59,6 +59,7 @@ class Call:
             assert (tokens[r], mass[r, 0], mass[r, 1], kept[r]) == want and status[r] == 0, (r, tokens[r], mass[r], kept[r], want)
 
 
+WIDE = "a tenth of all tokens"      # more than the first list has
 LIMITS = [dict(), dict(top_k=1), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=40, top_p=0.95), dict(top_k=900, top_p=0.7, min_p=0.001), dict(top_p=0.5, min_p=0.3)]
 
 
@@ -72,6 +73,16 @@ def test_sizes(gpu_lib, torch, vocab, limits):
 @pytest.mark.parametrize("limits", LIMITS)
 def test_every_number_of_blocks(gpu_lib, torch, rows, vocab, limits):
     Call(gpu_lib, torch, make(2, rows, vocab, **limits)).check()
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (3, 40009), (30, 60000), (90, 30001), (200, 40000)])
+@pytest.mark.parametrize("top_p,spread,min_p", [(0.5, 4.0, 0.0), (0.9, 4.0, 0.0), (0.9, 3.0, 0.00001), (0.99, 2.5, 0.0), (0.9, 0.1, 0.0), (0.3, 0.01, 0.9), (0.99999, 3.0, 0.0), (0.9, 9.0, 0.0)])
+def test_what_top_p_keeps_is_long(gpu_lib, torch, rows, vocab, top_p, spread, min_p):
+    """temperatures that spread the weights: a window around the end of what is kept, behind thousands of tokens"""
+    g = np.random.default_rng(16)
+    logits = np.rint(g.normal(0, spread * NAT, (rows, vocab)))
+    case = make(16, rows, vocab, top_p=top_p, min_p=min_p, logits=logits)
+    Call(gpu_lib, torch, case).check()
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1 << 20), (2, 300001), (200, 262000)])
@@ -223,13 +234,18 @@ def test_probabilities(gpu_lib, torch):
     assert (upto[tokens] >= u - 1.4e-5).all() and (upto[tokens] - p[tokens] <= u + 1.4e-5).all()
 
 
-@pytest.mark.parametrize("exchange,limits", [(0, dict()), (1, dict()), (0, dict(top_k=40)), (1, dict(top_k=40, top_p=0.9)), (2, dict(top_k=40, top_p=0.9))])
+@pytest.mark.parametrize("exchange,limits", [(0, dict()), (1, dict(top_k=40, top_p=0.9)), (2, dict(top_k=40, top_p=0.9)), (3, WIDE), (4, WIDE), (5, WIDE), (6, WIDE), (7, WIDE)])
 def test_a_wait_that_runs_out(gpu_lib, torch, exchange, limits):
     """block 0 waits for more than its peers send: its row is reported, the others are right, and so is the next call"""
     arm = gpu_lib.dll.sslm_b200_debug_withhold_exchange
     arm.argtypes = [C.c_int32, C.c_int32]
-    assert arm(8, 3) == abi.ST["SSLM_INVALID_ARGUMENT"]
-    c = Call(gpu_lib, torch, make(30, 3, 100000, **limits))
+    assert arm(8, 8) == abi.ST["SSLM_INVALID_ARGUMENT"]
+    if limits is WIDE:
+        case = make(30, 3, 100000, top_p=0.9, logits=np.random.default_rng(30).normal(0, 2.5 * NAT, (3, 100000)))
+        case["params"][:, :2] = abi.sample_params(1 / NAT)[:2]
+    else:
+        case = make(30, 3, 100000, **limits)
+    c = Call(gpu_lib, torch, case)
     try:
         assert arm(8, exchange) == 0
         c.call.run()
@@ -238,6 +254,8 @@ def test_a_wait_that_runs_out(gpu_lib, torch, exchange, limits):
         arm(-1, 0)
     assert c.status.tolist() == [100, 0, 0]
     c.check()
+    if limits is WIDE:
+        assert (c.kept > 4000).all()
 
 
 def test_what_a_caller_leaves_out(gpu_lib, torch):
