@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/sslm_b200.h"
 #include "sslm_cluster.cuh"
@@ -42,7 +43,8 @@ constexpr int kMostSlice = (kPlaces - 2) * 128 & ~127;      // a sum for every 1
 constexpr uint32_t kLate = 0xFFFFFFFFu;
 // exchanges, in order: maxima and bounds; sums and lists' lengths; the lists; and where the list is too short the window's ends, its sums, its
 // lists, the last key that is kept, sums and numbers of what is kept
-enum { kTop = 0, kSums, kLists, kEnds, kWindow, kWindowLists, kBound, kKept, kBars };
+// (a window's sums take two exchanges in turn, where one window is not enough)
+enum { kTop = 0, kSums, kLists, kEnds, kWindow, kWindowLists, kBound, kKept, kWindowOdd, kBars };
 
 struct SampleArgs {
 	int rows, vocab, shift, slice;      // a row is cut over 1 << shift blocks of `slice` tokens (a multiple of 128)
@@ -68,21 +70,33 @@ struct Row {
 };
 
 // ---- weights
-__device__ __forceinline__ uint32_t weight_of(uint32_t d, uint32_t most, uint32_t slope, uint32_t cut) {
-	const uint32_t t = (uint32_t)(((unsigned long long)d * slope) >> cut);      // (below 2^29 up to `most`)
-	const uint32_t f = t << 8;
+// d slope / 2^cut with the slope's leading bit moved to bit 30, which changes no quotient: t = hi(d 2^a, m) >> b. `most` is the largest d with a
+// weight (t below 2^29), so d 2^a is below 2^31 up to there; it leaves out INT32_MIN too.
+struct Scaled {
+	uint32_t m, most;
+	int a, b;
+};
+__device__ __forceinline__ Scaled scaled_of(uint32_t slope, uint32_t cut, int32_t top) {
+	Scaled s{0u, 0xFFFFFFFFu, 0, 0};
+	if (slope != 0u) {
+		const int z = __clz((int)slope) - 1, c = (int)cut + z;
+		s.m = slope << z;
+		s.a = c <= 32 ? min(32 - c, 31) : 0;
+		s.b = c <= 32 ? 0 : min(c - 32, 31);
+		if (cut < 34u) s.most = (uint32_t)min((unsigned long long)0xFFFFFFFFu, ((1ull << (29 + cut)) - 1ull) / slope);      // (d slope is below 2^63 anyhow)
+	}
+	s.most = min(s.most, (uint32_t)top - 0x80000001u);
+	return s;
+}
+__device__ __forceinline__ uint32_t weight_of(uint32_t d, const Scaled& s) {
+	const uint32_t t = __umulhi(d << s.a, s.m) >> s.b, f = t << 8;
 	uint32_t p = 14555373u;
 	p = 114090822u - __umulhi(f, p);
 	p = 514119776u - __umulhi(f, p);
 	p = 1488326151u - __umulhi(f, p);
 	p = 2147483648u - __umulhi(f, p);
-	return d <= most ? p >> (t >> 24) : 0u;
-}
-// the largest d with a weight: d slope < 2^(29 + cut)
-__device__ __forceinline__ uint32_t farthest(uint32_t slope, uint32_t cut) {
-	if (slope == 0u || cut >= 34u) return 0xFFFFFFFFu;      // (d slope is below 2^63)
-	const unsigned long long q = ((1ull << (29 + cut)) - 1ull) / slope;
-	return q > 0xFFFFFFFFull ? 0xFFFFFFFFu : (uint32_t)q;
+	p = __funnelshift_rc(p, 0u, t >> 24);
+	return d <= s.most ? p : 0u;
 }
 // floor(total part / 2^bits), part <= 2^bits
 __device__ __forceinline__ unsigned long long share_of(unsigned long long total, uint32_t part, int bits) {
@@ -108,12 +122,12 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, un
 }
 
 // ---- the keys of a block in rising order, E of them a thread (thread t those at E t ..), by a bitonic network: partners in the thread, in the warp,
-// or by way of `room` (E * kThreads words)
+// or by way of `room` (E * kThreads words). The first n of them; those behind are ~0 and stay so.
 template <int E>
-__device__ __forceinline__ void sort_keys(unsigned long long (&x)[E], unsigned long long* room) {
+__device__ __forceinline__ void sort_keys(unsigned long long (&x)[E], int n, unsigned long long* room) {
 	const int t = threadIdx.x;
 #pragma unroll 1
-	for (int k = 2; k <= E * kThreads; k *= 2) {
+	for (int k = 2; k < 2 * n; k *= 2) {
 #pragma unroll 1
 		for (int j = k / 2; j >= E; j /= 2) {
 			const int far = j / E;      // threads apart
@@ -266,7 +280,9 @@ struct SampleSmem {
 
 // What a list of a row is cut by, and what came of it.
 struct Cut {
-	uint32_t most, slope, cut, floor_w, top_p, draw;
+	Scaled scale;
+	unsigned long long origin;   // of the list's keys: they are (INT32_MAX - x) 2^20 + v, and less it d 2^20 + v
+	uint32_t floor_w, top_p, draw;
 	int top_k;
 	unsigned long long sum;      // of all weights, where top-k does not say what counts
 };
@@ -275,7 +291,7 @@ struct Drawn {
 	uint32_t weight, number;
 	unsigned long long sum;
 };
-__device__ __forceinline__ uint32_t key_weight(unsigned long long key, const Cut& c) { return weight_of((uint32_t)(key >> kIndexBits), c.most, c.slope, c.cut); }
+__device__ __forceinline__ uint32_t key_weight(unsigned long long key, const Cut& c) { return weight_of((uint32_t)(key >> kIndexBits), c.scale); }
 
 // The list in the order of falling logits, cut, and drawn from. n <= E * kThreads keys, which are overwritten. For the threads of a whole block.
 template <int E>
@@ -284,9 +300,9 @@ __device__ __noinline__ Drawn draw_sorted(unsigned long long* list, int n, const
 	unsigned long long x[E], before[E];
 	uint32_t w[E];
 #pragma unroll
-	for (int e = 0; e < E; ++e) x[e] = E * t + e < n ? list[E * t + e] : ~0ull;
+	for (int e = 0; e < E; ++e) x[e] = E * t + e < n ? list[E * t + e] - c.origin : ~0ull;
 	__syncthreads();
-	sort_keys<E>(x, list);
+	sort_keys<E>(x, n, list);
 	unsigned long long sum = 0;
 	const int limit = c.top_k > 0 ? min(n, c.top_k) : n;
 #pragma unroll
@@ -327,7 +343,7 @@ __device__ __noinline__ Drawn draw_sorted(unsigned long long* list, int n, const
 	} else {
 #pragma unroll
 		for (int e = 0; e < E; ++e) x[e] = E * t + e < kept ? (x[e] & (kMostVocab - 1)) << 32 | w[e] : ~0ull;
-		sort_keys<E>(x, list);
+		sort_keys<E>(x, kept, list);
 #pragma unroll
 		for (int e = 0; e < E; ++e) w[e] = E * t + e < kept ? (uint32_t)x[e] : 0u;
 		sums_before<E>(w, before, s_scan);
@@ -342,12 +358,12 @@ __device__ __noinline__ Drawn draw_sorted(unsigned long long* list, int n, const
 template <bool RESIDENT, bool KEEP>
 __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_constant__ SampleArgs a) {
 	extern __shared__ __align__(16) unsigned char smem[];
-	__shared__ __align__(8) unsigned long long s_bar[kBars], s_sum[2][16], s_scan[kWarps], s_bound;
+	__shared__ __align__(8) unsigned long long s_bar[kBars], s_sum[3][16], s_scan[kWarps], s_bound;
 	__shared__ int2 s_top[16], s_warp[kWarps], s_ends;
-	__shared__ uint32_t s_count[2][16], s_n;
+	__shared__ uint32_t s_count[3][16], s_n;
 	__shared__ Row s_row;
 	__shared__ Drawn s_drawn;
-	__shared__ unsigned long long s_listed[2][16];
+	__shared__ unsigned long long s_listed[3][16];
 	__shared__ SelectSmem s_select;
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
 	const int sub = 1 << a.shift, rank = (int)blockIdx.x;
@@ -367,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			exchange_init(cta_addr(&s_bar[kWindow]), (uint32_t)(sub * 20) + (held == 1 + kWindow ? 4u : 0u));
 			ring_init(cta_addr(&s_bar[kWindowLists]), 1);
 			exchange_init(cta_addr(&s_bar[kBound]), 8u + (held == 1 + kBound ? 4u : 0u));
+			exchange_init(cta_addr(&s_bar[kWindowOdd]), (uint32_t)(sub * 20));
 			exchange_init(cta_addr(&s_bar[kKept]), (uint32_t)(sub * 12) + (held == 1 + kKept ? 4u : 0u));
 			exchange_fence_init();
 		}
@@ -424,20 +441,44 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	const int32_t end_x = end >= 0 ? w.logits[end] : INT32_MIN;
 	constexpr int U = 4;
 	const int rounds = (words + U * kThreads - 1) / (U * kThreads);      // of U words a thread
-	auto word = [&](int k) { return KEEP ? kept[k] : __ldcg(from + k); };
-	// f(the word, its first token), over the block's words, from the last ones on (what was read last is likelier still in L2)
-	auto each_word = [&](auto f) {
+	// f(the word, its first token, its number), over the block's words, the next ones asked for ahead; LAST: from the last ones on (what was read last is
+	// likelier still in L2). Words behind the last are INT32_MIN where ALL threads of a warp are to take part.
+	auto each_word = [&](auto last_first, auto all, auto stored, auto f) {
+		constexpr bool LAST = decltype(last_first)::value, ALL = decltype(all)::value, STORED = decltype(stored)::value;
+		int4 q[U], y[U];
+		auto fetch = [&](int4 (&to)[U], int i) {
+			const int k = (LAST ? rounds - 1 - i : i) * U * kThreads + t;
+#pragma unroll
+			for (int u = 0; u < U; ++u)
+				if (k + u * kThreads < words) to[u] = STORED ? kept[k + u * kThreads] : __ldcg(from + k + u * kThreads);
+		};
+		if (rounds > 0) fetch(q, 0);
 #pragma unroll 1
-		for (int i = rounds - 1; i >= 0; --i) {
-			const int k = i * U * kThreads + t;
-			int4 q[U];
+		for (int i = 0; i < rounds; ++i) {
+			if (i + 1 < rounds) fetch(y, i + 1);
+			const int k = (LAST ? rounds - 1 - i : i) * U * kThreads + t;
 #pragma unroll
-			for (int u = 0; u < U; ++u)
-				if (k + u * kThreads < words) q[u] = word(k + u * kThreads);
-#pragma unroll
-			for (int u = 0; u < U; ++u)
-				if (k + u * kThreads < words) f(q[u], first + 4 * (k + u * kThreads));
+			for (int u = 0; u < U; ++u) {
+				const bool there = k + u * kThreads < words;
+				if (ALL && !there) q[u] = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+				if (ALL || there) f(q[u], first + 4 * (k + u * kThreads), k + u * kThreads);
+				q[u] = y[u];
+			}
 		}
+	};
+	using Yes = std::true_type;
+	using No = std::false_type;
+	using Kept = std::integral_constant<bool, KEEP>;
+	auto put = [&](int32_t x, int v) {
+		const uint32_t at = atomicAdd(&s_n, 1u);
+		if (at < (uint32_t)kList) list[at] = (unsigned long long)(0x7FFFFFFFu - (uint32_t)x) << kIndexBits | (uint32_t)v;
+	};
+	auto put_from = [&](int4 q, int v, int32_t least) {      // the tokens of a word from `least` on
+		if (max(max(q.x, q.y), max(q.z, q.w)) < least) return;
+		if (q.x >= least) put(q.x, v);
+		if (q.y >= least) put(q.y, v + 1);
+		if (q.z >= least) put(q.z, v + 2);
+		if (q.w >= least) put(q.w, v + 3);
 	};
 	// a wait ran out: the row is reported, and the block stays until nothing can be sent to it any more
 	auto give_up = [&](bool stay) {
@@ -453,18 +494,35 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 
 	// ---- the maximum, and the least of the groups' maxima
 	int32_t top = end_x;
-#pragma unroll 1
-	for (int k = t; k < words; k += 2 * U * kThreads) {
-		int4 q[2 * U];
-#pragma unroll
-		for (int u = 0; u < 2 * U; ++u)
-			if (k + u * kThreads < words) q[u] = __ldcg(from + k + u * kThreads);
-#pragma unroll
-		for (int u = 0; u < 2 * U; ++u)
-			if (k + u * kThreads < words) {
-				if (KEEP) kept[k + u * kThreads] = q[u];
-				top = max(top, max(max(q[u].x, q[u].y), max(q[u].z, q[u].w)));
-			}
+	// One block has a long row and a small top-k: the least of the maxima of the row's first eighth, of 16 to 64 groups, leaves eight times as
+	// many tokens of the row as of that eighth, so the list can be made in the first pass already (256 rows: a pass less).
+	const bool early = !KEEP && sub == 1 && w.top_k > 0 && w.top_k <= 400 && words >= 16 * kThreads;
+	int32_t early_least = INT32_MIN;
+	if (early) {
+		int32_t m = INT32_MIN;
+		const int part = words / (8 * kThreads) * kThreads;
+#pragma unroll 4
+		for (int k = t; k < part; k += kThreads) {
+			const int4 q = __ldcg(from + k);
+			m = max(m, max(max(q.x, q.y), max(q.z, q.w)));
+		}
+		const int mates = w.top_k <= 64 ? 32 : (w.top_k <= 160 ? 16 : 8);      // threads of a group
+		for (int o = 1; o < mates; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+		m = __reduce_min_sync(0xffffffffu, m);
+		if (lane == 0) s_warp[warp] = make_int2(m, 0);
+		__syncthreads();
+		early_least = max(INT32_MIN + 1, __reduce_min_sync(0xffffffffu, s_warp[lane & (kWarps - 1)].x));
+		if (end_x >= early_least) put(end_x, end);
+		each_word(No(), No(), No(), [&](int4 q, int v, int) {
+			top = max(top, max(max(q.x, q.y), max(q.z, q.w)));
+			put_from(q, v, early_least);
+		});
+		__syncthreads();      // (s_warp is used again)
+	} else {
+		each_word(No(), No(), No(), [&](int4 q, int, int k) {
+			if (KEEP) kept[k] = q;
+			top = max(top, max(max(q.x, q.y), max(q.z, q.w)));
+		});
 	}
 	const bool cuts = w.top_k > 0 || w.top_p < (1u << 30);
 	int32_t least = INT32_MAX;
@@ -511,12 +569,9 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		late = __syncthreads_or(late) != 0;
 	}
 	const bool none = top == INT32_MIN;
-	const uint32_t most = farthest(w.slope, w.cut), floor_w = max(1u, 2u * w.min_p);
-	auto weight = [&](int32_t x) { return x != INT32_MIN ? weight_of((uint32_t)top - (uint32_t)x, most, w.slope, w.cut) : 0u; };
-	auto put = [&](int32_t x, int v) {
-		const uint32_t at = atomicAdd(&s_n, 1u);
-		if (at < (uint32_t)kList) list[at] = (unsigned long long)((uint32_t)top - (uint32_t)x) << kIndexBits | (uint32_t)v;
-	};
+	const Scaled scale = scaled_of(w.slope, w.cut, none ? INT32_MAX : top);
+	const uint32_t most = scale.most, floor_w = max(1u, 2u * w.min_p);
+	auto weight = [&](int32_t x) { return weight_of((uint32_t)top - (uint32_t)x, scale); };
 	// sums over all tokens that counts() names, of 128 neighbours each: places 1 .. , the ends at 0 and behind
 	unsigned long long sum = 0, listed = 0;
 	uint32_t count = 0;
@@ -530,29 +585,27 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			count += g != 0u ? 1u : 0u;
 			atomicAdd(&places.sum[t < 4 ? 0 : steps - 1], (unsigned long long)g);
 		}
-#pragma unroll 1
-		for (int i = rounds - 1; i >= 0; --i) {
-			const int k = i * U * kThreads + t;
-			int4 q[U];
-#pragma unroll
-			for (int u = 0; u < U; ++u) q[u] = k + u * kThreads < words ? word(k + u * kThreads) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-#pragma unroll
-			for (int u = 0; u < U; ++u) {
-				const int at = k + u * kThreads, v = first + 4 * at;
-				const uint32_t g0 = counts(q[u].x, v), g1 = counts(q[u].y, v + 1), g2 = counts(q[u].z, v + 2), g3 = counts(q[u].w, v + 3);
-				const unsigned long long g = (unsigned long long)g0 + g1 + g2 + g3;
-				sum += g;
-				count += (g0 != 0u ? 1u : 0u) + (g1 != 0u ? 1u : 0u) + (g2 != 0u ? 1u : 0u) + (g3 != 0u ? 1u : 0u);
-				const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(g >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)g & 0xFFFFu);
-				if (lane == 0 && at < words) places.sum[1 + (at >> 5)] = ((unsigned long long)high << 16) + low;
-			}
-		}
+		each_word(Yes(), Yes(), Kept(), [&](int4 q, int v, int k) {
+			const uint32_t g0 = counts(q.x, v), g1 = counts(q.y, v + 1), g2 = counts(q.z, v + 2), g3 = counts(q.w, v + 3);
+			const unsigned long long g = (unsigned long long)g0 + g1 + g2 + g3;
+			sum += g;
+			count += (g0 != 0u ? 1u : 0u) + (g1 != 0u ? 1u : 0u) + (g2 != 0u ? 1u : 0u) + (g3 != 0u ? 1u : 0u);
+			const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(g >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)g & 0xFFFFu);
+			if (lane == 0 && k < words) places.sum[1 + (k >> 5)] = ((unsigned long long)high << 16) + low;
+		});
 	};
 
 	// ---- the second pass
 	const uint32_t reach = least == INT32_MIN ? 0xFFFFFFFFu : (uint32_t)top - (uint32_t)max(least, INT32_MIN + 1), far = min(reach, most);      // the list's farthest
-	const bool complete = reach >= most;      // the list has every token that has a weight
-	if (!late && !none) {
+	bool complete = reach >= most;      // the list has every token that has a weight
+	const bool have_list = early && s_n >= (uint32_t)w.top_k && s_n <= (uint32_t)kList;
+	if (early) {
+		__syncthreads();      // (all have seen how long it is)
+		if (have_list) complete = false;
+		else if (t == 0) s_n = 0u;
+		__syncthreads();
+	}
+	if (!late && !none && !have_list) {
 		if (!cuts) {
 			add_steps([&](int32_t x, int) {
 				const uint32_t g = weight(x);
@@ -570,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 					}
 				};
 				one(end_x, end);
-				each_word([&](int4 q, int v) {
+				each_word(Yes(), No(), Kept(), [&](int4 q, int v, int) {
 					one(q.x, v);
 					one(q.y, v + 1);
 					one(q.z, v + 2);
@@ -578,13 +631,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 				});
 			} else {
 				if (end_x >= from_x) put(end_x, end);
-				each_word([&](int4 q, int v) {
-					if (max(max(q.x, q.y), max(q.z, q.w)) < from_x) return;
-					if (q.x >= from_x) put(q.x, v);
-					if (q.y >= from_x) put(q.y, v + 1);
-					if (q.z >= from_x) put(q.z, v + 2);
-					if (q.w >= from_x) put(q.w, v + 3);
-				});
+				each_word(Yes(), No(), Kept(), [&](int4 q, int v, int) { put_from(q, v, from_x); });
 			}
 		}
 	}
@@ -598,13 +645,13 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	int owner = 0;                          // the block that finds the token among its sums
 	unsigned long long mark = 0;            // what it looks for
 	// sums of all blocks: of `what` words; false where a wait ran out here or elsewhere
-	auto tell = [&](int bar, int slot, bool both) {
+	auto tell = [&](int bar, int slot, bool both, uint32_t turn) {
 		if (t < sub) {
 			exchange_send(&s_sum[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, sum);
 			if (both) exchange_send(&s_listed[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, listed);
 			exchange_send(&s_count[slot][rank], cta_addr(&s_bar[bar]), (uint32_t)t, late ? kLate : count);
 		}
-		const bool waited = exchange_wait(cta_addr(&s_bar[bar]));
+		const bool waited = bounded_wait<true>(cta_addr(&s_bar[bar]), turn & 1u);
 		const bool gave_up = __syncthreads_or(late || !waited) != 0;
 		const uint32_t c = s_count[slot][lane & (sub - 1)];
 		if (!__any_sync(0xffffffffu, c == kLate) && !gave_up) return true;
@@ -627,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	uint32_t others = 0;                    // tokens of the lists of lower blocks
 	uint32_t total = count;
 	if (sub > 1) {
-		if (!tell(kSums, 0, true)) return;
+		if (!tell(kSums, 0, true, 0u)) return;
 		sum = listed = 0;
 		total = 0;
 		for (int i = 0; i < sub; ++i) {
@@ -640,104 +687,149 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	Drawn out{-2, 0u, 0u, 0ull};
 	bool by_steps = !cuts;
 	if (cuts && !none) {
-		const Cut cut{most, w.slope, w.cut, floor_w, w.top_p, w.draw, w.top_k, sum};
+		const Cut cut{scale, (unsigned long long)(0x7FFFFFFFu - (uint32_t)top) << kIndexBits, floor_w, w.top_p, w.draw, w.top_k, sum};
 		const unsigned long long enough = w.top_k == 0 ? share_of(sum, w.top_p, 30) : 0ull;
 		bool wide = false;
 		unsigned long long bound = ~0ull, sure = 0;      // the last key that is kept; weights in front of the window
+		unsigned long long kept_sum = 0;                 // this block's kept ones in front of the window
+		uint32_t kept_count = 0;
 		const bool fits = total <= (uint32_t)kList && (complete || (w.top_k > 0 ? total >= (uint32_t)w.top_k : listed >= enough));
 		if (!fits) {
 			wide = w.top_k == 0 && total <= (uint32_t)kList;
-			if (wide) {
-				// ---- a sample (32,768 to 65,536 of the first block's tokens, or all) of what lies behind the list says where the share that is still wanted
-				// ends, to one or two in a hundred; the window is three to either side
+			// what is kept ends at a d in (begin, stop], up to which exactly `before` and `through` of the weights lie
+			uint32_t begin = far, stop = most, turn = 0;
+			unsigned long long before_begin = listed, through_stop = sum;
+			while (wide) {
+				// ---- a sample (32,768 to 65,536 of the first block's tokens, or all) says where in between, to one or two in a hundred; the window
+				// is three to either side, or less where that would be too many tokens
 				if (rank == 0) {
-					const int down = max(0, 32 - __clz((int)(most - far)) - 11);
+					const int down = max(0, 32 - __clz((int)(stop - begin)) - 11);
 					for (int i = t; i < kPlaces; i += kThreads) places.count[i] = 0u;
 					__syncthreads();
 					const int every = max(1, words / 8192);
 					for (int k = t * every; k < words; k += kThreads * every) {
-						const int4 q = word(k);
+						const int4 q = KEEP ? kept[k] : __ldcg(from + k);
 						const int32_t y[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
 						for (int j = 0; j < 4; ++j) {
 							const uint32_t d = (uint32_t)top - (uint32_t)y[j];
-							if (y[j] != INT32_MIN && d > far && d <= most) atomicAdd(&places.count[min((d - far - 1u) >> down, (uint32_t)kPlaces - 1u)], 1u);
+							if (d > begin && d <= stop) atomicAdd(&places.count[min((d - begin - 1u) >> down, (uint32_t)kPlaces - 1u)], 1u);
 						}
 					}
 					__syncthreads();
 					// weights of the places, in units such that none is above 2^15 (and no place's sum above 2^31)
-					const int shift = max(0, 17 - __clz((int)weight_of(far, most, w.slope, w.cut)));
+					const int shift = max(0, 17 - __clz((int)weight_of(begin, scale)));
 					uint32_t v[4];
-					unsigned long long before[4], all = 0;
+					unsigned long long at[4], all = 0;
 #pragma unroll
 					for (int j = 0; j < 4; ++j) {
-						const uint32_t i = 4 * t + j, mid = far + 1u + (i << down) + ((1u << down) >> 1);
-						v[j] = mid > far ? places.count[i] * (weight_of(mid, most, w.slope, w.cut) >> shift) : 0u;
+						const uint32_t i = 4 * t + j, mid = begin + 1u + (i << down) + ((1u << down) >> 1);
+						v[j] = mid > begin ? places.count[i] * (weight_of(mid, scale) >> shift) : 0u;
 						all += v[j];
 					}
 					all = block_sum(all, s_scan);
-					sums_before<4>(v, before, s_scan);
-					const double want = (double)(enough - listed) / (double)(sum - listed), slack = 0.03;
-					const double low = (want - slack) * (double)all, high = (want + slack) * (double)all;
-					if (t == 0) s_ends = make_int2((int)far, (int)most);
-					__syncthreads();
+					sums_before<4>(v, at, s_scan);
+					const double want = (double)(enough - before_begin) / (double)(through_stop - before_begin);
+					double slack = 0.03;
+					unsigned long long number[2];      // of the sample, in the window
+					for (int turn_of = 0; turn_of < 2; ++turn_of) {
+						const double low = (want - slack) * (double)all, high = (want + slack) * (double)all;
+						if (t == 0) s_ends = make_int2((int)begin, (int)stop);
+						__syncthreads();
+						uint32_t in = 0;
 #pragma unroll
-					for (int j = 0; j < 4; ++j) {
-						const uint32_t i = 4 * t + j;
-						if ((double)before[j] <= low && low < (double)(before[j] + v[j])) s_ends.x = (int)(far + (i << down));
-						if ((double)before[j] <= high && high < (double)(before[j] + v[j])) s_ends.y = (int)min((unsigned long long)most, (unsigned long long)far + ((unsigned long long)(i + 1) << down));
+						for (int j = 0; j < 4; ++j) {
+							const uint32_t i = 4 * t + j;
+							if ((double)at[j] <= low && low < (double)(at[j] + v[j])) s_ends.x = (int)(begin + (i << down));
+							if ((double)at[j] <= high && high < (double)(at[j] + v[j]))
+								s_ends.y = (int)min((unsigned long long)stop, (unsigned long long)begin + ((unsigned long long)(i + 1) << down));
+							if ((double)(at[j] + v[j]) > low && (double)at[j] <= high) in += places.count[i];
+						}
+						number[turn_of] = block_sum(in, s_scan) * (unsigned long long)(every * sub);
+						if (number[turn_of] <= (unsigned long long)kList * 3 / 4) break;
+						slack = max(0.01, slack * (double)(kList / 2) / (double)number[turn_of]);
+						__syncthreads();
 					}
 					__syncthreads();
 					if (sub > 1 && t < sub && t != 0) exchange_send(&s_ends, cta_addr(&s_bar[kEnds]), (uint32_t)t, s_ends);
 				} else {
-					late = !exchange_wait(cta_addr(&s_bar[kEnds]));
+					late = !bounded_wait<true>(cta_addr(&s_bar[kEnds]), turn & 1u);
 					if (__syncthreads_or(late)) {
 						give_up(true);
 						return;
 					}
 				}
-				const uint32_t begin = (uint32_t)s_ends.x, stop = (uint32_t)s_ends.y;      // the window: begin < d <= stop
+				const uint32_t near = (uint32_t)s_ends.x, until = (uint32_t)s_ends.y;      // the window: near < d <= until
 				__syncthreads();
 				if (t == 0) s_n = 0u;
-				__syncthreads();
+				// ---- a pass: weights up to the window, and of what is kept of them by 128 tokens; weights and list of the window
 				sum = listed = 0;
-				auto one = [&](int32_t x, int v) {
-					const uint32_t d = (uint32_t)top - (uint32_t)x;
-					if (x == INT32_MIN || d > stop) return;
-					const uint32_t g = weight_of(d, most, w.slope, w.cut);
-					if (d <= begin) sum += g;
-					else {
-						listed += g;
-						put(x, v);
+				count = 0;
+				kept_sum = 0;
+				const int32_t until_x = (int32_t)max((long long)top - (long long)until, -2147483647ll), near_x = (int32_t)max((long long)top - (long long)near, -2147483647ll);
+				add_steps([&](int32_t x, int v) {
+					uint32_t g = 0;
+					if (x >= until_x) {
+						g = weight(x);
+						if (x >= near_x) {
+							kept_sum += g;
+							g = g >= floor_w ? g : 0u;
+						} else {
+							listed += g;
+							put(x, v);
+							g = 0u;
+						}
 					}
-				};
-				one(end_x, end);
-				each_word([&](int4 q, int v) {
-					one(q.x, v);
-					one(q.y, v + 1);
-					one(q.z, v + 2);
-					one(q.w, v + 3);
+					return g;
 				});
-				sum = block_sum(sum, s_scan);
+				const unsigned long long own_sum = sum;
+				kept_count = count;
+				sum = block_sum(kept_sum, s_scan);      // (of all weights up to the window)
 				listed = block_sum(listed, s_scan);
+				kept_sum = block_sum(own_sum, s_scan);
+				kept_count = (uint32_t)block_sum(kept_count, s_scan);
 				count = total = s_n;
+				others = 0;
 				if (sub > 1) {
-					if (!tell(kWindow, 1, true)) return;
+					const int slot = 1 + (int)(turn & 1u);
+					if (!tell(slot == 1 ? kWindow : kWindowOdd, slot, true, turn >> 1)) return;
 					sum = listed = 0;
-					others = total = 0;
+					total = 0;
 					for (int i = 0; i < sub; ++i) {
-						sum += s_sum[1][i];
-						listed += s_listed[1][i];
-						if (i < rank) others += s_count[1][i];
-						total += s_count[1][i];
+						sum += s_sum[slot][i];
+						listed += s_listed[slot][i];
+						if (i < rank) others += s_count[slot][i];
+						total += s_count[slot][i];
 					}
 				}
 				sure = sum;
-				wide = total <= (uint32_t)kList && sure < enough && enough <= sure + listed;      // (the last kept one is the first up to which `enough` lies)
+				if (sure < enough && enough <= sure + listed && total <= (uint32_t)kList) break;      // (the last kept one is the first up to which `enough` lies)
+				// not in the window, or more tokens than the list holds: closer in, for a few turns
+				if (enough <= sure) {
+					stop = near;
+					through_stop = sure;
+				} else if (enough <= sure + listed) {
+					begin = near;
+					before_begin = sure;
+					stop = until;
+					through_stop = sure + listed;
+				} else {
+					begin = until;
+					before_begin = sure + listed;
+				}
+				wide = ++turn < 6u && stop - begin > 1u;
+				if (sub > 1 && wide) {
+					if (t == 0) {      // (of the next turn's ends and the next but one's sums; what comes may have come already)
+						asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[(turn & 1u) != 0u ? kWindow : kWindowOdd])), "r"((uint32_t)(sub * 20)) : "memory");
+						if (rank != 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[kEnds])), "r"(8u) : "memory");
+					}
+					__syncthreads();
+				}
 			}
 			if (!wide && rank != 0) return;
 		}
 		const bool do_list = wide || fits;
+		const uint32_t own_listed = count;      // (at the front of the list)
 		if (sub > 1 && do_list) {      // the lists, to the first block
 			const uint32_t bar = cta_addr(&s_bar[wide ? kWindowLists : kLists]);
 			if (rank != 0) {
@@ -757,11 +849,17 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		}
 		if (wide) {
 			if (rank == 0) {
+				unsigned long long aside[4];      // (the sums of 128 tokens: the selection needs their places)
+#pragma unroll
+				for (int j = 0; j < 4; ++j) aside[j] = places.sum[4 * t + j];
+				__syncthreads();
 				bound = select_key(
 				    [&](auto f) {
-					    for (int i = t; i < (int)total; i += kThreads) f(list[i], key_weight(list[i], cut));
+					    for (int i = t; i < (int)total; i += kThreads) f(list[i] - cut.origin, key_weight(list[i] - cut.origin, cut));
 				    },
 				    kIndexBits + 32 - __clz((int)most), enough - 1ull - sure, places, s_select);
+#pragma unroll
+				for (int j = 0; j < 4; ++j) places.sum[4 * t + j] = aside[j];
 				if (t == 0) s_bound = bound;
 				__syncthreads();
 				if (sub > 1 && t < sub && t != 0) exchange_send(&s_bound, cta_addr(&s_bar[kBound]), (uint32_t)t, bound);
@@ -773,19 +871,22 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 				}
 				bound = s_bound;
 			}
+			// the block's tokens of the window that are kept, to their 128 neighbours
 			sum = 0;
 			count = 0;
-			add_steps([&](int32_t x, int v) {
-				const uint32_t d = (uint32_t)top - (uint32_t)x;
-				const unsigned long long key = (unsigned long long)d << kIndexBits | (uint32_t)v;
-				if (x == INT32_MIN || key > bound) return 0u;
-				const uint32_t g = weight_of(d, most, w.slope, w.cut);
-				return g >= floor_w ? g : 0u;
-			});
-			sum = block_sum(sum, s_scan);
-			count = total = (uint32_t)block_sum(count, s_scan);
+			for (uint32_t i = t; i < own_listed; i += kThreads) {
+				const unsigned long long key = list[i] - cut.origin;
+				const uint32_t g = key_weight(key, cut);
+				if (key > bound || g < floor_w) continue;
+				const int v = (int)(key & (kMostVocab - 1));
+				sum += g;
+				++count;
+				atomicAdd(&places.sum[v < first ? 0 : (v >= last ? steps - 1 : 1 + ((v - first) >> 7))], (unsigned long long)g);
+			}
+			sum = block_sum(sum, s_scan) + kept_sum;
+			count = total = (uint32_t)block_sum(count, s_scan) + kept_count;
 			if (sub > 1) {
-				if (!tell(kKept, 0, false)) return;
+				if (!tell(kKept, 0, false, 0u)) return;
 				sum = 0;
 				total = 0;
 				for (int i = 0; i < sub; ++i) {
@@ -801,12 +902,12 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			// every element: of the list, or of the whole row
 			auto each_key = [&](auto f) {
 				if (do_list) {
-					for (int i = t; i < (int)total; i += kThreads) f(list[i]);
+					for (int i = t; i < (int)total; i += kThreads) f(list[i] - cut.origin);
 				} else {
 					const int head = min(V, (4 - mis) & 3), whole = (V - head) >> 2;
 					auto one = [&](int32_t x, int v) {
 						const uint32_t d = (uint32_t)top - (uint32_t)x;
-						if (x != INT32_MIN && d <= most) f((unsigned long long)d << kIndexBits | (uint32_t)v);
+						if (d <= most) f((unsigned long long)d << kIndexBits | (uint32_t)v);
 					};
 					const int4* q = (const int4*)(w.logits + head);
 #pragma unroll 1
@@ -911,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		for (int j = 0; j < 4; ++j) {
 			const int at = v0 + 4 * lane + j;
 			const int32_t x = at < v1 ? w.logits[at] : INT32_MIN;
-			g[j] = weight(x);
+			g[j] = weight(x);      // (none of INT32_MIN)
 			if (g[j] < floor_w || ((unsigned long long)((uint32_t)top - (uint32_t)x) << kIndexBits | (uint32_t)at) > bound) g[j] = 0u;
 			own_sum += g[j];
 		}
