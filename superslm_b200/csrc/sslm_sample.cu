@@ -14,10 +14,10 @@
 // Two passes over the logits. The first finds the row's maximum and a bound that is likely to lie below what is kept and above nearly all else:
 // the least of the maxima of g groups of threads, which leaves about g (ln g + 0.6) tokens above it, and g at least. The second pass lists these tokens,
 // a few hundred to two thousand, and adds up the weights where top-p needs that. The list is cut and drawn from by counting its weights into 512
-// places. Rows without top-k and top-p need no list: sums of 128 neighbouring tokens are enough to find the token.
+// places. Rows without top-k and top-p need no list: sums of 256 neighbouring tokens are enough to find the token.
 //
 // Where top-p keeps more than the list has (the sums tell), a sample of the row says where the end of what is kept must lie; a pass adds up
-// what is surely kept and lists a window around that end, which is cut as the list is; then the sums of 128 tokens as above. Whatever
+// what is surely kept and lists a window around that end, which is cut as the list is; then the sums of 256 tokens as above. Whatever
 // does not work out that way (a list that overflows, a top-k beyond some thousands) is counted by one block over the whole row.
 //
 // A row is cut over the blocks of a cluster while rows are few; they exchange maxima and sums, and send their lists to the first one.
@@ -33,14 +33,14 @@
 namespace sslm {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMostWarps = 32;                // of a block of T threads (512: 1,024 a multiprocessor took 21 rows from 13.8 to 17.8 us)
 constexpr int kList = 8192;                   // tokens of a row's list
-constexpr int kSteps = 2048;                  // sums of 128 tokens
+constexpr int kSteps = 1024;                  // sums of 256 tokens
 constexpr int kCounts = 2048;                 // places that a sample is counted into
-constexpr int kPlaces = kThreads;             // places that a selection counts into, four words each
+constexpr int kPlaces = 512;                  // places that a selection counts into, four words each
 constexpr int kIndexBits = 20;                // of a token
 constexpr int kMostVocab = 1 << kIndexBits;
-constexpr int kMostSlice = (kSteps - 2) * 128;      // a sum for every 128 tokens, and for the ends
+constexpr int kMostSlice = (kSteps - 2) * 256;      // a sum for every 256 tokens, and for the ends
 constexpr int kMostBlocks = 16;
 constexpr uint32_t kLate = 0xFFFFFFFFu;
 // exchanges, in order: maxima and bounds; sums and lists' lengths; the lists; and where the list is too short the window's ends, its sums, its
@@ -90,15 +90,34 @@ __device__ __forceinline__ Scaled scaled_of(uint32_t slope, uint32_t cut, int32_
 	s.most = min(s.most, (uint32_t)top - 0x80000001u);
 	return s;
 }
-__device__ __forceinline__ uint32_t weight_of(uint32_t d, const Scaled& s) {
+// (of d up to `most`; beyond, anything)
+__device__ __forceinline__ uint32_t weight_near(uint32_t d, const Scaled& s) {
 	const uint32_t t = __umulhi(d << s.a, s.m) >> s.b, f = t << 8;
 	uint32_t p = 14555373u;
 	p = 114090822u - __umulhi(f, p);
 	p = 514119776u - __umulhi(f, p);
 	p = 1488326151u - __umulhi(f, p);
 	p = 2147483648u - __umulhi(f, p);
-	p = __funnelshift_rc(p, 0u, t >> 24);
+	return __funnelshift_rc(p, 0u, t >> 24);
+}
+__device__ __forceinline__ uint32_t weight_of(uint32_t d, const Scaled& s) {
+	const uint32_t p = weight_near(d, s);
 	return d <= s.most ? p : 0u;
+}
+// the largest d with a weight of `least` or more (at most 2^31), by a warp: 32 places at a time
+__device__ __forceinline__ uint32_t farthest_with(uint32_t least, const Scaled& s) {
+	const uint32_t lane = threadIdx.x & 31;
+	uint32_t low = 0, high = s.most;
+	while (low < high) {
+		const uint32_t span = high - low;
+		const uint32_t d = span <= 32u ? low + 1u + min(lane, span - 1u) : low + (uint32_t)((unsigned long long)span * (lane + 1u) >> 5);
+		const int n = __popc(__ballot_sync(0xffffffffu, weight_near(d, s) >= least));      // (the first n: weights fall)
+		const uint32_t in = __shfl_sync(0xffffffffu, d, max(n - 1, 0)), out = __shfl_sync(0xffffffffu, d, min(n, 31));
+		if (n > 0) low = in;
+		if (n < 32) high = out - 1u;
+		else high = low;
+	}
+	return low;
 }
 // floor(total part / 2^bits), part <= 2^bits
 __device__ __forceinline__ unsigned long long share_of(unsigned long long total, uint32_t part, int bits) {
@@ -106,29 +125,24 @@ __device__ __forceinline__ unsigned long long share_of(unsigned long long total,
 	return lo >> bits | hi << (64 - bits);
 }
 
-// ---- block-wide sums; s: 2 * kWarps words
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
-#pragma unroll
-	for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-	return v;
+// ---- block-wide sums of numbers below 2^52 (2^20 weights of at most 2^31); s: 2 * kMostWarps words
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {      // (two words of 26 bits: five shuffles of 64 bits took three times as long)
+	const uint32_t low = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3FFFFFFu), high = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26));
+	return ((unsigned long long)high << 26) + low;
 }
 // both, and a barrier
-__device__ __noinline__ ulonglong2 block_sums(unsigned long long a, unsigned long long b, unsigned long long* s) {
+template <int T>
+__device__ __forceinline__ ulonglong2 block_sums(unsigned long long a, unsigned long long b, unsigned long long* s) {
 	a = warp_sum(a);
 	b = warp_sum(b);
 	__syncthreads();
 	if ((threadIdx.x & 31) == 0) {
 		s[threadIdx.x >> 5] = a;
-		s[kWarps + (threadIdx.x >> 5)] = b;
+		s[kMostWarps + (threadIdx.x >> 5)] = b;
 	}
 	__syncthreads();
-	ulonglong2 all{0ull, 0ull};
-#pragma unroll
-	for (int i = 0; i < kWarps; ++i) {
-		all.x += s[i];
-		all.y += s[kWarps + i];
-	}
-	return all;
+	const int lane = threadIdx.x & 31;
+	return ulonglong2{warp_sum(lane < T / 32 ? s[lane] : 0ull), warp_sum(lane < T / 32 ? s[kMostWarps + lane] : 0ull)};
 }
 // the sum of v over the threads in front of this one
 __device__ __forceinline__ unsigned long long block_before(unsigned long long v, unsigned long long* s) {
@@ -141,10 +155,7 @@ __device__ __forceinline__ unsigned long long block_before(unsigned long long v,
 	}
 	if (lane == 31) s[warp] = upto;
 	__syncthreads();
-	unsigned long long at = upto - v;
-#pragma unroll
-	for (int i = 0; i < kWarps; ++i) at += i < warp ? s[i] : 0ull;
-	return at;
+	return upto - v + warp_sum(lane < warp ? s[lane] : 0ull);
 }
 
 // ---- elements of a row: those of a list, or all that have a weight. Their keys are d 2^20 + v.
@@ -157,11 +168,11 @@ struct Elements {
 	Scaled scale;
 	uint32_t floor_w;
 };
-template <bool WHOLE, typename F>
+template <int T, bool WHOLE, typename F>
 __device__ __forceinline__ void each_key(const Elements& e, F f) {
 	const int t = threadIdx.x;
 	if (!WHOLE) {
-		for (int i = t; i < e.n; i += kThreads) f(e.list[i] - e.origin);
+		for (int i = t; i < e.n; i += T) f(e.list[i] - e.origin);
 		return;
 	}
 	const int head = min(e.vocab, (int)((4 - (((uintptr_t)e.logits >> 2) & 3)) & 3)), words = (e.vocab - head) >> 2;
@@ -171,15 +182,15 @@ __device__ __forceinline__ void each_key(const Elements& e, F f) {
 	};
 	const int4* q = (const int4*)(e.logits + head);
 #pragma unroll 1
-	for (int k = t; k < words; k += 4 * kThreads) {
+	for (int k = t; k < words; k += 4 * T) {
 		int4 y[4];
 #pragma unroll
 		for (int u = 0; u < 4; ++u)
-			if (k + u * kThreads < words) y[u] = __ldcg(q + k + u * kThreads);
+			if (k + u * T < words) y[u] = __ldcg(q + k + u * T);
 #pragma unroll
 		for (int u = 0; u < 4; ++u) {
-			if (k + u * kThreads >= words) break;
-			const int v = head + 4 * (k + u * kThreads);
+			if (k + u * T >= words) break;
+			const int v = head + 4 * (k + u * T);
 			one(y[u].x, v);
 			one(y[u].y, v + 1);
 			one(y[u].z, v + 2);
@@ -197,17 +208,22 @@ __device__ __forceinline__ uint32_t key_weight(unsigned long long key, const Ele
 // counted into 512 places by their keys' leading bits, those of the place that holds the one looked for again, until a place has at most 32.
 // A place's sum is kept in three parts of 11 bits of each weight, for 2^20 elements in words of 32.
 enum { kOnes = 0, kWeights, kByIndex };
+constexpr int kFew = 64;
 struct SelectSmem {
-	unsigned long long key[32], scan[2 * kWarps], target, found;
+	unsigned long long key[32], scan[2 * kMostWarps], target, found;
 	uint32_t weight[32], place, count, n;
+	unsigned long long few_key[kFew];
+	uint32_t few_weight[kFew], few_kept[kFew];
+	int token;
+	uint32_t token_weight;
 };
-template <bool WHOLE>
+template <int T, bool WHOLE>
 __device__ __noinline__ unsigned long long select_key(const Elements& e, int what, unsigned long long bound, int bits, unsigned long long target, uint32_t* places, SelectSmem& s) {
 	const int t = threadIdx.x, lane = t & 31;
 	uint32_t* number = places + 3 * kPlaces;
 	unsigned long long low = 0;
 	auto each = [&](auto f) {
-		each_key<WHOLE>(e, [&](unsigned long long key) {
+		each_key<T, WHOLE>(e, [&](unsigned long long key) {
 			if (key > bound) return;
 			const uint32_t w = what == kOnes ? 1u : key_weight(key, e);
 			if (what == kByIndex) {
@@ -219,20 +235,21 @@ __device__ __noinline__ unsigned long long select_key(const Elements& e, int wha
 	};
 	for (;;) {
 		const int down = max(0, bits - 9);
-		places[t] = places[kPlaces + t] = places[2 * kPlaces + t] = number[t] = 0u;
+		for (int i = t; i < 4 * kPlaces; i += T) places[i] = 0u;
 		if (t == 0) s.n = 0u;
 		__syncthreads();
 		each([&](unsigned long long key, uint32_t w) {
 			const unsigned long long i = (key - low) >> down;
 			if (key < low || i >= (unsigned long long)kPlaces) return;
 			uint32_t* p = places + (int)i;
+			atomicAdd(p + 3 * kPlaces, 1u);
+			if (what == kOnes) return;
 			atomicAdd(p, w & 0x7FFu);
 			atomicAdd(p + kPlaces, w >> 11 & 0x7FFu);
 			atomicAdd(p + 2 * kPlaces, w >> 22);
-			atomicAdd(p + 3 * kPlaces, 1u);
 		});
 		__syncthreads();
-		const unsigned long long v = ((unsigned long long)places[2 * kPlaces + t] << 22) + ((unsigned long long)places[kPlaces + t] << 11) + places[t];
+		const unsigned long long v = t >= kPlaces ? 0ull : what == kOnes ? (unsigned long long)number[t] : ((unsigned long long)places[2 * kPlaces + t] << 22) + ((unsigned long long)places[kPlaces + t] << 11) + places[t];
 		const unsigned long long before = block_before(v, s.scan);
 		if (before <= target && target < before + v) {      // (one thread's place)
 			s.place = t;
@@ -271,49 +288,118 @@ struct Drawn {
 	uint32_t weight, number;
 	unsigned long long sum;
 };
+// The draw from at most 64 elements (s.few_key, `few` of them), cut by top-p (of `sum`, or of their own sum where that is 0) and min-p: eight threads an
+// element compare it with eight others each. For 512 threads at least.
+__device__ __noinline__ Drawn draw_few(const Elements& e, int few, uint32_t top_p, uint32_t draw, unsigned long long sum, SelectSmem& s) {
+	const int t = threadIdx.x, i = t >> 3;
+	if (t < kFew) {
+		if (t >= few) s.few_key[t] = ~0ull;
+		s.few_weight[t] = t < few ? key_weight(s.few_key[t], e) : 0u;
+	}
+	__syncthreads();
+	auto eighth = [](unsigned long long v) {
+#pragma unroll
+		for (int o = 1; o < 8; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+		return v;
+	};
+	const unsigned long long key = i < kFew ? s.few_key[i] : ~0ull;
+	const uint32_t w = i < kFew ? s.few_weight[i] : 0u;
+	unsigned long long less = 0, all = 0;
+#pragma unroll
+	for (int j = t & 7; j < kFew; j += 8) {
+		all += s.few_weight[j];
+		less += s.few_key[j] < key ? s.few_weight[j] : 0u;
+	}
+	less = eighth(less);
+	all = eighth(all);
+	const unsigned long long enough = top_p < (1u << 30) ? share_of(sum != 0ull ? sum : all, top_p, 30) : ~0ull;
+	const bool kept = less < enough && w >= e.floor_w;
+	if (i < kFew && (t & 7) == 0) s.few_kept[i] = kept ? w : 0u;
+	__syncthreads();
+	uint32_t number = 0;
+	const uint32_t v = (uint32_t)key & (kMostVocab - 1);
+	less = all = 0;
+#pragma unroll
+	for (int j = t & 7; j < kFew; j += 8) {
+		const uint32_t g = s.few_kept[j];
+		all += g;
+		number += min(g, 1u);
+		less += ((uint32_t)s.few_key[j] & (kMostVocab - 1)) < v ? g : 0u;
+	}
+	less = eighth(less);
+	all = eighth(all);
+#pragma unroll
+	for (int o = 1; o < 8; o *= 2) number += __shfl_xor_sync(0xffffffffu, number, o);
+	const unsigned long long mark = share_of(all, draw, 31);
+	if (kept && (t & 7) == 0 && less <= mark && mark < less + w) {      // (one thread)
+		s.token = (int)v;
+		s.token_weight = w;
+	}
+	__syncthreads();
+	return Drawn{s.token, s.token_weight, number, all};
+}
 // What a row's elements are cut to, and the token drawn from them. sum: of all weights, where top-k does not say what counts.
-template <bool WHOLE>
+template <int T, bool WHOLE>
 __device__ __forceinline__ Drawn draw_from(const Elements& e, int top_k, uint32_t top_p, uint32_t draw, unsigned long long sum, uint32_t* places, SelectSmem& s) {
-	const int bits = kIndexBits + 32 - __clz((int)e.scale.most);
+	const int t = threadIdx.x, bits = kIndexBits + 32 - __clz((int)e.scale.most);
 	unsigned long long bound = ~0ull;      // the last key that is kept
+	auto take_few = [&]() {                // the elements up to it
+		if (t == 0) s.n = 0u;
+		__syncthreads();
+		each_key<T, WHOLE>(e, [&](unsigned long long key) {
+			if (key <= bound) s.few_key[atomicAdd(&s.n, 1u)] = key;
+		});
+		__syncthreads();
+	};
 	if (top_k > 0) {
 		unsigned long long have = (unsigned long long)e.n, x = 0;
 		if (WHOLE) {
-			each_key<WHOLE>(e, [&](unsigned long long) { ++x; });
-			have = block_sums(x, 0ull, s.scan).x;
+			each_key<T, WHOLE>(e, [&](unsigned long long) { ++x; });
+			have = block_sums<T>(x, 0ull, s.scan).x;
 		}
-		if (have > (unsigned long long)top_k) bound = select_key<WHOLE>(e, kOnes, bound, bits, (unsigned long long)top_k - 1ull, places, s);
+		if (have > (unsigned long long)top_k) bound = select_key<T, WHOLE>(e, kOnes, bound, bits, (unsigned long long)top_k - 1ull, places, s);
+		have = min(have, (unsigned long long)top_k);
+		if (have <= (unsigned long long)kFew) {
+			take_few();
+			return draw_few(e, (int)have, top_p, draw, 0ull, s);
+		}
 		if (top_p < (1u << 30)) {
 			x = 0;
-			each_key<WHOLE>(e, [&](unsigned long long key) { x += key <= bound ? key_weight(key, e) : 0u; });
-			sum = block_sums(x, 0ull, s.scan).x;
+			each_key<T, WHOLE>(e, [&](unsigned long long key) { x += key <= bound ? key_weight(key, e) : 0u; });
+			sum = block_sums<T>(x, 0ull, s.scan).x;
 		}
 	}
 	// (the sum is 2^31 at least, so the share is 2 at least)
-	if (top_p < (1u << 30)) bound = select_key<WHOLE>(e, kWeights, bound, bits, share_of(sum, top_p, 30) - 1ull, places, s);
+	if (top_p < (1u << 30)) bound = select_key<T, WHOLE>(e, kWeights, bound, bits, share_of(sum, top_p, 30) - 1ull, places, s);
 	unsigned long long mass = 0, many = 0;
-	each_key<WHOLE>(e, [&](unsigned long long key) {
+	each_key<T, WHOLE>(e, [&](unsigned long long key) {
+		if (key > bound) return;
 		const uint32_t g = key_weight(key, e);
-		if (key > bound || g < e.floor_w) return;
+		many += 1ull << 32;
+		if (g < e.floor_w) return;
 		mass += g;
 		++many;
 	});
-	const ulonglong2 all = block_sums(mass, many, s.scan);
-	const int token = (int)select_key<WHOLE>(e, kByIndex, bound, kIndexBits, share_of(all.x, draw, 31), places, s);
+	const ulonglong2 all = block_sums<T>(mass, many, s.scan);
+	if (all.y >> 32 <= (unsigned long long)kFew) {
+		take_few();
+		return draw_few(e, (int)(all.y >> 32), top_p, draw, sum, s);
+	}
+	const int token = (int)select_key<T, WHOLE>(e, kByIndex, bound, kIndexBits, share_of(all.x, draw, 31), places, s);
 	return Drawn{token, weight_of((uint32_t)e.top - (uint32_t)e.logits[token], e.scale), (uint32_t)all.y, all.x};
 }
 
 struct SampleSmem {
-	// keys of the list [kList], sums of 128 tokens [kSteps], counts [kCounts], the block's logits [slice] if they are kept
+	// keys of the list [kList], sums of 256 tokens [kSteps], counts [kCounts], the block's logits [slice] if they are kept
 	static size_t bytes(int keep, int slice) { return (size_t)kList * 8 + (size_t)kSteps * 8 + (size_t)kCounts * 4 + (keep ? (size_t)slice * 4 + 16 : 0); }
 };
 
-template <bool RESIDENT, bool KEEP>
-__global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_constant__ SampleArgs a) {
+template <bool RESIDENT, bool KEEP, int T, int BLOCKS>
+__global__ void __launch_bounds__(T, BLOCKS) k_sample(const __grid_constant__ SampleArgs a) {
 	extern __shared__ __align__(16) unsigned char smem[];
 	__shared__ __align__(8) unsigned long long s_bar[kBars], s_sum[3][kMostBlocks], s_listed[3][kMostBlocks], s_bound;
-	__shared__ int2 s_top[kMostBlocks], s_warp[kWarps], s_ends;
-	__shared__ uint32_t s_count[3][kMostBlocks], s_n;
+	__shared__ int2 s_top[kMostBlocks], s_warp[kMostWarps], s_ends;
+	__shared__ uint32_t s_count[3][kMostBlocks], s_n, s_kept_far;
 	__shared__ Row s_row;
 	__shared__ SelectSmem s_select;
 	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
@@ -395,67 +481,29 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	const int heads = first - s0, tails = s1 - last;
 	const int end = t < heads ? s0 + t : (t >= 4 && t - 4 < tails ? last + t - 4 : -1);      // the token of the ends that is this thread's
 	const int32_t end_x = end >= 0 ? logits[end] : INT32_MIN;
-	constexpr int U = 4;
-	using Yes = std::true_type;
-	using No = std::false_type;
-	using Kept = std::integral_constant<bool, KEEP>;
-	const int rounds = (words + U * kThreads - 1) / (U * kThreads);
-	// f(U words of a thread, the first one's number) over the block's words. The first pass asks for the next ones ahead; the others go from the last ones on
-	// (what was read last is likelier still in L2) and need the registers. Words behind the last are INT32_MIN, so that whole warps take part.
-	auto each_group = [&](auto again, auto stored, auto f) {
-		constexpr bool LAST = decltype(again)::value, STORED = decltype(stored)::value;
-		int4 q[U], y[U];
-		auto fetch = [&](int4 (&to)[U], int i) {
-			const int k = (LAST ? rounds - 1 - i : i) * U * kThreads + t;
-#pragma unroll
-			for (int u = 0; u < U; ++u) {
-				to[u] = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-				if (k + u * kThreads < words) to[u] = STORED ? kept[k + u * kThreads] : __ldcg(from + k + u * kThreads);
-			}
-		};
-		if (!LAST && rounds > 0) fetch(q, 0);
-#pragma unroll 1
-		for (int i = 0; i < rounds; ++i) {
-			if (LAST) fetch(q, i);
-			else if (i + 1 < rounds) fetch(y, i + 1);
-			f(q, (LAST ? rounds - 1 - i : i) * U * kThreads + t);
-			if (!LAST) {
-#pragma unroll
-				for (int u = 0; u < U; ++u) q[u] = y[u];
-			}
-		}
-	};
 	auto top_of = [&](int4 q) { return max(max(q.x, q.y), max(q.z, q.w)); };
 	auto at_least = [&](int4 q, int32_t least) { return (q.x >= least ? 1u : 0u) | (q.y >= least ? 2u : 0u) | (q.z >= least ? 4u : 0u) | (q.w >= least ? 8u : 0u); };
-	auto put = [&](int32_t x, int v) {
-		const uint32_t at = atomicAdd(&s_n, 1u);
-		if (at < (uint32_t)kList) list[at] = (unsigned long long)(0x7FFFFFFFu - (uint32_t)x) << kIndexBits | (uint32_t)v;
-	};
-	// the tokens that `which` names (bit 4 u + j: token j of word u), one atomic a warp (one a token, each waited for, took longer than a list's sums)
-	auto put_group = [&](const int4 (&q)[U], int k, uint32_t which) {
-		if (__ballot_sync(0xffffffffu, which != 0u) == 0u) return;
+	// Room in the list for the tokens that the lanes' `which` names, one atomic a warp (one a token, each waited for, took longer than a list's sums):
+	// this lane's place behind `base`, which the first lane has once it has arrived.
+	auto reserve = [&](uint32_t which, uint32_t& base) {
 		const uint32_t n = __popc(which), lower = (1u << lane) - 1u;
 		uint32_t at = 0, all = 0;
+		if (__ballot_sync(0xffffffffu, which != 0u) != 0u) {
 #pragma unroll
-		for (int b = 0; b < 5; ++b) {
-			const uint32_t who = __ballot_sync(0xffffffffu, (n >> b & 1u) != 0u);
-			at += __popc(who & lower) << b;
-			all += __popc(who) << b;
-		}
-		uint32_t base = 0;
-		if (lane == 0) base = atomicAdd(&s_n, all);
-		at += __shfl_sync(0xffffffffu, base, 0);
-		if (which == 0u) return;
-#pragma unroll
-		for (int u = 0; u < U; ++u) {
-			const int32_t y[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				if ((which >> (4 * u + j) & 1u) == 0u) continue;
-				if (at < (uint32_t)kList) list[at] = (unsigned long long)(0x7FFFFFFFu - (uint32_t)y[j]) << kIndexBits | (uint32_t)(first + 4 * (k + u * kThreads) + j);
-				++at;
+			for (int b = 0; b < 5; ++b) {
+				const uint32_t who = __ballot_sync(0xffffffffu, (n >> b & 1u) != 0u);
+				at += __popc(who & lower) << b;
+				all += __popc(who) << b;
 			}
+			if (lane == 0) base = atomicAdd(&s_n, all);
 		}
+		return at;
+	};
+	auto put = [&](uint32_t at, int32_t x, int v) {
+		if (at < (uint32_t)kList) list[at] = (unsigned long long)(0x7FFFFFFFu - (uint32_t)x) << kIndexBits | (uint32_t)v;
+	};
+	auto put_end = [&]() {
+		put(atomicAdd(&s_n, 1u), end_x, end);
 	};
 	// a wait ran out: the row is reported, and the block stays until nothing can be sent to it any more
 	auto give_up = [&](bool stay) {
@@ -473,53 +521,63 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	int32_t top = end_x;
 	bool early = false;
 	int32_t early_least = INT32_MIN;
-	if (KEEP || sub > 1) {      // (the row's record arrives meanwhile)
-		each_group(No(), No(), [&](const int4 (&q)[U], int k) {
-#pragma unroll
-			for (int u = 0; u < U; ++u) {
-				if (KEEP && k + u * kThreads < words) kept[k + u * kThreads] = q[u];
-				top = max(top, top_of(q[u]));
-			}
-		});
-		take_record();
-		__syncthreads();
-	} else {
+	if (!KEEP && sub == 1) {
 		take_record();
 		__syncthreads();
 		// One block has a long row and a small top-k: the least of the maxima of the row's first eighth, of 16 to 64 groups, leaves eight times as
 		// many tokens of the row as of that eighth, so the list can be made in the first pass already (256 rows: a pass less).
 		const int top_k = s_row.top_k;
-		early = s_row.code == 0 && top_k > 0 && top_k <= 400 && words >= 16 * kThreads;
+		early = s_row.code == 0 && top_k > 0 && top_k <= 400 && words >= 16 * T;
 		if (early) {
 			int32_t m = INT32_MIN;
-			const int part = words / (8 * kThreads) * kThreads;
+			const int part = words / (8 * T) * T;
 #pragma unroll 4
-			for (int k = t; k < part; k += kThreads) m = max(m, top_of(__ldcg(from + k)));
+			for (int k = t; k < part; k += T) m = max(m, top_of(__ldcg(from + k)));
 			const int mates = top_k <= 64 ? 32 : (top_k <= 160 ? 16 : 8);      // threads of a group
 			for (int o = 1; o < mates; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
 			m = __reduce_min_sync(0xffffffffu, m);
 			if (lane == 0) s_warp[warp] = make_int2(m, 0);
 			__syncthreads();
-			early_least = max(INT32_MIN + 1, __reduce_min_sync(0xffffffffu, s_warp[lane & (kWarps - 1)].x));
-			if (end_x >= early_least) put(end_x, end);
-			each_group(No(), No(), [&](const int4 (&q)[U], int k) {
-				uint32_t which = 0;
-#pragma unroll
-				for (int u = 0; u < U; ++u) {
-					const int32_t m4 = top_of(q[u]);
-					top = max(top, m4);
-					if (m4 >= early_least) which |= at_least(q[u], early_least) << (4 * u);
-				}
-				put_group(q, k, which);
-			});
-			__syncthreads();      // (s_warp is used again)
-		} else if (s_row.code == 0) {
-			each_group(No(), No(), [&](const int4 (&q)[U], int) {
-#pragma unroll
-				for (int u = 0; u < U; ++u) top = max(top, top_of(q[u]));
-			});
+			early_least = max(INT32_MIN + 1, __reduce_min_sync(0xffffffffu, s_warp[lane & (T / 32 - 1)].x));
+			if (end_x >= early_least) put_end();
 		}
 	}
+	{
+		constexpr int U = 4;
+		int4 q[U], y[U];
+		auto fetch = [&](int4 (&to)[U], int k) {
+#pragma unroll
+			for (int u = 0; u < U; ++u) {
+				to[u] = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+				if (k + u * T < words) to[u] = __ldcg(from + k + u * T);
+			}
+		};
+		fetch(q, t);
+#pragma unroll 1
+		for (int k = t; k - t < words; k += U * T) {
+			fetch(y, k + U * T);
+			uint32_t which = 0;
+#pragma unroll
+			for (int u = 0; u < U; ++u) {
+				if (KEEP && k + u * T < words) kept[k + u * T] = q[u];
+				const int32_t m = top_of(q[u]);
+				top = max(top, m);
+				if (!KEEP && early && m >= early_least) which |= at_least(q[u], early_least) << (4 * u);
+				q[u] = y[u];
+			}
+			if (!KEEP && early) {      // (few: read again)
+				uint32_t base = 0, at = reserve(which, base);
+				at += __shfl_sync(0xffffffffu, base, 0);
+#pragma unroll 1
+				for (; which != 0u; which &= which - 1u, ++at) {
+					const int j = __ffs((int)which) - 1, i = 4 * (k + (j >> 2) * T) + (j & 3);
+					put(at, __ldcg(logits + first + i), first + i);
+				}
+			}
+		}
+	}
+	if (KEEP || sub > 1) take_record();      // (it arrived meanwhile)
+	__syncthreads();
 	const Row w = s_row;
 	if (w.code != 0) {      // (all blocks of the cluster alike)
 		if (sub > 1) cluster_wait();
@@ -534,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			wanted = 32;
 			while (wanted < min(w.top_k, 512)) wanted *= 2;
 		}
-		while (group < kThreads && 2 * group * wanted <= sub * kThreads) group *= 2;
+		while (group < T && 2 * group * wanted <= sub * T) group *= 2;
 		const bool has = t < words || end >= 0;
 		least = has ? top : INT32_MIN;
 		for (int o = 1; o < min(group, 32); o *= 2) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -549,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	}
 	__syncthreads();
 	{
-		const int2 x = s_warp[lane & (kWarps - 1)];
+		const int2 x = s_warp[lane & (T / 32 - 1)];
 		top = __reduce_max_sync(0xffffffffu, x.x);
 		least = x.y;
 		for (int o = 1; o < group / 32; o *= 2) {
@@ -560,6 +618,12 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		if (top == INT32_MIN) least = INT32_MAX;      // (nothing is allowed here)
 	}
 	bool late = false;
+	const uint32_t floor_w = max(1u, 2u * w.min_p);
+	if (warp == T / 32 - 1 && w.top_k == 0) {      // (beside the exchange; the largest logit only makes it less)
+		const uint32_t d = farthest_with(floor_w, scaled_of(w.slope, w.cut, INT32_MAX));
+		if (lane == 0) s_kept_far = d;
+	}
+	if (sub == 1) __syncthreads();
 	if (sub > 1) {
 		cluster_wait();      // (all blocks run)
 		if (t < sub) exchange_send(&s_top[rank], cta_addr(&s_bar[kTop]), (uint32_t)t, make_int2(top, least));
@@ -571,30 +635,9 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 	}
 	const bool none = top == INT32_MIN;
 	const Scaled scale = scaled_of(w.slope, w.cut, none ? INT32_MAX : top);
-	const uint32_t most = scale.most, floor_w = max(1u, 2u * w.min_p);
+	const uint32_t most = scale.most;
 	auto weight = [&](int32_t x) { return weight_of((uint32_t)top - (uint32_t)x, scale); };      // (0 of INT32_MIN)
 	auto x_of = [&](uint32_t d) { return (int32_t)max((long long)top - (long long)d, -2147483647ll); };      // the logit that lies d below the largest
-	unsigned long long sum = 0, listed = 0;
-	uint32_t count = 0;
-	const int last_step = (words + 31) / 32 + 1;      // steps[0] and this one: the ends; in between 128 neighbouring tokens each
-	auto clear_steps = [&]() {
-		if (t < 2) steps[t == 0 ? 0 : last_step] = 0ull;
-		__syncthreads();
-	};
-	auto add_end = [&](uint32_t g) {
-		sum += g;
-		count += g != 0u ? 1u : 0u;
-		if (g != 0u) atomicAdd(&steps[t < 4 ? 0 : last_step], (unsigned long long)g);
-	};
-	auto add_word = [&](uint32_t g0, uint32_t g1, uint32_t g2, uint32_t g3, int k) {
-		const unsigned long long g = (unsigned long long)g0 + g1 + g2 + g3;
-		sum += g;
-		count += (g0 != 0u ? 1u : 0u) + (g1 != 0u ? 1u : 0u) + (g2 != 0u ? 1u : 0u) + (g3 != 0u ? 1u : 0u);
-		const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(g >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)g & 0xFFFFu);
-		if (lane == 0 && k < words) steps[1 + (k >> 5)] = ((unsigned long long)high << 16) + low;
-	};
-
-	// ---- the second pass
 	const uint32_t reach = least == INT32_MIN ? 0xFFFFFFFFu : (uint32_t)top - (uint32_t)max(least, INT32_MIN + 1), far = min(reach, most);      // the list's farthest
 	bool complete = reach >= most;      // the list has every token that has a weight
 	bool have_list = false;
@@ -603,51 +646,14 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		__syncthreads();      // (all have seen how long it is)
 		if (have_list) complete = false;
 		else if (t == 0) s_n = 0u;
-		__syncthreads();
 	}
-	if (!late && !none && !have_list) {
-		if (!cuts) {
-			auto kept_of = [&](int32_t x) {
-				const uint32_t g = weight(x);
-				return g >= floor_w ? g : 0u;
-			};
-			clear_steps();
-			add_end(kept_of(end_x));
-			each_group(Yes(), Kept(), [&](const int4 (&q)[U], int k) {
-#pragma unroll
-				for (int u = 0; u < U; ++u) add_word(kept_of(q[u].x), kept_of(q[u].y), kept_of(q[u].z), kept_of(q[u].w), k + u * kThreads);
-			});
-		} else {
-			const int32_t from_x = x_of(far);
-			const bool all = w.top_k == 0;      // all weights are added up, and those of the list
-			if (end_x >= from_x) put(end_x, end);
-			if (all) {
-				const uint32_t g = weight(end_x);
-				sum += g;
-				listed += end_x >= from_x ? g : 0u;
-			}
-			each_group(Yes(), Kept(), [&](const int4 (&q)[U], int k) {
-				uint32_t which = 0;
-#pragma unroll
-				for (int u = 0; u < U; ++u) {
-					const uint32_t in = top_of(q[u]) >= from_x ? at_least(q[u], from_x) : 0u;
-					which |= in << (4 * u);
-					if (all) {
-						const uint32_t g0 = weight(q[u].x), g1 = weight(q[u].y), g2 = weight(q[u].z), g3 = weight(q[u].w);
-						sum += (unsigned long long)g0 + g1 + g2 + g3;
-						if (in != 0u) listed += (unsigned long long)((in & 1u) != 0u ? g0 : 0u) + ((in & 2u) != 0u ? g1 : 0u) + ((in & 4u) != 0u ? g2 : 0u) + ((in & 8u) != 0u ? g3 : 0u);
-					}
-				}
-				put_group(q, k, which);
-			});
-		}
-	}
-	{
-		const ulonglong2 both = block_sums(sum, cuts ? listed : count, scan);      // (a barrier, behind which the list is whole)
-		sum = both.x;
-		if (cuts) listed = both.y;
-		count = cuts ? s_n : (uint32_t)both.y;
-	}
+
+	// ---- passes: the second one, and those over a window. A pass adds up the weights of the logits from near_x on (sum), and, where there are sums of
+	// 256 neighbouring tokens (the ends at steps[0] and steps[last_step]), what is kept of them; it lists the logits from from_x on, with those sums only
+	// the ones below near_x, and adds up their weights (listed).
+	const int last_step = (words + 63) / 64 + 1;
+	unsigned long long sum = 0, listed = 0, kept_sum = 0;
+	uint32_t count = 0, kept_count = 0, others = 0, total = 0;      // tokens of the block's list, of what it keeps, of lower blocks' lists, of all lists
 	// sums of all blocks; false where a wait ran out here or elsewhere
 	auto tell = [&](int bar, int slot, bool both, uint32_t turn) {
 		if (t < sub) {
@@ -663,7 +669,6 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		}
 		return true;
 	};
-	uint32_t others = 0, total = count;      // tokens of the lists of lower blocks, and of all
 	auto add_up = [&](int slot, bool both) {
 		sum = listed = 0;
 		others = total = 0;
@@ -674,128 +679,121 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			total += s_count[slot][i];
 		}
 	};
-	if (sub > 1) {
-		if (!tell(kSums, 0, true, 0u)) return;
-		add_up(0, true);
-	}
-	Drawn out{-2, 0u, 0u, 0ull};
-	unsigned long long bound = ~0ull;      // the last key that is kept
-	bool by_steps = !cuts;
-	if (cuts && !none) {
-		const unsigned long long origin = (unsigned long long)(0x7FFFFFFFu - (uint32_t)top) << kIndexBits, all_weights = sum;
-		const unsigned long long enough = w.top_k == 0 ? share_of(sum, w.top_p, 30) : 0ull;
-		const bool fits = total <= (uint32_t)kList && (complete || (w.top_k > 0 ? total >= (uint32_t)w.top_k : listed >= enough));
-		bool wide = !fits && w.top_k == 0 && total <= (uint32_t)kList;
-		unsigned long long sure = 0, kept_sum = 0;       // weights in front of the window, and this block's of them that are kept
-		uint32_t kept_count = 0;
-		// what is kept ends at a d in (begin, stop], up to which exactly `before_begin` and `through_stop` of the weights lie
-		uint32_t begin = far, stop = most, turn = 0;
-		unsigned long long before_begin = listed, through_stop = sum;
+	// with windows: what is kept ends at a d in (begin, stop], up to which exactly `before_begin` and `through_stop` of the weights lie; near < d <= until
+	// is the window, `sure` lies in front of it
+	uint32_t begin = far, stop = most, near = 0, until = far, turn = 0;
+	unsigned long long before_begin = 0, through_stop = 0, all_weights = 0, enough = 0, sure = 0;
+	const bool weigh = w.top_k == 0;      // (of a row with top-k the list alone)
+	bool by_steps = !cuts, wide = false, fits = false;
 #pragma unroll 1
-		while (wide) {
-			// ---- a sample (32,768 to 65,536 of the first block's tokens, or all) says where in between, to one or two in a hundred; the window
-			// is three to either side, or less where that would be too many tokens
-			if (rank == 0) {
-				const int down = max(0, 32 - __clz((int)(stop - begin)) - 11);
-				for (int i = t; i < kCounts; i += kThreads) counts[i] = 0u;
-				__syncthreads();
-				const int every = max(1, words / 8192);
-#pragma unroll 4
-				for (int k = t * every; k < words; k += kThreads * every) {
-					const int4 q = KEEP ? kept[k] : __ldcg(from + k);
-					const int32_t y[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-					for (int j = 0; j < 4; ++j) {
-						const uint32_t d = (uint32_t)top - (uint32_t)y[j];
-						if (d > begin && d <= stop) atomicAdd(&counts[min((d - begin - 1u) >> down, (uint32_t)kCounts - 1u)], 1u);
-					}
-				}
-				__syncthreads();
-				// weights of the places, in units such that none is above 2^15 (and no place's sum above 2^31)
-				const int shift = max(0, 17 - __clz((int)weight_of(begin, scale)));
-				unsigned long long v[4], at = 0;
-#pragma unroll
-				for (int j = 0; j < 4; ++j) {
-					const uint32_t i = 4 * t + j, mid = begin + 1u + (i << down) + ((1u << down) >> 1);
-					v[j] = mid > begin ? (unsigned long long)(counts[i] * (weight_of(mid, scale) >> shift)) : 0ull;
-					at += v[j];
-				}
-				const unsigned long long all = block_sums(at, 0ull, scan).x;
-				__syncthreads();
-				at = block_before(at, scan);
-				const double want = (double)(enough - before_begin) / (double)(through_stop - before_begin);
-				double slack = 0.03;
-#pragma unroll 1
-				for (int trial = 0; trial < 2; ++trial) {
-					const double low = (want - slack) * (double)all, high = (want + slack) * (double)all;
-					if (t == 0) s_ends = make_int2((int)begin, (int)stop);
-					__syncthreads();
-					unsigned long long in = 0, z = at;
-#pragma unroll
-					for (int j = 0; j < 4; ++j) {
-						const uint32_t i = 4 * t + j;
-						if ((double)z <= low && low < (double)(z + v[j])) s_ends.x = (int)(begin + (i << down));
-						if ((double)z <= high && high < (double)(z + v[j])) s_ends.y = (int)min((unsigned long long)stop, (unsigned long long)begin + ((unsigned long long)(i + 1) << down));
-						if ((double)(z + v[j]) > low && (double)z <= high) in += counts[i];
-						z += v[j];
-					}
-					in = block_sums(in, 0ull, scan).x * (unsigned long long)(every * sub);      // tokens of the row that are to be expected
-					if (in <= (unsigned long long)kList * 3 / 4) break;
-					slack = max(0.01, slack * (double)(kList / 2) / (double)in);
-					__syncthreads();
-				}
-				__syncthreads();
-				if (sub > 1 && t < sub && t != 0) exchange_send(&s_ends, cta_addr(&s_bar[kEnds]), (uint32_t)t, s_ends);
-			} else {
-				late = !bounded_wait<true>(cta_addr(&s_bar[kEnds]), turn & 1u);
-				if (__syncthreads_or(late)) {
-					give_up(true);
-					return;
+	for (;;) {
+		const int32_t near_x = turn == 0u ? INT32_MIN + 1 : x_of(near), from_x = x_of(until);
+		const int32_t first_x = turn == 0u ? x_of(most) : near_x, kept_x = max(first_x, x_of(s_kept_far));      // what is added up, and what of it is kept
+		unsigned long long first_sum = 0, in_list = 0;
+		uint32_t many = 0;
+		if (by_steps && t < 2) steps[t == 0 ? 0 : last_step] = 0ull;
+		__syncthreads();
+		if (!late && !none && !have_list) {
+			if (weigh && end_x >= near_x) {
+				const uint32_t g = weight(end_x);
+				first_sum += g;
+				if (by_steps && end_x >= kept_x) {
+					++many;
+					atomicAdd(&steps[t < 4 ? 0 : last_step], (unsigned long long)g);
 				}
 			}
-			const uint32_t near = (uint32_t)s_ends.x, until = (uint32_t)s_ends.y;      // the window: near < d <= until
-			__syncthreads();
-			if (t == 0) s_n = 0u;
-			clear_steps();
-			// ---- a pass: weights up to the window, and of what is kept of them by 128 tokens; weights and list of the window
-			sum = listed = kept_sum = 0;
-			count = 0;
-			const int32_t until_x = x_of(until), near_x = x_of(near);
-			auto sure_of = [&](int32_t x) {
-				uint32_t g = 0;
-				if (x >= until_x) {
-					g = weight(x);
-					if (x >= near_x) kept_sum += g;
-					else listed += g;
-					g = x >= near_x && g >= floor_w ? g : 0u;
-				}
-				return g;
+			if (cuts && end_x >= from_x && !(by_steps && end_x >= near_x)) {
+				in_list += weight(end_x);
+				put_end();
+			}
+			// (two neighbouring words a thread and round, from the last ones on: what was read last is likelier still in L2)
+			const int rounds = (words + 2 * T - 1) / (2 * T);
+			auto fetch = [&](int k) { return (uint32_t)k < (uint32_t)words ? (KEEP ? kept[k] : __ldcg(from + k)) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN); };
+			auto wanted = [&](int4 u, int4 v) {      // of the list
+				if (!cuts || max(top_of(u), top_of(v)) < from_x) return 0u;
+				const uint32_t in = at_least(u, from_x) | at_least(v, from_x) << 4;
+				return by_steps ? in & ~(at_least(u, near_x) | at_least(v, near_x) << 4) : in;
 			};
-			add_end(sure_of(end_x));
-			if (end_x >= until_x && end_x < near_x) put(end_x, end);
-			each_group(Yes(), Kept(), [&](const int4 (&q)[U], int k) {
-				uint32_t which = 0;
-#pragma unroll
-				for (int u = 0; u < U; ++u) {
-					which |= (at_least(q[u], until_x) & ~at_least(q[u], near_x)) << (4 * u);
-					add_word(sure_of(q[u].x), sure_of(q[u].y), sure_of(q[u].z), sure_of(q[u].w), k + u * kThreads);
+			int k = 2 * ((rounds - 1) * T + t);
+			int4 q0 = fetch(k), q1 = fetch(k + 1);
+			uint32_t which = wanted(q0, q1), base = 0, at = reserve(which, base);
+#pragma unroll 1
+			for (int i = 0; i < rounds; ++i, k -= 2 * T) {
+				int4 y0 = q0, y1 = q1;
+				if (i + 1 < rounds) {
+					y0 = KEEP ? kept[k - 2 * T] : __ldcg(from + k - 2 * T);
+					y1 = KEEP ? kept[k - 2 * T + 1] : __ldcg(from + k - 2 * T + 1);
 				}
-				put_group(q, k, which);
-			});
-			const unsigned long long own_kept = sum;
-			ulonglong2 both = block_sums(kept_sum, listed, scan);      // (of all weights up to the window, and in it)
-			sum = both.x;
-			listed = both.y;
-			both = block_sums(own_kept, count, scan);
+				const int32_t x[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+				uint32_t g[8];
+				if (weigh) {
+#pragma unroll
+					for (int j = 0; j < 8; ++j) g[j] = weight_near((uint32_t)top - (uint32_t)x[j], scale);
+					if (cuts) {
+#pragma unroll
+						for (int j = 0; j < 8; ++j) first_sum += x[j] >= first_x ? g[j] : 0u;
+					}
+					if (by_steps) {
+						unsigned long long s8 = 0;
+#pragma unroll
+						for (int j = 0; j < 8; ++j) {
+							const bool yes = x[j] >= kept_x;
+							s8 += yes ? g[j] : 0u;
+							if (yes) ++many;
+						}
+						const uint32_t high = __reduce_add_sync(0xffffffffu, (uint32_t)(s8 >> 16)), low = __reduce_add_sync(0xffffffffu, (uint32_t)s8 & 0xFFFFu);
+						if (lane == 0 && k < words) steps[1 + (k >> 6)] = ((unsigned long long)high << 16) + low;
+					}
+				}
+				if (cuts) {      // (the room for them was asked for a round ago)
+					if (__ballot_sync(0xffffffffu, which != 0u) != 0u) {
+						at += __shfl_sync(0xffffffffu, base, 0);
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+							if ((which >> j & 1u) != 0u) {
+								put(at++, x[j], first + 4 * k + j);
+								in_list += weigh ? g[j] : 0u;
+							}
+					}
+					which = i + 1 < rounds ? wanted(y0, y1) : 0u;
+					at = reserve(which, base);
+				}
+				q0 = y0;
+				q1 = y1;
+			}
+			__syncthreads();
+		}
+		// ---- sums over the block (behind which its list is whole), and over all blocks
+		if (by_steps) {
+			kept_sum = 0;
+			if (!none && !late)
+				for (int i = t; i <= last_step; i += T) kept_sum += steps[i];
+			const ulonglong2 both = block_sums<T>(kept_sum, many, scan);
 			kept_sum = both.x;
 			kept_count = (uint32_t)both.y;
-			count = total = s_n;
-			others = 0;
-			if (sub > 1) {
-				const int slot = 1 + (int)(turn & 1u);
-				if (!tell(slot == 1 ? kWindow : kWindowOdd, slot, true, turn >> 1)) return;
-				add_up(slot, true);
-			}
+		}
+		{
+			const ulonglong2 both = block_sums<T>(first_sum, in_list, scan);
+			sum = cuts ? both.x : kept_sum;
+			listed = both.y;
+			count = total = cuts ? s_n : kept_count;
+		}
+		if (sub > 1) {
+			const int slot = turn == 0u ? 0 : 2 - (int)(turn & 1u), bar = slot == 0 ? kSums : (slot == 1 ? kWindow : kWindowOdd);
+			if (!tell(bar, slot, true, turn == 0u ? 0u : (turn - 1u) >> 1)) return;
+			add_up(slot, true);
+		}
+		if (!cuts || none) break;
+		if (turn == 0u) {
+			all_weights = sum;
+			enough = weigh ? share_of(sum, w.top_p, 30) : 0ull;
+			fits = total <= (uint32_t)kList && (complete || (weigh ? listed >= enough : total >= (uint32_t)w.top_k));
+			wide = !fits && weigh && total <= (uint32_t)kList;
+			if (!wide) break;
+			by_steps = true;
+			before_begin = listed;
+			through_stop = sum;
+		} else {
 			sure = sum;
 			if (sure < enough && enough <= sure + listed && total <= (uint32_t)kList) break;      // (the last kept one is the first up to which `enough` lies)
 			// not in the window, or more tokens than the list holds: closer in, for a few turns
@@ -811,21 +809,91 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 				begin = until;
 				before_begin = sure + listed;
 			}
-			wide = ++turn < 6u && stop - begin > 1u;
-			if (sub > 1 && wide) {
-				if (t == 0) {      // (of the next turn's ends and the next but one's sums; what comes may have come already)
-					asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[(turn & 1u) != 0u ? kWindow : kWindowOdd])), "r"((uint32_t)(sub * 20)) : "memory");
-					if (rank != 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[kEnds])), "r"(8u) : "memory");
+			wide = turn < 6u && stop - begin > 1u;
+			if (!wide) break;
+			if (sub > 1 && t == 0) {      // (of the next turn's ends and the next but one's sums; what comes may have come already)
+				asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[(turn & 1u) != 0u ? kWindow : kWindowOdd])), "r"((uint32_t)(sub * 20)) : "memory");
+				if (rank != 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(cta_addr(&s_bar[kEnds])), "r"(8u) : "memory");
+			}
+			__syncthreads();
+		}
+		// ---- a window. A sample (32,768 to 65,536 of the first block's tokens, or all) says where between begin and stop, to one or two in a hundred; the
+		// window is three to either side, or less where that would be too many tokens
+		if (rank == 0) {
+			const int down = max(0, 32 - __clz((int)(stop - begin)) - 11);
+			for (int i = t; i < kCounts; i += T) counts[i] = 0u;
+			__syncthreads();
+			const int every = max(1, words / 8192);
+#pragma unroll 2
+			for (int k = t * every; k < words; k += T * every) {
+				const int4 q = KEEP ? kept[k] : __ldcg(from + k);
+				const int32_t y[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+				for (int j = 0; j < 4; ++j) {
+					const uint32_t d = (uint32_t)top - (uint32_t)y[j];
+					if (d > begin && d <= stop) atomicAdd(&counts[min((d - begin - 1u) >> down, (uint32_t)kCounts - 1u)], 1u);
 				}
+			}
+			__syncthreads();
+			// weights of the places, in units such that none is above 2^15 (and no place's sum above 2^31)
+			const int shift = max(0, 17 - __clz((int)weight_of(begin, scale)));
+			constexpr int N = kCounts / T;
+			unsigned long long v[N], at = 0;
+#pragma unroll
+			for (int j = 0; j < N; ++j) {
+				const uint32_t i = N * t + j, mid = begin + 1u + (i << down) + ((1u << down) >> 1);
+				v[j] = mid > begin ? (unsigned long long)(counts[i] * (weight_of(mid, scale) >> shift)) : 0ull;
+				at += v[j];
+			}
+			const unsigned long long all = block_sums<T>(at, 0ull, scan).x;
+			__syncthreads();
+			at = block_before(at, scan);
+			const double want = (double)(enough - before_begin) / (double)(through_stop - before_begin);
+			double slack = 0.03;
+#pragma unroll 1
+			for (int trial = 0; trial < 2; ++trial) {
+				const double low = (want - slack) * (double)all, high = (want + slack) * (double)all;
+				if (t == 0) s_ends = make_int2((int)begin, (int)stop);
+				__syncthreads();
+				unsigned long long in = 0, z = at;
+#pragma unroll
+				for (int j = 0; j < N; ++j) {
+					const uint32_t i = N * t + j;
+					if ((double)z <= low && low < (double)(z + v[j])) s_ends.x = (int)(begin + (i << down));
+					if ((double)z <= high && high < (double)(z + v[j])) s_ends.y = (int)min((unsigned long long)stop, (unsigned long long)begin + ((unsigned long long)(i + 1) << down));
+					if ((double)(z + v[j]) > low && (double)z <= high) in += counts[i];
+					z += v[j];
+				}
+				in = block_sums<T>(in, 0ull, scan).x * (unsigned long long)(every * sub);      // tokens of the row that are to be expected
+				if (in <= (unsigned long long)kList * 3 / 4) break;
+				slack = max(0.01, slack * (double)(kList / 2) / (double)in);
 				__syncthreads();
 			}
+			__syncthreads();
+			if (sub > 1 && t < sub && t != 0) exchange_send(&s_ends, cta_addr(&s_bar[kEnds]), (uint32_t)t, s_ends);
+		} else {
+			late = !bounded_wait<true>(cta_addr(&s_bar[kEnds]), turn & 1u);
+			if (__syncthreads_or(late)) {
+				give_up(true);
+				return;
+			}
 		}
+		near = (uint32_t)s_ends.x;
+		until = (uint32_t)s_ends.y;
+		if (t == 0) s_n = 0u;
+		++turn;
+	}
+	Drawn out{-2, 0u, 0u, 0ull};
+	unsigned long long bound = ~0ull;      // the last key that is kept
+	if (cuts) by_steps = false;
+	if (cuts && !none) {
+		const unsigned long long origin = (unsigned long long)(0x7FFFFFFFu - (uint32_t)top) << kIndexBits;
 		if (!fits && !wide && rank != 0) return;
 		const uint32_t own_listed = count;      // (at the front of the list)
 		if (sub > 1 && (fits || wide)) {        // the lists, to the first block
 			const uint32_t bar = cta_addr(&s_bar[wide ? kWindowLists : kLists]);
 			if (rank != 0) {
-				for (uint32_t i = t; i < count; i += kThreads) exchange_send(list + others + i, bar, 0u, list[i]);
+				for (uint32_t i = t; i < count; i += T) exchange_send(list + others + i, bar, 0u, list[i]);
 				if (!wide) return;      // (nothing is sent to it any more)
 			} else {
 				if (t == 0) {
@@ -842,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		const Elements e{list, origin, w.logits, (int)total, V, top, scale, floor_w};
 		if (wide) {
 			if (rank == 0) {
-				bound = select_key<false>(e, kWeights, ~0ull, kIndexBits + 32 - __clz((int)most), enough - 1ull - sure, counts, s_select);
+				bound = select_key<T, false>(e, kWeights, ~0ull, kIndexBits + 32 - __clz((int)most), enough - 1ull - sure, counts, s_select);
 				if (t == 0) s_bound = bound;
 				__syncthreads();
 				if (sub > 1 && t < sub && t != 0) exchange_send(&s_bound, cta_addr(&s_bar[kBound]), (uint32_t)t, bound);
@@ -854,19 +922,19 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 				}
 				bound = s_bound;
 			}
-			// the block's tokens of the window that are kept, to their 128 neighbours
+			// the block's tokens of the window that are kept, to the sums of their 256 neighbours
 			sum = 0;
 			count = 0;
-			for (uint32_t i = t; i < own_listed; i += kThreads) {
+			for (uint32_t i = t; i < own_listed; i += T) {
 				const unsigned long long key = list[i] - origin;
 				const uint32_t g = key_weight(key, e);
 				if (key > bound || g < floor_w) continue;
 				const int v = (int)(key & (kMostVocab - 1));
 				sum += g;
 				++count;
-				atomicAdd(&steps[v < first ? 0 : (v >= last ? last_step : 1 + ((v - first) >> 7))], (unsigned long long)g);
+				atomicAdd(&steps[v < first ? 0 : (v >= last ? last_step : 1 + ((v - first) >> 8))], (unsigned long long)g);
 			}
-			const ulonglong2 both = block_sums(sum, count, scan);
+			const ulonglong2 both = block_sums<T>(sum, count, scan);
 			sum = both.x + kept_sum;
 			count = total = (uint32_t)both.y + kept_count;
 			if (sub > 1) {
@@ -875,13 +943,13 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 			}
 			by_steps = true;
 		} else if (fits) {
-			out = draw_from<false>(e, w.top_k, w.top_p, w.draw, all_weights, counts, s_select);
+			out = draw_from<T, false>(e, w.top_k, w.top_p, w.draw, all_weights, counts, s_select);
 		} else {
-			out = draw_from<true>(e, w.top_k, w.top_p, w.draw, all_weights, counts, s_select);
+			out = draw_from<T, true>(e, w.top_k, w.top_p, w.draw, all_weights, counts, s_select);
 		}
 	}
 	if (by_steps && !none) {
-		// the block whose sums the mark lies in, the 128 tokens, then the token
+		// the block whose sums the mark lies in, the 256 tokens, then the token
 		unsigned long long mark = share_of(sum, w.draw, 31);
 		int owner = 0;
 		if (sub > 1) {
@@ -898,18 +966,19 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		if (rank != owner) return;
 		out.sum = sum;
 		out.number = total;
-		unsigned long long v[4], at = 0;
+		constexpr int N = kSteps / T;
+		unsigned long long v[N], at = 0;
 #pragma unroll
-		for (int j = 0; j < 4; ++j) {
-			v[j] = 4 * t + j <= last_step ? steps[4 * t + j] : 0ull;
+		for (int j = 0; j < N; ++j) {
+			v[j] = N * t + j <= last_step ? steps[N * t + j] : 0ull;
 			at += v[j];
 		}
 		__syncthreads();
 		at = block_before(at, scan);
 #pragma unroll
-		for (int j = 0; j < 4; ++j) {
+		for (int j = 0; j < N; ++j) {
 			if (at <= mark && mark < at + v[j]) {
-				s_select.place = 4 * t + j;
+				s_select.place = N * t + j;
 				s_select.target = mark - at;
 			}
 			at += v[j];
@@ -918,13 +987,13 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		if (warp != 0) return;
 		const int step = (int)s_select.place;
 		mark = s_select.target;
-		const int v0 = step == 0 ? s0 : (step == last_step ? last : first + 128 * (step - 1)), v1 = step == 0 ? first : (step == last_step ? s1 : min(last, v0 + 128));
-		uint32_t g[4];
+		const int v0 = step == 0 ? s0 : (step == last_step ? last : first + 256 * (step - 1)), v1 = step == 0 ? first : (step == last_step ? s1 : min(last, v0 + 256));
+		uint32_t g[8];
 		unsigned long long own = 0;
 #pragma unroll
-		for (int j = 0; j < 4; ++j) {
-			const int i = v0 + 4 * lane + j;
-			const int32_t x = i < v1 ? w.logits[i] : INT32_MIN;
+		for (int j = 0; j < 8; ++j) {
+			const int i = v0 + 8 * lane + j;
+			const int32_t x = i < v1 ? logits[i] : INT32_MIN;
 			g[j] = weight(x);
 			if (g[j] < floor_w || ((unsigned long long)((uint32_t)top - (uint32_t)x) << kIndexBits | (uint32_t)i) > bound) g[j] = 0u;
 			own += g[j];
@@ -938,9 +1007,9 @@ __global__ void __launch_bounds__(kThreads, KEEP ? 1 : 2) k_sample(const __grid_
 		unsigned long long before = upto - own;
 		const int who = __ffs(__ballot_sync(0xffffffffu, before <= mark && mark < upto)) - 1;
 #pragma unroll
-		for (int j = 0; j < 4; ++j) {
+		for (int j = 0; j < 8; ++j) {
 			if (out.token < 0 && before <= mark && mark < before + g[j]) {
-				out.token = v0 + 4 * lane + j;
+				out.token = v0 + 8 * lane + j;
 				out.weight = g[j];
 			}
 			before += g[j];
@@ -972,10 +1041,10 @@ void sample_plan(SampleArgs* a) {
 	a->keep = a->rows * a->sub <= sms && SampleSmem::bytes(1, a->slice) <= (size_t)220 * 1024 ? 1 : 0;
 }
 
-template <bool RESIDENT, bool KEEP>
-cudaError_t sample_launch(SampleArgs a, cudaStream_t st) {
+template <bool RESIDENT, bool KEEP, int T, int BLOCKS>
+cudaError_t sample_launch_as(SampleArgs a, cudaStream_t st) {
 	static PerDeviceOnce once;
-	const auto kernel = k_sample<RESIDENT, KEEP>;
+	const auto kernel = k_sample<RESIDENT, KEEP, T, BLOCKS>;
 	cudaError_t e = once_per_device(once, [&] {
 		const cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 		return x != cudaSuccess ? x : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KEEP ? 220 * 1024 : (int)SampleSmem::bytes(0, 0));
@@ -984,7 +1053,7 @@ cudaError_t sample_launch(SampleArgs a, cudaStream_t st) {
 	a.debug_withhold = exchange_debug_take(kExchangeSample);
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3(a.sub, a.rows);
-	cfg.blockDim = dim3(kThreads);
+	cfg.blockDim = dim3(T);
 	cfg.dynamicSmemBytes = SampleSmem::bytes(KEEP, a.slice);
 	cfg.stream = st;
 	cudaLaunchAttribute attr[2];
@@ -998,6 +1067,11 @@ cudaError_t sample_launch(SampleArgs a, cudaStream_t st) {
 	cfg.numAttrs = pdl_enabled() ? 2 : 1;
 	return cudaLaunchKernelEx(&cfg, kernel, a);
 }
+template <bool RESIDENT>
+cudaError_t sample_launch(const SampleArgs& a, cudaStream_t st) {
+	if (a.keep) return sample_launch_as<RESIDENT, true, 512, 1>(a, st);
+	return a.rows * a.sub <= sm_count() ? sample_launch_as<RESIDENT, false, 512, 1>(a, st) : sample_launch_as<RESIDENT, false, 512, 2>(a, st);
+}
 
 }  // namespace
 
@@ -1006,7 +1080,7 @@ cudaError_t launch_sample(const SampleRow* rows, int m, int vocab, const Scale* 
 	a.rows = m; a.vocab = vocab;
 	a.desc = rows; a.scales = scales; a.best = best; a.status = status;
 	sample_plan(&a);
-	return a.keep ? sample_launch<false, true>(a, st) : sample_launch<false, false>(a, st);
+	return sample_launch<false>(a, st);
 }
 
 }  // namespace sslm
@@ -1029,7 +1103,7 @@ extern "C" sslm_status sslm_b200_sample_resident(const sslm_b200_sample* call, v
 	a.out_tokens = c.out_tokens; a.out_mass = c.out_mass; a.out_kept = c.out_kept;
 	a.status = c.row_status;
 	sample_plan(&a);
-	if ((a.keep ? sample_launch<true, true>(a, (cudaStream_t)stream) : sample_launch<true, false>(a, (cudaStream_t)stream)) != cudaSuccess) {
+	if (sample_launch<true>(a, (cudaStream_t)stream) != cudaSuccess) {
 		cudaGetLastError();
 		return SSLM_ALLOCATION_FAILED;
 	}
