@@ -282,7 +282,8 @@ SSLM_API sslm_status sslm_b200_debug_withhold_tc_load(int32_t launches);
  * where K is cut over a cluster (exchange 0); 1: attention of few rows (0 maxima, 1 sums, 2 contexts, 3 the
  * funnel's maximum); 2: attention of prefill chunks in tiles cut over a cluster (0 to 2); 3: the activation
  * site (0); 5: attention of few biased rows with the q/k/v site inside (0 the biased elements' maximum); 6: attention of
- * rows that share a prefix (0 to 2, 3 its copies of V); 7: the pick (0, 1 its first copy of logits). kernel -1 takes the request back. */
+ * rows that share a prefix (0 to 2, 3 its copies of V); 7: the pick (0, 1 its first copy of logits); 8: the draw (0 maxima, 1 sums,
+ * 2 lists, and of a window 3 its ends, 4 its sums, 5 its lists, 6 the last key, 7 what is kept; 3 and 6 in the second block). kernel -1 takes the request back. */
 SSLM_API sslm_status sslm_b200_debug_withhold_exchange(int32_t kernel, int32_t exchange);
 /* Tests only: the first kernel of each of the next `launches` (0..16) row groups counts as refused by the CUDA
  * runtime, as for want of resources. The verb returns SSLM_ALLOCATION_FAILED and launches nothing behind it. */
@@ -351,6 +352,33 @@ typedef struct sslm_b200_controls {
 	const int32_t* bias_values;
 } sslm_b200_controls;
 SSLM_API sslm_status sslm_b200_seq_set_controls(sslm_seq seq, const sslm_b200_controls* controls);
+
+/* Sampling: from this call on sslm_decode_step draws the sequence's tokens from its logit row as sslm_b200_sample_resident (below) does, after
+ * its controls and its schema's mask if it has them (where that allows nothing the step answers as before). A logit unit is worth the scale of the row that the
+ * head multiplies times that of the head's weights, (head_m, head_e), 2^30 <= head_m < 2^31 and |head_e| <= 4,096, or with head_m = 0 the
+ * embedding's (a model whose head has weights of its own: SSLM_INVALID_ARGUMENT); a row's temperature divides it. The first n_draws tokens take draws[i]
+ * (0 .. 2^31 - 1), later ones numbers made from the seed and how many tokens were drawn since this call, or since the last sslm_seq_reset. Other
+ * sequences of a call are chosen for as ever, and a save blob has nothing of this. NULL goes back to the greedy token; a second call
+ * replaces the first. Outside these ranges, or with a list missing: SSLM_INVALID_ARGUMENT; nothing changes then. Room for logit rows as with controls. */
+typedef struct sslm_b200_sampling {
+	uint32_t struct_size;
+	int32_t temperature;             /* Q16: 65,536 is 1.0 */
+	int32_t top_k;                   /* 0: no limit */
+	int32_t top_p, min_p;            /* shares of 2^30; 2^30 and 0: no limit */
+	int32_t n_draws;
+	int64_t head_m, head_e;
+	uint64_t seed;
+	const int32_t* draws;
+	uint64_t reserved;
+} sslm_b200_sampling;
+SSLM_API sslm_status sslm_b200_seq_set_sampling(sslm_seq seq, const sslm_b200_sampling* sampling);
+
+/* `seq` becomes a copy of `parent` as it is now, between two tokens (else SSLM_SEQ_RESET_MIDTOKEN_REJECTED, for either of them): several answers to
+ * one question, the branches of a search. What it was is gone. It has the parent's adapter, schema and walk, and its history; its controls and its
+ * sampling stay its own (its draws begin again). Both go on by themselves as if each had been given all that was before: same tokens, same save blobs. The
+ * full 16-token pages are shared, the partly filled one is copied; the call does not wait for that. Sequences of one pool of one model
+ * (else SSLM_INVALID_ARGUMENT). */
+SSLM_API sslm_status sslm_b200_seq_fork(sslm_seq seq, sslm_seq parent);
 
 /* Bytes of HBM held by the model's weights, tables and constants. */
 SSLM_API size_t sslm_b200_model_device_bytes(sslm_model model);

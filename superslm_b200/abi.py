@@ -53,6 +53,11 @@ class SslmControls(C.Structure):
                 ("count_given", C.c_int32), ("n_bias", C.c_int32), ("bias_tokens", C.POINTER(C.c_int32)), ("bias_values", C.POINTER(C.c_int32))]
 
 
+class SslmSampling(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("temperature", C.c_int32), ("top_k", C.c_int32), ("top_p", C.c_int32), ("min_p", C.c_int32), ("n_draws", C.c_int32),
+                ("head_m", C.c_int64), ("head_e", C.c_int64), ("seed", C.c_uint64), ("draws", C.POINTER(C.c_int32)), ("reserved", C.c_uint64)]
+
+
 _H = C.c_void_p  # opaque handle
 
 
@@ -268,6 +273,32 @@ class Sequence:
         c = SslmControls(C.sizeof(SslmControls), repetition, presence, frequency, int(count_given), len(biases),
                          C.cast(tokens, C.POINTER(C.c_int32)), C.cast(values, C.POINTER(C.c_int32)))
         _chk("sslm_b200_seq_set_controls", fn(self.handle, C.addressof(c)))
+
+    def set_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=0, draws=(), head_scale=None):
+        """sslm_b200_seq_set_sampling: tokens are drawn; draws: the first ones' random numbers (31 bits); head_scale: (m, e) of the head's weights where they
+        are not the embedding's. temperature=None goes back to the greedy token."""
+        fn = self.eng.lib.dll.sslm_b200_seq_set_sampling
+        fn.restype, fn.argtypes = C.c_int, [_H, C.c_void_p]
+        if temperature is None:
+            _chk("sslm_b200_seq_set_sampling", fn(self.handle, None))
+            return
+        draws = list(draws)
+        numbers = (C.c_int32 * len(draws))(*draws)
+        m, e = (0, 0) if head_scale is None else head_scale
+        c = SslmSampling(C.sizeof(SslmSampling), int(round(temperature * 65536)), top_k, max(1, int(top_p * (1 << 30))), int(min_p * (1 << 30)), len(draws), m, e, seed,
+                         C.cast(numbers, C.POINTER(C.c_int32)), 0)
+        _chk("sslm_b200_seq_set_sampling", fn(self.handle, C.addressof(c)))
+
+    def fork(self, into: "Sequence" = None) -> "Sequence":
+        """sslm_b200_seq_fork: a sequence (a new one of the engine, or `into`) that goes on from where this one is."""
+        child = self.eng.new_seq() if into is None else into
+        fn = self.eng.lib.dll.sslm_b200_seq_fork
+        fn.restype, fn.argtypes = C.c_int, [_H, _H]
+        st = fn(child.handle, self.handle)
+        if st != SSLM_OK and into is None:
+            child.release()
+        _chk("sslm_b200_seq_fork", st)
+        return child
 
     def save(self) -> bytes:
         n = C.c_size_t(0)

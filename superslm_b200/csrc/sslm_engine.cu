@@ -20,6 +20,7 @@ namespace {
 std::atomic<int> g_device{-1};
 std::mutex g_seq_registry_mutex;
 std::unordered_set<sslm_seq_s*> g_live_seqs;
+std::atomic<uint64_t> g_seq_uid{0};      // of sequences and of forks' common pages
 
 int current_device_choice() {
 	int d = g_device.load();
@@ -398,7 +399,7 @@ bool config_ok(const sslm_model_s* model, const sslm_config* c) {
 	return c->reserved == 0;
 }
 
-constexpr size_t kUpBytesPerRow = sizeof(RowDesc) + sizeof(RowSource) + sizeof(RowSink) + 4 * sizeof(int32_t) + sizeof(void*) + sizeof(PickRow);
+constexpr size_t kUpBytesPerRow = sizeof(RowDesc) + sizeof(RowSource) + sizeof(RowSink) + 4 * sizeof(int32_t) + sizeof(void*) + sizeof(PickRow) + sizeof(SampleRow);
 constexpr size_t kDownBytesPerRow = 8 + 8 + 4 + 4;      // arg-max key, saturations, status, finished layers
 
 // Lay the upload and read-back blocks out for a call of n rows.
@@ -415,6 +416,7 @@ void bind_rows(sslm_workspace_s* w, int n) {
 	up(w->h_group, w->d_group, n * 4 * sizeof(int32_t));
 	up(w->h_row_mask, w->d_row_mask, n * sizeof(void*));
 	up(w->h_pick, w->d_pick, n * sizeof(PickRow));
+	up(w->h_sample, w->d_sample, n * sizeof(SampleRow));
 	w->h_best = (unsigned long long*)w->h_down;
 	w->h_sat = w->h_best + n;
 	w->h_status = (int32_t*)(w->h_sat + n);

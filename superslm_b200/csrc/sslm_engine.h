@@ -61,10 +61,11 @@ struct sslm_workspace_s {
 	unsigned int* d_tc_counters = nullptr;
 	int32_t* logit_capture = nullptr;   // host buffer for full logit rows (tests), or nullptr
 	int32_t* d_logits = nullptr;
-	// full logit rows of a decode call in which some sequence has controls (pick_room: allocated by the first such call); records of their picks
+	// full logit rows of a decode call in which some sequence has controls or is sampled (pick_room: allocated by the first such call); records of their picks
 	int32_t* d_pick_logits = nullptr;
 	size_t pick_rows = 0;
 	sslm::PickRow *h_pick = nullptr, *d_pick = nullptr;
+	sslm::SampleRow *h_sample = nullptr, *d_sample = nullptr;      // and of their draws
 	cudaEvent_t ev[2][2] = {};    // start and end: of the call at hand [ev_now] and of the last completed one [ev_now ^ 1]
 	int ev_now = 0;
 	float last_ms = 0.f;
@@ -177,7 +178,7 @@ struct sslm_seq_s {
 	size_t pages_on_device = 0;     // entries of it that are in place
 	uint64_t batch_mark = 0;        // the decode batch the sequence was last put into
 	uint64_t uid = 0;               // of the sequences created so far
-	// the first pages are those of the frozen prefix with this uid (0: none): sequences of one prefix have the same ones
+	// the first pages are those of the frozen prefix with this uid, or of the fork it was given out for (0: none): sequences with one uid have the same ones
 	// tokens the sequence was given and tokens it produced, in order (since it was created, reset or restored)
 	std::vector<int32_t> given, produced;
 	// penalties and biases of its picks (sslm_b200_seq_set_controls); their ids and the biases lie in the sequence's slot of the pool
@@ -185,6 +186,13 @@ struct sslm_seq_s {
 	int32_t theta = 0, presence = 0, frequency = 0, n_bias = 0;
 	int32_t *d_history = nullptr, *d_bias = nullptr;
 	size_t given_on_device = 0, produced_on_device = 0;      // ids that count and are in d_history (given ones before later produced ones or behind)
+	// how its tokens are drawn (sslm_b200_seq_set_sampling): octaves a logit unit of a row of scale one, limits, and the random numbers
+	bool sampled = false;
+	int64_t slope_m = 0, slope_e = 0;
+	int32_t top_k = 0;
+	uint32_t top_p = 0, min_p = 0;
+	uint64_t seed = 0, drawn = 0;      // tokens drawn so far
+	std::vector<int32_t> draws;
 	uint64_t shared_uid = 0;
 	int32_t shared_pages = 0;
 	int64_t context_length = 0;

@@ -204,7 +204,8 @@ void launch_lora_u(const RowBatch& b, const int8_t* x, int k_in, int layer, int 
 // ---- the pick of rows whose sequences carry controls (sslm_pick.cu)
 constexpr int kPickMaxBias = 1024;      // biases of a row
 // best[r] of the rows whose record has logits; names: ids that a row's history, its extra one and its biases have at most, biases of them
-cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* status, cudaStream_t st);
+// (out: the changed rows, [m][vocab], which may be the rows themselves, or nullptr)
+cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* out, int32_t* status, cudaStream_t st);
 
 // ---- the draw of rows whose sequences are sampled (sslm_sample.cu): best[r] of the rows whose record has logits; scales: of the rows
 // that the head multiplied

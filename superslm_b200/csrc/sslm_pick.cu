@@ -575,11 +575,13 @@ cudaError_t pick_launch(PickArgs a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* status, cudaStream_t st) {
+cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int biases, unsigned long long* best, int32_t* out, int32_t* status, cudaStream_t st) {
 	PickArgs a{};
 	a.rows = m; a.vocab = vocab;
 	a.desc = rows; a.best = best; a.status = status;
+	a.out_logits = out; a.out_stride = vocab;
 	const bool table = pick_plan(names, biases, &a);
+	if (out != nullptr) return table ? pick_launch<false, true, true>(a, st) : pick_launch<false, false, true>(a, st);
 	return table ? pick_launch<false, true, false>(a, st) : pick_launch<false, false, false>(a, st);
 }
 
