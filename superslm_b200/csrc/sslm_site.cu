@@ -8,7 +8,8 @@
 //   rotation: pairs of channels, neighbours or rotary / 2 apart, on codes, with angles of 30 bits
 //
 // A thread takes four neighbouring elements (a quad), so a head is 8, 16 or 32 neighbouring lanes: what a head needs of itself (its maximum,
-// its sum of squares, the other half of its pairs) is exchanged in the warp. Only the funnel's maximum needs the block.
+// its sum of squares, the other half of its pairs) is exchanged in the warp. Only the funnel's maximum needs the block. Two forms: a block a
+// row, and for many rows eight rows a block.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -26,7 +27,102 @@ struct SiteArgs {
 	sslm_b200_qkv_site c;
 	int nq, nk, total;      // quads of q, of K (and as many of V), of the row
 	int lanes;              // of a head
+	int q_warps, k_warps;   // of q, of K (and as many of V) when a warp has 32 quads of one of them
 };
+
+// what a row says of itself; code 0 and a position: it is worked on. (Everything but the page is asked for at once.)
+struct SiteRow {
+	int pos, place, page, code;
+	int in_m, in_e;
+};
+__device__ __forceinline__ SiteRow site_row(const sslm_b200_qkv_site& a, int64_t r, bool lands) {
+	const bool scaled = a.q_gain == nullptr || lands;
+	SiteRow w{a.positions[r], 0, 0, 0, 1 << 30, 0};
+	const int64_t m = scaled ? a.in_scales[2 * r] : (int64_t)1 << 30, e = scaled ? a.in_scales[2 * r + 1] : 0;
+	const int place = lands && a.places != nullptr ? a.places[r] : w.pos, table = lands && a.table_of != nullptr ? a.table_of[r] : (int)r;
+	if (w.pos == -1) return w;
+	if (w.pos < 0 || w.pos >= a.num_positions) w.code = SSLM_B200_ROW_LENGTH;
+	if (m < ((int64_t)1 << 30) || m >= ((int64_t)1 << 31) || e < -4096 || e > 4096) w.code = w.code != 0 ? w.code : SSLM_B200_ROW_CONSTANTS;
+	else {
+		w.in_m = (int)m;
+		w.in_e = (int)e;
+	}
+	if (lands) {
+		w.place = place;
+		if (place < 0 || place >= a.table_pages * kPageTokens) w.code = w.code != 0 ? w.code : SSLM_B200_ROW_LENGTH;
+		else if (table < 0 || table >= a.num_tables) w.code = w.code != 0 ? w.code : SSLM_B200_ROW_INDEX;
+		else {
+			w.page = a.pages[table * a.pages_stride + place / kPageTokens];
+			if (w.page < 0 || w.page >= a.num_pages) w.code = w.code != 0 ? w.code : SSLM_B200_ROW_INDEX;
+		}
+	}
+	return w;
+}
+
+// four elements landed on their head's scale: codes in the low word, how many were held in the high one
+static __device__ __noinline__ uint64_t land_quad_exact(int32_t x0, int32_t x1, int32_t x2, int32_t x3, int64_t m, int64_t r_t, int64_t e, int64_t e_t) {
+	const int32_t x[4] = {x0, x1, x2, x3};
+	int c[4];
+	uint32_t held = 0;
+	for (int j = 0; j < 4; ++j) {
+		bool over;
+		const int64_t v = landing_rescale(x[j], m, r_t, e, e_t, &over, nullptr);
+		c[j] = over ? (x[j] < 0 ? -127 : 127) : (int)v;
+		held += over ? 1u : 0u;
+	}
+	return (uint64_t)held << 32 | pack4(c[0], c[1], c[2], c[3]);
+}
+__device__ __forceinline__ uint32_t land_quad(const int32_t (&x)[4], Scale in, int64_t e_t, int64_t r_t, uint32_t& held) {
+	const Lander l = make_lander(in.m, r_t, in.e, e_t);
+	if (!l.fast) {
+		const uint64_t v = land_quad_exact(x[0], x[1], x[2], x[3], in.m, r_t, in.e, e_t);
+		held += (uint32_t)(v >> 32);
+		return (uint32_t)v;
+	}
+	int c[4];
+#pragma unroll
+	for (int j = 0; j < 4; ++j) {
+		const uint64_t m = land_magnitude(abs_u32(x[j]), l);
+		held += m > 127 ? 1u : 0u;
+		c[j] = (int)min(m, (uint64_t)127);
+		if (x[j] < 0) c[j] = -c[j];
+	}
+	return pack4(c[0], c[1], c[2], c[3]);
+}
+
+// the codes c at elements e to e + 3 of a head turned by a row of the tables (all lanes of the warp take part)
+__device__ __forceinline__ uint32_t turn_quad(const sslm_b200_qkv_site& a, uint32_t c, int e, const int32_t* cos, const int32_t* sin, bool turned) {
+	const int lane = threadIdx.x & 31, half_lanes = a.rotary >> 3;
+	const uint32_t other = a.halves ? __shfl_sync(0xffffffffu, c, e < a.rotary ? (e < a.rotary / 2 ? lane + half_lanes : lane - half_lanes) : lane) : 0u;
+	if (!turned || e >= a.rotary) return c;
+	if (!a.halves) return rope_quad(c, *(const int2*)(cos + (e >> 1)), *(const int2*)(sin + (e >> 1)));
+	const bool low = e < a.rotary / 2;
+	const int at = low ? e : e - a.rotary / 2;
+	const int4 cs = *(const int4*)(cos + at), sn = *(const int4*)(sin + at);
+	const int co[4] = {cs.x, cs.y, cs.z, cs.w}, si[4] = {sn.x, sn.y, sn.z, sn.w};
+	int out[4];
+#pragma unroll
+	for (int j = 0; j < 4; ++j) {
+		const int mine = byte_of(c, j), theirs = byte_of(other, j);
+		out[j] = rope_round(low ? (int64_t)mine * co[j] - (int64_t)theirs * si[j] : (int64_t)theirs * si[j] + (int64_t)mine * co[j]);
+	}
+	return pack4(out[0], out[1], out[2], out[3]);
+}
+
+// softmax constants of row r for the kv heads first, first + step, ...; true where one cannot be
+static __device__ __noinline__ bool site_consts(const int64_t* khead, int64_t* consts, int kv_heads, int64_t r, Scale q, int first, int step) {
+	bool bad = false;
+	for (int h = first; h < kv_heads; h += step) {
+		SoftmaxConsts sc;
+		const bool none = softmax_consts(q, Scale{khead[2 * h], khead[2 * h + 1]}, 1, &sc) != kOk;
+		int64_t* to = consts + (r * kv_heads + h) * 3;
+		to[0] = none ? 0 : sc.c.q_ln2;
+		to[1] = none ? 0 : sc.c.q_b;
+		to[2] = none ? 0 : sc.c.q_c;
+		bad = bad || none;
+	}
+	return bad;
+}
 
 // u = y R / 2^36 in Q15 and the code of it: R = floor(2^54 / root) below 2^32, y at most 2^24, u below 2^19
 __device__ __forceinline__ uint32_t norm_reciprocal(uint64_t mean) {
@@ -70,6 +166,9 @@ __device__ __forceinline__ void norm_quad(const int32_t (&x)[4], const int16_t* 
 	}
 }
 
+// A block a row, NV quads a thread. One quad where there is a block for every SM at most, the shortest way through a row (32 rows, 16 + 2 + 2
+// heads of 128, from a cold cache: 8.2 us, two quads 10.2); two up to kRows rows for every SM, because a block does a row's scalars in every warp
+// (512 rows: 10.1, one quad 14.3, four 10.4; normed 13.5, 16.7, 16.3); more only for rows that need more threads than a block has.
 template <int NV>
 __global__ void __launch_bounds__(NV == 1 ? 1024 : 512)
 k_qkv_site(const __grid_constant__ SiteArgs g) {
@@ -89,30 +188,9 @@ k_qkv_site(const __grid_constant__ SiteArgs g) {
 		else if (i < g.nq + g.nk) load_quad(a.k + r * a.k_stride + 4 * (i - g.nq), x[v]);
 		else if (i < g.total) load_quad(a.v + r * a.v_stride + 4 * (i - g.nq - g.nk), x[v]);
 	}
-	// the row's record (all threads alike)
-	const int pos = a.positions[r];
-	int code = 0, place = 0;
-	int64_t page = 0;
-	Scale in{(int64_t)1 << 30, 0};
-	if (pos != -1) {
-		if (pos < 0 || pos >= a.num_positions) code = SSLM_B200_ROW_LENGTH;
-		if (a.q_gain == nullptr || g.nk > 0) {
-			in = Scale{a.in_scales[2 * r], a.in_scales[2 * r + 1]};
-			if (in.m < ((int64_t)1 << 30) || in.m >= ((int64_t)1 << 31) || in.e < -4096 || in.e > 4096) code = code != 0 ? code : SSLM_B200_ROW_CONSTANTS;
-		}
-		if (g.nk > 0) {
-			place = a.places != nullptr ? a.places[r] : pos;
-			const int table = a.table_of != nullptr ? a.table_of[r] : (int)r;
-			if (place < 0 || place >= a.table_pages * kPageTokens) code = code != 0 ? code : SSLM_B200_ROW_LENGTH;
-			else if (table < 0 || table >= a.num_tables) code = code != 0 ? code : SSLM_B200_ROW_INDEX;
-			else {
-				page = a.pages[table * a.pages_stride + place / kPageTokens];
-				if (page < 0 || page >= a.num_pages) code = code != 0 ? code : SSLM_B200_ROW_INDEX;
-			}
-		}
-	}
-	if (pos == -1 || code != 0) {
-		if (t == 0 && a.row_status != nullptr) a.row_status[r] = code;
+	const SiteRow w = site_row(a, r, g.nk > 0);      // (all threads alike)
+	if (w.pos == -1 || w.code != 0) {
+		if (t == 0 && a.row_status != nullptr) a.row_status[r] = w.code;
 		return;
 	}
 	const Scale site{a.q_site_m, a.q_site_e};
@@ -123,10 +201,13 @@ k_qkv_site(const __grid_constant__ SiteArgs g) {
 #pragma unroll
 		for (int v = 0; v < NV; ++v)
 			if (t + v * T < g.nq) top = max(max(max(top, abs_u32(x[v][0])), abs_u32(x[v][1])), max(abs_u32(x[v][2]), abs_u32(x[v][3])));
-		const FunnelFold fold = funnel_prefold(&in, 1, site);
+		const Scale scale{w.in_m, w.in_e};
+		const FunnelFold fold = funnel_prefold(&scale, 1, site);
 		fp = quad_funnel(T > 32 ? block_max_u32(top, bank) : __reduce_max_sync(0xffffffffu, top), fold);      // (canonical scales: never refused)
 	}
-	const int half_lanes = a.rotary >> 3, slot = place % kPageTokens;
+	const int slot = w.place % kPageTokens;
+	const int64_t turn = (int64_t)w.pos * (a.rotary >> 1);
+	const Scale in{w.in_m, w.in_e};
 	uint32_t held = 0;
 #pragma unroll
 	for (int v = 0; v < NV; ++v) {
@@ -149,50 +230,15 @@ k_qkv_site(const __grid_constant__ SiteArgs g) {
 		if (!is_q && !normed && i < g.total) {
 			const int64_t* rec = (is_k ? a.k_landing : a.v_landing) + 3 * head;
 			const int64_t e_t = rec[1], r_t = rec[2];
-			const Lander l = make_lander(in.m, r_t, in.e, e_t);
-			int lc[4];
-#pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				bool s1;
-				if (l.fast) {
-					const uint64_t m = land_magnitude(abs_u32(x[v][j]), l);
-					s1 = m > 127;
-					lc[j] = s1 ? 127 : (int)m;
-					if (x[v][j] < 0) lc[j] = -lc[j];
-				} else {
-					const int64_t m = landing_rescale(x[v][j], in.m, r_t, in.e, e_t, &s1, nullptr);
-					lc[j] = s1 ? (x[v][j] < 0 ? -127 : 127) : (int)m;
-				}
-				held += s1 ? 1u : 0u;
-			}
-			c = pack4(lc[0], lc[1], lc[2], lc[3]);
+			c = land_quad(x[v], in, e_t, r_t, held);
 		}
-		// rotation
-		const uint32_t other = a.halves ? __shfl_sync(0xffffffffu, c, e < a.rotary ? (e < a.rotary / 2 ? lane + half_lanes : lane - half_lanes) : lane) : 0u;
-		if ((is_q || is_k) && e < a.rotary) {
-			const int64_t row = (int64_t)pos * (a.rotary >> 1);
-			if (!a.halves) {
-				c = rope_quad(c, *(const int2*)(a.cos + row + (e >> 1)), *(const int2*)(a.sin + row + (e >> 1)));
-			} else {
-				const bool low = e < a.rotary / 2;
-				const int at = low ? e : e - a.rotary / 2;
-				const int4 cs = *(const int4*)(a.cos + row + at), sn = *(const int4*)(a.sin + row + at);
-				const int co[4] = {cs.x, cs.y, cs.z, cs.w}, si[4] = {sn.x, sn.y, sn.z, sn.w};
-				int out[4];
-#pragma unroll
-				for (int j = 0; j < 4; ++j) {
-					const int mine = byte_of(c, j), theirs = byte_of(other, j);
-					out[j] = rope_round(low ? (int64_t)mine * co[j] - (int64_t)theirs * si[j] : (int64_t)theirs * si[j] + (int64_t)mine * co[j]);
-				}
-				c = pack4(out[0], out[1], out[2], out[3]);
-			}
-		}
+		c = turn_quad(a, c, e, a.cos + turn, a.sin + turn, is_q || is_k);
 		if (is_q) {
 			*(uint32_t*)(a.q_codes + r * a.q_codes_stride + 4 * i) = c;
 		} else if (is_k) {
-			*(uint32_t*)(a.kv + ((2 * (int64_t)head * a.num_pages + page) * kPageTokens + slot) * hd + e) = c;
+			*(uint32_t*)(a.kv + ((2 * (int64_t)head * a.num_pages + (int64_t)w.page) * kPageTokens + slot) * hd + e) = c;
 		} else if (is_v) {
-			int8_t* to = a.kv + (((2 * (int64_t)head + 1) * a.num_pages + page) * hd + e) * kPageTokens + slot;
+			int8_t* to = a.kv + (((2 * (int64_t)head + 1) * a.num_pages + (int64_t)w.page) * hd + e) * kPageTokens + slot;
 #pragma unroll
 			for (int j = 0; j < 4; ++j) to[j * kPageTokens] = (int8_t)byte_of(c, j);
 		}
@@ -209,27 +255,394 @@ k_qkv_site(const __grid_constant__ SiteArgs g) {
 			a.q_scales[2 * r] = fp.out.m;
 			a.q_scales[2 * r + 1] = fp.out.e;
 		}
-		if (a.consts != nullptr) {
-			for (int h = lane; h < a.kv_heads; h += 32) {
-				const Scale kh{a.khead[2 * h], a.khead[2 * h + 1]};
-				SoftmaxConsts sc;
-				const bool none = softmax_consts(fp.out, kh, 1, &sc) != kOk;
-				int64_t* to = a.consts + (r * a.kv_heads + h) * 3;
-				to[0] = none ? 0 : sc.c.q_ln2;
-				to[1] = none ? 0 : sc.c.q_b;
-				to[2] = none ? 0 : sc.c.q_c;
-				bad = bad || none;
-			}
-		}
+		if (a.consts != nullptr) bad = site_consts(a.khead, a.consts, a.kv_heads, r, fp.out, lane, 32);
 	}
 	bad = __any_sync(0xffffffffu, bad);
 	if (lane == 0 && a.row_status != nullptr) a.row_status[r] = bad ? SSLM_B200_ROW_SOFTMAX : 0;
+}
+
+// Landing and rotation of many rows find their integers in float, and leave to the integer forms what is too close to a tie to know.
+//   landing:  v = x rho, rho = m r_t / 2^k. Five roundings (of x, m, r_t, and two products) move a v of at most 128 by 128 * 2^-24 each, 3.9e-5 in all.
+//   rotation: v = a c - b s, c and s in Q30 rounded to 24 bits (|c| <= 2: by 2^-24), |a|, |b| <= 127. Both terms together move by
+//             2 * 127 * 2^-24, b s rounds by 2^-17 and a result that is not held by 2^-18: 2.7e-5.
+// The distance to the nearest integer is exact (both are multiples of the float's last bit, and it is at most a half).
+constexpr float kLandTie = 0.49995f, kTurnTie = 0.49997f;
+// rf, ef: r_t and e_t, rf zero where they are out of range; mf: m
+__device__ __forceinline__ float land_factor(float mf, int e, float rf, int ef) {
+	const int k = 62 - (e - ef);
+	return k >= 33 && k <= 94 ? mf * rf * __int_as_float((127 - k) << 23) : 0.0f;
+}
+// four elements as whole floats from -127 to 127; returns how near to a tie the nearest is (1 where this form does not apply)
+__device__ __forceinline__ float land_floats(const int4& x, float rho, float (&code)[4], uint32_t& held) {
+	const int xs[4] = {x.x, x.y, x.z, x.w};
+	float far = rho > 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+	for (int j = 0; j < 4; ++j) {
+		const float v = fminf(fmaxf(__int2float_rn(xs[j]) * rho, -200.0f), 200.0f), q = (v + kRoundMagic) - kRoundMagic;
+		far = fmaxf(far, fabsf(v - q));
+		held += fabsf(q) > 127.0f ? 1u : 0u;
+		code[j] = fminf(fmaxf(q, -127.0f), 127.0f);
+	}
+	return far;
+}
+__device__ __forceinline__ uint32_t pack_floats(const float (&code)[4]) {
+	return pack4(__float_as_int(code[0] + kRoundMagic), __float_as_int(code[1] + kRoundMagic), __float_as_int(code[2] + kRoundMagic), __float_as_int(code[3] + kRoundMagic));
+}
+// the integer form, with the caller's tables
+static __device__ __noinline__ uint32_t turn_quad_exact(uint32_t c, uint32_t other, const int32_t* cos, const int32_t* sin, bool halves, bool low) {
+	if (!halves) return rope_quad(c, make_int2(cos[0], cos[1]), make_int2(sin[0], sin[1]));
+	int out[4];
+	for (int j = 0; j < 4; ++j) {
+		const int64_t mine = byte_of(c, j), theirs = byte_of(other, j);
+		out[j] = rope_round(low ? mine * cos[j] - theirs * sin[j] : theirs * sin[j] + mine * cos[j]);
+	}
+	return pack4(out[0], out[1], out[2], out[3]);
+}
+// what a lane's quads have in common
+struct TurnLane {
+	int half, angle, partner;      // words of a table row, the quad's first, the lane with the other half
+	bool turned, low;
+};
+__device__ __forceinline__ TurnLane turn_lane(const sslm_b200_qkv_site& a, int e) {
+	const int lane = threadIdx.x & 31, half = a.rotary >> 1, half_lanes = a.rotary >> 3;
+	const bool low = e < half, turned = e < a.rotary;
+	return TurnLane{half, a.halves ? (low ? e : e - half) : e >> 1, turned && a.halves ? (low ? lane + half_lanes : lane - half_lanes) : lane, turned, low};
+}
+// U rows' quads turned: the table rows as floats, cosines then sines, step apart
+template <int U>
+__device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const float (&code)[U][4], const TurnLane& l, const float* turn, int step, const int* pos, uint32_t (&c)[U]) {
+	float other[U][4] = {}, far = 0.0f;
+	if (a.halves) {
+#pragma unroll
+		for (int u = 0; u < U; ++u)
+#pragma unroll
+			for (int j = 0; j < 4; ++j) other[u][j] = __shfl_sync(0xffffffffu, code[u][j], l.partner);
+	}
+	if (!l.turned) {
+#pragma unroll
+		for (int u = 0; u < U; ++u) c[u] = pack_floats(code[u]);
+		return;
+	}
+#pragma unroll
+	for (int u = 0; u < U; ++u, turn += step) {
+		float v[4];
+		if (a.halves) {
+			const float4 co = *(const float4*)(turn + l.angle), si = *(const float4*)(turn + l.half + l.angle);
+			const float cs[4] = {co.x, co.y, co.z, co.w}, sn[4] = {si.x, si.y, si.z, si.w};
+#pragma unroll
+			for (int j = 0; j < 4; ++j) v[j] = fmaf(code[u][j], cs[j], l.low ? -(other[u][j] * sn[j]) : other[u][j] * sn[j]);
+		} else {
+			const float2 co = *(const float2*)(turn + l.angle), si = *(const float2*)(turn + l.half + l.angle);
+			v[0] = fmaf(code[u][0], co.x, -(code[u][1] * si.x));
+			v[1] = fmaf(code[u][0], si.x, code[u][1] * co.x);
+			v[2] = fmaf(code[u][2], co.y, -(code[u][3] * si.y));
+			v[3] = fmaf(code[u][2], si.y, code[u][3] * co.y);
+		}
+		int out[4];
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			v[j] = fminf(fmaxf(v[j], -127.0f), 127.0f);
+			const float m = v[j] + kRoundMagic;
+			far = fmaxf(far, fabsf(v[j] - (m - kRoundMagic)));
+			out[j] = __float_as_int(m);
+		}
+		c[u] = pack4(out[0], out[1], out[2], out[3]);
+	}
+	if (far > kTurnTie)
+#pragma unroll
+		for (int u = 0; u < U; ++u) {
+			if (pos[u] < 0) continue;      // (of a row that is not worked on the table's row may be missing)
+			const int64_t at = (int64_t)pos[u] * l.half + l.angle;
+			c[u] = turn_quad_exact(pack_floats(code[u]), pack_floats(other[u]), a.cos + at, a.sin + at, a.halves != 0, l.low);
+		}
+}
+
+// kRows rows a block. A warp has 32 quads (whole heads, as a rule) of q, of K or of V in all of them; the last warp has what the rows say of
+// themselves, the funnel's scalars and the softmax constants, a lane a row. From eight rows for every SM on, where it costs a third to a
+// half less than a block a row: 12 + 2 + 2 heads of 128, 8,191 rows: 44 us (a block a row: 64 with four quads a thread, 76 with two, 111 with one), 2,047
+// rows: 14.8 (17.9, 20.0, 26.8); below, its few blocks leave SMs idle: 1,000 rows 12.9 (11.3, 11.5, 15.7), 300 rows 9.4 (7.5, 7.3, 8.4).
+// The floor of 8,191 rows is 13.6 us of memory traffic; what bounds it are instructions, about 150 for a quad of 32 lanes and row (a scheduler
+// issues one in 53 % of its cycles, and 25 us would remain if it always did), and a block's chain of three waits (positions, tables, maxima)
+// that one other block of the SM covers. Measured and left: 4 rows a block (56 us), 16 (one block a SM: 102), three blocks a SM with 32
+// registers (55), one or four rows side by side (46.6, 65), the rotation in integers (58).
+constexpr int kRows = 8, kMostColumns = 31;
+struct SiteShared {
+	uint32_t top[32 * kRows], held[kRows], live;
+	int pos[kRows], page[kRows], slot[kRows], in_m[kRows], in_e[kRows];      // (of a row that is worked on; -1)
+	float4 funnel[kRows];      // f, f_lo and d (as bits)
+};
+template <bool NORMS, int MOST, int MIN>
+__global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_constant__ SiteArgs g) {
+	extern __shared__ __align__(16) int32_t s_x[];      // a thread's quads: kRows, x_step apart; then the tables' rows
+	__shared__ SiteShared s;
+	const sslm_b200_qkv_site& a = g.c;
+	const int t = threadIdx.x, lane = t & 31, warp = t >> 5, hd = a.head_dim, own = lane % kRows;      // (own: the lane's row)
+	const int64_t r0 = (int64_t)blockIdx.x * kRows;
+	const int rows = (int)min((int64_t)kRows, a.rows - r0), half = a.rotary >> 1;
+	const bool is_q = warp < g.q_warps, is_k = !is_q && warp < g.q_warps + g.k_warps, last = warp == g.q_warps + 2 * g.k_warps, is_v = !is_q && !is_k && !last;
+	constexpr int U = 2;      // rows side by side: their instructions fill each other's waits, and they share the tests for ties
+	const bool funnel = g.nq > 0 && a.q_gain == nullptr;
+	const int x_step = 128 * (g.q_warps + 2 * g.k_warps), turn_step = 2 * half;
+	int32_t *x_at = s_x + 4 * t, *s_turn = s_x + kRows * x_step;
+	pdl_wait();
+	pdl_release();
+	if (last) {
+		const SiteRow w = site_row(a, r0 + min(own, rows - 1), g.nk > 0);
+		const bool lives = own < rows && w.pos != -1 && w.code == 0;
+		const uint32_t live = __ballot_sync(0xffffffffu, lives) & ((1u << kRows) - 1u);
+		const Scale in{lives ? w.in_m : 1 << 30, lives ? w.in_e : 0}, site{a.q_site_m, a.q_site_e};
+		if (lane < kRows) {
+			s.held[lane] = 0;
+			s.pos[lane] = lives ? w.pos : -1;
+			s.page[lane] = lives ? w.page : -1;
+			s.slot[lane] = w.place % kPageTokens;
+			s.in_m[lane] = (int)in.m;
+			s.in_e[lane] = (int)in.e;
+			if (lane == 0) s.live = live;
+		}
+		FunnelFold fold{};
+		if (funnel) fold = funnel_prefold(&in, 1, site);
+		__syncthreads();
+		Scale out = site;
+		if (funnel) {
+			uint32_t top = 0;
+			for (int k = lane; k < g.q_warps * kRows; k += 32) top = max(top, s.top[k]);
+#pragma unroll
+			for (int o = kRows; o < 32; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+			const QuadFunnel fp = quad_funnel(top, fold);      // (canonical scales: never refused)
+			if (lane < kRows) s.funnel[lane] = make_float4(fp.f, fp.f_lo, __uint_as_float(fp.d), 0.0f);
+			out = fp.out;
+			asm volatile("bar.sync 1, %0;" ::"r"(32 * (g.q_warps + 1)) : "memory");
+		}
+		bool bad = false;
+		const int64_t row = r0 + own;
+		if (g.nq > 0 && lives) {
+			if (lane < kRows && a.q_scales != nullptr) {
+				a.q_scales[2 * row] = out.m;
+				a.q_scales[2 * row + 1] = out.e;
+			}
+			if (a.consts != nullptr) bad = site_consts(a.khead, a.consts, a.kv_heads, row, out, lane / kRows, 32 / kRows);
+		}
+		uint32_t none = __ballot_sync(0xffffffffu, bad);
+#pragma unroll
+		for (int o = 16; o >= kRows; o >>= 1) none |= none >> o;
+		if (lane < rows && a.row_status != nullptr) a.row_status[row] = w.code != 0 ? w.code : (((none >> lane) & 1) ? SSLM_B200_ROW_SOFTMAX : 0);
+		return;
+	}
+	const int i = 32 * (is_q ? warp : (is_k ? warp - g.q_warps : warp - g.q_warps - g.k_warps)) + lane;
+	const bool in = i < (is_q ? g.nq : g.nk);
+	{
+		const int64_t stride = is_q ? a.q_stride : (is_k ? a.k_stride : a.v_stride);
+		const int32_t* from = (is_q ? a.q : (is_k ? a.k : a.v)) + r0 * stride + 4 * i;
+		const uint32_t to = (uint32_t)__cvta_generic_to_shared(x_at);
+		const int pos = a.positions[r0 + min(own, rows - 1)];
+		if (in && rows == kRows) {
+#pragma unroll
+			for (int r = 0; r < kRows; ++r, from += stride) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * r * x_step), "l"(from) : "memory");
+		} else {
+			for (int r = 0; r < kRows; ++r, from += stride) {
+				if (in && r < rows) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * r * x_step), "l"(from) : "memory");
+				else *(int4*)(x_at + r * x_step) = make_int4(0, 0, 0, 0);
+			}
+		}
+		// the rows of the tables, 16 bytes a thread; each makes what it copied to floats
+		const bool known = pos >= 0 && pos < a.num_positions;
+		const int32_t* angles = (const int32_t*)a.cos + (int64_t)pos * half;
+		const int64_t sines = a.sin - a.cos;
+		if (known)
+			for (int k = 4 * (t / kRows); k < turn_step; k += x_step / (4 * kRows) * 4)
+				asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(s_turn + own * turn_step + k)), "l"(k < half ? angles + k : angles + sines + (k - half)) : "memory");
+		asm volatile("cp.async.wait_all;" ::: "memory");
+		if (known)
+			for (int k = 4 * (t / kRows); k < turn_step; k += x_step / (4 * kRows) * 4) {
+				int4* at = (int4*)(s_turn + own * turn_step + k);
+				const int4 v = *at;
+				constexpr float q30 = 1.0f / (1 << 30);
+				*(float4*)at = make_float4(q30 * __int2float_rn(v.x), q30 * __int2float_rn(v.y), q30 * __int2float_rn(v.z), q30 * __int2float_rn(v.w));
+			}
+	}
+	if (funnel && is_q) {
+		uint32_t mine = 0;
+#pragma unroll
+		for (int r = 0; r < kRows; ++r) {
+			const int4 x = *(const int4*)(x_at + r * x_step);
+			const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(abs_u32(x.x), abs_u32(x.y)), max(abs_u32(x.z), abs_u32(x.w))));
+			mine = lane == r ? top : mine;
+		}
+		if (lane < kRows) s.top[warp * kRows + lane] = mine;
+	}
+	__syncthreads();
+	const uint32_t live = s.live;
+	if (funnel && is_q) asm volatile("bar.sync 1, %0;" ::"r"(32 * (g.q_warps + 1)) : "memory");
+	const int e = (4 * i) & (hd - 1);
+	const float* turns = (const float*)s_turn;
+	if (is_q) {
+		const TurnLane l = turn_lane(a, e);
+		int8_t* to = a.q_codes + r0 * a.q_codes_stride + 4 * i;
+		for (int r = 0; r < kRows; r += U) {
+			int32_t x[U][4];
+			float code[U][4];
+#pragma unroll
+			for (int u = 0; u < U; ++u) {
+				const int4 xv = *(const int4*)(x_at + (r + u) * x_step);
+				x[u][0] = xv.x; x[u][1] = xv.y; x[u][2] = xv.z; x[u][3] = xv.w;
+			}
+			if (NORMS && a.q_gain != nullptr) {
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					int lc[4];
+					uint32_t over = 0;
+					norm_quad(x[u], a.q_gain + e, a.q_shift, g.lanes, lc, over);
+#pragma unroll
+					for (int j = 0; j < 4; ++j) code[u][j] = __int2float_rn(lc[j]);
+				}
+			} else {
+				QuadFunnel f[U];
+				int near[U][4];
+				float far = 0.0f;
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					const float4 row = s.funnel[r + u];
+					f[u].f = row.x;
+					f[u].f_lo = row.y;
+					f[u].d = __float_as_uint(row.z);
+					far = fmaxf(far, code_quad_try(x[u], f[u], near[u]));
+				}
+				if (far > kNearTie)
+#pragma unroll
+					for (int u = 0; u < U; ++u) code_quad_settle(x[u], f[u], near[u]);
+#pragma unroll
+				for (int u = 0; u < U; ++u)
+#pragma unroll
+					for (int j = 0; j < 4; ++j) code[u][j] = __int_as_float(near[u][j]) - kRoundMagic;
+			}
+			uint32_t c[U];
+			turn_floats(a, code, l, turns + r * turn_step, turn_step, s.pos + r, c);
+#pragma unroll
+			for (int u = 0; u < U; ++u, to += a.q_codes_stride)
+				if (in && ((live >> (r + u)) & 1)) *(uint32_t*)to = c[u];
+		}
+		return;
+	}
+	{
+		const int head = 4 * min(i, g.nk - 1) / hd;
+		const int64_t* rec = (is_k ? a.k_landing : a.v_landing) + 3 * head;
+		const bool normed = NORMS && is_k && a.k_gain != nullptr;
+		float rf = 0.0f;
+		int ef = 0;
+		if (!normed) {
+			const int64_t e_t = rec[1], r_t = rec[2];
+			if (r_t > 0 && r_t <= ((int64_t)1 << 32) && e_t > -(1 << 24) && e_t < (1 << 24)) {
+				rf = __ll2float_rn(r_t);
+				ef = (int)e_t;
+			}
+		}
+		int8_t* plane = a.kv + (2 * (int64_t)head + (is_v ? 1 : 0)) * a.num_pages * (kPageTokens * hd);
+		const TurnLane l = turn_lane(a, e);
+		for (int r = 0; r < kRows; r += U) {
+			int4 x[U];
+			float code[U][4];
+			uint32_t held[U], c[U];
+#pragma unroll
+			for (int u = 0; u < U; ++u) {
+				x[u] = *(const int4*)(x_at + (r + u) * x_step);
+				held[u] = 0;
+			}
+			if (normed) {
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					const int32_t xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+					int lc[4];
+					norm_quad(xs, a.k_gain + e, a.k_shift, g.lanes, lc, held[u]);
+#pragma unroll
+					for (int j = 0; j < 4; ++j) code[u][j] = __int2float_rn(lc[j]);
+				}
+			} else {
+				float far = 0.0f;
+				int in_m[U], in_e[U];
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					in_m[u] = s.in_m[r + u];
+					in_e[u] = s.in_e[r + u];
+					const float at = land_floats(x[u], land_factor(__int2float_rn(in_m[u]), in_e[u], rf, ef), code[u], held[u]);
+					if ((live >> (r + u)) & 1) far = fmaxf(far, at);
+				}
+				if (far > kLandTie)
+#pragma unroll
+					for (int u = 0; u < U; ++u) {
+						const uint64_t v = land_quad_exact(x[u].x, x[u].y, x[u].z, x[u].w, in_m[u], rec[2], in_e[u], rec[1]);
+						held[u] = (uint32_t)(v >> 32);
+#pragma unroll
+						for (int j = 0; j < 4; ++j) code[u][j] = (float)byte_of((uint32_t)v, j);
+					}
+			}
+			if (is_k) {
+				turn_floats(a, code, l, turns + r * turn_step, turn_step, s.pos + r, c);
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					const int64_t token = (int64_t)s.page[r + u] * kPageTokens + s.slot[r + u];
+					if (in && ((live >> (r + u)) & 1)) *(uint32_t*)(plane + token * hd + e) = c[u];
+				}
+			} else {
+#pragma unroll
+				for (int u = 0; u < U; ++u) x_at[(r + u) * x_step] = (int32_t)pack_floats(code[u]);
+			}
+			uint32_t any = 0;
+#pragma unroll
+			for (int u = 0; u < U; ++u) any |= held[u];
+			if (a.saturations != nullptr && __any_sync(0xffffffffu, in && any != 0))
+#pragma unroll
+				for (int u = 0; u < U; ++u) {
+					held[u] = __reduce_add_sync(0xffffffffu, in ? held[u] : 0u);
+					if (lane == 0) atomicAdd(&s.held[r + u], held[u]);
+				}
+		}
+		// V has the tokens of a page side by side: four rows on neighbouring places are one word
+		if (is_v)
+			for (int q = 0; q < kRows; q += 4) {
+				const int pg = s.page[q], at = s.slot[q];
+				const bool near = own < q || own >= q + 4 || (pg >= 0 && s.page[own] == pg && s.slot[own] == at + own - q);
+				const uint32_t c0 = (uint32_t)x_at[q * x_step], c1 = (uint32_t)x_at[(q + 1) * x_step], c2 = (uint32_t)x_at[(q + 2) * x_step], c3 = (uint32_t)x_at[(q + 3) * x_step];
+				if (__all_sync(0xffffffffu, near) && (at & 3) == 0) {
+					const uint32_t a0 = __byte_perm(c0, c1, 0x5140), a1 = __byte_perm(c2, c3, 0x5140);
+					const uint32_t b0 = __byte_perm(c0, c1, 0x7362), b1 = __byte_perm(c2, c3, 0x7362);
+					uint32_t* to = (uint32_t*)(plane + ((int64_t)pg * hd + e) * kPageTokens + at);
+					if (in) {
+						to[0] = __byte_perm(a0, a1, 0x5410);
+						to[kPageTokens / 4] = __byte_perm(a0, a1, 0x7632);
+						to[2 * kPageTokens / 4] = __byte_perm(b0, b1, 0x5410);
+						to[3 * kPageTokens / 4] = __byte_perm(b0, b1, 0x7632);
+					}
+					continue;
+				}
+				for (int r = q; r < q + 4; ++r) {
+					int8_t* to = plane + ((int64_t)s.page[r] * hd + e) * kPageTokens + s.slot[r];
+					const uint32_t c = (uint32_t)x_at[r * x_step];
+					if (in && ((live >> r) & 1))
+#pragma unroll
+						for (int j = 0; j < 4; ++j) to[j * kPageTokens] = (int8_t)byte_of(c, j);
+				}
+			}
+	}
+	if (a.saturations != nullptr) {
+		asm volatile("bar.sync 2, %0;" ::"r"(64 * g.k_warps) : "memory");      // (the warps of K and V)
+		if (is_k && i < kRows && ((live >> i) & 1)) a.saturations[r0 + i] = (int32_t)s.held[i];
+	}
 }
 
 template <int NV>
 cudaError_t site_launch(const SiteArgs& g, cudaStream_t st) {
 	const int threads = ((g.total + NV - 1) / NV + 31) & ~31;
 	return launch_pdl(k_qkv_site<NV>, dim3(g.c.rows), dim3(threads), 0, st, g);
+}
+
+template <bool NORMS, int MOST, int MIN>
+cudaError_t site_launch_rows(const SiteArgs& g, cudaStream_t st) {
+	static PerDeviceOnce once;
+	const cudaError_t e = once_per_device(once, [] { return cudaFuncSetAttribute(k_qkv_site_rows<NORMS, MOST, MIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRows * (MOST * 16 + 512)); });
+	if (e != cudaSuccess) return e;
+	const int threads = 32 * (g.q_warps + 2 * g.k_warps + 1);
+	return launch_pdl(k_qkv_site_rows<NORMS, MOST, MIN>, dim3((g.c.rows + kRows - 1) / kRows), dim3(threads), kRows * ((threads - 32) * 16 + g.c.rotary * 4), st, g);
 }
 
 }  // namespace
@@ -271,8 +684,17 @@ extern "C" sslm_status sslm_b200_qkv_site_resident(const sslm_b200_qkv_site* cal
 	g.nq = turns ? c.heads * g.lanes : 0;
 	g.nk = lands ? c.kv_heads * g.lanes : 0;
 	g.total = g.nq + 2 * g.nk;
+	g.q_warps = (g.nq + 31) / 32;
+	g.k_warps = (g.nk + 31) / 32;
 	const cudaStream_t st = (cudaStream_t)stream;
-	const cudaError_t e = g.total > 4096 ? site_launch<16>(g, st) : (g.total > 1024 || c.rows >= 512 ? site_launch<4>(g, st) : site_launch<1>(g, st));
+	const int columns = g.q_warps + 2 * g.k_warps;
+	const bool norms = c.q_gain != nullptr || c.k_gain != nullptr;
+	cudaError_t e;
+	if (c.rows >= kRows * sm_count() && columns <= kMostColumns) {
+		if (columns <= 16) e = norms ? site_launch_rows<true, 32 * 17, 2>(g, st) : site_launch_rows<false, 32 * 17, 2>(g, st);
+		else e = norms ? site_launch_rows<true, 1024, 1>(g, st) : site_launch_rows<false, 1024, 1>(g, st);
+	} else if (g.total <= 1024) e = c.rows <= sm_count() ? site_launch<1>(g, st) : site_launch<2>(g, st);
+	else e = g.total <= 2048 ? site_launch<4>(g, st) : site_launch<16>(g, st);
 	if (e != cudaSuccess) {
 		cudaGetLastError();
 		return SSLM_ALLOCATION_FAILED;

@@ -89,7 +89,7 @@ def test_part_of_a_head(gpu_lib, torch, rotary, halves):
 
 @pytest.mark.parametrize("rows", [1, 2, 511, 513])
 def test_rows_of_a_few_sequences(gpu_lib, torch, rows):
-    """more than 511 rows take the kernel of four quads a thread"""
+    """up to a row for every SM, and more"""
     c = Call(gpu_lib, torch, site_case(3, (2, 1, 32), rows, positions=400, tables=min(rows, 3), norm="k"))
     c.check(only=None if rows < 600 else range(0, rows, 17))
 
@@ -98,6 +98,132 @@ def test_rows_of_a_few_sequences(gpu_lib, torch, rows):
 def test_wide_rows(gpu_lib, torch, shape):
     """up to 32,768 elements: four and sixteen quads a thread"""
     Call(gpu_lib, torch, site_case(4, shape, 2, norm="k")).check()
+
+
+@pytest.mark.parametrize("quads", [1024, 1056, 2048, 2080, 4096, 4128, 8192])
+def test_where_the_threads_of_a_row_change(gpu_lib, torch, quads):
+    Call(gpu_lib, torch, site_case(15, (quads // 32 - 2, 1, 128), 1)).check()
+
+
+def by_hundreds(gpu_lib, torch, case):
+    """the same rows in calls of 100, a block a row"""
+    whole, parts = Call(gpu_lib, torch, case), []
+    whole.call.run()
+    kv = torch.from_numpy(case["kv"]).cuda()
+    for r in range(0, len(case["wide"]), 100):
+        cut = dict(case, **{k: case[k][r:r + 100] for k in ("wide", "in_scales", "positions", "places", "table_of")})
+        parts.append(Call(gpu_lib, torch, cut, kv=kv))
+        parts[-1].call.run()
+    torch.cuda.synchronize()
+    for name in ("q_codes", "q_scales", "consts", "saturations", "status"):
+        assert torch.equal(getattr(whole, name), torch.cat([getattr(c, name) for c in parts])), name
+    assert torch.equal(whole.d["kv"], kv)
+    return whole
+
+
+def many_rows(torch, seed, shape, more=5, first=3, **kind):
+    """eight rows for every SM and a few more; three sequences' places run on from `first`, the other rows' are drawn"""
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count + more
+    case = site_case(seed, shape, rows, positions=512, tables=6, **kind)
+    g = np.random.default_rng(seed)
+    places = np.zeros(rows, dtype=np.int64)
+    at = 0
+    for s, n in enumerate((300, 211, rows - 511 - 400)):
+        case["table_of"][at:at + n], places[at:at + n], at = s, np.arange(first, first + n), at + n
+    case["table_of"][at:] = 3 + np.arange(400) % 3
+    for s in range(3, 6):
+        mine = np.flatnonzero(case["table_of"] == s)
+        places[mine] = g.choice(512, len(mine), replace=False)
+    assert places.max() < 512
+    case["places"] = places.astype(np.int32)
+    return case
+
+
+@pytest.mark.parametrize("shape,norm,halves,part", [((14, 2, 64), "", False, 1), ((12, 2, 128), "", False, 1), ((12, 2, 128), "q", True, 2), ((4, 2, 32), "k", True, 1), ((5, 1, 32), "", True, 4),
+                                                    ((1, 1, 128), "qk", False, 1), ((16, 2, 128), "", True, 1), ((16, 4, 128), "qk", False, 2), ((3, 3, 64), "", False, 1), ((27, 2, 128), "", False, 1)])
+def test_many_rows(gpu_lib, torch, shape, norm, halves, part):
+    case = many_rows(torch, 16, shape, rotary=shape[2] // part, halves=halves, norm=norm)
+    c = by_hundreds(gpu_lib, torch, case)
+    c.compare(only=[0, 1, 2, 3, 4, 298, 299, 300, 301, 510, 511, 800, len(case["wide"]) - 1])
+
+
+@pytest.mark.parametrize("first,more", [(0, 0), (4, 1), (7, 8), (16, 13)])
+def test_many_rows_that_begin_anywhere(gpu_lib, torch, first, more):
+    by_hundreds(gpu_lib, torch, many_rows(torch, 17, (2, 1, 64), more=more, first=first))
+
+
+@pytest.mark.parametrize("parts", ["q", "k"])
+@pytest.mark.parametrize("norm", ["", "qk"])
+def test_parts_of_many_rows(gpu_lib, torch, parts, norm):
+    case = many_rows(torch, 18, (6, 2, 64), norm=norm)
+    c = Call(gpu_lib, torch, case, parts)
+    c.check(only=[0, 5, 9, 299, 300, 700, len(case["wide"]) - 1])
+    c = Call(gpu_lib, torch, dict(case, cos=np.zeros((512, 0), dtype=np.int32), sin=np.zeros((512, 0), dtype=np.int32)), parts)      # (nothing is turned)
+    c.check(only=[0, 5, 9, 299, 300, 700, len(case["wide"]) - 1])
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_many_rows_of_ties(gpu_lib, torch, halves):
+    """angles of whole eighths and landings by powers of two: a half is common, and a result out of range"""
+    case = many_rows(torch, 19, (4, 2, 64), halves=halves, deviation=3000.0)
+    g = np.random.default_rng(19)
+    rows = len(case["wide"])
+    case["cos"], case["sin"] = ((g.integers(-12, 13, case["cos"].shape) << 27).astype(np.int32) for _ in range(2))
+    case["cos"][0], case["sin"][0] = -(1 << 31), (1 << 31) - 1
+    case["positions"][::50] = 0
+    case["in_scales"][:, 0] = 1 << 30
+    for name in ("k_landing", "v_landing"):
+        case[name][:] = 1 << 30, -50 + 6, 1 << 32
+    case["in_scales"][:, 1] = -50 + g.integers(-2, 3, rows)
+    c = by_hundreds(gpu_lib, torch, case)
+    c.compare(only=[0, 1, 50, 77, 299, 300, 600, rows - 1])
+
+
+def test_many_rows_with_values_at_the_ends(gpu_lib, torch):
+    case = many_rows(torch, 20, (2, 1, 32))
+    w = case["wide"]
+    w[0], w[1], w[2], w[3], w[3, 5] = 0, -(1 << 31), (1 << 31) - 1, 0, 1
+    w[4] = np.where(np.arange(128) % 2, 1 << 24, -(1 << 24) - 1)
+    w[5], w[6] = 1 << 30, np.arange(128) - 64
+    w[60:90] = np.random.default_rng(20).integers(-(1 << 31), 1 << 31, (30, 128))
+    for r, (m, e) in {7: (1 << 30, 20), 8: ((1 << 31) - 1, -100), 9: (1 << 30, 60), 10: (1 << 30, 4096), 11: ((1 << 31) - 1, -4096), 61: (1 << 30, -60), 62: (1 << 30, -70)}.items():
+        case["in_scales"][r] = m, e
+    c = by_hundreds(gpu_lib, torch, case)
+    c.compare(only=list(range(0, 13)) + list(range(58, 92)))
+    case["k_landing"][0, 1], case["v_landing"][0, 1] = 1 << 40, -(1 << 62)
+    c = by_hundreds(gpu_lib, torch, case)
+    c.case = dict(case, k_landing=case["k_landing"].copy(), v_landing=case["v_landing"].copy())
+    c.case["k_landing"][0, 1], c.case["v_landing"][0, 1] = 20000, -20000      # as far out of range, and a number that the definition can shift by
+    c.compare(only=[0, 1, 4, 9, 70])
+    case["k_landing"][0, 2], case["v_landing"][0, 2] = 0, (1 << 40) + 1
+    by_hundreds(gpu_lib, torch, case)
+
+
+def test_many_rows_some_refused_and_left_out(gpu_lib, torch):
+    case = many_rows(torch, 21, (4, 2, 64))
+    n = len(case["wide"])
+    case["positions"][1] = -1
+    case["positions"][2] = -2
+    case["positions"][3] = 512
+    case["places"][4] = 512
+    case["places"][5] = -1
+    case["table_of"][6] = 6
+    case["table_of"][7] = -1
+    case["pages"][3, case["places"][np.flatnonzero(case["table_of"] == 3)[-1]] // PAGE] = -1
+    case["in_scales"][10, 0] = (1 << 30) - 1
+    case["in_scales"][11, 0] = 1 << 31
+    case["in_scales"][12, 1] = 4097
+    case["positions"][16:24] = -1                             # a tile of padding
+    case["positions"][n - 1] = -1
+    c = by_hundreds(gpu_lib, torch, case)
+    status = c.status.cpu().numpy()
+    assert list(status[:13]) == [0, 0, 7, 7, 7, 7, 101, 101, 0, 0, 20, 20, 20] and (status[16:24] == 0).all() and status[n - 1] == 0
+    assert 101 in status[511:] and (c.q_codes[16:24] == 55).all() and (c.saturations[1:8] == 55).all()
+    c.compare(only=[0, 8, 9, 13, 15, 24])
+    c = Call(gpu_lib, torch, dict(case, positions=np.full(n, 512, dtype=np.int32)))
+    c.call.run()
+    torch.cuda.synchronize()
+    assert (c.status == 7).all() and (c.q_codes == 55).all()
 
 
 @pytest.mark.parametrize("parts", ["q", "k"])
