@@ -421,7 +421,7 @@ class _ResidentCall:
             with torch.cuda.device(self._device):
                 return self.run(stream)
         if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
+            stream = torch._C._cuda_getCurrentRawStream(self._device.index)      # (torch.cuda.current_stream() makes an object: 3.2 us)
         st = self._fn(C.addressof(self.args), stream)
         if st != SSLM_OK:
             raise SslmError(self.verb, st)
