@@ -631,8 +631,8 @@ __global__ void __launch_bounds__(T, BLOCKS) k_sample(const __grid_constant__ Sa
 	const uint32_t reach = least == INT32_MIN ? 0xFFFFFFFFu : (uint32_t)top - (uint32_t)max(least, INT32_MIN + 1), far = min(reach, most);      // the list's farthest
 	bool complete = reach >= most;      // the list has every token that has a weight
 	bool have_list = false;
-	if (early) {
-		have_list = s_n >= (uint32_t)w.top_k && s_n <= (uint32_t)kList;
+	if (early) {      // (of no use where some of its tokens have no weight: they do not count)
+		have_list = s_n >= (uint32_t)w.top_k && s_n <= (uint32_t)kList && (uint32_t)top - (uint32_t)early_least <= most;
 		__syncthreads();      // (all have seen how long it is)
 		if (have_list) complete = false;
 		else if (t == 0) s_n = 0u;

@@ -140,6 +140,17 @@ def test_slopes(gpu_lib, torch, slope, cut):
     Call(gpu_lib, torch, case).check()
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 151936), (70, 33001), (150, 40000)])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 0.03, 30.0, 1e5])
+@pytest.mark.parametrize("limits", [dict(top_k=50, top_p=0.95), dict(top_k=400), dict(top_k=900, min_p=0.01), dict(top_p=0.9), dict()])
+def test_steep_and_flat(gpu_lib, torch, rows, vocab, temperature, limits):
+    """fewer tokens have a weight than top-k asks for, or all have nearly the same"""
+    case = make(21, rows, vocab, **limits)
+    case["params"][:] = [abi.sample_params(1 / NAT, temperature, **limits) for _ in range(rows)]
+    case["logits"][1] = np.arange(vocab) % 7 * 1000
+    Call(gpu_lib, torch, case).check()
+
+
 def test_draws_and_limits_at_their_ends(gpu_lib, torch):
     case = make(8, 8, 4099)
     case["draws"][:4] = 0, (1 << 31) - 1, 1, 1 << 30
