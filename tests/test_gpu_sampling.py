@@ -289,3 +289,24 @@ def test_many_rows(gpu_lib, rows):
             assert st == 0 and toks[0::2] == toks[1::2]
     finally:
         eng.close()
+
+
+def test_many_rows_of_a_large_vocabulary(gpu_lib):
+    """cut over one block each; few tokens of theirs have a weight"""
+    rows = 72
+    eng = engine(gpu_lib, n=rows, vocab=33001)
+    try:
+        seqs = []
+        for i in range(rows):
+            s = eng.new_seq()
+            s.prefill(A.stream_uniform(i // 3, "prompt", 4 + i // 3 % 20, 0, 100), 64)
+            if i % 3 == 1:
+                s.set_sampling(top_k=1, seed=i)
+            elif i % 3 == 2:
+                s.set_sampling(temperature=1 / 65536, top_k=40, seed=i)      # (the second largest logit weighs nothing)
+            seqs.append(s)
+        for _ in range(3):
+            st, toks = eng.decode_step(seqs, eng.num_layers)
+            assert st == 0 and toks[0::3] == toks[1::3] == toks[2::3]
+    finally:
+        eng.close()
