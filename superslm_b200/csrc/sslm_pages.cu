@@ -23,7 +23,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostSequences = 65535, kMostTable = 65536;
 constexpr int kMostRange = 4096;      // sequences of a block: kMostSequences over 16 blocks
-constexpr uint32_t kCopies = 0x80000000u;
+constexpr uint32_t kCopies = 0x80000000u, kRefused = 0xFFFFFFFFu;
 
 // sums that every block has of every block
 struct Told { uint32_t v[16][2]; };
@@ -77,16 +77,26 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 	pdl_release();
 	cluster_wait();
 	const Range seqs = range_of(n, blocks, rank), pages = range_of(a.num_pages, blocks, rank);
+	const int first_held = pages.from + t < pages.to ? a.holders[pages.from + t] : 0;      // (asked for early; most ranges are a page a thread,
+	auto held = [&](int64_t p) { return p == pages.from + t ? first_held : a.holders[p]; };
+	// and a sequence a warp, whose record stays in registers)
+	struct Seq { int parent, own, before, grow; } first{-1, 0, 0, 0};
+	auto seq_of = [&](int64_t i) {
+		Seq q{a.parents[i], a.lengths[i], 0, a.grow != nullptr ? a.grow[i] : 0};
+		if (q.parent >= 0 && q.parent < n) q.before = q.parent == (int)i ? q.own : a.lengths[q.parent];
+		return q;
+	};
 	const int room = a.table_pages * kPageTokens;
 	auto used_of = [&](int length) { return length >= 0 && length <= room ? (length + kPageTokens - 1) / kPageTokens : 0; };
 	// ---- what each sequence wants: a warp a sequence
 	for (int64_t i = seqs.from + warp; i < seqs.to; i += kWarps) {
-		const int parent = a.parents[i];
+		const Seq q = seq_of(i);
+		if (i == seqs.from + warp) first = q;
+		const int parent = q.parent, before = q.before, grow = q.grow;
 		int code = 0;
 		uint32_t want = 0;
 		if (parent < -1 || parent >= n) code = SSLM_B200_ROW_INDEX;
 		else if (parent >= 0) {
-			const int before = a.lengths[parent], grow = a.grow != nullptr ? a.grow[i] : 0;
 			if (before < 0 || grow < 0 || before > room || grow > room - before) code = SSLM_B200_ROW_LENGTH;
 			else {
 				const bool moved = parent != (int)i;
@@ -103,13 +113,13 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 		}
 		if (lane == 0) {
 			a.status[i] = code;
-			s_want[i - seqs.from] = code == 0 ? want : 0u;
+			s_want[i - seqs.from] = code == 0 ? want : kRefused;
 		}
 	}
 	// ---- free pages of this block's range
 	uint32_t unheld = 0;
 	for (int64_t p = pages.from + t; p < pages.to; p += kThreads) {
-		const int h = a.holders[p];
+		const int h = held(p);
 		a.out_holders[p] = h;
 		unheld += h == 0 ? 1u : 0u;
 	}
@@ -117,8 +127,9 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 	const int mine = (int)(seqs.to - seqs.from);
 	uint32_t wanted = 0, copies = 0;
 	for (int i = t; i < mine; i += kThreads) {
-		wanted += s_want[i] & ~kCopies;
-		copies += s_want[i] >> 31;
+		const uint32_t want = s_want[i] == kRefused ? 0u : s_want[i];
+		wanted += want & ~kCopies;
+		copies += want >> 31;
 	}
 	wanted = block_total(wanted, s_part);
 	copies = block_total(copies, s_part);
@@ -139,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 	// ---- the pages that are drawn, in order
 	const uint32_t last = min(want_all, free_all);
 	for (int64_t p0 = pages.from; p0 < pages.to && free_before < last; p0 += kThreads) {
-		const bool is_free = p0 + t < pages.to && a.holders[p0 + t] == 0;
+		const bool is_free = p0 + t < pages.to && held(p0 + t) == 0;
 		uint32_t all;
 		const uint32_t at = free_before + block_before(is_free ? 1u : 0u, s_part, &all);
 		if (is_free && at < last) a.drawn[at] = (int32_t)(p0 + t);
@@ -150,7 +161,8 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 	uint32_t drawn = 0, moves = 0;
 	for (int i0 = 0; i0 < mine; i0 += kThreads) {
 		const int i = i0 + t;
-		const uint32_t want = i < mine ? s_want[i] : 0u;
+		const bool refused = i < mine && s_want[i] == kRefused;
+		const uint32_t want = i < mine && !refused ? s_want[i] : 0u;
 		uint32_t all_want, all_copies;
 		const uint32_t at = want_before + block_before(want & ~kCopies, s_part, &all_want), move = copies_before + block_before(want >> 31, s_part, &all_copies);
 		want_before += all_want;
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 		if (i < mine) {
 			const int64_t s = seqs.from + i;
 			const uint32_t count = want & ~kCopies;
-			const bool served = count == 0u || (at <= free_all && count <= free_all - at);
+			const bool served = refused || count == 0u || (at <= free_all && count <= free_all - at);
 			if (!served) a.status[s] = SSLM_B200_ROW_PAGES;
 			else {
 				drawn += count;
@@ -169,16 +181,17 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 					a.moves[2 * move + 1] = a.drawn[at];
 				}
 			}
-			s_want[i] = served ? at : kCopies;      // (no place is that far back: the pages are fewer)
+			s_want[i] = served && !refused ? at : kRefused;      // (no place is that far back: the pages are fewer)
 		}
 	}
 	__syncthreads();
 	for (int64_t i = seqs.from + warp; i < seqs.to; i += kWarps) {
 		const uint32_t at = s_want[i - seqs.from];
-		const int parent = a.parents[i], own_length = a.lengths[i];
+		const Seq q = i == seqs.from + warp ? first : seq_of(i);
+		const int parent = q.parent, own_length = q.own;
 		const int32_t* own = a.tables + i * a.tables_stride;
 		int32_t* out = a.out_tables + i * a.out_stride;
-		if (a.status[i] != 0 || at == kCopies) {      // as it was
+		if (at == kRefused) {      // as it was
 			for (int j = lane; j < used_of(own_length); j += 32) out[j] = own[j];
 			if (lane == 0) a.out_lengths[i] = own_length;
 			continue;
@@ -189,8 +202,8 @@ __global__ void __launch_bounds__(kThreads) k_fork(const __grid_constant__ sslm_
 				if (own[j] >= 0 && own[j] < a.num_pages) atomicSub(&a.out_holders[own[j]], 1);
 		int length = 0;
 		if (parent >= 0) {
-			const int before = a.lengths[parent], taken = moved ? before / kPageTokens : used_of(before);
-			length = before + (a.grow != nullptr ? a.grow[i] : 0);
+			const int before = q.before, taken = moved ? before / kPageTokens : used_of(before);
+			length = before + q.grow;
 			const int32_t* from = a.tables + parent * a.tables_stride;
 			for (int j = lane; j < used_of(length); j += 32) {
 				const int page = j < taken ? from[j] : a.drawn[at + (uint32_t)(j - taken)];
@@ -220,8 +233,13 @@ __global__ void __launch_bounds__(kThreads) k_compact(const __grid_constant__ ss
 	pdl_release();
 	cluster_wait();
 	const Range pages = range_of(a.num_pages, blocks, rank);
+	// (asked for early; most ranges are a page a thread, a sequence a warp, and a page of its table a lane)
+	const int first_held = pages.from + t < pages.to ? a.holders[pages.from + t] : 0;
+	auto held = [&](int64_t p) { return p == pages.from + t ? first_held : a.holders[p]; };
+	const int64_t first_seq = (int64_t)rank * kWarps + warp;
+	const int first_length = first_seq < n ? a.lengths[first_seq] : 0, first_page = first_seq < n && lane < a.table_pages ? a.tables[first_seq * a.tables_stride + lane] : -1;
 	uint32_t used = 0;
-	for (int64_t p = pages.from + t; p < pages.to; p += kThreads) used += a.holders[p] != 0 ? 1u : 0u;
+	for (int64_t p = pages.from + t; p < pages.to; p += kThreads) used += held(p) != 0 ? 1u : 0u;
 	used = block_total(used, s_part);
 	tell(s_told, blocks, used, 0u);
 	meet();
@@ -229,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) k_compact(const __grid_constant__ ss
 	for (int i = 0; i < blocks; ++i) live += s_told.v[i][0];
 	uint32_t holes = 0, late = 0;
 	for (int64_t p = pages.from + t; p < pages.to; p += kThreads) {
-		const int h = a.holders[p];
+		const int h = held(p);
 		holes += h == 0 && p < live ? 1u : 0u;
 		late += h != 0 && p >= live ? 1u : 0u;
 		if (h == 0) a.new_of[p] = -1;
@@ -251,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) k_compact(const __grid_constant__ ss
 	if (holes + late > 0)
 		for (int64_t p0 = pages.from; p0 < pages.to; p0 += kThreads) {
 			const int64_t p = p0 + t;
-			const bool is_used = p < pages.to && a.holders[p] != 0, hole = p < pages.to && p < live && !is_used, behind = is_used && p >= live;
+			const bool is_used = p < pages.to && held(p) != 0, hole = p < pages.to && p < live && !is_used, behind = is_used && p >= live;
 			uint32_t all;      // (both sums in one: a tile has 512 pages)
 			const uint32_t before = block_before((hole ? 1u : 0u) | (behind ? 1u << 16 : 0u), s_part, &all);
 			if (hole) a.moves[2 * (int64_t)(holes_before + (before & 0xFFFFu)) + 1] = (int32_t)p;
@@ -260,26 +278,39 @@ __global__ void __launch_bounds__(kThreads) k_compact(const __grid_constant__ ss
 			late_before += all >> 16;
 		}
 	meet();
+	int2 last{0, 0};      // (what the last one's page is held by is waited for behind the barrier)
+	int last_held = 0;
+	bool any = false;
 	for (int64_t k = (int64_t)rank * kThreads + t; k < moves; k += (int64_t)blocks * kThreads) {
-		const int2 m = *(const int2*)(a.moves + 2 * k);
-		a.new_of[m.x] = m.y;
-		a.out_holders[m.y] = a.holders[m.x];
+		if (any) a.out_holders[last.y] = last_held;
+		last = *(const int2*)(a.moves + 2 * k);
+		a.new_of[last.x] = last.y;
+		last_held = a.holders[last.x];
+		any = true;
 	}
 	if (rank == 0 && t == 0) {
 		a.counts[0] = (int32_t)moves;
 		a.counts[1] = (int32_t)live;
 	}
 	meet();
+	if (any) a.out_holders[last.y] = last_held;
 	const int room = a.table_pages * kPageTokens;
-	for (int64_t i = (int64_t)rank * kWarps + warp; i < n; i += (int64_t)blocks * kWarps) {
-		const int length = a.lengths[i], entries = length >= 0 && length <= room ? (length + kPageTokens - 1) / kPageTokens : 0;
+	for (int64_t i = first_seq; i < n; i += (int64_t)blocks * kWarps) {
+		const int length = i == first_seq ? first_length : a.lengths[i], entries = length >= 0 && length <= room ? (length + kPageTokens - 1) / kPageTokens : 0;
 		const int32_t* from = a.tables + i * a.tables_stride;
 		int32_t* out = a.out_tables + i * a.out_stride;
-		bool bad = false;
-		for (int j = lane; j < entries; j += 32) bad = bad || from[j] < 0 || from[j] >= a.num_pages || a.new_of[from[j]] < 0;
+		auto new_page = [&](int j) {
+			const int page = i == first_seq && j == lane ? first_page : from[j];
+			return page < 0 || page >= a.num_pages ? -1 : a.new_of[page];
+		};
+		const int page = lane < entries ? new_page(lane) : 0;
+		bool bad = page < 0;
+		for (int j = lane + 32; j < entries; j += 32) bad = bad || new_page(j) < 0;
 		bad = __any_sync(0xffffffffu, bad);
-		if (!bad)
-			for (int j = lane; j < entries; j += 32) out[j] = a.new_of[from[j]];
+		if (!bad) {
+			if (lane < entries) out[lane] = page;
+			for (int j = lane + 32; j < entries; j += 32) out[j] = new_page(j);
+		}
 		if (lane == 0 && a.status != nullptr) a.status[i] = length < 0 || length > room ? SSLM_B200_ROW_LENGTH : (bad ? SSLM_B200_ROW_INDEX : 0);
 	}
 }
