@@ -642,7 +642,7 @@ cudaError_t site_launch_rows(const SiteArgs& g, cudaStream_t st) {
 	const cudaError_t e = once_per_device(once, [] { return cudaFuncSetAttribute(k_qkv_site_rows<NORMS, MOST, MIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRows * (MOST * 16 + 512)); });
 	if (e != cudaSuccess) return e;
 	const int threads = 32 * (g.q_warps + 2 * g.k_warps + 1);
-	return launch_pdl(k_qkv_site_rows<NORMS, MOST, MIN>, dim3((g.c.rows + kRows - 1) / kRows), dim3(threads), kRows * ((threads - 32) * 16 + g.c.rotary * 4), st, g);
+	return launch_pdl(k_qkv_site_rows<NORMS, MOST, MIN>, dim3((g.c.rows - 1) / kRows + 1), dim3(threads), kRows * ((threads - 32) * 16 + g.c.rotary * 4), st, g);
 }
 
 }  // namespace

@@ -54,7 +54,7 @@ def parents_of(seed, n, share=0.6, ended=0.1):
     return p
 
 
-@pytest.mark.parametrize("sequences,longest", [(1, 0), (1, 16), (1, 17), (2, 40), (5, 15), (16, 100), (17, 300), (60, 33), (300, 500), (1000, 64)])
+@pytest.mark.parametrize("sequences,longest", [(1, 0), (1, 16), (1, 17), (2, 40), (5, 15), (16, 100), (17, 300), (60, 33), (300, 500), (1000, 64), (3, 1500)])
 @pytest.mark.parametrize("grow", [None, 1, 16, 50])
 def test_forks(gpu_lib, torch, sequences, longest, grow):
     case = cache_case(1, sequences, longest, grow=grow or 0, spare=sequences * (2 + (grow or 0) // 16) + 9)
@@ -199,7 +199,7 @@ class Compact:
         return want
 
 
-@pytest.mark.parametrize("sequences,longest,spare", [(1, 0, 0), (1, 1, 0), (1, 16, 1), (2, 40, 100), (7, 200, 3), (40, 300, 500), (300, 200, 4000), (30, 100, 40000)])
+@pytest.mark.parametrize("sequences,longest,spare", [(1, 0, 0), (1, 1, 0), (1, 16, 1), (2, 40, 100), (7, 200, 3), (40, 300, 500), (300, 200, 4000), (30, 100, 40000), (3, 1500, 50), (20, 700, 9000)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_compacts(gpu_lib, torch, sequences, longest, spare, in_place):
     Compact(gpu_lib, torch, cache_case(14, sequences, longest, spare=spare), in_place).check()
