@@ -166,9 +166,10 @@ __device__ __forceinline__ void norm_quad(const int32_t (&x)[4], const int16_t* 
 	}
 }
 
-// A block a row, NV quads a thread. One quad where there is a block for every SM at most, the shortest way through a row (32 rows, 16 + 2 + 2
-// heads of 128, from a cold cache: 8.2 us, two quads 10.2); two up to kRows rows for every SM, because a block does a row's scalars in every warp
-// (512 rows: 10.1, one quad 14.3, four 10.4; normed 13.5, 16.7, 16.3); more only for rows that need more threads than a block has.
+// A block a row, NV quads a thread. One quad where there is a block for every SM at most, the shortest way through a row (148 rows of 16 + 2 + 2
+// heads of 128 4.9 us, two quads 5.3; normed 5.5 and 6.6); two beyond, because a block does a row's scalars in every warp (300 rows 7.1, one quad
+// 11.0; normed 8.9, 12.7); more only for rows that need more threads than a block has. One row: 4.6 us with 12 + 2 + 2 heads, of which the host's
+// part of the call is most.
 template <int NV>
 __global__ void __launch_bounds__(NV == 1 ? 1024 : 512)
 k_qkv_site(const __grid_constant__ SiteArgs g) {
@@ -288,7 +289,7 @@ __device__ __forceinline__ float land_floats(const int4& x, float rho, float (&c
 __device__ __forceinline__ uint32_t pack_floats(const float (&code)[4]) {
 	return pack4(__float_as_int(code[0] + kRoundMagic), __float_as_int(code[1] + kRoundMagic), __float_as_int(code[2] + kRoundMagic), __float_as_int(code[3] + kRoundMagic));
 }
-// the integer form, with the caller's tables
+// the integer form
 static __device__ __noinline__ uint32_t turn_quad_exact(uint32_t c, uint32_t other, const int32_t* cos, const int32_t* sin, bool halves, bool low) {
 	if (!halves) return rope_quad(c, make_int2(cos[0], cos[1]), make_int2(sin[0], sin[1]));
 	int out[4];
@@ -308,9 +309,9 @@ __device__ __forceinline__ TurnLane turn_lane(const sslm_b200_qkv_site& a, int e
 	const bool low = e < half, turned = e < a.rotary;
 	return TurnLane{half, a.halves ? (low ? e : e - half) : e >> 1, turned && a.halves ? (low ? lane + half_lanes : lane - half_lanes) : lane, turned, low};
 }
-// U rows' quads turned: the table rows as floats, cosines then sines, step apart
+// U rows' quads turned: the tables' rows, cosines then sines, step apart
 template <int U>
-__device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const float (&code)[U][4], const TurnLane& l, const float* turn, int step, const int* pos, uint32_t (&c)[U]) {
+__device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const float (&code)[U][4], const TurnLane& l, const int32_t* turn, int step, uint32_t (&c)[U]) {
 	float other[U][4] = {}, far = 0.0f;
 	if (a.halves) {
 #pragma unroll
@@ -323,52 +324,54 @@ __device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const f
 		for (int u = 0; u < U; ++u) c[u] = pack_floats(code[u]);
 		return;
 	}
+	turn += l.angle;
 #pragma unroll
-	for (int u = 0; u < U; ++u, turn += step) {
-		float v[4];
+	for (int u = 0; u < U; ++u) {
+		float v[4];      // 30 bits behind the point
 		if (a.halves) {
-			const float4 co = *(const float4*)(turn + l.angle), si = *(const float4*)(turn + l.half + l.angle);
-			const float cs[4] = {co.x, co.y, co.z, co.w}, sn[4] = {si.x, si.y, si.z, si.w};
+			const int4 co = *(const int4*)(turn + u * step), si = *(const int4*)(turn + u * step + l.half);
+			const int cs[4] = {co.x, co.y, co.z, co.w}, sn[4] = {si.x, si.y, si.z, si.w};
 #pragma unroll
-			for (int j = 0; j < 4; ++j) v[j] = fmaf(code[u][j], cs[j], l.low ? -(other[u][j] * sn[j]) : other[u][j] * sn[j]);
+			for (int j = 0; j < 4; ++j) {
+				const float b = other[u][j] * __int2float_rn(sn[j]);
+				v[j] = fmaf(code[u][j], __int2float_rn(cs[j]), l.low ? -b : b);
+			}
 		} else {
-			const float2 co = *(const float2*)(turn + l.angle), si = *(const float2*)(turn + l.half + l.angle);
-			v[0] = fmaf(code[u][0], co.x, -(code[u][1] * si.x));
-			v[1] = fmaf(code[u][0], si.x, code[u][1] * co.x);
-			v[2] = fmaf(code[u][2], co.y, -(code[u][3] * si.y));
-			v[3] = fmaf(code[u][2], si.y, code[u][3] * co.y);
+			const int2 co = *(const int2*)(turn + u * step), si = *(const int2*)(turn + u * step + l.half);
+			const float c0 = __int2float_rn(co.x), c1 = __int2float_rn(co.y), s0 = __int2float_rn(si.x), s1 = __int2float_rn(si.y);
+			v[0] = fmaf(code[u][0], c0, -(code[u][1] * s0));
+			v[1] = fmaf(code[u][0], s0, code[u][1] * c0);
+			v[2] = fmaf(code[u][2], c1, -(code[u][3] * s1));
+			v[3] = fmaf(code[u][2], s1, code[u][3] * c1);
 		}
 		int out[4];
+		constexpr float top = 127.0f * (1 << 30), q30 = 1.0f / (1 << 30);
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			v[j] = fminf(fmaxf(v[j], -127.0f), 127.0f);
-			const float m = v[j] + kRoundMagic;
-			far = fmaxf(far, fabsf(v[j] - (m - kRoundMagic)));
+			v[j] = fminf(fmaxf(v[j], -top), top);
+			const float m = fmaf(v[j], q30, kRoundMagic);
+			far = fmaxf(far, fabsf(fmaf(v[j], q30, kRoundMagic - m)));
 			out[j] = __float_as_int(m);
 		}
 		c[u] = pack4(out[0], out[1], out[2], out[3]);
 	}
 	if (far > kTurnTie)
 #pragma unroll
-		for (int u = 0; u < U; ++u) {
-			if (pos[u] < 0) continue;      // (of a row that is not worked on the table's row may be missing)
-			const int64_t at = (int64_t)pos[u] * l.half + l.angle;
-			c[u] = turn_quad_exact(pack_floats(code[u]), pack_floats(other[u]), a.cos + at, a.sin + at, a.halves != 0, l.low);
-		}
+		for (int u = 0; u < U; ++u) c[u] = turn_quad_exact(pack_floats(code[u]), pack_floats(other[u]), turn + u * step, turn + u * step + l.half, a.halves != 0, l.low);
 }
 
-// kRows rows a block. A warp has 32 quads (whole heads, as a rule) of q, of K or of V in all of them; the last warp has what the rows say of
-// themselves, the funnel's scalars and the softmax constants, a lane a row. From eight rows for every SM on, where it costs a third to a
-// half less than a block a row: 12 + 2 + 2 heads of 128, 8,191 rows: 44 us (a block a row: 64 with four quads a thread, 76 with two, 111 with one), 2,047
-// rows: 14.8 (17.9, 20.0, 26.8); below, its few blocks leave SMs idle: 1,000 rows 12.9 (11.3, 11.5, 15.7), 300 rows 9.4 (7.5, 7.3, 8.4).
-// The floor of 8,191 rows is 13.6 us of memory traffic; what bounds it are instructions, about 150 for a quad of 32 lanes and row (a scheduler
-// issues one in 53 % of its cycles, and 25 us would remain if it always did), and a block's chain of three waits (positions, tables, maxima)
-// that one other block of the SM covers. Measured and left: 4 rows a block (56 us), 16 (one block a SM: 102), three blocks a SM with 32
-// registers (55), one or four rows side by side (46.6, 65), the rotation in integers (58).
+// kRows rows a block. A warp has 32 quads (whole heads) of q, of K or of V in all of them; the last warp has what the rows say of
+// themselves, the funnel's scalars and the softmax constants, a lane a row. From four rows for every SM on (eight where heads are normed) it takes
+// less than a block a row with two or four quads a thread: 12 + 2 + 2 heads of 128, 8,191 rows 39.5 us (76, 64), 2,047 rows 12.7 (19.9, 17.6), 700 rows
+// 8.6 (9.9, 11.0), 512 rows 9.3 (7.5, 8.0); normed 1,184 rows 16.0 (16.7, 17.6), 700 rows 15.0 (12.9, 16.5).
+// The floor of 8,191 rows is 13.6 us of memory traffic; what bounds it are instructions, about 140 for 32 quads and a row, half of them on the half-rate
+// pipe of comparisons and conversions (9,000 of a block's 14,000 cycles, with two blocks an SM), and the chain in front of them (positions and tables,
+// maxima, scalars: 4,400). Measured and left: 4 rows a block (56 us), 16 (one block an SM: 102), three blocks an SM with 32 registers (55), one or four
+// rows side by side (46.6, 65 where two took 45), the rotation in integers (58 where it took 53).
 constexpr int kRows = 8, kMostColumns = 31;
 struct SiteShared {
 	uint32_t top[32 * kRows], held[kRows], live;
-	int pos[kRows], page[kRows], slot[kRows], in_m[kRows], in_e[kRows];      // (of a row that is worked on; -1)
+	int page[kRows], slot[kRows], in_m[kRows], in_e[kRows];      // (page: -1 where the row is not worked on)
 	float4 funnel[kRows];      // f, f_lo and d (as bits)
 };
 template <bool NORMS, int MOST, int MIN>
@@ -393,7 +396,6 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 		const Scale in{lives ? w.in_m : 1 << 30, lives ? w.in_e : 0}, site{a.q_site_m, a.q_site_e};
 		if (lane < kRows) {
 			s.held[lane] = 0;
-			s.pos[lane] = lives ? w.pos : -1;
 			s.page[lane] = lives ? w.page : -1;
 			s.slot[lane] = w.place % kPageTokens;
 			s.in_m[lane] = (int)in.m;
@@ -445,21 +447,15 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 				else *(int4*)(x_at + r * x_step) = make_int4(0, 0, 0, 0);
 			}
 		}
-		// the rows of the tables, 16 bytes a thread; each makes what it copied to floats
-		const bool known = pos >= 0 && pos < a.num_positions;
+		asm volatile("cp.async.commit_group;" ::: "memory");
+		// the rows of the tables, 16 bytes a thread
 		const int32_t* angles = (const int32_t*)a.cos + (int64_t)pos * half;
 		const int64_t sines = a.sin - a.cos;
-		if (known)
+		if (pos >= 0 && pos < a.num_positions)
 			for (int k = 4 * (t / kRows); k < turn_step; k += x_step / (4 * kRows) * 4)
 				asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(s_turn + own * turn_step + k)), "l"(k < half ? angles + k : angles + sines + (k - half)) : "memory");
-		asm volatile("cp.async.wait_all;" ::: "memory");
-		if (known)
-			for (int k = 4 * (t / kRows); k < turn_step; k += x_step / (4 * kRows) * 4) {
-				int4* at = (int4*)(s_turn + own * turn_step + k);
-				const int4 v = *at;
-				constexpr float q30 = 1.0f / (1 << 30);
-				*(float4*)at = make_float4(q30 * __int2float_rn(v.x), q30 * __int2float_rn(v.y), q30 * __int2float_rn(v.z), q30 * __int2float_rn(v.w));
-			}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+		asm volatile("cp.async.wait_group 1;" ::: "memory");      // (the quads: a thread reads what it copied itself)
 	}
 	if (funnel && is_q) {
 		uint32_t mine = 0;
@@ -471,11 +467,11 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 		}
 		if (lane < kRows) s.top[warp * kRows + lane] = mine;
 	}
+	asm volatile("cp.async.wait_group 0;" ::: "memory");
 	__syncthreads();
 	const uint32_t live = s.live;
 	if (funnel && is_q) asm volatile("bar.sync 1, %0;" ::"r"(32 * (g.q_warps + 1)) : "memory");
 	const int e = (4 * i) & (hd - 1);
-	const float* turns = (const float*)s_turn;
 	if (is_q) {
 		const TurnLane l = turn_lane(a, e);
 		int8_t* to = a.q_codes + r0 * a.q_codes_stride + 4 * i;
@@ -517,7 +513,7 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 					for (int j = 0; j < 4; ++j) code[u][j] = __int_as_float(near[u][j]) - kRoundMagic;
 			}
 			uint32_t c[U];
-			turn_floats(a, code, l, turns + r * turn_step, turn_step, s.pos + r, c);
+			turn_floats(a, code, l, s_turn + r * turn_step, turn_step, c);
 #pragma unroll
 			for (int u = 0; u < U; ++u, to += a.q_codes_stride)
 				if (in && ((live >> (r + u)) & 1)) *(uint32_t*)to = c[u];
@@ -528,12 +524,14 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 		const int head = 4 * min(i, g.nk - 1) / hd;
 		const int64_t* rec = (is_k ? a.k_landing : a.v_landing) + 3 * head;
 		const bool normed = NORMS && is_k && a.k_gain != nullptr;
-		float rf = 0.0f;
+		float rf = 0.0f;      // r_t, zero where the float form does not apply
+		uint32_t r_less = 0;  // r_t - 1
 		int ef = 0;
 		if (!normed) {
 			const int64_t e_t = rec[1], r_t = rec[2];
 			if (r_t > 0 && r_t <= ((int64_t)1 << 32) && e_t > -(1 << 24) && e_t < (1 << 24)) {
 				rf = __ll2float_rn(r_t);
+				r_less = (uint32_t)(r_t - 1);
 				ef = (int)e_t;
 			}
 		}
@@ -570,14 +568,14 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 				if (far > kLandTie)
 #pragma unroll
 					for (int u = 0; u < U; ++u) {
-						const uint64_t v = land_quad_exact(x[u].x, x[u].y, x[u].z, x[u].w, in_m[u], rec[2], in_e[u], rec[1]);
+						const uint64_t v = land_quad_exact(x[u].x, x[u].y, x[u].z, x[u].w, in_m[u], rf > 0.0f ? (int64_t)r_less + 1 : rec[2], in_e[u], rf > 0.0f ? (int64_t)ef : rec[1]);
 						held[u] = (uint32_t)(v >> 32);
 #pragma unroll
 						for (int j = 0; j < 4; ++j) code[u][j] = (float)byte_of((uint32_t)v, j);
 					}
 			}
 			if (is_k) {
-				turn_floats(a, code, l, turns + r * turn_step, turn_step, s.pos + r, c);
+				turn_floats(a, code, l, s_turn + r * turn_step, turn_step, c);
 #pragma unroll
 				for (int u = 0; u < U; ++u) {
 					const int64_t token = (int64_t)s.page[r + u] * kPageTokens + s.slot[r + u];
@@ -598,31 +596,32 @@ __global__ void __launch_bounds__(MOST, MIN) k_qkv_site_rows(const __grid_consta
 				}
 		}
 		// V has the tokens of a page side by side: four rows on neighbouring places are one word
-		if (is_v)
-			for (int q = 0; q < kRows; q += 4) {
-				const int pg = s.page[q], at = s.slot[q];
-				const bool near = own < q || own >= q + 4 || (pg >= 0 && s.page[own] == pg && s.slot[own] == at + own - q);
-				const uint32_t c0 = (uint32_t)x_at[q * x_step], c1 = (uint32_t)x_at[(q + 1) * x_step], c2 = (uint32_t)x_at[(q + 2) * x_step], c3 = (uint32_t)x_at[(q + 3) * x_step];
-				if (__all_sync(0xffffffffu, near) && (at & 3) == 0) {
+		if (is_v) {
+			const int page = s.page[own], slot = s.slot[own], next = min(own + 1, kRows - 1);
+			const uint32_t goes_on = __ballot_sync(0xffffffffu, page >= 0 && own + 1 < kRows && s.page[next] == page && s.slot[next] == slot + 1);      // (row r + 1 behind row r)
+			for (int r = 0; r < kRows;) {
+				const int at = s.slot[r];
+				int8_t* to = plane + ((int64_t)s.page[r] * hd + e) * kPageTokens + at;
+				const uint32_t c0 = (uint32_t)x_at[r * x_step];
+				if ((at & 3) == 0 && (goes_on >> r & 7u) == 7u) {
+					const uint32_t c1 = (uint32_t)x_at[(r + 1) * x_step], c2 = (uint32_t)x_at[(r + 2) * x_step], c3 = (uint32_t)x_at[(r + 3) * x_step];
 					const uint32_t a0 = __byte_perm(c0, c1, 0x5140), a1 = __byte_perm(c2, c3, 0x5140);
 					const uint32_t b0 = __byte_perm(c0, c1, 0x7362), b1 = __byte_perm(c2, c3, 0x7362);
-					uint32_t* to = (uint32_t*)(plane + ((int64_t)pg * hd + e) * kPageTokens + at);
 					if (in) {
-						to[0] = __byte_perm(a0, a1, 0x5410);
-						to[kPageTokens / 4] = __byte_perm(a0, a1, 0x7632);
-						to[2 * kPageTokens / 4] = __byte_perm(b0, b1, 0x5410);
-						to[3 * kPageTokens / 4] = __byte_perm(b0, b1, 0x7632);
+						*(uint32_t*)to = __byte_perm(a0, a1, 0x5410);
+						*(uint32_t*)(to + kPageTokens) = __byte_perm(a0, a1, 0x7632);
+						*(uint32_t*)(to + 2 * kPageTokens) = __byte_perm(b0, b1, 0x5410);
+						*(uint32_t*)(to + 3 * kPageTokens) = __byte_perm(b0, b1, 0x7632);
 					}
+					r += 4;
 					continue;
 				}
-				for (int r = q; r < q + 4; ++r) {
-					int8_t* to = plane + ((int64_t)s.page[r] * hd + e) * kPageTokens + s.slot[r];
-					const uint32_t c = (uint32_t)x_at[r * x_step];
-					if (in && ((live >> r) & 1))
+				if (in && ((live >> r) & 1))
 #pragma unroll
-						for (int j = 0; j < 4; ++j) to[j * kPageTokens] = (int8_t)byte_of(c, j);
-				}
+					for (int j = 0; j < 4; ++j) to[j * kPageTokens] = (int8_t)byte_of(c0, j);
+				++r;
 			}
+		}
 	}
 	if (a.saturations != nullptr) {
 		asm volatile("bar.sync 2, %0;" ::"r"(64 * g.k_warps) : "memory");      // (the warps of K and V)
@@ -690,7 +689,7 @@ extern "C" sslm_status sslm_b200_qkv_site_resident(const sslm_b200_qkv_site* cal
 	const int columns = g.q_warps + 2 * g.k_warps;
 	const bool norms = c.q_gain != nullptr || c.k_gain != nullptr;
 	cudaError_t e;
-	if (c.rows >= kRows * sm_count() && columns <= kMostColumns) {
+	if (c.rows >= (norms ? kRows : kRows / 2) * sm_count() && columns <= kMostColumns) {
 		if (columns <= 16) e = norms ? site_launch_rows<true, 32 * 17, 2>(g, st) : site_launch_rows<false, 32 * 17, 2>(g, st);
 		else e = norms ? site_launch_rows<true, 1024, 1>(g, st) : site_launch_rows<false, 1024, 1>(g, st);
 	} else if (g.total <= 1024) e = c.rows <= sm_count() ? site_launch<1>(g, st) : site_launch<2>(g, st);

@@ -122,7 +122,7 @@ def by_hundreds(gpu_lib, torch, case):
 
 
 def many_rows(torch, seed, shape, more=5, first=3, **kind):
-    """eight rows for every SM and a few more; three sequences' places run on from `first`, the other rows' are drawn"""
+    """eight rows for every SM and a few more, enough for the form of many rows; three sequences' places run on from `first`, the other rows' are drawn"""
     rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count + more
     case = site_case(seed, shape, rows, positions=512, tables=6, **kind)
     g = np.random.default_rng(seed)
