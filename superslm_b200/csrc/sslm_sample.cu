@@ -21,6 +21,11 @@
 // does not work out that way (a list that overflows, a top-k beyond some thousands) is counted by one block over the whole row.
 //
 // A row is cut over the blocks of a cluster while rows are few; they exchange maxima and sums, and send their lists to the first one.
+//
+// Rows of 151,936 logits, us: one row with top-k 50 and top-p 10.0, 21 rows with a temperature alone 13.2, 64 with top-p 0.9 of which 2,400 tokens are kept on
+// the average 79, 256 with top-k 40 and top-p 44.5; 40 rows of 32,003 of which a schema allows 1,000, top-p, 16.3. One row is bound by its chain of passes and
+// exchanges, 256 rows by the first pass (35), the others by instructions: a weight is 15 of them a token, a pass of weights alone keeps a scheduler busy
+// for 49 cycles a warp's 32 tokens, one that lists besides 60 to 85.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -1019,8 +1024,9 @@ __global__ void __launch_bounds__(T, BLOCKS) k_sample(const __grid_constant__ Sa
 	}
 }
 
-// blocks a row: with few rows as many as leave every block a multiprocessor of its own (clusters do not fill the device: 132 of its 148),
-// with slices of 4,096 tokens and more, else one
+// Blocks a row: with few rows as many as leave every block a multiprocessor of its own (clusters do not fill the device: 132 of its 148), with
+// slices of 4,096 tokens and more, else one. 64 rows of 151,936: two blocks 97 us with top-p and 27 with top-k (one 156 and 28, three 131 and 35, four
+// 109 and 30, eight 133 and 48, as the kernel stood then); 32 rows: four 63 and 17 (two 92 and 23, eight 72 and 28).
 void sample_plan(SampleArgs* a) {
 	const int sms = sm_count(), most = std::max(1, (sms - 16) / a->rows), need = (a->vocab + kMostSlice - 128 - 1) / (kMostSlice - 128);
 	a->sub = std::min(kMostBlocks, std::max(need, std::min(most, std::max(1, a->vocab / 4096))));
