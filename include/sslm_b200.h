@@ -359,7 +359,7 @@ SSLM_API sslm_status sslm_b200_seq_set_controls(sslm_seq seq, const sslm_b200_co
  * embedding's (a model whose head has weights of its own: SSLM_INVALID_ARGUMENT); a row's temperature divides it. The first n_draws tokens take draws[i]
  * (0 .. 2^31 - 1), later ones numbers made from the seed and how many tokens were drawn since this call, or since the last sslm_seq_reset. Other
  * sequences of a call are chosen for as ever, and a save blob has nothing of this. NULL goes back to the greedy token; a second call
- * replaces the first. Outside these ranges, or with a list missing: SSLM_INVALID_ARGUMENT; nothing changes then. Room for logit rows as with controls. */
+ * replaces the first. Outside these ranges, with a list missing or a vocabulary above 2^20: SSLM_INVALID_ARGUMENT; nothing changes then. Room for logit rows as with controls. */
 typedef struct sslm_b200_sampling {
 	uint32_t struct_size;
 	int32_t temperature;             /* Q16: 65,536 is 1.0 */

@@ -209,6 +209,7 @@ cudaError_t launch_pick(const PickRow* rows, int m, int vocab, int names, int bi
 
 // ---- the draw of rows whose sequences are sampled (sslm_sample.cu): best[r] of the rows whose record has logits; scales: of the rows
 // that the head multiplied
+constexpr int kSampleIndexBits = 20, kSampleMostVocab = 1 << kSampleIndexBits;
 cudaError_t launch_sample(const SampleRow* rows, int m, int vocab, const Scale* scales, unsigned long long* best, int32_t* status, cudaStream_t st);
 
 // ---- attention over the paged KV pool (sslm_attn.cu)

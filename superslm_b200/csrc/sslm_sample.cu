@@ -43,8 +43,8 @@ constexpr int kList = 8192;                   // tokens of a row's list
 constexpr int kSteps = 1024;                  // sums of 256 tokens
 constexpr int kCounts = 2048;                 // places that a sample is counted into
 constexpr int kPlaces = 512;                  // places that a selection counts into, four words each
-constexpr int kIndexBits = 20;                // of a token
-constexpr int kMostVocab = 1 << kIndexBits;
+constexpr int kIndexBits = kSampleIndexBits;  // of a token
+constexpr int kMostVocab = kSampleMostVocab;
 constexpr int kMostSlice = (kSteps - 2) * 256;      // a sum for every 256 tokens, and for the ends
 constexpr int kMostBlocks = 16;
 constexpr uint32_t kLate = 0xFFFFFFFFu;

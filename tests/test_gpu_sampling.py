@@ -310,3 +310,22 @@ def test_many_rows_of_a_large_vocabulary(gpu_lib):
             assert st == 0 and toks[0::3] == toks[1::3] == toks[2::3]
     finally:
         eng.close()
+
+
+def test_a_vocabulary_that_is_too_large(gpu_lib):
+    for vocab, more in ((1 << 20, 0), ((1 << 20) + 8, 1)):
+        eng = engine(gpu_lib, n=1, cap=32, vocab=vocab)
+        try:
+            s = eng.new_seq()
+            s.prefill([1, 2, 3], 64)
+            if more:
+                with pytest.raises(abi.SslmError):
+                    s.set_sampling(top_k=1)
+                continue
+            st, want = eng.decode_step([s], eng.num_layers)
+            s.reset()
+            s.prefill([1, 2, 3], 64)
+            s.set_sampling(top_k=1)
+            assert st == 0 and eng.decode_step([s], eng.num_layers) == (0, want)
+        finally:
+            eng.close()
