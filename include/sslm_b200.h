@@ -592,10 +592,10 @@ SSLM_API sslm_status sslm_b200_sample_resident(const sslm_b200_sample* call, voi
  * What a sequence held and no longer holds it lets go. Pages that are drawn were free before the call, lowest first, in the order of the
  * sequences: drawn[0 .. counts[1]) (behind these, free pages that were too few for a sequence may follow). moves[0 .. counts[0]) are the pages
  * copied, (from, to), whole, in every plane of kv (NULL: none are copied, for a caller whose planes lie apart). Entries of out_tables behind a
- * sequence's pages, and of moves behind the count, stay as they were. status[i]: 0, or why the sequence stays what it was: a parent that does not exist or a page id of it that does not
- * (SSLM_B200_ROW_INDEX), a length or growth below 0 or together above the table's room (_LENGTH), not enough free pages for it (_PAGES: those
- * in front of it are served). Outputs may not overlap inputs. At most 65,535 sequences and 65,536 pages a table; page_bytes a multiple of
- * 16, kv on a 16-byte boundary, moves on an 8-byte one. Two launches. */
+ * sequence's pages, and of moves behind the count, stay as they were. status[i]: 0, or why the sequence stays what it was: a parent that does not exist or
+ * a page id of it that does not (SSLM_B200_ROW_INDEX), a length or growth below 0 or together above the table's room (_LENGTH), not enough free pages for it
+ * (_PAGES: those in front of it are served). Without sequences holders go to out_holders as they are and counts are zeros. Outputs may not overlap
+ * inputs. At most 65,535 sequences and 65,536 pages a table; page_bytes a multiple of 16, kv on a 16-byte boundary, moves on an 8-byte one. Two launches. */
 #define SSLM_B200_ROW_PAGES 102
 typedef struct sslm_b200_fork {
 	uint32_t struct_size;

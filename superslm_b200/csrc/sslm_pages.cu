@@ -382,6 +382,13 @@ sslm_status pages_check(const A& c) {
 }
 template <typename... P>
 bool words(P... p) { return ((((uintptr_t)p & 3) == 0) && ...); }
+// memory that the runtime knows, or none
+bool reachable(const void* p) {
+	cudaPointerAttributes at;
+	if (p == nullptr || (cudaPointerGetAttributes(&at, p) == cudaSuccess && at.type != cudaMemoryTypeUnregistered)) return true;
+	cudaGetLastError();
+	return false;
+}
 
 }  // namespace
 }  // namespace sslm
@@ -393,15 +400,17 @@ extern "C" sslm_status sslm_b200_fork_resident(const sslm_b200_fork* call, void*
 	const sslm_b200_fork& c = *call;
 	const sslm_status st = pages_check(c);
 	if (st != SSLM_OK) return st;
-	if (c.sequences == 0) return SSLM_OK;
-	if (!c.lengths || !c.parents || !c.out_lengths || !c.status || !c.moves || !c.counts) return SSLM_INVALID_ARGUMENT;
-	if (c.table_pages > 0 && (!c.tables || !c.out_tables)) return SSLM_INVALID_ARGUMENT;
-	if (c.num_pages > 0 && (!c.holders || !c.out_holders || !c.drawn)) return SSLM_INVALID_ARGUMENT;
+	const bool any = c.sequences > 0;
+	if (!c.counts || (any && (!c.lengths || !c.parents || !c.out_lengths || !c.status || !c.moves))) return SSLM_INVALID_ARGUMENT;
+	if (any && c.table_pages > 0 && (!c.tables || !c.out_tables)) return SSLM_INVALID_ARGUMENT;
+	if (c.num_pages > 0 && (!c.holders || !c.out_holders || (any && !c.drawn))) return SSLM_INVALID_ARGUMENT;
 	if (c.holders && c.holders == c.out_holders) return SSLM_INVALID_ARGUMENT;      // (read when others are written)
-	if ((c.tables && c.tables == c.out_tables) || c.lengths == c.out_lengths) return SSLM_INVALID_ARGUMENT;
+	if (any && ((c.tables && c.tables == c.out_tables) || c.lengths == c.out_lengths)) return SSLM_INVALID_ARGUMENT;
 	if (!words(c.holders, c.tables, c.lengths, c.parents, c.grow, c.out_holders, c.out_tables, c.out_lengths, c.status, c.drawn, c.counts) || ((uintptr_t)c.moves & 7) ||
 	    ((uintptr_t)c.kv & 15))
 		return SSLM_MISALIGNED_BUFFER;
+	// (no sequences: the holders are still to be handed on. A caller without sequences may have no cache either; such addresses are left alone)
+	if (!any && (!reachable(c.holders) || !reachable(c.out_holders) || !reachable(c.counts))) return SSLM_OK;
 	if (pages_launch(k_fork, c, c.sequences, (cudaStream_t)stream) != cudaSuccess) {
 		cudaGetLastError();
 		return SSLM_ALLOCATION_FAILED;
