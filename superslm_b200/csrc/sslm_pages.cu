@@ -27,8 +27,9 @@ constexpr int kMostRange = 4096;      // sequences of a block: kMostSequences ov
 constexpr uint32_t kCopies = 0x80000000u, kRefused = 0xFFFFFFFFu;
 
 // sums that every block has of every block
-struct Told { uint32_t v[16][2]; };
+struct Told { alignas(8) uint32_t v[16][2]; };      // (a pair is stored as one word of 8 bytes)
 __device__ __forceinline__ void tell(Told& told, int blocks, uint32_t a, uint32_t b) {      // (one thread per peer; a cluster barrier follows)
+	static_assert(alignof(Told) == 8 && sizeof(told.v[0]) == 8, "a pair's place");
 	if ((int)threadIdx.x < blocks) {
 		const uint32_t at = cta_addr(told.v[cluster_rank()]);
 		asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\tst.shared::cluster.v2.u32 [ra], {%2, %3};\n\t}" ::"r"(at), "r"((uint32_t)threadIdx.x), "r"(a), "r"(b)
