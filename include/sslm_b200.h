@@ -624,8 +624,8 @@ SSLM_API sslm_status sslm_b200_fork_resident(const sslm_b200_fork* call, void* s
  * in front of it, the lowest to the lowest. new_of[p] is page p's new id, -1 where it is free; moves[0 .. counts[0]) are (from, to), copied in every
  * plane of kv (NULL: not); counts[1] = live. out_holders and out_tables are holders and tables under the new ids; entries behind a sequence's
  * pages, and of moves behind the count, stay as they were. status[i] (may be NULL): 0, or a length below 0 or above the table's room
- * (SSLM_B200_ROW_LENGTH), a page id that does not exist or is free (_INDEX): such a table is not written. out_tables may be tables; other
- * outputs may not overlap inputs. Limits and alignment as above. Two launches. */
+ * (SSLM_B200_ROW_LENGTH), a page id that does not exist or is free (_INDEX): such a table is not written. out_tables may be tables with
+ * the same stride; other outputs may not overlap inputs. Limits and alignment as above. Two launches. */
 typedef struct sslm_b200_compact {
 	uint32_t struct_size;
 	int32_t sequences, table_pages, planes, page_bytes;

@@ -428,6 +428,7 @@ extern "C" sslm_status sslm_b200_compact_resident(const sslm_b200_compact* call,
 	if (c.sequences > 0 && (!c.lengths || (c.table_pages > 0 && (!c.tables || !c.out_tables)))) return SSLM_INVALID_ARGUMENT;
 	if (c.num_pages > 0 && (!c.holders || !c.out_holders || !c.new_of || (c.num_pages > 1 && !c.moves))) return SSLM_INVALID_ARGUMENT;
 	if (c.holders && c.holders == c.out_holders) return SSLM_INVALID_ARGUMENT;
+	if (c.sequences > 1 && c.table_pages > 0 && c.tables == c.out_tables && c.tables_stride != c.out_stride) return SSLM_INVALID_ARGUMENT;      // (a row would be another one's input)
 	if (!words(c.holders, c.tables, c.lengths, c.out_holders, c.out_tables, c.new_of, c.counts, c.status) || ((uintptr_t)c.moves & 7) || ((uintptr_t)c.kv & 15))
 		return SSLM_MISALIGNED_BUFFER;
 	if (pages_launch(k_compact, c, (int)(c.num_pages / 2), (cudaStream_t)stream) != cudaSuccess) {
