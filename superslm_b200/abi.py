@@ -421,7 +421,9 @@ class _ResidentCall:
             with torch.cuda.device(self._device):
                 return self.run(stream)
         if stream is None:
-            stream = torch._C._cuda_getCurrentRawStream(self._device.index)      # (torch.cuda.current_stream() makes an object: 3.2 us)
+            # (torch.cuda.current_stream() makes an object, 3.2 us; the handle alone is not of torch's public interface)
+            handle = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            stream = handle(self._device.index) if handle is not None else torch.cuda.current_stream(self._device).cuda_stream
         st = self._fn(C.addressof(self.args), stream)
         if st != SSLM_OK:
             raise SslmError(self.verb, st)
