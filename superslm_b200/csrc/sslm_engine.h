@@ -164,6 +164,14 @@ struct sslm_adapter_s {
 	std::atomic<uint32_t> live_refs{0};
 };
 
+// Sequences with one uid (of a frozen prefix, or given out for a fork) have the same first pages. A sequence that forks again and again keeps the
+// share of fewest pages, which most others have, and the latest ones.
+struct SharedPages {
+	uint64_t uid;
+	int32_t pages;
+};
+constexpr int kMostShares = 4;
+
 struct sslm_seq_s {
 	sslm_model_s* model = nullptr;
 	sslm_kv_pool_s* pool = nullptr;
@@ -178,7 +186,6 @@ struct sslm_seq_s {
 	size_t pages_on_device = 0;     // entries of it that are in place
 	uint64_t batch_mark = 0;        // the decode batch the sequence was last put into
 	uint64_t uid = 0;               // of the sequences created so far
-	// the first pages are those of the frozen prefix with this uid, or of the fork it was given out for (0: none): sequences with one uid have the same ones
 	// tokens the sequence was given and tokens it produced, in order (since it was created, reset or restored)
 	std::vector<int32_t> given, produced;
 	// penalties and biases of its picks (sslm_b200_seq_set_controls); their ids and the biases lie in the sequence's slot of the pool
@@ -193,8 +200,9 @@ struct sslm_seq_s {
 	uint32_t top_p = 0, min_p = 0;
 	uint64_t seed = 0, drawn = 0;      // tokens drawn so far
 	std::vector<int32_t> draws;
-	uint64_t shared_uid = 0;
-	int32_t shared_pages = 0;
+	// its first pages that others have too, fewest pages first: those of the prefix it adopted, of forks it was a side of
+	SharedPages shares[kMostShares] = {};
+	int n_shares = 0;
 	int64_t context_length = 0;
 	uint32_t layer_index = 0;
 	int32_t current_token = -1;
@@ -208,6 +216,13 @@ struct sslm_seq_s {
 	int64_t forced_token_count = 0;
 	std::mutex lifecycle_mutex;
 
+	void share(SharedPages with) {      // (more pages than it shares so far)
+		if (n_shares == kMostShares) {
+			for (int i = 1; i + 1 < kMostShares; ++i) shares[i] = shares[i + 1];
+			--n_shares;
+		}
+		shares[n_shares++] = with;
+	}
 	int8_t* hidden(int slot) const { return (int8_t*)(d_state + (size_t)slot * state_stride); }
 	sslm::Scale* scale(int slot) const { return (sslm::Scale*)(d_state + (size_t)slot * state_stride + scale_off); }
 };
