@@ -361,9 +361,15 @@ __device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const f
 }
 
 // kRows rows a block. A warp has 32 quads (whole heads) of q, of K or of V in all of them; the last warp has what the rows say of
-// themselves, the funnel's scalars and the softmax constants, a lane a row. From four rows for every SM on (eight where heads are normed) it takes
-// less than a block a row with two or four quads a thread: 12 + 2 + 2 heads of 128, 8,191 rows 39.5 us (76, 64), 2,047 rows 12.7 (19.9, 17.6), 700 rows
-// 8.6 (9.9, 11.0), 512 rows 9.3 (7.5, 8.0); normed 1,184 rows 16.0 (16.7, 17.6), 700 rows 15.0 (12.9, 16.5).
+// themselves, the funnel's scalars and the softmax constants, a lane a row. It takes less than a block a row with two quads a thread where those
+// blocks no longer fit the device at once, from about 2,048 quads for every SM on and four rows (5,000 where q is normed, whose roots the warps do one behind the
+// other). Eleven widths, 1,536 to 12,288 quads an SM, this form / a block a row, us:
+//   12 + 2 + 2 heads of 128   593 rows 9.0 / 8.4   723 9.2 / 9.6   917 8.7 / 10.6   1,777 13.0 / 17.3   3,553 23.0 / 31.0
+//    4 + 2 + 2 heads of 32  2,368 rows 6.8 / 6.0   4,737 7.9 / 9.3   9,473 12.3 / 15.4   28,417 29.7 / 40.9
+//   20 + 4 + 4 heads of 128   413 rows 11.6 / 10.9   677 12.3 / 15.0   2,030 22.7 / 34.7
+//   q and K normed: 12 + 2 + 2 of 128 1,185 rows 22.7 / 17.5, 1,777 23.1 / 23.8, 3,553 41.2 / 43.4; 4 + 2 + 2 of 32 4,737 rows 13.7 / 12.4, 14,209 31.4 / 29.8, 28,417
+//   52.2 / 57.3; 16 + 2 + 2 of 128 1,157 rows 16.6 / 19.5. K alone: 12 + 2 + 2 of 128 723 rows 13.4 / 13.6, 1,185 17.5 / 19.8.
+// Both go up by steps, as their blocks fill the device once more, so near the border either may be a tenth ahead.
 // The floor of 8,191 rows is 13.6 us of memory traffic; what bounds it are instructions, about 140 for 32 quads and a row, half of them on the half-rate
 // pipe of comparisons and conversions (9,000 of a block's 14,000 cycles, with two blocks an SM), and the chain in front of them (positions and tables,
 // maxima, scalars: 4,400). Measured and left: 4 rows a block (56 us), 16 (one block an SM: 102), three blocks an SM with 32 registers (55), one or four
@@ -689,7 +695,8 @@ extern "C" sslm_status sslm_b200_qkv_site_resident(const sslm_b200_qkv_site* cal
 	const int columns = g.q_warps + 2 * g.k_warps;
 	const bool norms = c.q_gain != nullptr || c.k_gain != nullptr;
 	cudaError_t e;
-	if (c.rows >= (norms ? kRows : kRows / 2) * sm_count() && columns <= kMostColumns) {
+	const int64_t sms = sm_count(), quads = (int64_t)c.rows * g.total;
+	if (c.rows >= kRows / 2 * sms && quads > (turns && c.q_gain != nullptr ? 5000 : 2048) * sms && columns <= kMostColumns) {
 		if (columns <= 16) e = norms ? site_launch_rows<true, 32 * 17, 2>(g, st) : site_launch_rows<false, 32 * 17, 2>(g, st);
 		else e = norms ? site_launch_rows<true, 1024, 1>(g, st) : site_launch_rows<false, 1024, 1>(g, st);
 	} else if (g.total <= 1024) e = c.rows <= sm_count() ? site_launch<1>(g, st) : site_launch<2>(g, st);
