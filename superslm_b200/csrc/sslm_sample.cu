@@ -18,18 +18,26 @@
 //
 // Where top-p keeps more than the list has (the sums tell), a sample of the row says where the end of what is kept must lie; a pass adds up
 // what is surely kept and lists a window around that end, which is cut as the list is; then the sums of 256 tokens as above. Whatever
-// does not work out that way (a list that overflows, a top-k beyond some thousands) is counted by one block over the whole row.
+// does not work out that way is counted by one block over the whole row, in some 20 passes: a list that overflows, or one with fewer tokens
+// than top-k. The groups are 512 at most, and the least of 512 maxima leaves 3,440 tokens on the average (of normal logits; 2,500 to 4,900
+// in 60 rows), so that is where a large top-k ends up: in some rows from 2,500 on, in nearly all above 4,500. Rows of 151,936, us: 64 rows with top-k
+// 2,000 41, 2,500 286, 4,000 399; one row 22, 22, 361.
 //
 // A row is cut over the blocks of a cluster while rows are few; they exchange maxima and sums, and send their lists to the first one.
 //
 // Rows of 151,936 logits, us: one row with top-k 50 and top-p 10.0, 21 rows with a temperature alone 13.2, 64 with top-p 0.9 of which 2,400 tokens are kept on
-// the average 79, 256 with top-k 40 and top-p 44.5; 40 rows of 32,003 of which a schema allows 1,000, top-p, 16.3. One row is bound by its chain of passes and
-// exchanges, 256 rows by the first pass (35), the others by instructions: a weight is 15 of them a token, a pass of weights alone keeps a scheduler busy
-// for 49 cycles a warp's 32 tokens, one that lists besides 60 to 85.
+// the average 79, 256 with top-k 40 and top-p 44.5; 40 rows of 32,003 of which a schema allows 1,000, top-p, 16.3. What bounds them, by a block's clock
+// (cycles at 1.9 GHz):
+//   one row    its chain: the maximum 2,900, the list 3,900, their exchanges 900 and 2,400, the lists' exchange, cut and draw 7,800
+//   21 rows    the second pass with 12,100 of 23,700 (a pass of weights keeps a scheduler busy for 49 cycles a warp's 32 tokens, one that lists besides 60 to
+//              85), then the first pass 3,000, exchanges 2,000 and 2,400, the search of the token 3,000
+//   40 rows    the lists' exchange and the selections in one block with 13,200 of 28,400, then the second pass with 8,000, which weighs masked tokens too
+//   64 rows    their passes, the window's among them, which weighs every token though few count there (45 % of the issue slots are used)
+//   256 rows   the first pass, 57,000 of 76,000 at 4.5 TB/s: two blocks a multiprocessor leave 64 registers, of which 322 bytes are stored and 454 loaded,
+//              and the loads are what it waits for
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "../../include/sslm_b200.h"
 #include "sslm_cluster.cuh"

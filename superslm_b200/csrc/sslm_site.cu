@@ -372,8 +372,9 @@ __device__ __forceinline__ void turn_floats(const sslm_b200_qkv_site& a, const f
 // Both go up by steps, as their blocks fill the device once more, so near the border either may be a tenth ahead.
 // The floor of 8,191 rows is 13.6 us of memory traffic; what bounds it are instructions, about 140 for 32 quads and a row, half of them on the half-rate
 // pipe of comparisons and conversions (9,000 of a block's 14,000 cycles, with two blocks an SM), and the chain in front of them (positions and tables,
-// maxima, scalars: 4,400). Measured and left: 4 rows a block (56 us), 16 (one block an SM: 102), three blocks an SM with 32 registers (55), one or four
-// rows side by side (46.6, 65 where two took 45), the rotation in integers (58 where it took 53).
+// maxima, scalars: 4,400). Two blocks of 17 warps leave 56 registers, so 92 bytes are stored and 192 loaded again. Measured and left: 4 rows a block (56 us), 16
+// (one block an SM: 102), three blocks an SM with 32 registers (55), one or four rows side by side (46.6, 65 where two took 45), the rotation in integers
+// (58 where it took 53).
 constexpr int kRows = 8, kMostColumns = 31;
 struct SiteShared {
 	uint32_t top[32 * kRows], held[kRows], live;
